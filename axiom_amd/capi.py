@@ -76,6 +76,31 @@ class GemmParams(C.Structure):
     ]
 
 
+class RowsQ8Params(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("eps", C.c_float),
+        ("rows", C.c_int64), ("cols", C.c_int64),
+        ("ld_x", C.c_int64), ("ld_residual", C.c_int64), ("ld_sum", C.c_int64), ("ld_q", C.c_int64),
+    ]
+
+
+class GemmQ8Params(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("epilogue_op", C.c_int32),
+        ("m", C.c_int64), ("n", C.c_int64), ("k", C.c_int64),
+        ("lda", C.c_int64), ("ldb", C.c_int64), ("ldc", C.c_int64),
+        ("scale_a", C.c_void_p), ("scale_b", C.c_void_p), ("bias", C.c_void_p), ("residual", C.c_void_p),
+    ]
+
+
+class SampleParams(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32),
+        ("rows", C.c_int64), ("vocab", C.c_int64), ("ld", C.c_int64),
+        ("temperature", C.c_void_p), ("top_k", C.c_void_p), ("top_p", C.c_void_p), ("min_p", C.c_void_p), ("u", C.c_void_p),
+    ]
+
+
 _lib = None
 
 
@@ -140,6 +165,14 @@ def lib() -> C.CDLL:
         l.axhip_reduce_axis_ws.argtypes = [C.c_void_p, C.c_int32, C.c_int64, C.c_int64, C.c_int64, C.c_int32, C.c_void_p, C.c_int32, C.c_void_p, C.c_size_t, C.c_void_p]
         l.axhip_softmax_axis.argtypes = [C.c_void_p, C.c_int32, C.c_int64, C.c_int64, C.c_int64, C.c_int32, C.c_void_p, C.c_void_p]
         l.axhip_gather_rows.argtypes = [C.c_void_p, C.c_int32, C.c_int64, C.c_int64, C.c_void_p, C.c_int32, C.c_int64, C.c_void_p, C.c_void_p]
+        l.axhip_quantize_q8.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.POINTER(RowsQ8Params), C.c_void_p]
+        l.axhip_rms_norm_q8.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.POINTER(RowsQ8Params), C.c_void_p]
+        l.axhip_gemm_q8.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.POINTER(GemmQ8Params), C.c_void_p]
+        l.axhip_gemm_q8_last_kernel.restype = C.c_char_p
+        l.axhip_sample.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.POINTER(SampleParams), C.c_void_p]
+        l.axhip_sample_workspace_bytes.restype = C.c_size_t
+        l.axhip_sample_workspace_bytes.argtypes = [C.POINTER(SampleParams)]
+        l.axhip_sample_ws.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.POINTER(SampleParams), C.c_void_p, C.c_size_t, C.c_void_p]
         _lib = l
     return _lib
 

@@ -53,6 +53,9 @@ size_t axhip_sizeof(int which) {
     case 2: return sizeof(AxhipGemmParams);
     case 3: return sizeof(AxhipOperand);
     case 4: return sizeof(AxhipChainOp);
+    case 5: return sizeof(AxhipRowsQ8Params);
+    case 6: return sizeof(AxhipGemmQ8Params);
+    case 7: return sizeof(AxhipSampleParams);
     default: return 0;
     }
 }

@@ -464,10 +464,86 @@ int axhip_gemm_ws(const void *a, const void *b, void *c, const AxhipGemmParams *
  * tile), the same with "_parts" (fp32 by products of bf16 parts), "fma", "empty". */
 const char *axhip_gemm_last_kernel(void);
 
+/* ------------------------------------------------------------- 8-bit rows
+ * Rows of values as int8 with one fp32 scale each: q[r][j] * scales[r] stands for the value.  q lies in [-127, 127]; the nearest
+ * integer is taken, halves to the even one, decided on exact products (a value next to a half falls on the right side of it).
+ * A row of zeros has scale 0; a row that holds an infinity or a NaN (or whose products overflow fp32) has scale NaN and zeros, so
+ * that every product with it comes out as NaN.  Rows are contiguous, ld_* elements apart (at least cols; any alignment).
+ *
+ * axhip_quantize_q8: scales[r] = max_j |x[r][j]| / 127.  The weight (n, k) of nn::Linear by output channel, activations by token.
+ *
+ * axhip_rms_norm_q8: the residual's addition and the RMS norm of a pre-norm block (ops::add, then ops::rms_norm,
+ * include/axiom/operations.hpp and src/nn/normalization.cpp), out in 8 bits for the product that follows: with
+ *     h = x + residual, rounded to dtype (residual NULL: h = x),   y = h / sqrt(mean(h^2) + eps) * weight
+ * q and scales stand for y, which is rounded nowhere else; the statistics are fp32.  sum: NULL, or where h goes for the
+ * next residual addition (x or residual itself, with the same ld, is allowed; needs a residual).  x, residual, weight (NULL: ones) and sum are of
+ * `dtype`.  No temporary memory; axhip_quantize_q8 reads dtype, rows, cols, ld_x and ld_q only. */
+typedef struct {
+    int32_t dtype; /* of x, residual, weight and sum */
+    float eps;
+    int64_t rows, cols;
+    int64_t ld_x, ld_residual, ld_sum, ld_q; /* elements */
+} AxhipRowsQ8Params;
+
+int axhip_quantize_q8(const void *x, int8_t *q, float *scales, const AxhipRowsQ8Params *params_host, void *stream);
+int axhip_rms_norm_q8(const void *x, const void *residual, const void *weight, void *sum, int8_t *q, float *scales,
+                      const AxhipRowsQ8Params *params_host, void *stream);
+
+/* ------------------------------------------------------- products in 8 bits
+ * nn::Linear (src/nn/linear.cpp:15-27) on rows in 8 bits: C = act(scale_a[m] scale_b[n] sum_k A[m][k] B[n][k] (+ bias[n]) (+ residual)),
+ * A (m, k) and B (n, k) int8, row-major, lda / ldb / ldc in elements, any alignment.  The sums are int32 and exact: k up to
+ * 131071, beyond which rows of -128 could overflow (AXHIP_ERR_UNSUPPORTED).  scale_a [m] and scale_b [n] are fp32; the rest is fp32 arithmetic,
+ * rounded once to dtype.  residual has C's layout and may be C itself.  No temporary memory. */
+typedef struct {
+    int32_t dtype;       /* of C, bias and residual: Float32, Float16 or BFloat16 */
+    int32_t epilogue_op; /* 0 or AXHIP_OP_RELU / GELU / SILU / SIGMOID / TANH */
+    int64_t m, n, k;
+    int64_t lda, ldb, ldc;
+    const float *scale_a; /* [m] */
+    const float *scale_b; /* [n] */
+    const void *bias;     /* [n] or NULL */
+    const void *residual; /* same layout as C or NULL */
+} AxhipGemmQ8Params;
+
+int axhip_gemm_q8(const int8_t *a, const int8_t *b, void *c, const AxhipGemmQ8Params *params_host, void *stream);
+/* diagnostic: the kernel of the calling thread's last axhip_gemm_q8 */
+const char *axhip_gemm_q8_last_kernel(void);
+
+/* ---------------------------------------------------------------- sampling
+ * A token from each row of logits [rows, vocab]: what axhip_argreduce does for greedy decoding, for the rest.  It has no
+ * counterpart in the reference.  Each setting is an array of `rows` values on the device, or NULL (off).  With
+ * w_i = exp((l_i - max l) / temperature) and the order "larger logit first, equal ones by index":
+ *     top_k  (k > 0)      keeps the first k;
+ *     top_p  (p < 1)      of those, keeps the ones in front of which less than p of their sum of w lies (always the first);
+ *     min_p  (0 < m)      of those, keeps the ones with w_i >= m (more than 1 counts as 1);
+ *     u                   in [0, 1): the token is the first kept index, by index, at which the running sum of w exceeds u times
+ *                         the sum of all that are kept.
+ * temperature 0 (or less, or NaN) takes the first largest logit.  NULL: 1.  -inf and NaN are never drawn; +inf shares the draw with
+ * its equals alone.  A row that has nothing else gets token -1.  probs (or NULL): the kept probability of the token (1 for
+ * temperature 0, 0 for token -1).  The same arguments give the same tokens, whatever else runs: sums are of
+ * multiples of 2^-43 of the largest weight, so that no order changes them; a token below 2^-44 of the most likely one is never drawn.
+ * vocab up to 2^20 (AXHIP_ERR_UNSUPPORTED beyond), rows ld elements apart, any alignment. */
+typedef struct {
+    int32_t dtype;
+    int64_t rows, vocab, ld;
+    const float *temperature; /* [rows] or NULL */
+    const int32_t *top_k;     /* [rows] or NULL; 0 or less: off for the row */
+    const float *top_p;       /* [rows] or NULL; 1 or more: off for the row */
+    const float *min_p;       /* [rows] or NULL; 0 or less: off for the row */
+    const float *u;           /* [rows] */
+} AxhipSampleParams;
+
+int axhip_sample(const void *logits, int64_t *tokens, float *probs, const AxhipSampleParams *params_host, void *stream);
+/* The same with its temporary memory handed in by the caller (0 bytes for every shape that needs none). */
+size_t axhip_sample_workspace_bytes(const AxhipSampleParams *params_host);
+int axhip_sample_ws(const void *logits, int64_t *tokens, float *probs, const AxhipSampleParams *params_host,
+                    void *workspace, size_t workspace_bytes, void *stream);
+
 /* sizeof() of the parameter structs as this library was compiled, so that a
  * foreign-language binding can verify its own struct layout at load time:
  * which = 0 AxhipSdpaParams, 1 AxhipRowsProgram, 2 AxhipGemmParams,
- * 3 AxhipOperand, 4 AxhipChainOp; anything else returns 0. */
+ * 3 AxhipOperand, 4 AxhipChainOp, 5 AxhipRowsQ8Params, 6 AxhipGemmQ8Params,
+ * 7 AxhipSampleParams; anything else returns 0. */
 size_t axhip_sizeof(int which);
 
 #ifdef __cplusplus
