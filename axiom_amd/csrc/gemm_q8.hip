@@ -1,11 +1,15 @@
 // Products of int8 rows with scales: axhip_gemm_q8.
+#include "gemm_q8.hpp"
 #include "gemm_skinny.hpp"
+
+#include <algorithm>
+#include <utility>
 
 namespace axhip {
 namespace {
 thread_local const char *q8_last_kernel = "none";
 
-struct Q8Args {
+struct GenericArgs {
     const int8_t *a, *b;
     void *c;
     const float *scale_a, *scale_b;
@@ -15,7 +19,7 @@ struct Q8Args {
 };
 
 // Any size and alignment: a work-group owns 16 x 16 of C, k goes through LDS.
-__global__ __launch_bounds__(256) void gemm_q8_generic_kernel(const Q8Args g, int64_t tiles_n) {
+__global__ __launch_bounds__(256) void gemm_q8_generic_kernel(const GenericArgs g, int64_t tiles_n) {
     __shared__ int8_t As[16][68], Bs[16][68];
     const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
     const int64_t m0 = blockIdx.x / tiles_n * 16, n0 = blockIdx.x % tiles_n * 16;
@@ -36,6 +40,82 @@ __global__ __launch_bounds__(256) void gemm_q8_generic_kernel(const Q8Args g, in
         if (g.residual) y += load_any(g.residual, g.dtype, m * g.ldc + n);
         store_any(g.c, g.dtype, m * g.ldc + n, gemm_epilogue(g.epilogue, y));
     }
+}
+
+// Within the 32-bit offsets the matrix-core kernels address with, and a whole chunk of k.
+bool takes_q8_kernels(const AxhipGemmQ8Params &p) {
+    constexpr int64_t LD = int64_t(1) << 22;
+    return p.k >= 16 && p.lda < LD && p.ldb < LD && p.ldc < (int64_t(1) << 31);
+}
+
+// The candidates with the time each takes, in us: start + k (per_k + per_k_full u) r + per_round (r - 1), r being the rounds its work-groups take on
+// the 256 CUs and u how full the first is.
+struct Q8Kernel {
+    enum Kind { BIG256, TILE, SMALL } kind;
+    int shape, waves;
+    float start, per_k, per_k_full, per_round;
+    bool ragged;
+    const char *name;
+};
+constexpr Q8Kernel Q8_KERNELS[] = {
+    {Q8Kernel::BIG256, 0, 8, 7.0f, 0.0160f, 0.0057f, 4.0f, false, "big"},
+    {Q8Kernel::TILE, TILE_256x128, 8, 6.5f, 0.0080f, 0.0034f, 6.4f, false, "tile_256x128"},
+    {Q8Kernel::TILE, TILE_192x128, 8, 5.7f, 0.0063f, 0.0024f, 4.9f, false, "tile_192x128"},
+    {Q8Kernel::TILE, TILE_128x128, 8, 4.9f, 0.0048f, 0.0014f, 4.1f, false, "tile_128x128"},
+    {Q8Kernel::TILE, TILE_64x128, 8, 4.9f, 0.0032f, 0.0009f, 3.7f, false, "tile_64x128"},
+    {Q8Kernel::TILE, TILE_128x128, 8, 6.5f, 0.0080f, 0.0f, 5.9f, true, "tile_128x128_ragged"},
+    {Q8Kernel::SMALL, SMALL_64x64, 8, 4.35f, 0.00245f, 0.00148f, 3.6f, false, "small_64x64_8"},
+    {Q8Kernel::SMALL, SMALL_64x64, 4, 4.15f, 0.00324f, 0.00047f, 1.65f, false, "small_64x64_4"},
+    {Q8Kernel::SMALL, SMALL_32x64, 8, 3.50f, 0.00170f, 0.00085f, 2.3f, false, "small_32x64_8"},
+    {Q8Kernel::SMALL, SMALL_32x64, 4, 3.30f, 0.00210f, 0.00030f, 0.6f, false, "small_32x64_4"},
+    {Q8Kernel::SMALL, SMALL_32x32, 8, 3.07f, 0.00105f, 0.00045f, 0.76f, false, "small_32x32_8"},
+    {Q8Kernel::SMALL, SMALL_32x32, 4, 2.95f, 0.00148f, 0.00005f, 0.26f, false, "small_32x32_4"},
+    {Q8Kernel::SMALL, SMALL_32x16, 8, 2.92f, 0.00074f, 0.00032f, 0.33f, false, "small_32x16_8"},
+    {Q8Kernel::SMALL, SMALL_32x16, 4, 2.91f, 0.00102f, 0.00004f, 0.10f, false, "small_32x16_4"},
+    {Q8Kernel::SMALL, SMALL_16x16, 8, 2.95f, 0.00045f, 0.00024f, 0.19f, false, "small_16x16_8"},
+    {Q8Kernel::SMALL, SMALL_16x16, 4, 2.94f, 0.00069f, 0.00004f, 0.02f, false, "small_16x16_4"},
+};
+constexpr size_t Q8_CANDIDATES = sizeof(Q8_KERNELS) / sizeof(Q8_KERNELS[0]);
+
+struct Q8Choice { const Q8Kernel *best; float cost; };
+// One candidate.  (A parameter of the template, so that its tiles are constants here: divisions by what a table holds cost a small product's caller.)
+template <size_t I> void consider(const AxhipGemmQ8Params &p, bool aligned, Q8Choice &c) {
+    constexpr const Q8Kernel &h = Q8_KERNELS[I];
+    if (h.kind != Q8Kernel::SMALL && h.ragged == aligned) return;
+    if (h.kind == Q8Kernel::BIG256 && (p.k % 128 != 0 || p.m < 256 || p.n < 256)) return;
+    constexpr uint32_t tm = h.kind == Q8Kernel::BIG256 ? 256 : h.kind == Q8Kernel::TILE ? TILE_GEOMETRY[h.kind == Q8Kernel::TILE ? h.shape : 0].tm : SMALL_GEOMETRY[h.kind == Q8Kernel::SMALL ? h.shape : 0].tm;
+    constexpr uint32_t tn = h.kind == Q8Kernel::BIG256 ? 256 : h.kind == Q8Kernel::TILE ? TILE_GEOMETRY[h.kind == Q8Kernel::TILE ? h.shape : 0].tn : SMALL_GEOMETRY[h.kind == Q8Kernel::SMALL ? h.shape : 0].tn;
+    const uint32_t rows = (static_cast<uint32_t>(p.m) + tm - 1) / tm, cols = (static_cast<uint32_t>(p.n) + tn - 1) / tn;
+    if (!launch_fits(static_cast<int64_t>(rows) * cols + 7, 64 * h.waves)) return;
+    const float k = static_cast<float>((p.k + 127) / 128 * 64);
+    const float full = static_cast<float>(rows) * static_cast<float>(cols) * (1.0f / 256.0f);
+    float r = 1.0f;
+    if (full > 1.0f) {
+        float whole = full < 1e9f ? static_cast<float>(static_cast<int>(full)) : full;
+        if (whole < full) whole += 1.0f;
+        r = h.kind == Q8Kernel::SMALL ? 0.5f * (whole + full) : whole;
+    }
+    const float slower = aligned ? 1.0f : h.kind == Q8Kernel::SMALL ? 1.5f : 1.0f;
+    const float cost = h.start + k * (h.per_k + h.per_k_full * std::min(full, 1.0f)) * slower * r + h.per_round * (r - 1.0f);
+    if (!c.best || cost < c.cost) c = {&h, cost};
+}
+template <size_t... I> const Q8Kernel *choose(const AxhipGemmQ8Params &p, bool aligned, std::index_sequence<I...>) {
+    Q8Choice c{nullptr, 0.0f};
+    (consider<I>(p, aligned, c), ...);
+    return c.best;
+}
+
+int launch_chosen(const Q8Args &g, const AxhipGemmQ8Params &p, bool aligned, hipStream_t s) {
+    if (p.m <= 8) {
+        q8_last_kernel = "skinny";
+        return launch_q8_skinny(g, p.dtype, 1, s);
+    }
+    const Q8Kernel *k = choose(p, aligned, std::make_index_sequence<Q8_CANDIDATES>{});
+    AXHIP_REQUIRE(k != nullptr, AXHIP_ERR_UNSUPPORTED, "axhip_gemm_q8: too many tiles");
+    q8_last_kernel = k->name;
+    if (k->kind == Q8Kernel::BIG256) return launch_q8_big(g, p.dtype, s);
+    if (k->kind == Q8Kernel::SMALL) return launch_q8_small(g, p.dtype, k->shape, k->waves, s);
+    return p.dtype == AXHIP_DTYPE_F32 ? launch_q8_tile_f32(g, k->shape, aligned, s) : p.dtype == AXHIP_DTYPE_F16 ? launch_q8_tile_f16(g, k->shape, aligned, s) : launch_q8_tile_bf16(g, k->shape, aligned, s);
 }
 } // namespace
 } // namespace axhip
@@ -63,11 +143,19 @@ extern "C" int axhip_gemm_q8(const int8_t *a, const int8_t *b, void *c, const Ax
     int rc = ensure_init();
     if (rc) return rc;
     hipStream_t s = resolve_stream(stream);
-    const Q8Args g{a, b, c, p.scale_a, p.scale_b, p.bias, p.residual, p.m, p.n, p.k, p.lda, p.ldb, p.ldc, p.dtype, p.epilogue_op};
-    const int64_t tiles_n = (p.n + 15) / 16, tiles = (p.m + 15) / 16 * tiles_n;
-    AXHIP_REQUIRE(launch_fits(tiles, 256), AXHIP_ERR_UNSUPPORTED, "axhip_gemm_q8: too many tiles");
-    hipLaunchKernelGGL(gemm_q8_generic_kernel, dim3(static_cast<unsigned>(tiles)), dim3(256), 0, s, g, tiles_n);
-    q8_last_kernel = "generic";
+    if (takes_q8_kernels(p)) {
+        const Q8Args g{a, b, c, p.bias, p.residual, p.scale_a, p.scale_b, static_cast<int>(p.m), static_cast<int>(p.n), static_cast<int>(p.k),
+                       static_cast<int>(p.lda), static_cast<int>(p.ldb), static_cast<int>(p.ldc), p.epilogue_op};
+        const bool aligned = ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15u) == 0 && (p.k | p.lda | p.ldb) % 16 == 0;
+        rc = launch_chosen(g, p, aligned, s);
+        if (rc) return rc;
+    } else {
+        const GenericArgs g{a, b, c, p.scale_a, p.scale_b, p.bias, p.residual, p.m, p.n, p.k, p.lda, p.ldb, p.ldc, p.dtype, p.epilogue_op};
+        const int64_t tiles_n = (p.n + 15) / 16, tiles = (p.m + 15) / 16 * tiles_n;
+        AXHIP_REQUIRE(launch_fits(tiles, 256), AXHIP_ERR_UNSUPPORTED, "axhip_gemm_q8: too many tiles");
+        hipLaunchKernelGGL(gemm_q8_generic_kernel, dim3(static_cast<unsigned>(tiles)), dim3(256), 0, s, g, tiles_n);
+        q8_last_kernel = "generic";
+    }
     AXHIP_CHECK_HIP(hipGetLastError());
     return AXHIP_OK;
 }
