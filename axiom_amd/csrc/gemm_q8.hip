@@ -51,7 +51,7 @@ bool takes_q8_kernels(const AxhipGemmQ8Params &p) {
 // The candidates with the time each takes, in us: start + k (per_k + per_k_full u) r + per_round (r - 1), r being the rounds its work-groups take on
 // the 256 CUs and u how full the first is.
 struct Q8Kernel {
-    enum Kind { BIG256, TILE, SMALL } kind;
+    enum Kind { BIG256, TILE, PAIR, SMALL } kind;
     int shape, waves;
     float start, per_k, per_k_full, per_round;
     bool ragged;
@@ -64,6 +64,7 @@ constexpr Q8Kernel Q8_KERNELS[] = {
     {Q8Kernel::TILE, TILE_128x128, 8, 4.9f, 0.0048f, 0.0014f, 4.1f, false, "tile_128x128"},
     {Q8Kernel::TILE, TILE_64x128, 8, 4.9f, 0.0032f, 0.0009f, 3.7f, false, "tile_64x128"},
     {Q8Kernel::TILE, TILE_128x128, 8, 6.5f, 0.0080f, 0.0f, 5.9f, true, "tile_128x128_ragged"},
+    {Q8Kernel::PAIR, Q8_128x128_PAIR, 4, 4.9f, 0.0048f, 0.0014f, 4.1f, false, "tile_128x128_pair"},
     {Q8Kernel::SMALL, SMALL_64x64, 8, 4.35f, 0.00245f, 0.00148f, 3.6f, false, "small_64x64_8"},
     {Q8Kernel::SMALL, SMALL_64x64, 4, 4.15f, 0.00324f, 0.00047f, 1.65f, false, "small_64x64_4"},
     {Q8Kernel::SMALL, SMALL_32x64, 8, 3.50f, 0.00170f, 0.00085f, 2.3f, false, "small_32x64_8"},
@@ -83,8 +84,8 @@ template <size_t I> void consider(const AxhipGemmQ8Params &p, bool aligned, Q8Ch
     constexpr const Q8Kernel &h = Q8_KERNELS[I];
     if (h.kind != Q8Kernel::SMALL && h.ragged == aligned) return;
     if (h.kind == Q8Kernel::BIG256 && (p.k % 128 != 0 || p.m < 256 || p.n < 256)) return;
-    constexpr uint32_t tm = h.kind == Q8Kernel::BIG256 ? 256 : h.kind == Q8Kernel::TILE ? TILE_GEOMETRY[h.kind == Q8Kernel::TILE ? h.shape : 0].tm : SMALL_GEOMETRY[h.kind == Q8Kernel::SMALL ? h.shape : 0].tm;
-    constexpr uint32_t tn = h.kind == Q8Kernel::BIG256 ? 256 : h.kind == Q8Kernel::TILE ? TILE_GEOMETRY[h.kind == Q8Kernel::TILE ? h.shape : 0].tn : SMALL_GEOMETRY[h.kind == Q8Kernel::SMALL ? h.shape : 0].tn;
+    constexpr uint32_t tm = h.kind == Q8Kernel::BIG256 ? 256 : h.kind == Q8Kernel::PAIR ? 128 : h.kind == Q8Kernel::TILE ? TILE_GEOMETRY[h.kind == Q8Kernel::TILE ? h.shape : 0].tm : SMALL_GEOMETRY[h.kind == Q8Kernel::SMALL ? h.shape : 0].tm;
+    constexpr uint32_t tn = h.kind == Q8Kernel::BIG256 ? 256 : h.kind == Q8Kernel::PAIR ? 128 : h.kind == Q8Kernel::TILE ? TILE_GEOMETRY[h.kind == Q8Kernel::TILE ? h.shape : 0].tn : SMALL_GEOMETRY[h.kind == Q8Kernel::SMALL ? h.shape : 0].tn;
     const uint32_t rows = (static_cast<uint32_t>(p.m) + tm - 1) / tm, cols = (static_cast<uint32_t>(p.n) + tn - 1) / tn;
     if (!launch_fits(static_cast<int64_t>(rows) * cols + 7, 64 * h.waves)) return;
     const float k = static_cast<float>((p.k + 127) / 128 * 64);

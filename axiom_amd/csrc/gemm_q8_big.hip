@@ -46,6 +46,8 @@ __global__ __launch_bounds__(512, 1) void gemm_q8_big_kernel(const Q8Args g) {
     };
 
     const int wm = (wave / 4) * 128, wn = (wave % 4) * 64;
+    Q8Scales<DT, 8> scales;
+    scales.load(g, m0 + wm, n0 + wn, lane);
     int f_off[2];
 #pragma unroll
     for (int s = 0; s < 2; ++s) f_off[s] = l16 * ROWB + (((4 * s + g4) ^ ((l16 >> 1) & 7)) * 16);
@@ -137,19 +139,11 @@ __global__ __launch_bounds__(512, 1) void gemm_q8_big_kernel(const Q8Args g) {
 
     // the tile buffers become the staging area of the epilogue: no load of this work-group is still on its way into them (past the last tile they
     // write zeros), and every wavefront has its last fragments
+    Q8Residual<DT, 4> res;
+    res.load(g, m0 + wm, n0 + wn, lane);
     __builtin_amdgcn_s_waitcnt(0x0F70);
     __syncthreads();
-    unsigned char *stage = big_lds + wave * 16384;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        int4_t half[4][4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) half[i][j] = acc[4 * h + i][j];
-        q8_store_blocks<DT, 4>(g, half, m0 + wm + 64 * h, n0 + wn, lane, stage);
-        wave_lds_fence();
-    }
+    q8_store_pieces<DT, 8, 4>(g, acc, scales, res, m0 + wm, n0 + wn, lane, big_lds + wave * 16384);
 }
 
 template <int DT> int launch(const Q8Args &g, hipStream_t s) {

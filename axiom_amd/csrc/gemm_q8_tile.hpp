@@ -20,7 +20,7 @@ namespace axhip {
 namespace {
 
 template <int DT, bool DMA, int MI, int WM, int WN, int WK, int TKB, int S>
-__global__ __launch_bounds__(64 * WM * WN * WK, 1) void gemm_q8_tile_kernel(const Q8Args g) {
+__global__ __launch_bounds__(64 * WM * WN * WK, 2) void gemm_q8_tile_kernel(const Q8Args g) {
     constexpr int NW = WM * WN * WK, TM = 16 * MI * WM, TN = 64 * WN;
     constexpr int KS = TKB / 64 / WK;         // k-steps of 64 per k-tile and wavefront
     constexpr int CH = TKB / 16;              // 16-byte chunks per LDS row
@@ -45,6 +45,10 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 1) void gemm_q8_tile_kernel(cons
     const int m0 = (first_m + rem % gsz) * TM, n0 = (rem / gsz) * TN;
     const int8_t *A = g.a + static_cast<int64_t>(m0) * g.lda, *B = g.b + static_cast<int64_t>(n0) * g.ldb;
     const int rows_a = min(TM, g.M - m0), rows_b = min(TN, g.N - n0);
+
+    constexpr int MB = MI / WK, MP = MB > 4 ? 4 : MB; // row blocks that a wavefront finishes, and stages at a time
+    Q8Scales<DT, MB> scales;
+    scales.load(g, m0 + wm + wk * MB * 16, n0 + wn, lane);
 
     // ---- tile loads: load n of a wavefront moves chunks 64 (n NW + wave) + lane of the tile's LDS image
     const int ld_row = (wave * 64 + lane) / CH, ld_pos = lane % CH;
@@ -238,10 +242,11 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 1) void gemm_q8_tile_kernel(cons
 #undef AXHIP_FENCE
 
     // ---- the WK groups' sums meet in LDS: group w finishes row blocks [w MB, (w + 1) MB) of its wavefront tile
+    Q8Residual<DT, MP> res;
+    res.load(g, m0 + wm + wk * MB * 16, n0 + wn, lane);
     AXHIP_VMCNT(0); // no load of this wavefront is still on its way into the ring
 #undef AXHIP_VMCNT
     __syncthreads();
-    constexpr int MB = MI / WK;
     int4_t own[MB][4];
     auto part = [&](int owner, int source, int i) -> unsigned char * { // 4 KiB: block i of `owner`, from `source` (!= owner)
         const int src = source - (source > owner ? 1 : 0);
@@ -278,14 +283,14 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 1) void gemm_q8_tile_kernel(cons
             }
     }
     // (the blocks that a wavefront has just read are its staging area)
-    unsigned char *stage = tile_lds + (WK > 1 ? (wt * WK + wk) * (WK - 1) * MB * 4096 : wave * MB * 4096);
-    q8_store_blocks<DT, MB>(g, own, m0 + wm + wk * MB * 16, n0 + wn, lane, stage);
+    unsigned char *stage = tile_lds + (WK > 1 ? (wt * WK + wk) * (WK - 1) * MB * 4096 : wave * MP * 4096);
+    q8_store_pieces<DT, MB, MP>(g, own, scales, res, m0 + wm + wk * MB * 16, n0 + wn, lane, stage);
 }
 
 // bytes of LDS: the ring, or what the groups exchange at the end where that is more
 template <int MI, int WM, int WN, int WK, int TKB, int S> constexpr size_t q8_tile_lds_bytes() {
     const size_t ring = size_t(S) * (16 * MI * WM + 64 * WN) * TKB;
-    const size_t parts = WK > 1 ? size_t(WM * WN) * WK * (WK - 1) * (MI / WK) * 4096 : size_t(WM * WN) * MI * 4096;
+    const size_t parts = WK > 1 ? size_t(WM * WN) * WK * (WK - 1) * (MI / WK) * 4096 : size_t(WM * WN) * (MI > 4 ? 4 : MI) * 4096;
     return ring > parts ? ring : parts;
 }
 
@@ -307,6 +312,7 @@ template <int DT> int launch_q8_tile_as(const Q8Args &g, int shape, bool aligned
     switch (shape) {
     case TILE_256x128: return launch_q8_tile_kernel<DT, true, 8, 2, 2, 2, 128, 3>(g, s);
     case TILE_192x128: return launch_q8_tile_kernel<DT, true, 6, 2, 2, 2, 128, 3>(g, s);
+    case Q8_128x128_PAIR: return launch_q8_tile_kernel<DT, true, 4, 2, 2, 1, 128, 2>(g, s);
     case TILE_128x128: return launch_q8_tile_kernel<DT, true, 4, 2, 2, 2, 128, 4>(g, s);
     default: return launch_q8_tile_kernel<DT, true, 4, 1, 2, 4, 256, 3>(g, s);
     }
