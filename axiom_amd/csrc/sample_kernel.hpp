@@ -1,0 +1,823 @@
+// Sampling: the kernel.
+#pragma once
+#include "sample.hpp"
+
+namespace axhip {
+namespace {
+
+// A work-group of 1024 threads to a row, which it holds in registers where it fits (IT steps of eight elements a lane).  No sorting: a filter keeps a prefix of the order "larger
+// logit first, equal ones by index", and where it ends is found by what lies in front (numbers of logits, or sums of weights).  The draw is the same search in
+// the order of the indexes.  Weights are integers, multiples of 2^-43 of the largest, of which 2^20 fit 64 bits: sums do not depend on the order in which
+// atomics arrive.  Three ways, by what is asked of the row:
+//   * top_k up to SMALL_K (and short rows): of the threads' 1024 largest logits the k-th largest is a bound that at least k logits reach, and hardly more do; they go to a list
+//     in LDS, and each entry of the list adds up what lies in front of it.
+//   * other 16-bit rows: all 65535 values are counted in LDS (128 KiB), and every filter is answered by the counts: one weight for each value that occurs
+//     instead of one for each logit.  The draw takes weights from a table of the values that are kept.  Counts are 16 bits wide; if one overflows, the sum of all shows
+//     it and the row goes the third way.
+//   * other fp32 rows: a histogram of 2048 bins that are linear in the logit, from the largest to 31 temperatures below it, from where on weights round to zero (bins by the
+//     bits of the float hold most logits in a few dozen bins, on which a wavefront's atomics wait for each other).  All logits in the bin in which a filter ends, or in
+//     front of it, go to a list in LDS if they fit, and everything after happens there.
+constexpr int THREADS = 1024, WAVES = THREADS / WAVE, E = 8; // elements of a lane's vector
+constexpr int STEP = WAVE * E;                               // consecutive elements of a wavefront's step
+constexpr int BINS = 2048, FEW = 128;
+constexpr int DIRECT = 128, FEW_LOGITS = 1024, SMALL_K = 512;
+constexpr int LIST = 16384, FRONT = 12288; // of which this many for what lies in front of the bin
+constexpr int BLOCK = 64, BLOCKS = 65536 / BLOCK; // 16-bit values are summed up by blocks
+static_assert(MOST_VOCAB <= int64_t(BINS) * STEP, "a bin for a step");
+constexpr uint64_t ONE = uint64_t(1) << 43, MARK = uint64_t(1) << 53;
+constexpr double REACH = 31.0; // temperatures: exp(-31) is below half of 2^-43
+
+struct SampleShared {
+    uint64_t bins[BINS];
+    uint64_t block_mass[BLOCKS];
+    uint64_t few_place[FEW], few_value[FEW];
+    uint64_t scratch[WAVES + 2], other_scratch[WAVES];
+    float top[WAVES];
+    uint32_t where[WAVES], few, front, inside;
+    union {
+        uint64_t list[LIST];
+        uint32_t counts[32768]; // two values to a word
+        uint64_t weights[LIST];
+    };
+};
+static_assert(sizeof(SampleShared) <= 160 * 1024, "LDS of a CU");
+
+// ---- sums over a wavefront's lanes in 64 bits
+template <int CTRL, int ROWS = 0xF> __device__ __forceinline__ uint64_t dpp64(uint64_t v) {
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(static_cast<uint32_t>(v)), CTRL, ROWS, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(static_cast<uint32_t>(v >> 32)), CTRL, ROWS, 0xF, false);
+    return static_cast<uint64_t>(hi) << 32 | lo;
+}
+__device__ __forceinline__ uint64_t sum16(uint64_t v) { // over rows of 16 lanes
+    v += dpp64<0x128>(v); // row_ror:8, 4, 2, 1
+    v += dpp64<0x124>(v);
+    v += dpp64<0x122>(v);
+    return v + dpp64<0x121>(v);
+}
+__device__ __forceinline__ uint64_t sum32(uint64_t v) { // over halves
+    v = sum16(v);
+    const auto lo = __builtin_amdgcn_permlane16_swap(static_cast<uint32_t>(v), static_cast<uint32_t>(v), false, false);
+    const auto hi = __builtin_amdgcn_permlane16_swap(static_cast<uint32_t>(v >> 32), static_cast<uint32_t>(v >> 32), false, false);
+    return (static_cast<uint64_t>(hi[0]) << 32 | lo[0]) + (static_cast<uint64_t>(hi[1]) << 32 | lo[1]);
+}
+__device__ __forceinline__ uint64_t wave_sum64(uint64_t v) {
+    v = sum32(v);
+    const auto lo = __builtin_amdgcn_permlane32_swap(static_cast<uint32_t>(v), static_cast<uint32_t>(v), false, false);
+    const auto hi = __builtin_amdgcn_permlane32_swap(static_cast<uint32_t>(v >> 32), static_cast<uint32_t>(v >> 32), false, false);
+    return (static_cast<uint64_t>(hi[0]) << 32 | lo[0]) + (static_cast<uint64_t>(hi[1]) << 32 | lo[1]);
+}
+__device__ __forceinline__ uint64_t wave_upto64(uint64_t v) { // of the lanes up to this one
+    v += dpp64<0x111>(v); // row_shr:1, 2, 4, 8
+    v += dpp64<0x112>(v);
+    v += dpp64<0x114>(v);
+    v += dpp64<0x118>(v);
+    v += dpp64<0x142, 0xA>(v); // the row in front, to rows 1 and 3
+    return v + dpp64<0x143, 0xC>(v); // the first half, to the second
+}
+__device__ __forceinline__ uint64_t lane_of(uint64_t v, int lane) {
+    return static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(v >> 32)), lane))) << 32 |
+           static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(v)), lane));
+}
+// A counter's old value; lane by lane (the compiler makes a sum over the wavefront of additions to one address, which is the longer way for the few lanes that come here)
+__device__ __forceinline__ uint32_t take_from(uint32_t &counter, uint32_t n) {
+    uint32_t offset = 0;
+    asm volatile("" : "+v"(offset));
+    return atomicAdd(&counter + offset, n);
+}
+__device__ __forceinline__ void add_to_bin(uint64_t &bin, uint64_t v) { atomicAdd(reinterpret_cast<unsigned long long *>(&bin), static_cast<unsigned long long>(v)); }
+
+// ---- the order: smaller numbers first.  Larger logits (-0 is +0), and of equal ones smaller indexes.
+__device__ __forceinline__ uint64_t order_of(float v, uint32_t i) {
+    const uint32_t b = __float_as_uint(v + 0.0f);
+    return static_cast<uint64_t>(b & 0x80000000u ? b : ~b & 0x7FFFFFFFu) << 20 | i;
+}
+__device__ __forceinline__ float logit_of(uint64_t order) {
+    const uint32_t b = static_cast<uint32_t>(order >> 20);
+    return __uint_as_float(b & 0x80000000u ? b : ~b & 0x7FFFFFFFu);
+}
+__device__ __forceinline__ uint32_t index_of(uint64_t order) { return static_cast<uint32_t>(order) & 0xFFFFFu; }
+
+// The same of two 16-bit logits at a time: 0x7FFF - h of a positive one, h - 1 of a negative one (so that -0 has the number of +0).
+__device__ __forceinline__ uint32_t orders_of_pair(uint32_t w) {
+    const uint32_t sign = (w >> 15) & 0x00010001u;
+    return (w ^ 0x7FFF7FFFu ^ ((sign << 15) - sign)) - sign;
+}
+template <int DT> constexpr uint32_t INFINITY16 = DT == AXHIP_DTYPE_BF16 ? 0x7F80u : 0x7C00u;
+template <int DT> constexpr uint32_t FIRST_ORDER = 0x7FFFu ^ INFINITY16<DT>;                                    // of infinity,
+template <int DT> constexpr uint32_t DRAWN_ORDERS = (0x8000u | INFINITY16<DT>) - 1 - FIRST_ORDER<DT>;          // and how many there are before -infinity and the NaNs
+template <int DT> __device__ __forceinline__ float logit_of16(uint32_t order) {
+    const uint32_t h = order <= 0x7FFFu ? order ^ 0x7FFFu : order + 1;
+    return DT == AXHIP_DTYPE_BF16 ? bf16_bits_to_f32(h) : f16_bits_to_f32(h);
+}
+
+template <int DT> struct Step { uint4_t v[DT == AXHIP_DTYPE_F32 ? 2 : 1]; };
+template <int DT> __device__ __forceinline__ float element(const Step<DT> &s, int e) {
+    if constexpr (DT == AXHIP_DTYPE_F32) return __uint_as_float(s.v[e / 4][e % 4]);
+    else if constexpr (DT == AXHIP_DTYPE_BF16) return e % 2 ? __uint_as_float(s.v[0][e / 2] & 0xFFFF0000u) : __uint_as_float(s.v[0][e / 2] << 16);
+    else return f16_bits_to_f32((s.v[0][e / 2] >> (16 * (e % 2))) & 0xFFFFu);
+}
+
+template <int DT> struct Row {
+    const char *logits;
+    int vocab;
+    float top = 0.0f;      // the largest logit
+    double base = 0.0;     // ... or the largest finite number
+    double rate = 0.0;     // log2(e) / temperature
+    float floor = 0.0f;    // from here on weights may be more than nothing
+    uint64_t last = ~0ull; // kept: up to this one in the order,
+    double least = 0.0;    // and with at least this weight
+
+    __device__ __forceinline__ Step<DT> load(int step) const {
+        constexpr int ES = DT == AXHIP_DTYPE_F32 ? 4 : 2;
+        const int at = step * STEP + static_cast<int>(threadIdx.x % WAVE) * E;
+        Step<DT> s;
+        if (at + E <= vocab) {
+#pragma unroll
+            for (int i = 0; i < ES / 2; ++i) s.v[i] = reinterpret_cast<const uint4_unaligned_t *>(logits + static_cast<int64_t>(at) * ES + 16 * i)->v;
+        } else { // (past the end: NaN, which is never drawn)
+#pragma unroll
+            for (int i = 0; i < ES / 2; ++i) s.v[i] = uint4_t{~0u, ~0u, ~0u, ~0u};
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (at + e < vocab) {
+                    if constexpr (ES == 4) s.v[e / 4][e % 4] = reinterpret_cast<const uint32_t *>(logits)[at + e];
+                    else s.v[0][e / 2] = e % 2 ? (s.v[0][e / 2] & 0xFFFFu) | static_cast<uint32_t>(reinterpret_cast<const uint16_t *>(logits)[at + e]) << 16
+                                              : (s.v[0][e / 2] & 0xFFFF0000u) | reinterpret_cast<const uint16_t *>(logits)[at + e];
+                }
+        }
+        return s;
+    }
+    __device__ __forceinline__ int steps() const { return (vocab + STEP - 1) / STEP; }
+
+    // log2 of the weight, within [-64, 0].  (An infinite largest logit: `base` is the largest finite number, and only infinities are asked for.)
+    __device__ __forceinline__ double power(float v) const { return fmin(fmax((static_cast<double>(v) - base) * rate, -64.0), 0.0); }
+    // exp((v - top) / temperature) in multiples of 2^-43: 2^z with z = i + r, |r| <= 1/2, by a polynomial through the Chebyshev points of 2^r, off by less than 5e-15 of the weight
+    // (a table of 2^(i / 256) and four terms waited longer for LDS than the six terms more take).
+    __device__ __forceinline__ double scaled_weight(double z) const {
+        constexpr double SPLIT = 6755399441055744.0; // 1.5 * 2^52: its last bit is 1
+        const double t = z + SPLIT, r = z - (t - SPLIT);
+        const uint32_t i = static_cast<uint32_t>(__double_as_longlong(t));
+        double p = 6.422412339320131e-09;
+        p = __builtin_fma(r, p, 1.02053706737851e-07);
+        p = __builtin_fma(r, p, 1.3219110032865315e-06);
+        p = __builtin_fma(r, p, 1.5252674086943783e-05);
+        p = __builtin_fma(r, p, 0.00015403523472909156);
+        p = __builtin_fma(r, p, 0.0013333558203519715);
+        p = __builtin_fma(r, p, 0.00961812911264106);
+        p = __builtin_fma(r, p, 0.05550410866458426);
+        p = __builtin_fma(r, p, 0.2402265069589931);
+        p = __builtin_fma(r, p, 0.6931471805599488);
+        p = __builtin_fma(r, p, 1.0);
+        return __longlong_as_double(__double_as_longlong(p) + (static_cast<long long>(static_cast<uint64_t>(i + 43u) << 52)));
+    }
+    static __device__ __forceinline__ uint64_t integer(double w) {
+        constexpr double TO_INTEGER = 4503599627370496.0; // 2^52: the integer is what its last bits say
+        return static_cast<uint64_t>(__double_as_longlong(w + TO_INTEGER)) & ((uint64_t(1) << 52) - 1);
+    }
+    __device__ __forceinline__ uint64_t mass(float v) const { return integer(scaled_weight(power(v))); }
+    __device__ __forceinline__ uint64_t mass_of_least(float v) const { // ... 0 below min_p
+        const double w = scaled_weight(power(v));
+        return w >= least ? integer(w) : 0;
+    }
+    // bins of the power, BINS to REACH temperatures; the last one holds everything from there on
+    __device__ __forceinline__ uint32_t bin_of_power(double z) const {
+        constexpr double PER_POWER = (BINS - 1) / (REACH * 1.4426950408889634), TO_INTEGER = 4503599627370496.0;
+        return min(static_cast<uint32_t>(__double_as_longlong(__builtin_fma(z, -PER_POWER, TO_INTEGER))), static_cast<uint32_t>(BINS - 1));
+    }
+    __device__ __forceinline__ uint32_t bin_of(float v) const { return bin_of_power(power(v)); }
+    // Below every logit of bins up to `bin` (-inf where rounding leaves nothing to say).
+    __device__ __forceinline__ float below(int bin) const {
+        const double edge = base - (bin + 2) * (REACH * 1.4426950408889634 / (BINS - 1)) / rate;
+        const float low = static_cast<float>(edge) - fabsf(static_cast<float>(edge)) * 1e-6f;
+        return low > -3e38f ? low : -3.402823466e38f;
+    }
+    __device__ __forceinline__ bool counts(float v, uint32_t i) const { return v >= floor && (last == ~0ull || order_of(v, i) <= last); }
+};
+
+// ---- All of these are called by the whole work-group, and their answers are every thread's.
+__device__ __forceinline__ void clear_bins(SampleShared &sh) {
+    sh.bins[threadIdx.x] = 0;
+    sh.bins[threadIdx.x + THREADS] = 0;
+    __syncthreads();
+}
+__device__ __forceinline__ uint64_t sum_of_all(SampleShared &sh, uint64_t v) {
+    v = wave_sum64(v);
+    if (threadIdx.x % WAVE == 0) sh.other_scratch[threadIdx.x / WAVE] = v;
+    __syncthreads();
+    v = sum16(sh.other_scratch[threadIdx.x % WAVES]);
+    __syncthreads();
+    return v;
+}
+// (behind a barrier behind the additions to the bins)
+__device__ __forceinline__ uint64_t sum_of_bins(SampleShared &sh) { return sum_of_all(sh, sh.bins[threadIdx.x] + sh.bins[threadIdx.x + THREADS]); }
+// The first bin at which the running sum, `before` in front, exceeds `than`, and the sum in front of it; -1 if none does.
+__device__ __forceinline__ int find_bin(SampleShared &sh, uint64_t before, uint64_t than, uint64_t &in_front) {
+    const int t = threadIdx.x, lane = t % WAVE, wave = t / WAVE;
+    const uint64_t v0 = sh.bins[2 * t], v1 = sh.bins[2 * t + 1], upto = wave_upto64(v0 + v1);
+    if (lane == WAVE - 1) sh.scratch[wave] = upto;
+    if (t == 0) sh.scratch[WAVES] = ~0ull;
+    __syncthreads();
+    const uint64_t others = sum16(lane % WAVES < wave ? sh.scratch[lane % WAVES] : 0);
+    const uint64_t all = before + others + upto, mine = all - v0 - v1;
+    if (all > than && mine <= than) {
+        sh.scratch[WAVES] = mine + v0 > than ? 2 * t : 2 * t + 1;
+        sh.scratch[WAVES + 1] = mine + v0 > than ? mine : mine + v0;
+    }
+    __syncthreads();
+    const int bin = static_cast<int>(sh.scratch[WAVES]);
+    in_front = sh.scratch[WAVES + 1];
+    __syncthreads();
+    return bin;
+}
+__device__ __forceinline__ void smallest_and_largest(SampleShared &sh, uint64_t &lo, uint64_t &hi) {
+#pragma unroll
+    for (int d = 32; d; d /= 2) {
+        const uint64_t l = __shfl_xor(lo, d, WAVE), h = __shfl_xor(hi, d, WAVE);
+        lo = l < lo ? l : lo;
+        hi = h > hi ? h : hi;
+    }
+    if (threadIdx.x % WAVE == 0) {
+        sh.scratch[threadIdx.x / WAVE] = lo;
+        sh.other_scratch[threadIdx.x / WAVE] = hi;
+    }
+    __syncthreads();
+    for (int w = 0; w < WAVES; ++w) {
+        lo = sh.scratch[w] < lo ? sh.scratch[w] : lo;
+        hi = sh.other_scratch[w] > hi ? sh.other_scratch[w] : hi;
+    }
+    __syncthreads();
+}
+
+// Of the elements that `all(f)` hands to f(place, value()), those with places in [lo, hi]: the place at which the running sum of values, by place and with `before` in
+// front, exceeds than(sum of them all) -- hi if it never does.  Places are unique, values may be 0.  `count`: how many they are at most.
+template <class Than, class All> __device__ __forceinline__ uint64_t find_place(SampleShared &sh, uint64_t lo, uint64_t hi, uint64_t before, int count, Than than_of, All all) {
+    uint64_t than = 0;
+    for (bool first = true; lo < hi; first = false) {
+        // (each round leaves a bin, at most 1 / 2047 of the places, or fewer than FEW elements)
+        const double rate = (BINS - 0.5) / (static_cast<double>(hi - lo) + 1.0);
+        auto bin_of = [&](uint64_t place) { return static_cast<int>(static_cast<double>(place - lo) * rate); };
+        const bool all_few = first && count <= FEW;
+        int bin = 0;
+        if (threadIdx.x == 0) sh.few = 0;
+        if (!all_few) {
+            clear_bins(sh);
+            all([&](uint64_t place, auto value) __attribute__((always_inline)) {
+                if (place >= lo && place <= hi) {
+                    const uint64_t v = value();
+                    if (v) add_to_bin(sh.bins[bin_of(place)], v);
+                }
+            });
+            __syncthreads();
+            if (first) than = than_of([&] { return sum_of_bins(sh); });
+            bin = find_bin(sh, before, than, before);
+            if (bin < 0) return hi;
+        } else {
+            __syncthreads();
+        }
+        uint64_t l = ~0ull, h = 0;
+        all([&](uint64_t place, auto value) __attribute__((always_inline)) {
+            if (place >= lo && place <= hi && (all_few || bin_of(place) == bin)) {
+                const uint64_t v = value();
+                if (v) {
+                    const uint32_t at = take_from(sh.few, 1);
+                    if (at < FEW) {
+                        sh.few_place[at] = place;
+                        sh.few_value[at] = v;
+                    }
+                    l = place < l ? place : l;
+                    h = place > h ? place : h;
+                }
+            }
+        });
+        __syncthreads();
+        const int n = static_cast<int>(sh.few);
+        if (n <= FEW) {
+            if (all_few) than = than_of([&] { return sum_of_all(sh, static_cast<int>(threadIdx.x) < n ? sh.few_value[threadIdx.x] : 0); });
+            if (threadIdx.x == 0) sh.scratch[WAVES] = hi;
+            __syncthreads();
+            if (static_cast<int>(threadIdx.x) < n) {
+                const uint64_t mine = sh.few_place[threadIdx.x];
+                uint64_t front = before;
+                for (int i = 0; i < n; ++i) front += sh.few_place[i] < mine ? sh.few_value[i] : 0;
+                if (front <= than && front + sh.few_value[threadIdx.x] > than) sh.scratch[WAVES] = mine;
+            }
+            __syncthreads();
+            lo = sh.scratch[WAVES];
+            __syncthreads();
+            return lo;
+        }
+        smallest_and_largest(sh, l, h);
+        lo = l;
+        hi = h;
+    }
+    return lo;
+}
+
+template <int DT, int IT> __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleArgs a) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char sample_lds[];
+    SampleShared &sh = *reinterpret_cast<SampleShared *>(sample_lds);
+    const int t = threadIdx.x, lane = t % WAVE, wave = t / WAVE;
+    const int64_t row = blockIdx.x;
+    constexpr int64_t ES = DT == AXHIP_DTYPE_F32 ? 4 : 2;
+    Row<DT> r{static_cast<const char *>(a.logits) + row * a.ld * ES, a.vocab};
+    const int steps = r.steps();
+    Step<DT> held[IT > 0 ? IT : 1];
+#pragma unroll
+    for (int i = 0; i < IT; ++i)
+        if (i * WAVES + wave < steps) held[i] = r.load(i * WAVES + wave);
+    // f(vectors, index of the first, step) for the wavefront's steps, from memory with the next ones' loads in flight
+    auto each_step_of_memory = [&](auto f) __attribute__((always_inline)) {
+        constexpr int AHEAD = 3;
+        Step<DT> next[AHEAD];
+#pragma unroll
+        for (int d = 0; d < AHEAD; ++d) next[d] = r.load(min(wave + d * WAVES, steps - 1));
+#pragma unroll 1
+        for (int step = wave; step < steps; step += WAVES) {
+            const Step<DT> s = next[0];
+#pragma unroll
+            for (int d = 0; d + 1 < AHEAD; ++d) next[d] = next[d + 1];
+            next[AHEAD - 1] = r.load(min(step + AHEAD * WAVES, steps - 1));
+            f(s, static_cast<uint32_t>(step * STEP + lane * E), step);
+        }
+    };
+    // ... from the registers, for passes of few instructions.  (The compiler is not to see that a later pass forms the same numbers of the same vectors: it would keep them all.)
+    auto each_step = [&](auto f) __attribute__((always_inline)) {
+        if constexpr (IT > 0) {
+            int first = lane * E;
+#pragma unroll
+            for (int i = 0; i < IT; ++i) {
+                const int step = i * WAVES + wave;
+                Step<DT> s = held[i];
+#pragma unroll
+                for (int v = 0; v < ES / 2; ++v)
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) asm volatile("" : "+v"(s.v[v][w]));
+                asm volatile("" : "+v"(first));
+                if (step < steps) f(s, static_cast<uint32_t>(step * STEP + first), step);
+            }
+        } else {
+            each_step_of_memory(f);
+        }
+    };
+    auto each_of = [&](auto steps_of, auto f) __attribute__((always_inline)) { // f(logit, index)
+        steps_of([&](const Step<DT> &s, uint32_t at, int) __attribute__((always_inline)) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) f(element<DT>(s, e), at + e);
+        });
+    };
+
+    float temperature = a.temperature ? a.temperature[row] : 1.0f;
+    temperature = temperature > 1e30f ? 1e30f : temperature;
+    const float p = a.top_p ? a.top_p[row] : 1.0f, m = a.min_p ? a.min_p[row] : 0.0f, u = a.u[row];
+    const int32_t k = a.top_k && a.top_k[row] > 0 && a.top_k[row] < a.vocab ? a.top_k[row] : 0;
+    if (t == 0) sh.front = sh.inside = 0;
+    sh.bins[t] = 0;
+    sh.bins[t + THREADS] = 0;
+
+    // kept by top_p: those with less than p of the sum in front of them, so up to the one at which the running sum reaches p of it
+    auto than_of_p = [&](auto total) __attribute__((always_inline)) {
+        const double reach = static_cast<double>(p) * static_cast<double>(total());
+        return reach > 1.0 ? static_cast<uint64_t>(__builtin_ceil(reach)) - 1 : uint64_t(0);
+    };
+    auto than_of_u = [&](uint64_t total) __attribute__((always_inline)) {
+        const double reach = u > 0.0f ? static_cast<double>(u) * static_cast<double>(total) : 0.0;
+        return reach < static_cast<double>(total - 1) ? static_cast<uint64_t>(reach) : total - 1;
+    };
+    auto answer = [&](uint32_t index, uint64_t mass, uint64_t total) {
+        a.tokens[row] = static_cast<int64_t>(index);
+        if (a.probs) a.probs[row] = static_cast<float>(static_cast<double>(mass) / static_cast<double>(total));
+    };
+
+    // ---- the largest logit
+    float mine = -__builtin_inff(); // of this thread's
+    each_of(each_step, [&](float v, uint32_t) { mine = fmaxf(mine, v); });
+    float top = wave_max(mine);
+    if (lane == 0) sh.top[wave] = top;
+    __syncthreads();
+    top = sh.top[lane % WAVES];
+    top = wave_max(top);
+    if (top == -__builtin_inff() || !(temperature > 0.0f)) { // (the same in every thread)
+        uint32_t first = ~0u;
+        if (top != -__builtin_inff()) each_of(each_step_of_memory, [&](float v, uint32_t i) { first = v == top ? min(first, i) : first; });
+#pragma unroll
+        for (int d = 32; d; d /= 2) first = min(first, static_cast<uint32_t>(__shfl_xor(first, d, WAVE)));
+        if (lane == 0) sh.where[wave] = first;
+        __syncthreads();
+        for (int w = 0; w < WAVES; ++w) first = min(first, sh.where[w]);
+        if (t == 0) {
+            a.tokens[row] = first == ~0u ? -1 : static_cast<int64_t>(first);
+            if (a.probs) a.probs[row] = first == ~0u ? 0.0f : 1.0f;
+        }
+        return;
+    }
+    constexpr float LARGEST = 3.402823466e38f;
+    r.top = top;
+    r.base = static_cast<double>(fminf(top, LARGEST));
+    r.rate = 1.4426950408889634 / static_cast<double>(temperature);
+    r.floor = fmaxf(top - static_cast<float>(REACH) * temperature, -LARGEST); // (NaN, of an infinite logit and temperature: everything finite)
+    if (top > LARGEST) r.floor = top;                                         // (only its equals)
+    const double least = m > 0.0f ? (m < 1.0f ? static_cast<double>(m) : 1.0) * static_cast<double>(ONE) : 0.0;
+    r.least = least;
+
+    // Those that `taken(logit, index)` gives a kind, 1 or 2, to the list: the first kind from its start, the second from FRONT on.
+    auto gather = [&](auto steps_of, int front_room, auto taken) __attribute__((always_inline)) {
+        steps_of([&](const Step<DT> &s, uint32_t at, int) __attribute__((always_inline)) {
+            uint32_t kinds = 0; // two bits an element
+#pragma unroll
+            for (int e = 0; e < E; ++e) kinds |= taken(element<DT>(s, e), at + e) << (2 * e);
+            if (kinds) {
+                const uint32_t ones = __builtin_popcount(kinds & 0x5555u), twos = __builtin_popcount(kinds & 0xAAAAu);
+                uint32_t f = ones ? take_from(sh.front, ones) : 0, i = twos ? FRONT + take_from(sh.inside, twos) : 0;
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const uint32_t kind = (kinds >> (2 * e)) & 3u, to = kind == 1 ? f : i;
+                    f += kind == 1;
+                    i += kind == 2;
+                    if (kind && to < static_cast<uint32_t>(kind == 1 ? front_room : LIST)) sh.list[to] = order_of(element<DT>(s, e), at + e);
+                }
+            }
+        });
+        __syncthreads();
+    };
+
+    // `listed`: the list holds all that is kept: `listed_front` from its start, `listed_inside` from FRONT on.
+    bool listed = false;
+    int listed_front = 0, listed_inside = 0;
+
+    // ================ top_k of a few, short rows: a list of little more than what is kept
+    if ((k && k <= SMALL_K) || a.vocab <= FEW_LOGITS) {
+        float low = r.floor;
+        bool bounded = a.vocab <= FEW_LOGITS;
+        if (!bounded) { // (the bins are clear: a barrier ago)
+            if (a.vocab >= THREADS * E) {
+                if (mine >= r.floor) add_to_bin(sh.bins[r.bin_of(mine)], 1);
+            } else { // (too few threads have any: all logits)
+                each_of(each_step_of_memory, [&](float v, uint32_t) {
+                    if (v >= r.floor) add_to_bin(sh.bins[r.bin_of(v)], 1);
+                });
+            }
+            __syncthreads();
+            uint64_t in_front;
+            const int bin = find_bin(sh, 0, static_cast<uint64_t>(k - 1), in_front);
+            bounded = bin >= 0 && bin < BINS - 1;
+            if (bounded) low = fmaxf(low, r.below(bin));
+        }
+        if (bounded) {
+            gather(each_step, FRONT, [&](float v, uint32_t) { return v >= low ? 1u : 0u; });
+            const int n = static_cast<int>(sh.front);
+            if (n <= DIRECT) {
+                // L threads to an entry, each of which looks at every L-th of the others
+                int shift = 4;
+                while (THREADS >> shift < n) --shift;
+                const int entry = t >> shift, part = t & ((1 << shift) - 1), L = 1 << shift;
+                const bool is = entry < n;
+                const uint64_t o = is ? sh.list[entry] : ~0ull;
+                const float v = logit_of(o);
+                uint64_t *const masses = sh.block_mass;
+                static_assert(BLOCKS >= DIRECT, "room for their weights");
+                auto all_parts = [&](uint64_t x) __attribute__((always_inline)) {
+                    for (int d = 1; d < L; d *= 2) x += __shfl_xor(x, d, WAVE);
+                    return x;
+                };
+                // in front of it in the order: how many (less than k are kept), and what they weigh (all of them are kept if it is)
+                uint64_t x = is ? r.mass(v) : 0;
+                if (is && part == 0) masses[entry] = x;
+                __syncthreads();
+                uint32_t rank = 0;
+                uint64_t front = 0;
+#pragma unroll 4
+                for (int j = part; j < n; j += L) {
+                    const bool before = sh.list[j] < o;
+                    rank += before ? 1 : 0;
+                    front += before ? masses[j] : 0;
+                }
+                bool kept = is && (k == 0 || all_parts(rank) < static_cast<uint64_t>(k));
+                if (p < 1.0f) {
+                    const uint64_t total = sum_of_all(sh, kept && part == 0 ? x : 0);
+                    kept = kept && all_parts(front) <= than_of_p([&] { return total; });
+                }
+                __syncthreads();
+                x = kept ? r.mass_of_least(v) : 0;
+                if (is && part == 0) masses[entry] = x;
+                const uint64_t total = sum_of_all(sh, part == 0 ? x : 0), than = than_of_u(total); // (a barrier behind the weights)
+                const uint32_t index = index_of(o);
+                front = 0;
+#pragma unroll 4
+                for (int j = part; j < n; j += L) front += index_of(sh.list[j]) < index ? masses[j] : 0;
+                front = all_parts(front);
+                if (is && part == 0 && front <= than && front + x > than) answer(index, x, total);
+                return;
+            }
+            // longer ones: searched, as the lists of the third way are
+            __syncthreads();
+            if (t == 0) sh.front = 0;
+            __syncthreads();
+            if (n <= FRONT) {
+                listed = true;
+                listed_front = n;
+                r.last = order_of(low, 0xFFFFFu);
+            }
+        }
+    }
+
+    // The draw by the sums of the wavefronts' steps, and then within one.  masses(vectors, index of the first, sums): of a lane's eight, MARK for a logit of which only the first
+    // `ties` are kept, with the weight `of_tie` each.
+    auto draw_by_steps = [&](auto steps_of, uint64_t of_tie, uint32_t ties, auto masses) __attribute__((always_inline)) {
+        clear_bins(sh);
+        steps_of([&](const Step<DT> &s, uint32_t at, int step) __attribute__((always_inline)) {
+            uint64_t x[E], sum = 0;
+            masses(s, at, x);
+#pragma unroll
+            for (int e = 0; e < E; ++e) sum += x[e];
+            sum = wave_sum64(sum); // (weights of a step are 2^52 at most, marks 512)
+            if (lane == 0) sh.bins[step] = sum;
+        });
+        __syncthreads();
+        uint64_t marks_in_front = 0; // of the step that is looked for
+        if (of_tie) { // marks -> the weights of those that are kept
+            const uint64_t b0 = sh.bins[2 * t], b1 = sh.bins[2 * t + 1], m0 = b0 / MARK, m1 = b1 / MARK, upto = wave_upto64(m0 + m1);
+            if (lane == WAVE - 1) sh.scratch[wave] = upto;
+            __syncthreads();
+            const uint64_t in_front = sum16(lane % WAVES < wave ? sh.scratch[lane % WAVES] : 0) + upto - m0 - m1;
+            auto kept = [&](uint64_t before, uint64_t marks) { return before >= ties ? uint64_t(0) : min(marks, ties - before); };
+            sh.bins[2 * t] = b0 % MARK + kept(in_front, m0) * of_tie;
+            sh.bins[2 * t + 1] = b1 % MARK + kept(in_front + m0, m1) * of_tie;
+            sh.block_mass[t] = in_front; // (in front of step 2 t; the other's are m0 more, whose steps are looked at again)
+            __syncthreads();
+        }
+        const uint64_t total = sum_of_bins(sh), than = than_of_u(total);
+        uint64_t front;
+        const int step = max(find_bin(sh, 0, than, front), 0); // (the largest logit's weight is there, and `than` is below the sum)
+        if (wave == 0) {
+            const uint32_t at = static_cast<uint32_t>(step * STEP + lane * E);
+            uint64_t x[E], own = 0;
+            if (of_tie) {
+                marks_in_front = sh.block_mass[step / 2];
+                if (step % 2) {
+                    masses(r.load(step - 1), at - STEP, x);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) own += x[e] / MARK;
+                    marks_in_front += wave_sum64(own);
+                }
+            }
+            masses(r.load(step), at, x);
+            if (of_tie) {
+                own = 0;
+#pragma unroll
+                for (int e = 0; e < E; ++e) own += x[e] / MARK;
+                uint64_t before = marks_in_front + wave_upto64(own) - own;
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (x[e] == MARK) x[e] = before++ < ties ? of_tie : 0;
+            }
+            own = 0;
+#pragma unroll
+            for (int e = 0; e < E; ++e) own += x[e];
+            const uint64_t upto = front + wave_upto64(own);
+            front = upto - own;
+            if (upto > than && front <= than) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    if (front <= than && front + x[e] > than) answer(at + e, x[e], total);
+                    front += x[e];
+                }
+            }
+        }
+    };
+
+    // ================ 16-bit logits: counts of their values
+    if (DT != AXHIP_DTYPE_F32 && !listed) {
+        const bool filtered = k || p < 1.0f; // (else there is nothing to count)
+        auto count_at = [&](uint32_t order) { return (sh.counts[order >> 1] >> (16 * (order & 1))) & 0xFFFFu; };
+        if (filtered)
+            for (int i = t; i < 8192; i += THREADS) reinterpret_cast<uint4_t *>(sh.counts)[i] = uint4_t{0, 0, 0, 0};
+        clear_bins(sh); // (and a barrier)
+        uint32_t drawn = 0;
+        if (filtered)
+            each_step([&](const Step<DT> &s, uint32_t, int) __attribute__((always_inline)) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t pair = orders_of_pair(s.v[0][i]);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t order = h ? pair >> 16 : pair & 0xFFFFu;
+                        if (order - FIRST_ORDER<DT> < DRAWN_ORDERS<DT>) {
+                            ++drawn;
+                            atomicAdd(&sh.counts[order >> 1], 1u << (16 * (order & 1)));
+                        }
+                    }
+                }
+            });
+        drawn = static_cast<uint32_t>(sum_of_all(sh, drawn)); // (a barrier behind the counts)
+        // f(block, pair of counts, the first one's order) of the blocks of 64 values in which any occurs, by the lanes of half a wavefront; others' sums are 0
+        auto each_block_pair = [&](auto f) __attribute__((always_inline)) {
+            constexpr int TOGETHER = 8;
+#pragma unroll 1
+            for (int j0 = wave; j0 < BLOCKS / 2; j0 += WAVES * TOGETHER) {
+                uint32_t w[TOGETHER];
+#pragma unroll
+                for (int i = 0; i < TOGETHER; ++i) w[i] = sh.counts[64 * (j0 + WAVES * i) + lane];
+#pragma unroll
+                for (int i = 0; i < TOGETHER; ++i) {
+                    const int j = j0 + WAVES * i;
+                    if (__ballot(w[i] != 0)) f(2 * j + lane / 32, w[i], static_cast<uint32_t>(128 * j + 2 * lane));
+                }
+            }
+        };
+        static_assert(BLOCKS / 2 % (WAVES * 8) == 0, "whole rounds");
+        if (filtered)
+            each_block_pair([&](int block, uint32_t w, uint32_t) __attribute__((always_inline)) {
+                const uint64_t sum = sum32((w & 0xFFFFu) + (w >> 16));
+                if (lane % 32 == 0) sh.bins[block] = sum;
+            });
+        __syncthreads();
+        if (sum_of_bins(sh) == drawn) { // (a count that overflowed takes 65535 or 65536 from the sum)
+            static_assert(BLOCK == WAVE && BLOCKS <= BINS, "a value to a lane, and a bin for a block");
+            // the first value of `block` at which the running sum exceeds `than`, and the sum in front of it
+            auto find_value = [&](int block, uint64_t front, uint64_t than, uint64_t own, uint64_t &in_front) __attribute__((always_inline)) {
+                const uint64_t upto = front + wave_upto64(own);
+                const int first = __builtin_ctzll(__ballot(upto > than) | uint64_t(1) << 63);
+                in_front = lane_of(upto - own, first);
+                return static_cast<uint32_t>(block * BLOCK + first);
+            };
+            const uint32_t first = orders_of_pair(DT == AXHIP_DTYPE_BF16 ? f32_to_bf16_bits(top) : f32_to_f16_bits(top)) & 0xFFFFu; // the largest's
+            uint64_t front, in_front;
+            const uint32_t lowest = (orders_of_pair(DT == AXHIP_DTYPE_BF16 ? f32_to_bf16_bits(r.floor) : f32_to_f16_bits(r.floor)) & 0xFFFFu) + 1; // (the floor, rounded)
+            uint32_t last = min(lowest, FIRST_ORDER<DT> + DRAWN_ORDERS<DT> - 1), ties = ~0u; // kept: orders up to `last`, and of that one so many, by index
+            if (k) {
+                const uint64_t than = static_cast<uint64_t>(k - 1);
+                const int block = find_bin(sh, 0, than, front);
+                if (block >= 0) {
+                    last = find_value(block, front, than, count_at(block * BLOCK + lane), in_front);
+                    ties = static_cast<uint32_t>(than - in_front) + 1;
+                }
+            }
+            if (p < 1.0f) {
+                auto kept_mass = [&](uint32_t order, uint32_t count) __attribute__((always_inline)) {
+                    const uint32_t c = order < last ? count : order == last ? min(count, ties) : 0u;
+                    return c ? c * r.mass(logit_of16<DT>(order)) : uint64_t(0);
+                };
+                clear_bins(sh);
+                each_block_pair([&](int block, uint32_t w, uint32_t order) __attribute__((always_inline)) {
+                    const uint64_t sum = sum32(kept_mass(order, w & 0xFFFFu) + kept_mass(order + 1, w >> 16));
+                    if (lane % 32 == 0) sh.bins[block] = sum;
+                });
+                __syncthreads();
+                const uint64_t than = than_of_p([&] { return sum_of_bins(sh); });
+                const int block = find_bin(sh, 0, than, front);
+                if (block >= 0) {
+                    const uint32_t order = block * BLOCK + lane;
+                    last = find_value(block, front, than, kept_mass(order, count_at(order)), in_front);
+                    ties = static_cast<uint32_t>((than - in_front) / r.mass(logit_of16<DT>(last))) + 1;
+                }
+            }
+            // Of the last value only the first `ties` by index are kept: its logits carry no weight but a mark, and their share is added when the steps' numbers of
+            // marks are known.
+            const uint64_t of_last = filtered && ties < count_at(last) ? r.mass_of_least(logit_of16<DT>(last)) : 0;
+            const bool in_part = of_last != 0; // (those that weigh nothing need no marks)
+            const uint32_t values = last - first + 1;
+            __syncthreads(); // (the counts make room for the weights)
+            // (weights of logits between two small ones of either sign are the same integer: one entry of the table for all of them, which lets it reach negative bfloat16 logits)
+            uint32_t zone = values, gap = 0; // entries zone .. zone + gap are one
+            if (DT == AXHIP_DTYPE_BF16 && values >= LIST) {
+                const uint32_t small = orders_of_pair(f32_to_bf16_bits(temperature * 7.105427357601002e-15f)) & 0xFFFFu; // 2^-47 temperatures
+                const uint32_t end = 0xFFFEu - small;                                                                       // ... and as much below zero
+                if (small > first && end < last) {
+                    zone = small - first;
+                    gap = end - small;
+                }
+            }
+            const uint32_t entries = values - gap;
+            if (entries < LIST) {
+                for (uint32_t i = t; i <= entries; i += THREADS)
+                    sh.weights[i] = i == entries ? 0 : in_part && i == entries - 1 ? MARK : r.mass_of_least(logit_of16<DT>(first + (i > zone ? i + gap : i)));
+                if (gap == 0) {
+                    draw_by_steps(each_step, of_last, ties, [&](const Step<DT> &s, uint32_t, uint64_t(&x)[E]) __attribute__((always_inline)) { // (a barrier in front of the loop)
+#pragma unroll
+                        for (int e = 0; e < E; ++e) {
+                            const uint32_t pair = orders_of_pair(s.v[0][e / 2]);
+                            x[e] = sh.weights[min((e % 2 ? pair >> 16 : pair & 0xFFFFu) - first, values)];
+                        }
+                    });
+                } else {
+                    draw_by_steps(each_step, of_last, ties, [&](const Step<DT> &s, uint32_t, uint64_t(&x)[E]) __attribute__((always_inline)) {
+#pragma unroll
+                        for (int e = 0; e < E; ++e) {
+                            const uint32_t pair = orders_of_pair(s.v[0][e / 2]), i = min((e % 2 ? pair >> 16 : pair & 0xFFFFu) - first, values);
+                            x[e] = sh.weights[i <= zone ? i : i - min(i - zone, gap)];
+                        }
+                    });
+                }
+            } else {
+                draw_by_steps(each_step_of_memory, of_last, ties, [&](const Step<DT> &s, uint32_t, uint64_t(&x)[E]) __attribute__((always_inline)) {
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        const uint32_t pair = orders_of_pair(s.v[0][e / 2]), i = (e % 2 ? pair >> 16 : pair & 0xFFFFu) - first;
+                        const float v = element<DT>(s, e);
+                        x[e] = v >= r.floor && i < values ? in_part && i == values - 1 ? MARK : r.mass_of_least(v) : 0;
+                    }
+                });
+            }
+            return;
+        }
+        __syncthreads(); // (the list takes the counts' place)
+    }
+
+    // ================ lists, other fp32 rows, and 16-bit ones with more than 65535 equal logits
+    auto each_listed = [&](auto f) __attribute__((always_inline)) {
+        for (int i = t; i < listed_front + listed_inside; i += THREADS) f(sh.list[i < listed_front ? i : FRONT + i - listed_front]);
+    };
+    // Keeps what is kept up to where the running sum of value(logit, power) exceeds than(sum of all).
+    auto cut = [&](auto value, auto than_of) __attribute__((always_inline)) {
+        auto value_of = [&](float v) __attribute__((always_inline)) { return value(r.power(v)); };
+        if (listed) {
+            r.last = find_place(sh, order_of(r.top, 0), r.last, 0, listed_front + listed_inside, than_of, [&](auto f) __attribute__((always_inline)) { each_listed([&](uint64_t o) { f(o, [&] { return value_of(logit_of(o)); }); }); });
+            return;
+        }
+        clear_bins(sh);
+        each_of(each_step_of_memory, [&](float v, uint32_t i) {
+            if (r.counts(v, i)) {
+                const double z = r.power(v);
+                add_to_bin(sh.bins[r.bin_of_power(z)], value(z));
+            }
+        });
+        __syncthreads();
+        const uint64_t than = than_of([&] { return sum_of_bins(sh); });
+        uint64_t before;
+        const int bin = find_bin(sh, 0, than, before);
+        if (bin < 0 || bin == BINS - 1) return; // (all are kept, or all that weigh anything)
+        const float low = fmaxf(r.floor, r.below(bin));
+        gather(each_step_of_memory, FRONT, [&](float v, uint32_t i) {
+            uint32_t kind = 0;
+            if (v >= low) {
+                const uint32_t b = r.bin_of(v);
+                if (b <= static_cast<uint32_t>(bin) && r.counts(v, i)) kind = b == static_cast<uint32_t>(bin) ? 2u : 1u;
+            }
+            return kind;
+        });
+        const int front = static_cast<int>(sh.front), inside = static_cast<int>(sh.inside);
+        __syncthreads();
+        if (t == 0) sh.front = sh.inside = 0;
+        listed = front <= FRONT && inside <= LIST - FRONT;
+        listed_front = front;
+        listed_inside = inside;
+        const uint64_t first = order_of(r.top, 0), behind = r.last < (uint64_t(1) << 52) ? r.last : (uint64_t(1) << 52) - 1;
+        auto known = [&](auto) { return than; };
+        if (inside <= LIST - FRONT) {
+            const int n = inside;
+            r.last = find_place(sh, first, behind, before, n, known, [&](auto f) __attribute__((always_inline)) {
+                for (int i = t; i < n; i += THREADS) {
+                    const uint64_t o = sh.list[FRONT + i];
+                    f(o, [&] { return value_of(logit_of(o)); });
+                }
+            });
+        } else {
+            r.last = find_place(sh, first, behind, before, inside, known, [&](auto f) __attribute__((always_inline)) {
+                each_of(each_step_of_memory, [&](float v, uint32_t i) {
+                    if (v >= r.floor && r.bin_of(v) == static_cast<uint32_t>(bin)) f(order_of(v, i), [&] { return value_of(v); });
+                });
+            });
+        }
+    };
+    if (k) cut([](double) { return uint64_t(1); }, [&](auto) { return static_cast<uint64_t>(k - 1); });
+    if (p < 1.0f) cut([&](double z) { return r.integer(r.scaled_weight(z)); }, than_of_p);
+
+    if (listed) {
+        uint64_t total = 0;
+        const uint64_t at = find_place(sh, 0, static_cast<uint64_t>(a.vocab), 0, listed_front + listed_inside, [&](auto sum) { return than_of_u(total = sum()); }, [&](auto f) __attribute__((always_inline)) {
+            each_listed([&](uint64_t o) { f(index_of(o), [&] { return o <= r.last ? r.mass_of_least(logit_of(o)) : uint64_t(0); }); });
+        });
+        each_listed([&](uint64_t o) {
+            if (index_of(o) == at && o <= r.last) answer(static_cast<uint32_t>(at), r.mass_of_least(logit_of(o)), total);
+        });
+        return;
+    }
+    draw_by_steps(each_step_of_memory, 0, 0, [&](const Step<DT> &s, uint32_t at, uint64_t(&x)[E]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const float v = element<DT>(s, e);
+            x[e] = r.counts(v, at + e) ? r.mass_of_least(v) : 0;
+        }
+    });
+}
+
+template <int DT, int IT> int launch(const SampleArgs &a, int64_t rows, hipStream_t s) {
+    const auto kernel = sample_kernel<DT, IT>;
+    static const hipError_t configured = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, sizeof(SampleShared));
+    AXHIP_CHECK_HIP(configured);
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(rows)), dim3(THREADS), sizeof(SampleShared), s, a);
+    return AXHIP_OK;
+}
+// Registers for a row: 64 of a thread's 128 (65536 fp32 or 131072 16-bit logits).
+template <int DT> int launch(const SampleArgs &a, int64_t rows, hipStream_t s) {
+    const int held = (a.vocab + STEP * WAVES - 1) / (STEP * WAVES);
+    if (held <= 2) return launch<DT, 2>(a, rows, s);
+    if (held <= 4) return launch<DT, 4>(a, rows, s);
+    if (held <= 8) return launch<DT, 8>(a, rows, s);
+    if constexpr (DT != AXHIP_DTYPE_F32)
+        if (held <= 16) return launch<DT, 16>(a, rows, s);
+    return launch<DT, 0>(a, rows, s);
+}
+
+} // namespace
+} // namespace axhip
