@@ -48,56 +48,58 @@ bool takes_q8_kernels(const AxhipGemmQ8Params &p) {
     return p.k >= 16 && p.lda < LD && p.ldb < LD && p.ldc < (int64_t(1) << 31);
 }
 
-// The candidates with the time each takes, in us: start + k (per_k + per_k_full u) r + per_round (r - 1), r being the rounds its work-groups take on
-// the 256 CUs and u how full the first is.
+// The candidates with the time each takes, in us: start + k (per_k + per_k_full u) r + per_round (r - 1), k in steps of 128, r being the rounds its work-groups
+// take on the 256 CUs (whole rounds of the tile kernels, of which a CU holds one, or two of a pair; the small ones share a CU, and a part of a round costs
+// about half of what is missing from a whole one) and u how full the first is.  Fitted to 460 products of m 9 .. 8192, n and k 64 .. 8192, results in bfloat16, every
+// candidate timed (mean error 5 - 12 %); the one picked takes 1.022 of the fastest one's time on average, 1.26 at worst (303 x 883 x 6416, 14.0 us instead of 11.1).
 struct Q8Kernel {
-    enum Kind { BIG256, TILE, PAIR, SMALL } kind;
-    int shape, waves;
+    bool small;
+    int tile, waves; // a Q8Tile, or a SmallShape and its wavefronts
     float start, per_k, per_k_full, per_round;
     bool ragged;
     const char *name;
 };
 constexpr Q8Kernel Q8_KERNELS[] = {
-    {Q8Kernel::BIG256, 0, 8, 7.0f, 0.0160f, 0.0057f, 4.0f, false, "big"},
-    {Q8Kernel::TILE, TILE_256x128, 8, 6.5f, 0.0080f, 0.0034f, 6.4f, false, "tile_256x128"},
-    {Q8Kernel::TILE, TILE_192x128, 8, 5.7f, 0.0063f, 0.0024f, 4.9f, false, "tile_192x128"},
-    {Q8Kernel::TILE, TILE_128x128, 8, 4.9f, 0.0048f, 0.0014f, 4.1f, false, "tile_128x128"},
-    {Q8Kernel::TILE, TILE_64x128, 8, 4.9f, 0.0032f, 0.0009f, 3.7f, false, "tile_64x128"},
-    {Q8Kernel::TILE, TILE_128x128, 8, 6.5f, 0.0080f, 0.0f, 5.9f, true, "tile_128x128_ragged"},
-    {Q8Kernel::PAIR, Q8_128x128_PAIR, 4, 4.9f, 0.0048f, 0.0014f, 4.1f, false, "tile_128x128_pair"},
-    {Q8Kernel::SMALL, SMALL_64x64, 8, 4.35f, 0.00245f, 0.00148f, 3.6f, false, "small_64x64_8"},
-    {Q8Kernel::SMALL, SMALL_64x64, 4, 4.15f, 0.00324f, 0.00047f, 1.65f, false, "small_64x64_4"},
-    {Q8Kernel::SMALL, SMALL_32x64, 8, 3.50f, 0.00170f, 0.00085f, 2.3f, false, "small_32x64_8"},
-    {Q8Kernel::SMALL, SMALL_32x64, 4, 3.30f, 0.00210f, 0.00030f, 0.6f, false, "small_32x64_4"},
-    {Q8Kernel::SMALL, SMALL_32x32, 8, 3.07f, 0.00105f, 0.00045f, 0.76f, false, "small_32x32_8"},
-    {Q8Kernel::SMALL, SMALL_32x32, 4, 2.95f, 0.00148f, 0.00005f, 0.26f, false, "small_32x32_4"},
-    {Q8Kernel::SMALL, SMALL_32x16, 8, 2.92f, 0.00074f, 0.00032f, 0.33f, false, "small_32x16_8"},
-    {Q8Kernel::SMALL, SMALL_32x16, 4, 2.91f, 0.00102f, 0.00004f, 0.10f, false, "small_32x16_4"},
-    {Q8Kernel::SMALL, SMALL_16x16, 8, 2.95f, 0.00045f, 0.00024f, 0.19f, false, "small_16x16_8"},
-    {Q8Kernel::SMALL, SMALL_16x16, 4, 2.94f, 0.00069f, 0.00004f, 0.02f, false, "small_16x16_4"},
+    {false, Q8_256x256, 8, 10.00f, 0.01722f, 0.00783f, 7.45f, false, "tile_256x256"},
+    {false, Q8_256x128, 8, 7.85f, 0.00961f, 0.00463f, 6.97f, false, "tile_256x128"},
+    {false, Q8_192x128, 8, 6.62f, 0.00736f, 0.00380f, 5.91f, false, "tile_192x128"},
+    {false, Q8_128x128, 8, 5.49f, 0.00542f, 0.00339f, 4.63f, false, "tile_128x128"},
+    {false, Q8_128x128_PAIR, 4, 5.23f, 0.00909f, 0.00089f, 2.35f, false, "tile_128x128_pair"},
+    {false, Q8_64x128, 8, 5.43f, 0.00333f, 0.00156f, 4.48f, false, "tile_64x128"},
+    {false, Q8_128x128, 8, 7.55f, 0.00981f, 0.00180f, 6.69f, true, "tile_128x128_ragged"}, // (through registers)
+    {true, SMALL_64x64, 8, 4.75f, 0.00246f, 0.00260f, 3.91f, false, "small_64x64_8"},
+    {true, SMALL_64x64, 4, 5.09f, 0.00338f, 0.00092f, 2.07f, false, "small_64x64_4"},
+    {true, SMALL_32x64, 8, 3.55f, 0.00158f, 0.00160f, 2.49f, false, "small_32x64_8"},
+    {true, SMALL_32x64, 4, 3.67f, 0.00207f, 0.00062f, 0.80f, false, "small_32x64_4"},
+    {true, SMALL_32x32, 8, 3.28f, 0.00095f, 0.00075f, 0.71f, false, "small_32x32_8"},
+    {true, SMALL_32x32, 4, 3.23f, 0.00129f, 0.00049f, 0.22f, false, "small_32x32_4"},
+    {true, SMALL_32x16, 8, 3.29f, 0.00054f, 0.00065f, 0.26f, false, "small_32x16_8"},
+    {true, SMALL_32x16, 4, 3.28f, 0.00075f, 0.00052f, 0.02f, false, "small_32x16_4"},
+    {true, SMALL_16x16, 8, 3.36f, 0.00019f, 0.00053f, 0.08f, false, "small_16x16_8"},
+    {true, SMALL_16x16, 4, 3.30f, 0.00040f, 0.00034f, 0.00f, false, "small_16x16_4"},
 };
 constexpr size_t Q8_CANDIDATES = sizeof(Q8_KERNELS) / sizeof(Q8_KERNELS[0]);
+// Rows off the 16-byte grid, or k no whole chunks: what that costs the small kernels per k.
+constexpr float Q8_MISALIGNED = 1.8f;
 
 struct Q8Choice { const Q8Kernel *best; float cost; };
 // One candidate.  (A parameter of the template, so that its tiles are constants here: divisions by what a table holds cost a small product's caller.)
 template <size_t I> void consider(const AxhipGemmQ8Params &p, bool aligned, Q8Choice &c) {
     constexpr const Q8Kernel &h = Q8_KERNELS[I];
-    if (h.kind != Q8Kernel::SMALL && h.ragged == aligned) return;
-    if (h.kind == Q8Kernel::BIG256 && (p.k % 128 != 0 || p.m < 256 || p.n < 256)) return;
-    constexpr uint32_t tm = h.kind == Q8Kernel::BIG256 ? 256 : h.kind == Q8Kernel::PAIR ? 128 : h.kind == Q8Kernel::TILE ? TILE_GEOMETRY[h.kind == Q8Kernel::TILE ? h.shape : 0].tm : SMALL_GEOMETRY[h.kind == Q8Kernel::SMALL ? h.shape : 0].tm;
-    constexpr uint32_t tn = h.kind == Q8Kernel::BIG256 ? 256 : h.kind == Q8Kernel::PAIR ? 128 : h.kind == Q8Kernel::TILE ? TILE_GEOMETRY[h.kind == Q8Kernel::TILE ? h.shape : 0].tn : SMALL_GEOMETRY[h.kind == Q8Kernel::SMALL ? h.shape : 0].tn;
+    if (!h.small && h.ragged == aligned) return;
+    constexpr uint32_t tm = h.small ? SMALL_GEOMETRY[h.small ? h.tile : 0].tm : Q8_GEOMETRY[h.small ? 0 : h.tile].tm;
+    constexpr uint32_t tn = h.small ? SMALL_GEOMETRY[h.small ? h.tile : 0].tn : Q8_GEOMETRY[h.small ? 0 : h.tile].tn;
     const uint32_t rows = (static_cast<uint32_t>(p.m) + tm - 1) / tm, cols = (static_cast<uint32_t>(p.n) + tn - 1) / tn;
     if (!launch_fits(static_cast<int64_t>(rows) * cols + 7, 64 * h.waves)) return;
     const float k = static_cast<float>((p.k + 127) / 128 * 64);
     const float full = static_cast<float>(rows) * static_cast<float>(cols) * (1.0f / 256.0f);
+    auto whole = [](float x) { // (rounded up)
+        const float down = x < 1e9f ? static_cast<float>(static_cast<int>(x)) : x;
+        return down < x ? down + 1.0f : down;
+    };
     float r = 1.0f;
-    if (full > 1.0f) {
-        float whole = full < 1e9f ? static_cast<float>(static_cast<int>(full)) : full;
-        if (whole < full) whole += 1.0f;
-        r = h.kind == Q8Kernel::SMALL ? 0.5f * (whole + full) : whole;
-    }
-    const float slower = aligned ? 1.0f : h.kind == Q8Kernel::SMALL ? 1.5f : 1.0f;
-    const float cost = h.start + k * (h.per_k + h.per_k_full * std::min(full, 1.0f)) * slower * r + h.per_round * (r - 1.0f);
+    if (full > 1.0f) r = h.small ? 0.5f * (whole(full) + full) : !h.ragged && h.tile == Q8_128x128_PAIR ? whole(0.5f * full) + 0.5f * full : whole(full);
+    const float cost = h.start + k * (h.per_k + h.per_k_full * std::min(full, 1.0f)) * (h.small && !aligned ? Q8_MISALIGNED : 1.0f) * r + h.per_round * (r - 1.0f);
     if (!c.best || cost < c.cost) c = {&h, cost};
 }
 template <size_t... I> const Q8Kernel *choose(const AxhipGemmQ8Params &p, bool aligned, std::index_sequence<I...>) {
@@ -107,16 +109,17 @@ template <size_t... I> const Q8Kernel *choose(const AxhipGemmQ8Params &p, bool a
 }
 
 int launch_chosen(const Q8Args &g, const AxhipGemmQ8Params &p, bool aligned, hipStream_t s) {
-    if (p.m <= 8) {
+    // One or two rows of x: the weights are read once, along k (1 x 4096 x 4096 5.2 us, on the small kernels 5.4; 1 x 1280 x 5120 4.1 and 5.3; of three rows and more the small
+    // ones take less).  Two rows of W to a wavefront where k is short (51865 x 1280 15.8 -> 11.9 us) or x has two and W is large (2 x 16384 x 16384 52.7 -> 48.2).
+    if (p.m <= 2) {
         q8_last_kernel = "skinny";
-        return launch_q8_skinny(g, p.dtype, 1, s);
+        return launch_q8_skinny(g, p.dtype, p.k < 2048 || (p.m == 2 && p.n * p.k >= int64_t(1) << 26) ? 2 : 1, s);
     }
     const Q8Kernel *k = choose(p, aligned, std::make_index_sequence<Q8_CANDIDATES>{});
     AXHIP_REQUIRE(k != nullptr, AXHIP_ERR_UNSUPPORTED, "axhip_gemm_q8: too many tiles");
     q8_last_kernel = k->name;
-    if (k->kind == Q8Kernel::BIG256) return launch_q8_big(g, p.dtype, s);
-    if (k->kind == Q8Kernel::SMALL) return launch_q8_small(g, p.dtype, k->shape, k->waves, s);
-    return p.dtype == AXHIP_DTYPE_F32 ? launch_q8_tile_f32(g, k->shape, aligned, s) : p.dtype == AXHIP_DTYPE_F16 ? launch_q8_tile_f16(g, k->shape, aligned, s) : launch_q8_tile_bf16(g, k->shape, aligned, s);
+    if (k->small) return launch_q8_small(g, p.dtype, k->tile, k->waves, s);
+    return p.dtype == AXHIP_DTYPE_F32 ? launch_q8_tile_f32(g, k->tile, aligned, s) : p.dtype == AXHIP_DTYPE_F16 ? launch_q8_tile_f16(g, k->tile, aligned, s) : launch_q8_tile_bf16(g, k->tile, aligned, s);
 }
 } // namespace
 } // namespace axhip

@@ -15,17 +15,17 @@ struct Q8Args {
 };
 static_assert(sizeof(Q8Args) <= 96, "kernel arguments");
 
-// The launchers.  The tiles are those of the 16-bit products (TileShape, SmallShape): a k of int8 is half as many bytes, so their k-tiles
-// hold twice as many k.  `aligned`: every row of a and b starts on a 16-byte boundary and K is a multiple of 16.  All but the skinny kernel's
-// grid are their own; K >= 16 for all.
-// one more tile: 128 x 128 on four wavefronts, of which a CU holds two work-groups
-constexpr int Q8_128x128_PAIR = TILE_SHAPES;
+// Work-group tiles (M x N) of the middle-sized and large products.  Q8_128x128_PAIR: on four wavefronts, of which a CU holds two work-groups.
+enum Q8Tile { Q8_256x256, Q8_256x128, Q8_192x128, Q8_128x128, Q8_128x128_PAIR, Q8_64x128, Q8_TILES };
+struct Q8Geometry { int tm, tn, waves; };
+constexpr Q8Geometry Q8_GEOMETRY[Q8_TILES] = {{256, 256, 8}, {256, 128, 8}, {192, 128, 8}, {128, 128, 8}, {128, 128, 4}, {64, 128, 8}};
 
-int launch_q8_big(const Q8Args &g, int dtype, hipStream_t s);  // 256 x 256: aligned, K a multiple of 128
-int launch_q8_tile_f32(const Q8Args &g, int shape, bool aligned, hipStream_t s); // (not aligned: TILE_128x128)
-int launch_q8_tile_f16(const Q8Args &g, int shape, bool aligned, hipStream_t s);
-int launch_q8_tile_bf16(const Q8Args &g, int shape, bool aligned, hipStream_t s);
+// The launchers, K >= 16.  `aligned`: every row of a and b starts on a 16-byte boundary and K is a multiple of 16 (if not: Q8_128x128, through registers).  The small products' tiles are
+// those of the 16-bit ones (SmallShape).
+int launch_q8_tile_f32(const Q8Args &g, int tile, bool aligned, hipStream_t s);
+int launch_q8_tile_f16(const Q8Args &g, int tile, bool aligned, hipStream_t s);
+int launch_q8_tile_bf16(const Q8Args &g, int tile, bool aligned, hipStream_t s);
 int launch_q8_small(const Q8Args &g, int dtype, int shape, int waves, hipStream_t s);
-int launch_q8_skinny(const Q8Args &g, int dtype, int rows_per_wave, hipStream_t s); // M <= 8
+int launch_q8_skinny(const Q8Args &g, int dtype, int rows_per_wave, hipStream_t s); // M 1 or 2; 1 or 2 rows of b to a wavefront
 
 } // namespace axhip

@@ -1,4 +1,4 @@
-// Products of at most eight int8 rows of x with a weight matrix: one read of the weights.
+// Products of one or two int8 rows of x with a weight matrix: one read of the weights.
 #include "gemm_q8_device.hpp"
 
 namespace axhip {
@@ -21,9 +21,9 @@ template <int P> __device__ __forceinline__ int q8_lane_sums(int (&v)[P], int la
     step(P, 32);
     step(P / 2, 16);
     step(P / 4, 8);
-    step(P / 8, 4);
-    step(P / 16, 2);
-    step(P / 32, 1);
+    step(1, 4);
+    step(1, 2);
+    step(1, 1);
     return v[0];
 }
 
@@ -35,10 +35,10 @@ __global__ __launch_bounds__(256) void gemm_q8_skinny_kernel(const Q8Args a) {
     const int lane = threadIdx.x % 64;
     const int n0 = (static_cast<int>(blockIdx.x) * 4 + threadIdx.x / 64) * R;
     if (n0 >= a.N) return; // (whole wavefronts)
-    constexpr int P = M * R <= 1 ? 1 : M * R <= 2 ? 2 : M * R <= 4 ? 4 : M * R <= 8 ? 8 : M * R <= 16 ? 16 : 32;
+    constexpr int P = M * R; // sums of a wavefront: 1, 2 or 4
     // after the sums, lane 64 / P i finishes value i = m R + r; what it needs is requested before W is
     const int value = lane / (64 / P), n = n0 + value % R;
-    const bool writes = lane % (64 / P) == 0 && value < M * R && n < a.N;
+    const bool writes = lane % (64 / P) == 0 && n < a.N;
     const int64_t at = static_cast<int64_t>(value / R) * a.ldc + n;
     const float bias = writes && a.bias ? Elem<DT>::load(a.bias, n) : 0.0f, residual = writes && a.residual ? Elem<DT>::load(a.residual, at) : 0.0f;
     const float scale = writes ? a.scale_a[value / R] * a.scale_b[n] : 0.0f;
@@ -46,7 +46,7 @@ __global__ __launch_bounds__(256) void gemm_q8_skinny_kernel(const Q8Args a) {
     const int8_t *wrow[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) wrow[r] = a.b + static_cast<int64_t>(min(n0 + r, a.N - 1)) * a.ldb; // (rows past N: the last row again, not stored)
-    constexpr int U = R == 1 ? 4 : R == 2 ? 2 : 1; // k steps requested together
+    constexpr int U = R == 1 ? 4 : 2; // k steps requested together
     for (int k0 = lane * 16; k0 < a.K; k0 += 1024 * U) {
         uint4_t wf[U][R], xf[U][M];
 #pragma unroll
@@ -74,28 +74,19 @@ __global__ __launch_bounds__(256) void gemm_q8_skinny_kernel(const Q8Args a) {
     }
     int v[P];
 #pragma unroll
-    for (int i = 0; i < P; ++i) v[i] = i < M * R ? acc[i / R][i % R] : 0;
+    for (int i = 0; i < P; ++i) v[i] = acc[i / R][i % R];
     const int sum = q8_lane_sums<P>(v, lane);
     if (writes) Elem<DT>::store(a.c, at, gemm_epilogue(a.epilogue, __builtin_fmaf(static_cast<float>(sum), scale, bias) + residual));
 }
 
 template <int DT, int M> void launch_rows(const Q8Args &g, int rows_per_wave, hipStream_t s) {
     const dim3 grid(static_cast<unsigned>((g.N + 4 * rows_per_wave - 1) / (4 * rows_per_wave)));
-    if (rows_per_wave == 4) hipLaunchKernelGGL((gemm_q8_skinny_kernel<DT, M, 4>), grid, dim3(256), 0, s, g);
-    else if (rows_per_wave == 2) hipLaunchKernelGGL((gemm_q8_skinny_kernel<DT, M, 2>), grid, dim3(256), 0, s, g);
+    if (rows_per_wave == 2) hipLaunchKernelGGL((gemm_q8_skinny_kernel<DT, M, 2>), grid, dim3(256), 0, s, g);
     else hipLaunchKernelGGL((gemm_q8_skinny_kernel<DT, M, 1>), grid, dim3(256), 0, s, g);
 }
 template <int DT> void launch_dtype(const Q8Args &g, int rows_per_wave, hipStream_t s) {
-    switch (g.M) { // (x's row count is a template constant: the sums live in registers)
-    case 1: return launch_rows<DT, 1>(g, rows_per_wave, s);
-    case 2: return launch_rows<DT, 2>(g, rows_per_wave, s);
-    case 3: return launch_rows<DT, 3>(g, rows_per_wave, s);
-    case 4: return launch_rows<DT, 4>(g, rows_per_wave, s);
-    case 5: return launch_rows<DT, 5>(g, rows_per_wave, s);
-    case 6: return launch_rows<DT, 6>(g, rows_per_wave, s);
-    case 7: return launch_rows<DT, 7>(g, rows_per_wave, s);
-    default: return launch_rows<DT, 8>(g, rows_per_wave, s);
-    }
+    if (g.M == 1) launch_rows<DT, 1>(g, rows_per_wave, s);
+    else launch_rows<DT, 2>(g, rows_per_wave, s);
 }
 } // namespace
 

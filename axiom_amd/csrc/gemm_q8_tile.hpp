@@ -1,4 +1,4 @@
-// ------------------------------------------------------- middle-sized products of int8 rows
+// ------------------------------------------------------- middle-sized and large products of int8 rows
 // C = A B^T, A [M, K], B [N, K].  Work-group tile TM x TN, k-tiles of TKB bytes in an S-stage ring in LDS; the schedule of the 16-bit tile
 // kernel, whose LDS rows and fragments hold the same bytes: v_mfma_i32_16x16x64_i8 takes as many cycles for 64 k of int8 as the 16-bit form does for
 // 32 k, and reads as many bytes.
@@ -307,13 +307,14 @@ int launch_q8_tile_kernel(const Q8Args &g, hipStream_t s) {
     hipLaunchKernelGGL(kernel, dim3(tile_grid(tiles, 1)), dim3(64 * WM * WN * WK), lds, s, g);
     return AXHIP_OK;
 }
-template <int DT> int launch_q8_tile_as(const Q8Args &g, int shape, bool aligned, hipStream_t s) {
+template <int DT> int launch_q8_tile_as(const Q8Args &g, int tile, bool aligned, hipStream_t s) {
     if (!aligned) return launch_q8_tile_kernel<DT, false, 4, 2, 2, 2, 128, 2>(g, s);
-    switch (shape) {
-    case TILE_256x128: return launch_q8_tile_kernel<DT, true, 8, 2, 2, 2, 128, 3>(g, s);
-    case TILE_192x128: return launch_q8_tile_kernel<DT, true, 6, 2, 2, 2, 128, 3>(g, s);
+    switch (tile) {
+    case Q8_256x256: return launch_q8_tile_kernel<DT, true, 8, 2, 4, 1, 128, 2>(g, s);
+    case Q8_256x128: return launch_q8_tile_kernel<DT, true, 8, 2, 2, 2, 128, 3>(g, s);
+    case Q8_192x128: return launch_q8_tile_kernel<DT, true, 6, 2, 2, 2, 128, 3>(g, s);
+    case Q8_128x128: return launch_q8_tile_kernel<DT, true, 4, 2, 2, 2, 128, 4>(g, s);
     case Q8_128x128_PAIR: return launch_q8_tile_kernel<DT, true, 4, 2, 2, 1, 128, 2>(g, s);
-    case TILE_128x128: return launch_q8_tile_kernel<DT, true, 4, 2, 2, 2, 128, 4>(g, s);
     default: return launch_q8_tile_kernel<DT, true, 4, 1, 2, 4, 256, 3>(g, s);
     }
 }
