@@ -2,6 +2,9 @@
 #pragma once
 #include "sample.hpp"
 
+#include <type_traits>
+#include <utility>
+
 namespace axhip {
 namespace {
 
@@ -60,6 +63,12 @@ __device__ __forceinline__ uint64_t sum32(uint64_t v) { // over halves
     const auto hi = __builtin_amdgcn_permlane16_swap(static_cast<uint32_t>(v >> 32), static_cast<uint32_t>(v >> 32), false, false);
     return (static_cast<uint64_t>(hi[0]) << 32 | lo[0]) + (static_cast<uint64_t>(hi[1]) << 32 | lo[1]);
 }
+// x's sum in the first half's lanes, y's in the second's
+__device__ __forceinline__ uint64_t sums_of_two(uint64_t x, uint64_t y) {
+    const auto lo = __builtin_amdgcn_permlane32_swap(static_cast<uint32_t>(x), static_cast<uint32_t>(y), false, false);
+    const auto hi = __builtin_amdgcn_permlane32_swap(static_cast<uint32_t>(x >> 32), static_cast<uint32_t>(y >> 32), false, false);
+    return sum32((static_cast<uint64_t>(hi[0]) << 32 | lo[0]) + (static_cast<uint64_t>(hi[1]) << 32 | lo[1]));
+}
 __device__ __forceinline__ uint64_t wave_sum64(uint64_t v) {
     v = sum32(v);
     const auto lo = __builtin_amdgcn_permlane32_swap(static_cast<uint32_t>(v), static_cast<uint32_t>(v), false, false);
@@ -78,6 +87,37 @@ __device__ __forceinline__ uint64_t lane_of(uint64_t v, int lane) {
     return static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(v >> 32)), lane))) << 32 |
            static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(v)), lane));
 }
+// The sums of P values (a power of two from 2 to 16), value i in lanes [64 / P i, 64 / P (i + 1)): at each step a lane hands half of them over and adds up the other half.
+template <int P> __device__ __forceinline__ uint64_t sums_of_many(uint64_t (&v)[P], int lane) {
+    static_assert(P == 2 || P == 4 || P == 8 || P == 16, "a power of two");
+    auto halve = [&](int p, auto swap) __attribute__((always_inline)) { // (swap(x, y): x's low and y's low lanes, x's high and y's high)
+#pragma unroll
+        for (int i = 0; i < (p > 1 ? p / 2 : 1); ++i) {
+            const uint64_t x = v[i], y = v[p > 1 ? i + p / 2 : i];
+            const auto lo = swap(static_cast<uint32_t>(x), static_cast<uint32_t>(y)), hi = swap(static_cast<uint32_t>(x >> 32), static_cast<uint32_t>(y >> 32));
+            v[i] = (static_cast<uint64_t>(hi[0]) << 32 | lo[0]) + (static_cast<uint64_t>(hi[1]) << 32 | lo[1]);
+        }
+    };
+    auto step = [&](int p, int d, auto from) __attribute__((always_inline)) { // (from(x): x of the lane d away)
+        if (p <= 1) {
+            v[0] += from(v[0]);
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < p / 2; ++i) {
+            const uint64_t mine = lane & d ? v[i + p / 2] : v[i], other = lane & d ? v[i] : v[i + p / 2];
+            v[i] = mine + from(other);
+        }
+    };
+    halve(P, [](uint32_t x, uint32_t y) { return __builtin_amdgcn_permlane32_swap(x, y, false, false); });
+    halve(P / 2, [](uint32_t x, uint32_t y) { return __builtin_amdgcn_permlane16_swap(x, y, false, false); });
+    step(P / 4, 8, [](uint64_t x) { return dpp64<0x128>(x); }); // (row_ror:8)
+    step(P / 8, 4, [](uint64_t x) { return __shfl_xor(x, 4, WAVE); });
+    v[0] += dpp64<0x4E>(v[0]); // (quad_perm: 2 and 1 apart)
+    return v[0] + dpp64<0xB1>(v[0]);
+}
+template <int N, class F, int... I> __device__ __forceinline__ void unrolled_as(F f, std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>{}), ...); }
+template <int N, class F> __device__ __forceinline__ void unrolled(F f) { unrolled_as<N>(f, std::make_integer_sequence<int, N>{}); }
 // A counter's old value; lane by lane (the compiler makes a sum over the wavefront of additions to one address, which is the longer way for the few lanes that come here)
 __device__ __forceinline__ uint32_t take_from(uint32_t &counter, uint32_t n) {
     uint32_t offset = 0;
@@ -98,10 +138,14 @@ __device__ __forceinline__ float logit_of(uint64_t order) {
 __device__ __forceinline__ uint32_t index_of(uint64_t order) { return static_cast<uint32_t>(order) & 0xFFFFFu; }
 
 // The same of two 16-bit logits at a time: 0x7FFF - h of a positive one, h - 1 of a negative one (so that -0 has the number of +0).
-__device__ __forceinline__ uint32_t orders_of_pair(uint32_t w) {
-    const uint32_t sign = (w >> 15) & 0x00010001u;
-    return (w ^ 0x7FFF7FFFu ^ ((sign << 15) - sign)) - sign;
+typedef uint16_t pair_t __attribute__((ext_vector_type(2)));
+typedef int16_t signed_pair_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ pair_t orders_of(uint32_t w) {
+    const signed_pair_t sign = __builtin_bit_cast(signed_pair_t, w) >> static_cast<int16_t>(15); // -1 or 0
+    const uint32_t m = ~__builtin_bit_cast(uint32_t, sign) & 0x7FFF7FFFu;
+    return __builtin_bit_cast(pair_t, w ^ m) + __builtin_bit_cast(pair_t, sign);
 }
+__device__ __forceinline__ uint32_t order_of16(uint32_t h) { return orders_of(h)[0]; }
 template <int DT> constexpr uint32_t INFINITY16 = DT == AXHIP_DTYPE_BF16 ? 0x7F80u : 0x7C00u;
 template <int DT> constexpr uint32_t FIRST_ORDER = 0x7FFFu ^ INFINITY16<DT>;                                    // of infinity,
 template <int DT> constexpr uint32_t DRAWN_ORDERS = (0x8000u | INFINITY16<DT>) - 1 - FIRST_ORDER<DT>;          // and how many there are before -infinity and the NaNs
@@ -341,23 +385,23 @@ template <int DT, int IT> __global__ __launch_bounds__(THREADS) void sample_kern
         }
     };
     // ... from the registers, for passes of few instructions.  (The compiler is not to see that a later pass forms the same numbers of the same vectors: it would keep them all.)
+    auto each_step_at = [&](auto f) __attribute__((always_inline)) { // f(vectors, index of the first, their place in `held`)
+        int first = lane * E;
+        unrolled<IT>([&](auto place) __attribute__((always_inline)) {
+            constexpr int i = decltype(place)::value;
+            const int step = i * WAVES + wave;
+            Step<DT> s = held[i];
+#pragma unroll
+            for (int v = 0; v < ES / 2; ++v)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) asm volatile("" : "+v"(s.v[v][w]));
+            asm volatile("" : "+v"(first));
+            if (step < steps) f(s, static_cast<uint32_t>(step * STEP + first), place);
+        });
+    };
     auto each_step = [&](auto f) __attribute__((always_inline)) {
-        if constexpr (IT > 0) {
-            int first = lane * E;
-#pragma unroll
-            for (int i = 0; i < IT; ++i) {
-                const int step = i * WAVES + wave;
-                Step<DT> s = held[i];
-#pragma unroll
-                for (int v = 0; v < ES / 2; ++v)
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) asm volatile("" : "+v"(s.v[v][w]));
-                asm volatile("" : "+v"(first));
-                if (step < steps) f(s, static_cast<uint32_t>(step * STEP + first), step);
-            }
-        } else {
-            each_step_of_memory(f);
-        }
+        if constexpr (IT > 0) each_step_at([&](const Step<DT> &s, uint32_t at, auto place) __attribute__((always_inline)) { f(s, at, decltype(place)::value * WAVES + wave); });
+        else each_step_of_memory(f);
     };
     auto each_of = [&](auto steps_of, auto f) __attribute__((always_inline)) { // f(logit, index)
         steps_of([&](const Step<DT> &s, uint32_t at, int) __attribute__((always_inline)) {
@@ -522,16 +566,33 @@ template <int DT, int IT> __global__ __launch_bounds__(THREADS) void sample_kern
 
     // The draw by the sums of the wavefronts' steps, and then within one.  masses(vectors, index of the first, sums): of a lane's eight, MARK for a logit of which only the first
     // `ties` are kept, with the weight `of_tie` each.
-    auto draw_by_steps = [&](auto steps_of, uint64_t of_tie, uint32_t ties, auto masses) __attribute__((always_inline)) {
+    auto draw_by_steps = [&](auto in_registers, uint64_t of_tie, uint32_t ties, auto masses) __attribute__((always_inline)) {
+        constexpr bool HELD = decltype(in_registers)::value;
         clear_bins(sh);
-        steps_of([&](const Step<DT> &s, uint32_t at, int step) __attribute__((always_inline)) {
-            uint64_t x[E], sum = 0;
-            masses(s, at, x);
+        if constexpr (HELD && IT > 0) { // (weights of a step are 2^52 at most, marks 512)
+            constexpr int N = IT > 0 ? IT : 2;
+            uint64_t sums[N];
 #pragma unroll
-            for (int e = 0; e < E; ++e) sum += x[e];
-            sum = wave_sum64(sum); // (weights of a step are 2^52 at most, marks 512)
-            if (lane == 0) sh.bins[step] = sum;
-        });
+            for (int i = 0; i < N; ++i) sums[i] = 0;
+            each_step_at([&](const Step<DT> &s, uint32_t at, auto place) __attribute__((always_inline)) {
+                uint64_t x[E];
+                masses(s, at, x);
+#pragma unroll
+                for (int e = 0; e < E; ++e) sums[place.value] += x[e];
+            });
+            const uint64_t sum = sums_of_many<N>(sums, lane);
+            const int step = lane / (WAVE / N) * WAVES + wave;
+            if (lane % (WAVE / N) == 0 && step < steps) sh.bins[step] = sum;
+        } else {
+            each_step_of_memory([&](const Step<DT> &s, uint32_t at, int step) __attribute__((always_inline)) {
+                uint64_t x[E], sum = 0;
+                masses(s, at, x);
+#pragma unroll
+                for (int e = 0; e < E; ++e) sum += x[e];
+                sum = wave_sum64(sum);
+                if (lane == 0) sh.bins[step] = sum;
+            });
+        }
         __syncthreads();
         uint64_t marks_in_front = 0; // of the step that is looked for
         if (of_tie) { // marks -> the weights of those that are kept
@@ -588,51 +649,87 @@ template <int DT, int IT> __global__ __launch_bounds__(THREADS) void sample_kern
     // ================ 16-bit logits: counts of their values
     if (DT != AXHIP_DTYPE_F32 && !listed) {
         const bool filtered = k || p < 1.0f; // (else there is nothing to count)
-        auto count_at = [&](uint32_t order) { return (sh.counts[order >> 1] >> (16 * (order & 1))) & 0xFFFFu; };
+        // The count of order o is a half of word o % 32768 (values next to each other lie in different banks).
+        auto count_at = [&](uint32_t order) { return (sh.counts[order & 0x7FFFu] >> (order >> 15 << 4)) & 0xFFFFu; };
         if (filtered)
             for (int i = t; i < 8192; i += THREADS) reinterpret_cast<uint4_t *>(sh.counts)[i] = uint4_t{0, 0, 0, 0};
         clear_bins(sh); // (and a barrier)
         uint32_t drawn = 0;
         if (filtered)
             each_step([&](const Step<DT> &s, uint32_t, int) __attribute__((always_inline)) {
+                // (most steps hold nothing that is never drawn: no look at every logit)
+                pair_t farthest = pair_t{0, 0};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) farthest = __builtin_elementwise_max(farthest, orders_of(s.v[0][i]) - static_cast<uint16_t>(FIRST_ORDER<DT>));
+                const bool whole = max(farthest[0], farthest[1]) < DRAWN_ORDERS<DT>;
+                const bool all_whole = __ballot(!whole) == 0;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const uint32_t pair = orders_of_pair(s.v[0][i]);
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const uint32_t order = h ? pair >> 16 : pair & 0xFFFFu;
-                        if (order - FIRST_ORDER<DT> < DRAWN_ORDERS<DT>) {
+                    const uint32_t orders = __builtin_bit_cast(uint32_t, orders_of(s.v[0][i])), halves = orders >> 11 & 0x00100010u; // 16 for counts in the upper half
+                    uint32_t *const first = &sh.counts[orders & 0x7FFFu], *const second = &sh.counts[orders >> 16 & 0x7FFFu];
+                    const uint32_t one = 1u << (halves & 31u), other = 1u << (halves >> 16);
+                    if (all_whole) {
+                        atomicAdd(first, one);
+                        atomicAdd(second, other);
+                    } else {
+                        const pair_t at = __builtin_bit_cast(pair_t, orders) - static_cast<uint16_t>(FIRST_ORDER<DT>);
+                        if (at[0] < DRAWN_ORDERS<DT>) {
                             ++drawn;
-                            atomicAdd(&sh.counts[order >> 1], 1u << (16 * (order & 1)));
+                            atomicAdd(first, one);
+                        }
+                        if (at[1] < DRAWN_ORDERS<DT>) {
+                            ++drawn;
+                            atomicAdd(second, other);
                         }
                     }
                 }
+                if (all_whole) drawn += E;
             });
         drawn = static_cast<uint32_t>(sum_of_all(sh, drawn)); // (a barrier behind the counts)
-        // f(block, pair of counts, the first one's order) of the blocks of 64 values in which any occurs, by the lanes of half a wavefront; others' sums are 0
-        auto each_block_pair = [&](auto f) __attribute__((always_inline)) {
+        // f(counts of the lane's value in block j and in block j + BLOCKS / 2, its order in the first) where either has any, a sum for each block; the others' sums are 0
+        auto sum_blocks = [&](auto f) __attribute__((always_inline)) {
             constexpr int TOGETHER = 8;
 #pragma unroll 1
             for (int j0 = wave; j0 < BLOCKS / 2; j0 += WAVES * TOGETHER) {
                 uint32_t w[TOGETHER];
 #pragma unroll
-                for (int i = 0; i < TOGETHER; ++i) w[i] = sh.counts[64 * (j0 + WAVES * i) + lane];
-#pragma unroll
+                for (int i = 0; i < TOGETHER; ++i) w[i] = sh.counts[BLOCK * (j0 + WAVES * i) + lane];
+#pragma unroll 1
                 for (int i = 0; i < TOGETHER; ++i) {
+                    uint32_t pair = w[0];
+#pragma unroll
+                    for (int d = 0; d + 1 < TOGETHER; ++d) w[d] = w[d + 1];
+                    if (__ballot(pair != 0) == 0) continue;
                     const int j = j0 + WAVES * i;
-                    if (__ballot(w[i] != 0)) f(2 * j + lane / 32, w[i], static_cast<uint32_t>(128 * j + 2 * lane));
+                    uint64_t of_first, of_second;
+                    f(pair & 0xFFFFu, pair >> 16, static_cast<uint32_t>(BLOCK * j + lane), of_first, of_second);
+                    const uint64_t sum = sums_of_two(of_first, of_second);
+                    if (lane % 32 == 0) sh.bins[lane ? j + BLOCKS / 2 : j] = sum;
                 }
             }
         };
-        static_assert(BLOCKS / 2 % (WAVES * 8) == 0, "whole rounds");
-        if (filtered)
-            each_block_pair([&](int block, uint32_t w, uint32_t) __attribute__((always_inline)) {
-                const uint64_t sum = sum32((w & 0xFFFFu) + (w >> 16));
-                if (lane % 32 == 0) sh.bins[block] = sum;
+        static_assert(BLOCKS / 2 % (WAVES * 8) == 0 && BLOCK == WAVE && BLOCKS <= BINS, "whole rounds, a value to a lane, and a bin for a block");
+        uint32_t counted = 0;
+        auto masses_of = [&](uint32_t last, uint32_t ties) __attribute__((always_inline)) {
+            return [&r, last, ties](uint32_t order, uint32_t count) __attribute__((always_inline)) {
+                const uint32_t c = order < last ? count : order == last ? min(count, ties) : 0u;
+                return c ? c * r.mass(logit_of16<DT>(order)) : uint64_t(0);
+            };
+        };
+        if (k) {
+            sum_blocks([&](uint32_t c0, uint32_t c1, uint32_t, uint64_t &first, uint64_t &second) __attribute__((always_inline)) {
+                first = c0;
+                second = c1;
+                counted += c0 + c1;
             });
-        __syncthreads();
-        if (sum_of_bins(sh) == drawn) { // (a count that overflowed takes 65535 or 65536 from the sum)
-            static_assert(BLOCK == WAVE && BLOCKS <= BINS, "a value to a lane, and a bin for a block");
+        } else if (p < 1.0f) { // (what the blocks weigh, at once)
+            sum_blocks([&, mass_of = masses_of(~0u, 0)](uint32_t c0, uint32_t c1, uint32_t order, uint64_t &first, uint64_t &second) __attribute__((always_inline)) {
+                first = mass_of(order, c0);
+                second = mass_of(order + 32768, c1);
+                counted += c0 + c1;
+            });
+        }
+        if (sum_of_all(sh, counted) == drawn) { // (a count that overflowed takes 65535 or 65536 from the sum)
             // the first value of `block` at which the running sum exceeds `than`, and the sum in front of it
             auto find_value = [&](int block, uint64_t front, uint64_t than, uint64_t own, uint64_t &in_front) __attribute__((always_inline)) {
                 const uint64_t upto = front + wave_upto64(own);
@@ -640,9 +737,9 @@ template <int DT, int IT> __global__ __launch_bounds__(THREADS) void sample_kern
                 in_front = lane_of(upto - own, first);
                 return static_cast<uint32_t>(block * BLOCK + first);
             };
-            const uint32_t first = orders_of_pair(DT == AXHIP_DTYPE_BF16 ? f32_to_bf16_bits(top) : f32_to_f16_bits(top)) & 0xFFFFu; // the largest's
+            const uint32_t first = order_of16(DT == AXHIP_DTYPE_BF16 ? f32_to_bf16_bits(top) : f32_to_f16_bits(top)); // the largest's
             uint64_t front, in_front;
-            const uint32_t lowest = (orders_of_pair(DT == AXHIP_DTYPE_BF16 ? f32_to_bf16_bits(r.floor) : f32_to_f16_bits(r.floor)) & 0xFFFFu) + 1; // (the floor, rounded)
+            const uint32_t lowest = order_of16(DT == AXHIP_DTYPE_BF16 ? f32_to_bf16_bits(r.floor) : f32_to_f16_bits(r.floor)) + 1; // (the floor, rounded)
             uint32_t last = min(lowest, FIRST_ORDER<DT> + DRAWN_ORDERS<DT> - 1), ties = ~0u; // kept: orders up to `last`, and of that one so many, by index
             if (k) {
                 const uint64_t than = static_cast<uint64_t>(k - 1);
@@ -653,22 +750,25 @@ template <int DT, int IT> __global__ __launch_bounds__(THREADS) void sample_kern
                 }
             }
             if (p < 1.0f) {
-                auto kept_mass = [&](uint32_t order, uint32_t count) __attribute__((always_inline)) {
-                    const uint32_t c = order < last ? count : order == last ? min(count, ties) : 0u;
-                    return c ? c * r.mass(logit_of16<DT>(order)) : uint64_t(0);
-                };
-                clear_bins(sh);
-                each_block_pair([&](int block, uint32_t w, uint32_t order) __attribute__((always_inline)) {
-                    const uint64_t sum = sum32(kept_mass(order, w & 0xFFFFu) + kept_mass(order + 1, w >> 16));
-                    if (lane % 32 == 0) sh.bins[block] = sum;
-                });
-                __syncthreads();
+                const auto kept_mass = masses_of(last, ties);
+                if (k) {
+                    clear_bins(sh);
+                    sum_blocks([&](uint32_t c0, uint32_t c1, uint32_t order, uint64_t &first, uint64_t &second) __attribute__((always_inline)) {
+                        first = kept_mass(order, c0);
+                        second = kept_mass(order + 32768, c1);
+                    });
+                    __syncthreads();
+                }
                 const uint64_t than = than_of_p([&] { return sum_of_bins(sh); });
                 const int block = find_bin(sh, 0, than, front);
                 if (block >= 0) {
                     const uint32_t order = block * BLOCK + lane;
                     last = find_value(block, front, than, kept_mass(order, count_at(order)), in_front);
-                    ties = static_cast<uint32_t>((than - in_front) / r.mass(logit_of16<DT>(last))) + 1;
+                    const uint64_t each_of_them = r.mass(logit_of16<DT>(last)), reached = than - in_front;
+                    ties = static_cast<uint32_t>(static_cast<double>(reached) / static_cast<double>(each_of_them)); // (to within one)
+                    if (ties * each_of_them > reached) --ties;
+                    else if ((ties + 1) * each_of_them <= reached) ++ties;
+                    ++ties;
                 }
             }
             // Of the last value only the first `ties` by index are kept: its logits carry no weight but a mark, and their share is added when the steps' numbers of
@@ -680,7 +780,7 @@ template <int DT, int IT> __global__ __launch_bounds__(THREADS) void sample_kern
             // (weights of logits between two small ones of either sign are the same integer: one entry of the table for all of them, which lets it reach negative bfloat16 logits)
             uint32_t zone = values, gap = 0; // entries zone .. zone + gap are one
             if (DT == AXHIP_DTYPE_BF16 && values >= LIST) {
-                const uint32_t small = orders_of_pair(f32_to_bf16_bits(temperature * 7.105427357601002e-15f)) & 0xFFFFu; // 2^-47 temperatures
+                const uint32_t small = order_of16(f32_to_bf16_bits(temperature * 7.105427357601002e-15f)); // 2^-47 temperatures
                 const uint32_t end = 0xFFFEu - small;                                                                       // ... and as much below zero
                 if (small > first && end < last) {
                     zone = small - first;
@@ -688,31 +788,32 @@ template <int DT, int IT> __global__ __launch_bounds__(THREADS) void sample_kern
                 }
             }
             const uint32_t entries = values - gap;
+            // of two logits, `values` where they are not kept (orders in front of the first, of NaNs, come out beyond it)
+            auto place_of = [&](uint32_t w) __attribute__((always_inline)) {
+                return __builtin_elementwise_min(orders_of(w) - static_cast<uint16_t>(first), pair_t{static_cast<uint16_t>(values), static_cast<uint16_t>(values)});
+            };
             if (entries < LIST) {
                 for (uint32_t i = t; i <= entries; i += THREADS)
                     sh.weights[i] = i == entries ? 0 : in_part && i == entries - 1 ? MARK : r.mass_of_least(logit_of16<DT>(first + (i > zone ? i + gap : i)));
                 if (gap == 0) {
-                    draw_by_steps(each_step, of_last, ties, [&](const Step<DT> &s, uint32_t, uint64_t(&x)[E]) __attribute__((always_inline)) { // (a barrier in front of the loop)
+                    draw_by_steps(std::true_type{}, of_last, ties, [&](const Step<DT> &s, uint32_t, uint64_t(&x)[E]) __attribute__((always_inline)) { // (a barrier in front of the loop)
 #pragma unroll
-                        for (int e = 0; e < E; ++e) {
-                            const uint32_t pair = orders_of_pair(s.v[0][e / 2]);
-                            x[e] = sh.weights[min((e % 2 ? pair >> 16 : pair & 0xFFFFu) - first, values)];
-                        }
+                        for (int e = 0; e < E; ++e) x[e] = sh.weights[place_of(s.v[0][e / 2])[e % 2]];
                     });
                 } else {
-                    draw_by_steps(each_step, of_last, ties, [&](const Step<DT> &s, uint32_t, uint64_t(&x)[E]) __attribute__((always_inline)) {
+                    draw_by_steps(std::true_type{}, of_last, ties, [&](const Step<DT> &s, uint32_t, uint64_t(&x)[E]) __attribute__((always_inline)) {
 #pragma unroll
                         for (int e = 0; e < E; ++e) {
-                            const uint32_t pair = orders_of_pair(s.v[0][e / 2]), i = min((e % 2 ? pair >> 16 : pair & 0xFFFFu) - first, values);
+                            const uint32_t i = place_of(s.v[0][e / 2])[e % 2];
                             x[e] = sh.weights[i <= zone ? i : i - min(i - zone, gap)];
                         }
                     });
                 }
             } else {
-                draw_by_steps(each_step_of_memory, of_last, ties, [&](const Step<DT> &s, uint32_t, uint64_t(&x)[E]) __attribute__((always_inline)) {
+                draw_by_steps(std::false_type{}, of_last, ties, [&](const Step<DT> &s, uint32_t, uint64_t(&x)[E]) __attribute__((always_inline)) {
 #pragma unroll
                     for (int e = 0; e < E; ++e) {
-                        const uint32_t pair = orders_of_pair(s.v[0][e / 2]), i = (e % 2 ? pair >> 16 : pair & 0xFFFFu) - first;
+                        const uint32_t i = place_of(s.v[0][e / 2])[e % 2];
                         const float v = element<DT>(s, e);
                         x[e] = v >= r.floor && i < values ? in_part && i == values - 1 ? MARK : r.mass_of_least(v) : 0;
                     }
@@ -792,7 +893,7 @@ template <int DT, int IT> __global__ __launch_bounds__(THREADS) void sample_kern
         });
         return;
     }
-    draw_by_steps(each_step_of_memory, 0, 0, [&](const Step<DT> &s, uint32_t at, uint64_t(&x)[E]) __attribute__((always_inline)) {
+    draw_by_steps(std::false_type{}, 0, 0, [&](const Step<DT> &s, uint32_t at, uint64_t(&x)[E]) __attribute__((always_inline)) {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             const float v = element<DT>(s, e);
