@@ -35,6 +35,7 @@ struct SampleShared {
     uint64_t block_mass[BLOCKS];
     uint64_t few_place[FEW], few_value[FEW];
     uint64_t scratch[WAVES + 2], other_scratch[WAVES];
+    double pow2[32];
     float top[WAVES];
     uint32_t where[WAVES], few, front, inside;
     union {
@@ -82,6 +83,15 @@ __device__ __forceinline__ uint64_t wave_upto64(uint64_t v) { // of the lanes up
     v += dpp64<0x118>(v);
     v += dpp64<0x142, 0xA>(v); // the row in front, to rows 1 and 3
     return v + dpp64<0x143, 0xC>(v); // the first half, to the second
+}
+template <int CTRL, int ROWS = 0xF> __device__ __forceinline__ uint32_t dpp32(uint32_t v) { return __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xF, false); }
+__device__ __forceinline__ uint32_t wave_upto32(uint32_t v) {
+    v += dpp32<0x111>(v);
+    v += dpp32<0x112>(v);
+    v += dpp32<0x114>(v);
+    v += dpp32<0x118>(v);
+    v += dpp32<0x142, 0xA>(v);
+    return v + dpp32<0x143, 0xC>(v);
 }
 __device__ __forceinline__ uint64_t lane_of(uint64_t v, int lane) {
     return static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(v >> 32)), lane))) << 32 |
@@ -168,6 +178,8 @@ template <int DT> struct Row {
     double base = 0.0;     // ... or the largest finite number
     double rate = 0.0;     // log2(e) / temperature
     float floor = 0.0f;    // from here on weights may be more than nothing
+    float lowest = 0.0f, highest = 0.0f; // finite bounds of what powers are formed of
+    const double *pow2 = nullptr; // 2^43 2^(i / 32)
     uint64_t last = ~0ull; // kept: up to this one in the order,
     double least = 0.0;    // and with at least this weight
 
@@ -193,30 +205,33 @@ template <int DT> struct Row {
     }
     __device__ __forceinline__ int steps() const { return (vocab + STEP - 1) / STEP; }
 
-    // log2 of the weight, within [-64, 0].  (An infinite largest logit: `base` is the largest finite number, and only infinities are asked for.)
-    __device__ __forceinline__ double power(float v) const { return fmin(fmax((static_cast<double>(v) - base) * rate, -64.0), 0.0); }
-    // exp((v - top) / temperature) in multiples of 2^-43: 2^z with z = i + r, |r| <= 1/2, by a polynomial through the Chebyshev points of 2^r, off by less than 5e-15 of the weight
-    // (a table of 2^(i / 256) and four terms waited longer for LDS than the six terms more take).
+    // log2 of the weight, 0 at most and -90 at least: logits below the floor count as the floor (NaN too), an infinite one as the largest finite number.
+    __device__ __forceinline__ double power(float v) const { return (static_cast<double>(__builtin_amdgcn_fmed3f(v, lowest, highest)) - base) * rate; }
+    // exp((v - top) / temperature) in multiples of 2^-43: 2^z with z = i / 32 + r, |r| <= 1/64: 2^(i / 32) from a table in LDS (of 64 banks: no two lanes wait for each
+    // other), with the power of two put into its exponent, and five terms of 2^r, which leave less than 3e-15 of the weight.  (Operations of 64 bits take a wavefront eight
+    // cycles, others four: eleven terms and no table took a fifth longer.)
     __device__ __forceinline__ double scaled_weight(double z) const {
-        constexpr double SPLIT = 6755399441055744.0; // 1.5 * 2^52: its last bit is 1
+        constexpr double SPLIT = 211106232532992.0; // 1.5 * 2^47: its last bit is 1/32
         const double t = z + SPLIT, r = z - (t - SPLIT);
         const uint32_t i = static_cast<uint32_t>(__double_as_longlong(t));
-        double p = 6.422412339320131e-09;
-        p = __builtin_fma(r, p, 1.02053706737851e-07);
-        p = __builtin_fma(r, p, 1.3219110032865315e-06);
-        p = __builtin_fma(r, p, 1.5252674086943783e-05);
-        p = __builtin_fma(r, p, 0.00015403523472909156);
-        p = __builtin_fma(r, p, 0.0013333558203519715);
-        p = __builtin_fma(r, p, 0.00961812911264106);
-        p = __builtin_fma(r, p, 0.05550410866458426);
-        p = __builtin_fma(r, p, 0.2402265069589931);
-        p = __builtin_fma(r, p, 0.6931471805599488);
+        const uint64_t power_of_two = static_cast<uint64_t>(__double_as_longlong(pow2[i & 31])) + (static_cast<uint64_t>((i & ~31u) << 15) << 32);
+        double p = 0.0013333558146428443;
+        p = __builtin_fma(r, p, 0.009618129107628477);
+        p = __builtin_fma(r, p, 0.05550410866482158);
+        p = __builtin_fma(r, p, 0.2402265069591007);
+        p = __builtin_fma(r, p, 0.6931471805599453);
         p = __builtin_fma(r, p, 1.0);
-        return __longlong_as_double(__double_as_longlong(p) + (static_cast<long long>(static_cast<uint64_t>(i + 43u) << 52)));
+        return __longlong_as_double(static_cast<long long>(power_of_two)) * p;
     }
     static __device__ __forceinline__ uint64_t integer(double w) {
         constexpr double TO_INTEGER = 4503599627370496.0; // 2^52: the integer is what its last bits say
         return static_cast<uint64_t>(__double_as_longlong(w + TO_INTEGER)) & ((uint64_t(1) << 52) - 1);
+    }
+    // (formed for all lanes, eight chains at a time, whether or not a lane's is used: behind a branch each would wait for the one before)
+    static __device__ __forceinline__ uint64_t formed(uint64_t x) {
+        uint32_t lo = static_cast<uint32_t>(x), hi = static_cast<uint32_t>(x >> 32);
+        asm("" : "+v"(lo), "+v"(hi));
+        return static_cast<uint64_t>(hi) << 32 | lo;
     }
     __device__ __forceinline__ uint64_t mass(float v) const { return integer(scaled_weight(power(v))); }
     __device__ __forceinline__ uint64_t mass_of_least(float v) const { // ... 0 below min_p
@@ -371,17 +386,17 @@ template <int DT, int IT> __global__ __launch_bounds__(THREADS) void sample_kern
         if (i * WAVES + wave < steps) held[i] = r.load(i * WAVES + wave);
     // f(vectors, index of the first, step) for the wavefront's steps, from memory with the next ones' loads in flight
     auto each_step_of_memory = [&](auto f) __attribute__((always_inline)) {
-        constexpr int AHEAD = 3;
+        constexpr int AHEAD = 2; // (sets of registers of their own: moved from one to the next, every load would be waited for)
         Step<DT> next[AHEAD];
 #pragma unroll
         for (int d = 0; d < AHEAD; ++d) next[d] = r.load(min(wave + d * WAVES, steps - 1));
 #pragma unroll 1
-        for (int step = wave; step < steps; step += WAVES) {
-            const Step<DT> s = next[0];
+        for (int step = wave; step < steps; step += AHEAD * WAVES) {
 #pragma unroll
-            for (int d = 0; d + 1 < AHEAD; ++d) next[d] = next[d + 1];
-            next[AHEAD - 1] = r.load(min(step + AHEAD * WAVES, steps - 1));
-            f(s, static_cast<uint32_t>(step * STEP + lane * E), step);
+            for (int d = 0; d < AHEAD; ++d) {
+                if (step + d * WAVES < steps) f(next[d], static_cast<uint32_t>((step + d * WAVES) * STEP + lane * E), step + d * WAVES);
+                next[d] = r.load(min(step + (d + AHEAD) * WAVES, steps - 1));
+            }
         }
     };
     // ... from the registers, for passes of few instructions.  (The compiler is not to see that a later pass forms the same numbers of the same vectors: it would keep them all.)
@@ -415,6 +430,8 @@ template <int DT, int IT> __global__ __launch_bounds__(THREADS) void sample_kern
     const float p = a.top_p ? a.top_p[row] : 1.0f, m = a.min_p ? a.min_p[row] : 0.0f, u = a.u[row];
     const int32_t k = a.top_k && a.top_k[row] > 0 && a.top_k[row] < a.vocab ? a.top_k[row] : 0;
     if (t == 0) sh.front = sh.inside = 0;
+    if (t < 32) sh.pow2[t] = exp2(43.0 + t * (1.0 / 32.0)); // (a barrier before they are used)
+    r.pow2 = sh.pow2;
     sh.bins[t] = 0;
     sh.bins[t + THREADS] = 0;
 
@@ -460,6 +477,8 @@ template <int DT, int IT> __global__ __launch_bounds__(THREADS) void sample_kern
     r.rate = 1.4426950408889634 / static_cast<double>(temperature);
     r.floor = fmaxf(top - static_cast<float>(REACH) * temperature, -LARGEST); // (NaN, of an infinite logit and temperature: everything finite)
     if (top > LARGEST) r.floor = top;                                         // (only its equals)
+    r.lowest = fminf(r.floor, LARGEST);
+    r.highest = fminf(top, LARGEST);
     const double least = m > 0.0f ? (m < 1.0f ? static_cast<double>(m) : 1.0) * static_cast<double>(ONE) : 0.0;
     r.least = least;
 
@@ -469,9 +488,17 @@ template <int DT, int IT> __global__ __launch_bounds__(THREADS) void sample_kern
             uint32_t kinds = 0; // two bits an element
 #pragma unroll
             for (int e = 0; e < E; ++e) kinds |= taken(element<DT>(s, e), at + e) << (2 * e);
+            if (__ballot(kinds != 0) == 0) return;
+            // places: one addition for the wavefront, and what the lanes in front have of either kind
+            const uint32_t own = __builtin_popcount(kinds & 0x5555u) | static_cast<uint32_t>(__builtin_popcount(kinds & 0xAAAAu)) << 16;
+            const uint32_t upto = wave_upto32(own), all = __builtin_amdgcn_readlane(upto, WAVE - 1);
+            uint32_t f0 = 0, i0 = 0;
+            if (lane == 0) {
+                if (all & 0xFFFFu) f0 = take_from(sh.front, all & 0xFFFFu);
+                if (all >> 16) i0 = take_from(sh.inside, all >> 16);
+            }
+            uint32_t f = __builtin_amdgcn_readfirstlane(f0) + ((upto - own) & 0xFFFFu), i = FRONT + __builtin_amdgcn_readfirstlane(i0) + ((upto - own) >> 16);
             if (kinds) {
-                const uint32_t ones = __builtin_popcount(kinds & 0x5555u), twos = __builtin_popcount(kinds & 0xAAAAu);
-                uint32_t f = ones ? take_from(sh.front, ones) : 0, i = twos ? FRONT + take_from(sh.inside, twos) : 0;
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     const uint32_t kind = (kinds >> (2 * e)) & 3u, to = kind == 1 ? f : i;
@@ -710,10 +737,15 @@ template <int DT, int IT> __global__ __launch_bounds__(THREADS) void sample_kern
         };
         static_assert(BLOCKS / 2 % (WAVES * 8) == 0 && BLOCK == WAVE && BLOCKS <= BINS, "whole rounds, a value to a lane, and a bin for a block");
         uint32_t counted = 0;
+        auto weight_of = [&](uint32_t order) __attribute__((always_inline)) { // (nothing below the floor: an infinite largest logit's is itself)
+            const float v = logit_of16<DT>(order);
+            return v >= r.floor ? r.mass_of_least(v) : uint64_t(0);
+        };
         auto masses_of = [&](uint32_t last, uint32_t ties) __attribute__((always_inline)) {
             return [&r, last, ties](uint32_t order, uint32_t count) __attribute__((always_inline)) {
                 const uint32_t c = order < last ? count : order == last ? min(count, ties) : 0u;
-                return c ? c * r.mass(logit_of16<DT>(order)) : uint64_t(0);
+                const float v = logit_of16<DT>(order);
+                return c && v >= r.floor ? c * r.mass(v) : uint64_t(0);
             };
         };
         if (k) {
@@ -773,7 +805,7 @@ template <int DT, int IT> __global__ __launch_bounds__(THREADS) void sample_kern
             }
             // Of the last value only the first `ties` by index are kept: its logits carry no weight but a mark, and their share is added when the steps' numbers of
             // marks are known.
-            const uint64_t of_last = filtered && ties < count_at(last) ? r.mass_of_least(logit_of16<DT>(last)) : 0;
+            const uint64_t of_last = filtered && ties < count_at(last) ? weight_of(last) : 0;
             const bool in_part = of_last != 0; // (those that weigh nothing need no marks)
             const uint32_t values = last - first + 1;
             __syncthreads(); // (the counts make room for the weights)
@@ -794,7 +826,7 @@ template <int DT, int IT> __global__ __launch_bounds__(THREADS) void sample_kern
             };
             if (entries < LIST) {
                 for (uint32_t i = t; i <= entries; i += THREADS)
-                    sh.weights[i] = i == entries ? 0 : in_part && i == entries - 1 ? MARK : r.mass_of_least(logit_of16<DT>(first + (i > zone ? i + gap : i)));
+                    sh.weights[i] = i == entries ? 0 : in_part && i == entries - 1 ? MARK : weight_of(first + (i > zone ? i + gap : i));
                 if (gap == 0) {
                     draw_by_steps(std::true_type{}, of_last, ties, [&](const Step<DT> &s, uint32_t, uint64_t(&x)[E]) __attribute__((always_inline)) { // (a barrier in front of the loop)
 #pragma unroll
@@ -815,7 +847,8 @@ template <int DT, int IT> __global__ __launch_bounds__(THREADS) void sample_kern
                     for (int e = 0; e < E; ++e) {
                         const uint32_t i = place_of(s.v[0][e / 2])[e % 2];
                         const float v = element<DT>(s, e);
-                        x[e] = v >= r.floor && i < values ? in_part && i == values - 1 ? MARK : r.mass_of_least(v) : 0;
+                        const uint64_t mass = r.formed(r.mass_of_least(v));
+                        x[e] = v >= r.floor && i < values ? in_part && i == values - 1 ? MARK : mass : 0;
                     }
                 });
             }
@@ -836,11 +869,19 @@ template <int DT, int IT> __global__ __launch_bounds__(THREADS) void sample_kern
             return;
         }
         clear_bins(sh);
-        each_of(each_step_of_memory, [&](float v, uint32_t i) {
-            if (r.counts(v, i)) {
-                const double z = r.power(v);
-                add_to_bin(sh.bins[r.bin_of_power(z)], value(z));
+        each_step_of_memory([&](const Step<DT> &s, uint32_t at, int) __attribute__((always_inline)) {
+            uint64_t x[E];
+            uint32_t bins[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const double z = r.power(element<DT>(s, e));
+                x[e] = r.formed(value(z));
+                bins[e] = r.bin_of_power(z);
+                asm("" : "+v"(bins[e]));
             }
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (r.counts(element<DT>(s, e), at + e)) add_to_bin(sh.bins[bins[e]], x[e]);
         });
         __syncthreads();
         const uint64_t than = than_of([&] { return sum_of_bins(sh); });
@@ -897,7 +938,8 @@ template <int DT, int IT> __global__ __launch_bounds__(THREADS) void sample_kern
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             const float v = element<DT>(s, e);
-            x[e] = r.counts(v, at + e) ? r.mass_of_least(v) : 0;
+            const uint64_t mass = r.formed(r.mass_of_least(v));
+            x[e] = r.counts(v, at + e) ? mass : 0;
         }
     });
 }

@@ -147,3 +147,68 @@ def test_the_same_call_gives_the_same_tokens_and_no_probabilities_are_asked_for(
         assert np.array_equal(tokens, again) and np.array_equal(probs, p)
     again, p = q8.sample(logits, "bf16", u, want_probs=False, **settings)
     assert np.array_equal(tokens, again) and p is None
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("values", [1, 2, 3])
+def test_more_than_65535_equal_logits(dt, values):
+    gen = torch.Generator()
+    gen.manual_seed(values)
+    vocab = 140003 if values < 3 else 230001
+    logits = torch.randint(0, values, (4, vocab), generator=gen).to(q8.DTYPES[dt][1]).cuda()
+    u = torch.rand(4, generator=gen)
+    check(logits, dt, u, top_p=[0.2, 0.618, 0.9, 0.98])
+    check(logits, dt, u, top_k=[700, 70000, 100001, vocab - 1])
+    check(logits, dt, u, top_k=[700, 70000, 100001, vocab - 1], top_p=0.71)
+    check(logits, dt, u, temperature=0.5, min_p=0.3)
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("vocab", [4000, 51865])
+def test_top_k_of_every_size(dt, vocab):
+    ks = [2, 64, 127, 128, 129, 300, 511, 512, 513, 1024, 3000, vocab // 2, vocab - 1, vocab, vocab + 7, 2**31 - 1]
+    logits, u = logits_of(vocab + 1, len(ks), vocab, dt)
+    check(logits, dt, u, top_k=ks)
+    check(logits, dt, u, top_k=ks, top_p=0.93, temperature=1.5)
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("scale", [1e-4, 0.02, 0.3, 40.0, 3000.0])
+@pytest.mark.parametrize("shift", [0.0, -500.0, 3000.0])
+def test_flat_and_steep_logits(dt, scale, shift):
+    """From rows whose every token is as likely as any other to rows with one that is; far from zero, where the type leaves few values."""
+    logits, u = logits_of(5, 6, 30000, dt, scale)
+    logits = (logits.float() + shift).clamp(-6e4, 6e4).to(logits.dtype)
+    check(logits, dt, u)
+    check(logits, dt, u, top_p=[0.1, 0.5, 0.9, 0.95, 0.99, 0.9999])
+    check(logits, dt, u, top_p=[0.1, 0.5, 0.9, 0.95, 0.99, 0.9999], temperature=[0.05, 0.3, 3.0, 20.0, 500.0, 1.0], min_p=0.001)
+    check(logits, dt, u, top_k=[1, 10, 100, 500, 5000, 29999], temperature=[0.05, 0.3, 3.0, 20.0, 500.0, 1.0])
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_the_largest_vocabulary(dt):
+    logits, u = logits_of(7, 2, 1 << 20, dt)
+    check(logits, dt, u)
+    check(logits, dt, u, top_k=[40, 2000], top_p=0.9)
+    check(logits, dt, u, top_p=[0.6, 0.97])
+
+
+def test_many_short_rows():
+    logits, u = logits_of(8, 3000, 37, "bf16")
+    check(logits, "bf16", u, top_k=9, top_p=0.8)
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+def test_masked_halves_and_infinities_under_every_filter(dt):
+    """Rows of 60000 of which most are masked by -inf, NaN or the lowest number, and rows with infinite logits."""
+    logits, u = logits_of(9, 6, 60000, dt)
+    lowest = torch.finfo(logits.dtype).min
+    logits[0, 100:] = -float("inf")
+    logits[1, :59900] = float("nan")
+    logits[2, 50:] = lowest
+    logits[3, ::2] = float("nan")
+    logits[4, [7, 50000, 59999]] = float("inf")
+    logits[5] = lowest
+    for settings in ({}, dict(top_k=3), dict(top_k=700), dict(top_p=0.9), dict(min_p=0.2), dict(top_k=1000, top_p=0.7, min_p=0.01)):
+        tokens = check(logits, dt, u, temperature=0.8, **settings)
+        assert tokens[0] < 100 and tokens[1] >= 59900 and tokens[2] < 50 and tokens[3] % 2 == 1 and tokens[4] in (7, 50000, 59999)
