@@ -1,6 +1,5 @@
 // Products of int8 rows with scales: axhip_gemm_q8.
-#include "gemm_q8.hpp"
-#include "gemm_skinny.hpp"
+#include "gemm_q8_device.hpp"
 
 #include <algorithm>
 #include <utility>
@@ -35,10 +34,9 @@ __global__ __launch_bounds__(256) void gemm_q8_generic_kernel(const GenericArgs 
     }
     const int64_t m = m0 + ty, n = n0 + tx;
     if (m < g.M && n < g.N) {
-        float y = static_cast<float>(acc) * (g.scale_a[m] * g.scale_b[n]);
-        if (g.bias) y += load_any(g.bias, g.dtype, n);
+        float y = q8_scaled(acc, g.scale_a[m], g.scale_b[n], g.bias ? load_any(g.bias, g.dtype, n) : 0.0f);
         if (g.residual) y += load_any(g.residual, g.dtype, m * g.ldc + n);
-        store_any(g.c, g.dtype, m * g.ldc + n, gemm_epilogue(g.epilogue, y));
+        store_any(g.c, g.dtype, m * g.ldc + n, g.dtype == AXHIP_DTYPE_F32 ? gemm_epilogue(g.epilogue, y) : gemm_epilogue16(g.epilogue, y));
     }
 }
 
@@ -111,9 +109,10 @@ template <size_t... I> const Q8Kernel *choose(const AxhipGemmQ8Params &p, bool a
 int launch_chosen(const Q8Args &g, const AxhipGemmQ8Params &p, bool aligned, hipStream_t s) {
     // One or two rows of x: the weights are read once, along k (1 x 4096 x 4096 5.2 us, on the small kernels 5.4; 1 x 1280 x 5120 4.1 and 5.3; of three rows and more the small
     // ones take less).  Two rows of W to a wavefront where k is short (51865 x 1280 15.8 -> 11.9 us) or x has two and W is large (2 x 16384 x 16384 52.7 -> 48.2).
-    if (p.m <= 2) {
+    const int rows_per_wave = p.k < 2048 || (p.m == 2 && p.n * p.k >= int64_t(1) << 26) ? 2 : 1;
+    if (p.m <= 2 && launch_fits((p.n + 4 * rows_per_wave - 1) / (4 * rows_per_wave), 256)) { // (vocabularies of 2^26 and more go on)
         q8_last_kernel = "skinny";
-        return launch_q8_skinny(g, p.dtype, p.k < 2048 || (p.m == 2 && p.n * p.k >= int64_t(1) << 26) ? 2 : 1, s);
+        return launch_q8_skinny(g, p.dtype, rows_per_wave, s);
     }
     const Q8Kernel *k = choose(p, aligned, std::make_index_sequence<Q8_CANDIDATES>{});
     AXHIP_REQUIRE(k != nullptr, AXHIP_ERR_UNSUPPORTED, "axhip_gemm_q8: too many tiles");

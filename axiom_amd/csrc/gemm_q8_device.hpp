@@ -25,14 +25,17 @@ __device__ __forceinline__ int4_t q8_mfma(const uint4_t &fb, const uint4_t &fa, 
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(int4_t, fb), __builtin_bit_cast(int4_t, fa), acc, 0, 0, 0);
 }
 
+// A sum with its scales and bias.  Every kernel rounds here, in this order (the sum to fp32, the scales' product, the whole once), then adds the residual, so that a row's results
+// have the same bits whichever kernel the other rows lead to.
+__device__ __forceinline__ float q8_scaled(int sum, float sa, float sb, float bias) { return __builtin_fmaf(static_cast<float>(sum), sa * sb, bias); }
+
 // N sums of row `row` from column `col` on, of which columns [first, last) exist, to C: scales (scale_b's in sb, bias in b), residual, activation.
-// Sums of up to 2^31 round to fp32 here, once; DT's rounding is the last.
 template <int DT, int N>
 __device__ __forceinline__ void q8_finish(const Q8Args &g, const int (&sum)[N], float sa, const float (&sb)[N], const float (&b)[N], int64_t at, int first, int last) {
     const bool whole = first == 0 && last == N;
     float x[N];
 #pragma unroll
-    for (int e = 0; e < N; ++e) x[e] = __builtin_fmaf(static_cast<float>(sum[e]), sa * sb[e], b[e]);
+    for (int e = 0; e < N; ++e) x[e] = q8_scaled(sum[e], sa, sb[e], b[e]);
     if (g.residual) {
         if (whole) {
             float r[N];
@@ -57,27 +60,28 @@ __device__ __forceinline__ void q8_finish(const Q8Args &g, const int (&sum)[N], 
 
 // What the epilogue of a wavefront's MB blocks of 16 x 64 needs of A's and B's rows, requested while the last products are still under way.
 template <int DT, int MB> struct Q8Scales {
-    float sa[MB], sb[8], b[8]; // of rows 16 i + lane % 16, of the eight columns from 8 (lane & 7) on
+    float sa[MB], sb[4][4], b[4][4]; // as the sums lie: of rows 16 i + lane % 16, of columns 16 j + 4 (lane / 16) + e
     __device__ __forceinline__ void load(const Q8Args &g, int m_base, int n_base, int lane) {
 #pragma unroll
         for (int i = 0; i < MB; ++i) sa[i] = g.scale_a[min(m_base + 16 * i + lane % 16, g.M - 1)];
-        const int col = n_base + 8 * (lane & 7);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            sb[e] = col + e < g.N ? g.scale_b[col + e] : 0.0f;
-            b[e] = g.bias && col + e < g.N ? Elem<DT>::load(g.bias, col + e) : 0.0f;
+        for (int j = 0; j < 4; ++j) {
+            const int col = n_base + 16 * j + 4 * (lane / 16);
+            if (col + 4 <= g.N) {
+                load_vec<4, true>(g.scale_b, AXHIP_DTYPE_F32, col, sb[j]);
+                if (g.bias) load_vec<4, true>(g.bias, DT, col, b[j]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    sb[j][e] = col + e < g.N ? g.scale_b[col + e] : 0.0f;
+                    if (g.bias) b[j][e] = col + e < g.N ? Elem<DT>::load(g.bias, col + e) : 0.0f;
+                }
+            }
+            if (!g.bias) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) b[j][e] = 0.0f;
+            }
         }
-    }
-    template <int MP> __device__ __forceinline__ Q8Scales<DT, MP> part(int first) const { // blocks first .. first + MP - 1
-        Q8Scales<DT, MP> p;
-#pragma unroll
-        for (int i = 0; i < MP; ++i) p.sa[i] = sa[first + i];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            p.sb[e] = sb[e];
-            p.b[e] = b[e];
-        }
-        return p;
     }
 };
 
@@ -115,20 +119,20 @@ template <int DT, int MB> struct Q8Residual {
     }
 };
 
-// The wavefront's MB blocks of 16 x 64 sums -> C, through its own LDS (`stage`, 4 KiB per block), so that a lane holds eight consecutive columns of a
-// row: whole 128-byte lines per store, and one short loop of code.  In that loop nothing is loaded from memory: A's scales are multiplied in
+// Blocks first .. first + MP - 1 of the wavefront's sums of 16 x 64 -> C, through its own LDS (`stage`, 4 KiB per block), so that a lane holds eight consecutive columns of a
+// row: whole 128-byte lines per store, and one short loop of code.  In that loop nothing is loaded from memory: scales and bias are taken
 // on the way to LDS, and the residual (`res`, requested before the last products are over) is added to what lies there; then `behind` requests the next blocks' residual, which
 // arrives while these are written (row by row, each waited for the one before: 8192 x 4096 x 128 with a residual took 60 us, 26 without).
-template <int DT, int MB, class F>
-__device__ __forceinline__ void q8_store_blocks(const Q8Args &g, const int4_t (&own)[MB][4], Q8Scales<DT, MB> s, const Q8Residual<DT, MB> &res, int m_base, int n_base, int lane, unsigned char *stage, F behind) {
+template <int DT, int MB, int MP, class F>
+__device__ __forceinline__ void q8_store_blocks(const Q8Args &g, const int4_t (&own)[MB][4], int first, const Q8Scales<DT, MB> &s, const Q8Residual<DT, MP> &res, int m_base, int n_base, int lane, unsigned char *stage, F behind) {
     const int l16 = lane % 16, g4 = lane / 16;
 #pragma unroll
-    for (int i = 0; i < MB; ++i)
+    for (int i = 0; i < MP; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             float4_t v;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = static_cast<float>(own[i][j][e]) * s.sa[i]; // (sums of up to 2^31 round to fp32 here)
+            for (int e = 0; e < 4; ++e) v[e] = q8_scaled(own[first + i][j][e], s.sa[first + i], s.sb[j][e], s.b[j][e]);
             *reinterpret_cast<float4_t *>(stage + (16 * i + l16) * 256 + (((4 * j + g4) ^ l16) * 16)) = v;
         }
     wave_lds_fence();
@@ -136,26 +140,21 @@ __device__ __forceinline__ void q8_store_blocks(const Q8Args &g, const int4_t (&
     auto at = [&](int r, int h) { return reinterpret_cast<float4_t *>(stage + r * 256 + (((2 * q + h) ^ (r & 15)) * 16)); };
     if (g.residual && last > 0) {
 #pragma unroll
-        for (int n = 0; n < 2 * MB; ++n) {
+        for (int n = 0; n < 2 * MP; ++n) {
             const int r = (lane >> 3) + 8 * n;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 float4_t v = *at(r, h);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(v[e], s.sb[4 * h + e], s.b[4 * h + e]) + res.at(n, 4 * h + e);
+                for (int e = 0; e < 4; ++e) v[e] += res.at(n, 4 * h + e);
                 *at(r, h) = v;
             }
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            s.sb[e] = 1.0f;
-            s.b[e] = 0.0f;
         }
     }
     behind();
     if (last <= 0) return;
 #pragma unroll 1
-    for (int r = lane >> 3; r < 16 * MB; r += 8) {
+    for (int r = lane >> 3; r < 16 * MP; r += 8) {
         const int row = m_base + r;
         if (row >= g.M) break;
         float x[8];
@@ -163,7 +162,7 @@ __device__ __forceinline__ void q8_store_blocks(const Q8Args &g, const int4_t (&
         for (int h = 0; h < 2; ++h) {
             const float4_t v = *at(r, h);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[4 * h + e] = __builtin_fmaf(v[e], s.sb[4 * h + e], s.b[4 * h + e]);
+            for (int e = 0; e < 4; ++e) x[4 * h + e] = v[e];
         }
         gemm_epilogue_all_as<DT != AXHIP_DTYPE_F32>(g.epilogue, x);
         const int64_t to = static_cast<int64_t>(row) * g.ldc + col;
@@ -177,17 +176,12 @@ __device__ __forceinline__ void q8_store_blocks(const Q8Args &g, const int4_t (&
     }
 }
 
-// ... of PIECES times MP blocks, one piece staged at a time; `res`: the first piece's residual.
+// ... all MB blocks, MP staged at a time; `res`: the first ones' residual.
 template <int DT, int MB, int MP>
 __device__ __forceinline__ void q8_store_pieces(const Q8Args &g, const int4_t (&own)[MB][4], const Q8Scales<DT, MB> &s, Q8Residual<DT, MP> &res, int m_base, int n_base, int lane, unsigned char *stage) {
 #pragma unroll
     for (int h = 0; h < MB / MP; ++h) {
-        int4_t piece[MP][4];
-#pragma unroll
-        for (int i = 0; i < MP; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) piece[i][j] = own[MP * h + i][j];
-        q8_store_blocks<DT, MP>(g, piece, s.template part<MP>(MP * h), res, m_base + 16 * MP * h, n_base, lane, stage, [&]() __attribute__((always_inline)) {
+        q8_store_blocks<DT, MB, MP>(g, own, MP * h, s, res, m_base + 16 * MP * h, n_base, lane, stage, [&]() __attribute__((always_inline)) {
             if (h + 1 < MB / MP) res.load(g, m_base + 16 * MP * (h + 1), n_base, lane);
         });
         wave_lds_fence();

@@ -41,7 +41,7 @@ __global__ __launch_bounds__(256) void gemm_q8_skinny_kernel(const Q8Args a) {
     const bool writes = lane % (64 / P) == 0 && n < a.N;
     const int64_t at = static_cast<int64_t>(value / R) * a.ldc + n;
     const float bias = writes && a.bias ? Elem<DT>::load(a.bias, n) : 0.0f, residual = writes && a.residual ? Elem<DT>::load(a.residual, at) : 0.0f;
-    const float scale = writes ? a.scale_a[value / R] * a.scale_b[n] : 0.0f;
+    const float sa = writes ? a.scale_a[value / R] : 0.0f, sb = writes ? a.scale_b[n] : 0.0f;
     int acc[M][R] = {};
     const int8_t *wrow[R];
 #pragma unroll
@@ -76,7 +76,9 @@ __global__ __launch_bounds__(256) void gemm_q8_skinny_kernel(const Q8Args a) {
 #pragma unroll
     for (int i = 0; i < P; ++i) v[i] = acc[i / R][i % R];
     const int sum = q8_lane_sums<P>(v, lane);
-    if (writes) Elem<DT>::store(a.c, at, gemm_epilogue(a.epilogue, __builtin_fmaf(static_cast<float>(sum), scale, bias) + residual));
+    float x[1] = {q8_scaled(sum, sa, sb, bias) + residual};
+    gemm_epilogue_all_as<DT != AXHIP_DTYPE_F32>(a.epilogue, x);
+    if (writes) Elem<DT>::store(a.c, at, x[0]);
 }
 
 template <int DT, int M> void launch_rows(const Q8Args &g, int rows_per_wave, hipStream_t s) {

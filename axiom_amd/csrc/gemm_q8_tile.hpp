@@ -46,7 +46,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void gemm_q8_tile_kernel(cons
     const int8_t *A = g.a + static_cast<int64_t>(m0) * g.lda, *B = g.b + static_cast<int64_t>(n0) * g.ldb;
     const int rows_a = min(TM, g.M - m0), rows_b = min(TN, g.N - n0);
 
-    constexpr int MB = MI / WK, MP = MB > 4 ? 4 : MB; // row blocks that a wavefront finishes, and stages at a time
+    // row blocks that a wavefront finishes, and stages at a time (of eight in fp32 two: their residual's registers)
+    constexpr int MB = MI / WK, MP = MB <= 4 ? MB : DT == AXHIP_DTYPE_F32 ? 2 : 4;
     Q8Scales<DT, MB> scales;
     scales.load(g, m0 + wm + wk * MB * 16, n0 + wn, lane);
 

@@ -492,8 +492,9 @@ int axhip_rms_norm_q8(const void *x, const void *residual, const void *weight, v
 /* ------------------------------------------------------- products in 8 bits
  * nn::Linear (src/nn/linear.cpp:15-27) on rows in 8 bits: C = act(scale_a[m] scale_b[n] sum_k A[m][k] B[n][k] (+ bias[n]) (+ residual)),
  * A (m, k) and B (n, k) int8, row-major, lda / ldb / ldc in elements, any alignment.  The sums are int32 and exact: k up to
- * 131071, beyond which rows of -128 could overflow (AXHIP_ERR_UNSUPPORTED).  scale_a [m] and scale_b [n] are fp32; the rest is fp32 arithmetic,
- * rounded once to dtype.  residual has C's layout and may be C itself.  No temporary memory. */
+ * 131071, beyond which rows of -128 could overflow (AXHIP_ERR_UNSUPPORTED).  scale_a [m] and scale_b [n] are fp32; the rest is fp32 arithmetic (the sum as a
+ * float times the scales' product, plus bias, rounded once; plus residual), rounded once to dtype: a row of C has the same bits whatever the other rows are and however many.
+ * residual has C's layout and may be C itself.  No temporary memory. */
 typedef struct {
     int32_t dtype;       /* of C, bias and residual: Float32, Float16 or BFloat16 */
     int32_t epilogue_op; /* 0 or AXHIP_OP_RELU / GELU / SILU / SIGMOID / TANH */
@@ -534,7 +535,7 @@ typedef struct {
 } AxhipSampleParams;
 
 int axhip_sample(const void *logits, int64_t *tokens, float *probs, const AxhipSampleParams *params_host, void *stream);
-/* The same with its temporary memory handed in by the caller (0 bytes for every shape that needs none). */
+/* The same with its temporary memory handed in by the caller.  Rows are drawn from in registers and LDS: 0 bytes for every shape, workspace may be NULL. */
 size_t axhip_sample_workspace_bytes(const AxhipSampleParams *params_host);
 int axhip_sample_ws(const void *logits, int64_t *tokens, float *probs, const AxhipSampleParams *params_host,
                     void *workspace, size_t workspace_bytes, void *stream);

@@ -266,3 +266,47 @@ def test_the_same_call_twice_and_on_another_stream():
     q0, s0 = q8.quantize(x, "bf16")
     q1, s1 = q8.quantize(x, "bf16", stream=other.cuda_stream)
     assert torch.equal(q0, q1) and torch.equal(s0, s1)
+
+
+@pytest.mark.parametrize("k", [8, 100, 1280, 2049])
+@pytest.mark.parametrize("act", [None, "gelu", "silu", "tanh"])
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+def test_a_row_has_the_same_bits_whatever_the_others(dt, act, k):
+    m, n = 1500, 1000
+    a, b, sa, sb = operands(m, n, k, dt)
+    bias, residual = normal(m, n, dt=dt), normal(n, m, n, dt=dt)
+    want, whole = q8.gemm(a, b, sa, sb, dt, bias, residual, act)
+    kernels = {whole}
+    for first, last in [(0, 1), (700, 702), (5, 8), (3, 20), (64, 128), (100, 400), (800, 1499)]:
+        rows = slice(first, last)
+        c, kernel = q8.gemm(a[rows], b, sa[rows].contiguous(), sb, dt, bias, residual[rows].contiguous(), act)
+        assert torch.equal(c, want[rows]), kernel
+        kernels.add(kernel)
+    far = a[:1].as_strided((1, k), (1 << 22, 1))  # (one row, whatever its leading dimension)
+    c, kernel = q8.gemm(far, b, sa[:1].contiguous(), sb, dt, bias, residual[:1].contiguous(), act)
+    assert kernel == "generic" and torch.equal(c, want[:1])
+    assert k < 16 or len(kernels) > 2
+
+
+@pytest.mark.parametrize("m", [1, 20, 300, 2048])
+@pytest.mark.parametrize("large,small", [(1e33, 1e-20), (1e-20, 1e33), (1e-36, 1e30), (1e36, 1e-36)])
+def test_scales_of_which_one_is_huge(m, large, small):
+    """Their product is an ordinary number; the sum times either of them is not."""
+    a, b, sa, sb = operands(m, 520, 1024, "f32")
+    sa, sb = sa * large, sb * small
+    c, _ = q8.gemm(a, b, sa, sb, "f32")
+    close(c, a, b, sa, sb, "f32")
+
+
+@pytest.mark.parametrize("m", [1, 2])
+def test_more_columns_than_one_launch_has_threads_for(m):
+    n, k = (1 << 27) + 3, 16
+    a = int8s(m, m, k)
+    b = torch.empty(n, k, dtype=torch.int8, device="cuda")
+    b.view(-1)[:] = torch.arange(16 * 4099, dtype=torch.int32, device="cuda").remainder(251).sub(125).to(torch.int8).repeat(n // 4099 + 1)[: n * k]
+    one = torch.ones(n, device="cuda")
+    c, kernel = q8.gemm(a, b, one[:m], one, "f32")
+    assert kernel != "skinny"
+    for first in (0, 1 << 20, 1 << 26, n - 5000):
+        part = slice(first, first + 5000)
+        assert torch.equal(c[:, part].cpu(), (a.cpu().int()[:, None] * b[part].cpu().int()[None]).sum(-1).float())
