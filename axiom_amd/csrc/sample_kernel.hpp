@@ -23,7 +23,7 @@ namespace {
 constexpr int THREADS = 1024, WAVES = THREADS / WAVE, E = 8; // elements of a lane's vector
 constexpr int STEP = WAVE * E;                               // consecutive elements of a wavefront's step
 constexpr int BINS = 2048, FEW = 128;
-constexpr int DIRECT = 128, FEW_LOGITS = 1024, SMALL_K = 512;
+constexpr int FEW_LOGITS = 1024, SMALL_K = 512;
 constexpr int LIST = 16384, FRONT = 12288; // of which this many for what lies in front of the bin
 constexpr int BLOCK = 64, BLOCKS = 65536 / BLOCK; // 16-bit values are summed up by blocks
 static_assert(MOST_VOCAB <= int64_t(BINS) * STEP, "a bin for a step");
@@ -307,6 +307,68 @@ __device__ __forceinline__ void smallest_and_largest(SampleShared &sh, uint64_t 
     __syncthreads();
 }
 
+// The number of the lane D away (D a power of two).
+template <int D> __device__ __forceinline__ uint64_t lane_across(uint64_t v, int lane) {
+    if constexpr (D == 1) return dpp64<0xB1>(v); // (quad_perm)
+    else if constexpr (D == 2) return dpp64<0x4E>(v);
+    else if constexpr (D == 4) return dpp64<0x1B>(dpp64<0x141>(v)); // (7 away, 3 away)
+    else if constexpr (D == 8) return dpp64<0x128>(v);
+    else {
+        const uint32_t low = static_cast<uint32_t>(v), high = static_cast<uint32_t>(v >> 32);
+        const auto lo = D == 16 ? __builtin_amdgcn_permlane16_swap(low, low, false, false) : __builtin_amdgcn_permlane32_swap(low, low, false, false);
+        const auto hi = D == 16 ? __builtin_amdgcn_permlane16_swap(high, high, false, false) : __builtin_amdgcn_permlane32_swap(high, high, false, false);
+        return lane & D ? static_cast<uint64_t>(hi[0]) << 32 | lo[0] : static_cast<uint64_t>(hi[1]) << 32 | lo[1];
+    }
+}
+// Numbers, one to a thread of the first `waves` wavefronts (a power of two), the smallest to the first thread and so on: a bitonic sort, by exchanges between lanes where they are of
+// one wavefront and through LDS (`room`, two numbers a thread) where not.  Called by the whole work-group.
+__device__ __forceinline__ uint64_t sorted(uint64_t *room, uint64_t v, int waves) {
+    const int t = threadIdx.x, lane = t % WAVE;
+    auto keep = [&](uint64_t other, int d, bool up) __attribute__((always_inline)) { v = (other < v) == (up == ((t & d) == 0)) ? other : v; };
+    auto within = [&](auto from, bool up) __attribute__((always_inline)) { // distances from `from` down
+        constexpr int D = decltype(from)::value;
+        if constexpr (D >= 32) keep(lane_across<32>(v, lane), 32, up);
+        if constexpr (D >= 16) keep(lane_across<16>(v, lane), 16, up);
+        if constexpr (D >= 8) keep(lane_across<8>(v, lane), 8, up);
+        if constexpr (D >= 4) keep(lane_across<4>(v, lane), 4, up);
+        if constexpr (D >= 2) keep(lane_across<2>(v, lane), 2, up);
+        keep(lane_across<1>(v, lane), 1, up);
+    };
+    const bool mine = t < waves * WAVE;
+    if (mine) {
+        within(std::integral_constant<int, 1>{}, (t & 2) == 0);
+        within(std::integral_constant<int, 2>{}, (t & 4) == 0);
+        within(std::integral_constant<int, 4>{}, (t & 8) == 0);
+        within(std::integral_constant<int, 8>{}, (t & 16) == 0);
+        within(std::integral_constant<int, 16>{}, (t & 32) == 0);
+        within(std::integral_constant<int, 32>{}, (t & 64) == 0 || waves == 1);
+    }
+    int half = 0;
+    for (int size = 2 * WAVE; size <= waves * WAVE; size *= 2) {
+        const bool up = (t & size) == 0 || size == waves * WAVE;
+        for (int d = size / 2; d >= WAVE; d /= 2, half ^= THREADS) {
+            if (mine) room[half + t] = v;
+            __syncthreads(); // (the numbers of the step before last have been read)
+            if (mine) keep(room[half + (t ^ d)], d, up);
+        }
+        if (mine) within(std::integral_constant<int, 32>{}, up);
+    }
+    __syncthreads();
+    return v;
+}
+// The sum of the threads in front of this one, and of all.
+__device__ __forceinline__ uint64_t sum_in_front(SampleShared &sh, uint64_t v, uint64_t &total) {
+    const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE;
+    const uint64_t upto = wave_upto64(v);
+    if (lane == WAVE - 1) sh.scratch[wave] = upto;
+    __syncthreads();
+    const uint64_t other = sh.scratch[lane % WAVES];
+    total = sum16(other);
+    const uint64_t front = sum16(lane % WAVES < wave ? other : 0) + upto - v;
+    __syncthreads();
+    return front;
+}
+
 // Of the elements that `all(f)` hands to f(place, value()), those with places in [lo, hi]: the place at which the running sum of values, by place and with `before` in
 // front, exceeds than(sum of them all) -- hi if it never does.  Places are unique, values may be 0.  `count`: how many they are at most.
 template <class Than, class All> __device__ __forceinline__ uint64_t find_place(SampleShared &sh, uint64_t lo, uint64_t hi, uint64_t before, int count, Than than_of, All all) {
@@ -534,58 +596,64 @@ template <int DT, int IT> __global__ __launch_bounds__(THREADS) void sample_kern
             if (bounded) low = fmaxf(low, r.below(bin));
         }
         if (bounded) {
-            gather(each_step, FRONT, [&](float v, uint32_t) { return v >= low ? 1u : 0u; });
-            const int n = static_cast<int>(sh.front);
-            if (n <= DIRECT) {
-                // L threads to an entry, each of which looks at every L-th of the others
-                int shift = 4;
-                while (THREADS >> shift < n) --shift;
-                const int entry = t >> shift, part = t & ((1 << shift) - 1), L = 1 << shift;
-                const bool is = entry < n;
-                const uint64_t o = is ? sh.list[entry] : ~0ull;
+            // each wavefront's to a part of the list of its own
+            constexpr uint32_t PART = LIST / WAVES;
+            uint32_t own = 0;
+            each_step([&](const Step<DT> &s, uint32_t at, int) __attribute__((always_inline)) {
+                float largest = element<DT>(s, 0);
+#pragma unroll
+                for (int e = 1; e < E; ++e) largest = fmaxf(largest, element<DT>(s, e));
+                if (__ballot(largest >= low) == 0) return;
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const float v = element<DT>(s, e);
+                    const uint64_t taken = __ballot(v >= low);
+                    if (taken == 0) continue;
+                    const uint32_t to = own + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(taken >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(taken), 0));
+                    if (v >= low && to < PART) sh.list[wave * PART + to] = order_of(v, at + e);
+                    own += __builtin_popcountll(taken);
+                }
+            });
+            if (lane == 0) sh.where[wave] = own;
+            __syncthreads();
+            uint32_t in_front = 0, n = 0;
+            for (int w = 0; w < WAVES; ++w) {
+                in_front += w < wave ? sh.where[w] : 0;
+                n += sh.where[w];
+            }
+            if (n <= THREADS) { // an entry to a thread
+                uint64_t *const entries = sh.bins;
+                for (uint32_t i = lane; i < own; i += WAVE) entries[in_front + i] = sh.list[wave * PART + i];
+                __syncthreads();
+                uint64_t o = static_cast<uint32_t>(t) < n ? entries[t] : ~0ull, total;
+                int waves = 1;
+                while (waves * WAVE < static_cast<int>(n)) waves *= 2;
+                if (k || p < 1.0f) o = sorted(sh.list, o, waves);
+                // (in their order: what lies in front of an entry is what the threads in front hold)
+                bool kept = static_cast<uint32_t>(t) < n && (k == 0 || t < k);
                 const float v = logit_of(o);
-                uint64_t *const masses = sh.block_mass;
-                static_assert(BLOCKS >= DIRECT, "room for their weights");
-                auto all_parts = [&](uint64_t x) __attribute__((always_inline)) {
-                    for (int d = 1; d < L; d *= 2) x += __shfl_xor(x, d, WAVE);
-                    return x;
-                };
-                // in front of it in the order: how many (less than k are kept), and what they weigh (all of them are kept if it is)
-                uint64_t x = is ? r.mass(v) : 0;
-                if (is && part == 0) masses[entry] = x;
-                __syncthreads();
-                uint32_t rank = 0;
-                uint64_t front = 0;
-#pragma unroll 4
-                for (int j = part; j < n; j += L) {
-                    const bool before = sh.list[j] < o;
-                    rank += before ? 1 : 0;
-                    front += before ? masses[j] : 0;
-                }
-                bool kept = is && (k == 0 || all_parts(rank) < static_cast<uint64_t>(k));
                 if (p < 1.0f) {
-                    const uint64_t total = sum_of_all(sh, kept && part == 0 ? x : 0);
-                    kept = kept && all_parts(front) <= than_of_p([&] { return total; });
+                    const uint64_t front = sum_in_front(sh, kept ? r.mass(v) : 0, total);
+                    kept = kept && front <= than_of_p([&] { return total; });
                 }
-                __syncthreads();
-                x = kept ? r.mass_of_least(v) : 0;
-                if (is && part == 0) masses[entry] = x;
-                const uint64_t total = sum_of_all(sh, part == 0 ? x : 0), than = than_of_u(total); // (a barrier behind the weights)
-                const uint32_t index = index_of(o);
-                front = 0;
-#pragma unroll 4
-                for (int j = part; j < n; j += L) front += index_of(sh.list[j]) < index ? masses[j] : 0;
-                front = all_parts(front);
-                if (is && part == 0 && front <= than && front + x > than) answer(index, x, total);
+                // by index, with their weights: 20 and 44 bits
+                static_assert(MOST_VOCAB <= int64_t(1) << 20 && ONE < uint64_t(1) << 44, "one number for both");
+                const uint64_t mass = kept ? r.mass_of_least(v) : 0;
+                const uint64_t drawn = sorted(sh.list, mass ? static_cast<uint64_t>(index_of(o)) << 44 | mass : ~0ull, waves);
+                const uint64_t x = drawn != ~0ull ? drawn & ((uint64_t(1) << 44) - 1) : 0;
+                const uint64_t front = sum_in_front(sh, x, total), than = than_of_u(total);
+                if (front <= than && front + x > than) answer(static_cast<uint32_t>(drawn >> 44), x, total);
                 return;
             }
-            // longer ones: searched, as the lists of the third way are
+            // many equal ones: a longer list, searched as those of the third way are
+            gather(each_step_of_memory, FRONT, [&](float v, uint32_t) { return v >= low ? 1u : 0u; });
+            const int listed_here = static_cast<int>(sh.front);
             __syncthreads();
             if (t == 0) sh.front = 0;
             __syncthreads();
-            if (n <= FRONT) {
+            if (listed_here <= FRONT) {
                 listed = true;
-                listed_front = n;
+                listed_front = listed_here;
                 r.last = order_of(low, 0xFFFFFu);
             }
         }
