@@ -8,18 +8,21 @@
 namespace axhip {
 namespace {
 
-// A work-group of 1024 threads to a row, which it holds in registers where it fits (IT steps of eight elements a lane).  No sorting: a filter keeps a prefix of the order "larger
+// A work-group of 1024 threads to a row, which it holds in registers where it fits (IT steps of eight elements a lane).  A filter keeps a prefix of the order "larger
 // logit first, equal ones by index", and where it ends is found by what lies in front (numbers of logits, or sums of weights).  The draw is the same search in
 // the order of the indexes.  Weights are integers, multiples of 2^-43 of the largest, of which 2^20 fit 64 bits: sums do not depend on the order in which
 // atomics arrive.  Three ways, by what is asked of the row:
-//   * top_k up to SMALL_K (and short rows): of the threads' 1024 largest logits the k-th largest is a bound that at least k logits reach, and hardly more do; they go to a list
-//     in LDS, and each entry of the list adds up what lies in front of it.
+//   * top_k up to SMALL_K (and short rows): of the threads' 1024 largest logits the k-th largest is a bound that at least k logits reach, and hardly more do (of k = 512, 1024 ln 2 = 710 where
+//     they lie anywhere; a larger k would often leave more than there are threads).  An entry to a thread, they are sorted by the order, and then those that are kept by index.
 //   * other 16-bit rows: all 65535 values are counted in LDS (128 KiB), and every filter is answered by the counts: one weight for each value that occurs
 //     instead of one for each logit.  The draw takes weights from a table of the values that are kept.  Counts are 16 bits wide; if one overflows, the sum of all shows
 //     it and the row goes the third way.
 //   * other fp32 rows: a histogram of 2048 bins that are linear in the logit, from the largest to 31 temperatures below it, from where on weights round to zero (bins by the
 //     bits of the float hold most logits in a few dozen bins, on which a wavefront's atomics wait for each other).  All logits in the bin in which a filter ends, or in
 //     front of it, go to a list in LDS if they fit, and everything after happens there.
+// What bounds it: few rows the chain of dependent passes and barriers (fp32 1 x 51865, top_k: 8.9 us, of which 3 are the launch; bf16 64 x 51865, top_k, top_p and min_p: 15.2);
+// 256 rows a CU's own work on its row.  bf16 256 x 128256, top_p, 49 us: 8 loading (at HBM's rate), 2 the largest, 11 counting (LDS atomics: a wavefront's 64 random banks take 12
+// cycles), 5 the blocks' weights (64-bit operations), 3 the cut, 8 the draw's table look-ups, 3 the step it falls in.  fp32, the same rows: without filters 61, top_k 45, top_p 140.
 constexpr int THREADS = 1024, WAVES = THREADS / WAVE, E = 8; // elements of a lane's vector
 constexpr int STEP = WAVE * E;                               // consecutive elements of a wavefront's step
 constexpr int BINS = 2048, FEW = 128;
@@ -780,7 +783,7 @@ template <int DT, int IT> __global__ __launch_bounds__(THREADS) void sample_kern
                 }
                 if (all_whole) drawn += E;
             });
-        drawn = static_cast<uint32_t>(sum_of_all(sh, drawn)); // (a barrier behind the counts)
+        __syncthreads();
         // f(counts of the lane's value in block j and in block j + BLOCKS / 2, its order in the first) where either has any, a sum for each block; the others' sums are 0
         auto sum_blocks = [&](auto f) __attribute__((always_inline)) {
             constexpr int TOGETHER = 8;
@@ -829,7 +832,7 @@ template <int DT, int IT> __global__ __launch_bounds__(THREADS) void sample_kern
                 counted += c0 + c1;
             });
         }
-        if (sum_of_all(sh, counted) == drawn) { // (a count that overflowed takes 65535 or 65536 from the sum)
+        if (sum_of_all(sh, uint64_t(drawn) - counted) == 0) { // (a count that overflowed takes 65535 or 65536 from the sum)
             // the first value of `block` at which the running sum exceeds `than`, and the sum in front of it
             auto find_value = [&](int block, uint64_t front, uint64_t than, uint64_t own, uint64_t &in_front) __attribute__((always_inline)) {
                 const uint64_t upto = front + wave_upto64(own);
@@ -862,13 +865,19 @@ template <int DT, int IT> __global__ __launch_bounds__(THREADS) void sample_kern
                 const uint64_t than = than_of_p([&] { return sum_of_bins(sh); });
                 const int block = find_bin(sh, 0, than, front);
                 if (block >= 0) {
-                    const uint32_t order = block * BLOCK + lane;
-                    last = find_value(block, front, than, kept_mass(order, count_at(order)), in_front);
-                    const uint64_t each_of_them = r.mass(logit_of16<DT>(last)), reached = than - in_front;
-                    ties = static_cast<uint32_t>(static_cast<double>(reached) / static_cast<double>(each_of_them)); // (to within one)
-                    if (ties * each_of_them > reached) --ties;
-                    else if ((ties + 1) * each_of_them <= reached) ++ties;
-                    ++ties;
+                    if (wave == 0) { // (operations of 64 bits, for all wavefronts)
+                        const uint32_t order = block * BLOCK + lane;
+                        last = find_value(block, front, than, kept_mass(order, count_at(order)), in_front);
+                        const uint64_t each_of_them = r.mass(logit_of16<DT>(last)), reached = than - in_front;
+                        ties = static_cast<uint32_t>(static_cast<double>(reached) / static_cast<double>(each_of_them)); // (to within one)
+                        if (ties * each_of_them > reached) --ties;
+                        else if ((ties + 1) * each_of_them <= reached) ++ties;
+                        ++ties;
+                        if (lane == 0) sh.other_scratch[0] = uint64_t(ties) << 32 | last;
+                    }
+                    __syncthreads();
+                    last = static_cast<uint32_t>(sh.other_scratch[0]);
+                    ties = static_cast<uint32_t>(sh.other_scratch[0] >> 32);
                 }
             }
             // Of the last value only the first `ties` by index are kept: its logits carry no weight but a mark, and their share is added when the steps' numbers of
