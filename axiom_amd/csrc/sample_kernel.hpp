@@ -18,16 +18,17 @@ namespace {
 //     instead of one for each logit.  The draw takes weights from a table of the values that are kept.  Counts are 16 bits wide; if one overflows, the sum of all shows
 //     it and the row goes the third way.
 //   * other fp32 rows: a histogram of 2048 bins that are linear in the logit, from the largest to 31 temperatures below it, from where on weights round to zero (bins by the
-//     bits of the float hold most logits in a few dozen bins, on which a wavefront's atomics wait for each other).  All logits in the bin in which a filter ends, or in
-//     front of it, go to a list in LDS if they fit, and everything after happens there.
+//     bits of the float hold most logits in a few dozen bins, on which a wavefront's atomics wait for each other).  The logits in the bin in which a filter ends go to a list
+//     in LDS if they fit, where the cut is found.  (Lists of all that is kept, for the draw, and weights formed of what is kept alone took as long as a pass over the row.)
 // What bounds it: few rows the chain of dependent passes and barriers (fp32 1 x 51865, top_k: 8.9 us, of which 3 are the launch; bf16 64 x 51865, top_k, top_p and min_p: 15.2);
 // 256 rows a CU's own work on its row.  bf16 256 x 128256, top_p, 49 us: 8 loading (at HBM's rate), 2 the largest, 11 counting (LDS atomics: a wavefront's 64 random banks take 12
-// cycles), 5 the blocks' weights (64-bit operations), 3 the cut, 8 the draw's table look-ups, 3 the step it falls in.  fp32, the same rows: without filters 61, top_k 45, top_p 140.
+// cycles), 5 the blocks' weights (64-bit operations), 3 the cut, 8 the draw's table look-ups, 3 the step it falls in.  fp32, the same rows: without filters 61, top_k 45, top_p 129: a pass over the row takes
+// 35 to 45, 200 cycles of a SIMD for each vector of 64 weights, half of them 64-bit operations.
 constexpr int THREADS = 1024, WAVES = THREADS / WAVE, E = 8; // elements of a lane's vector
 constexpr int STEP = WAVE * E;                               // consecutive elements of a wavefront's step
 constexpr int BINS = 2048, FEW = 128;
 constexpr int FEW_LOGITS = 1024, SMALL_K = 512;
-constexpr int LIST = 16384, FRONT = 12288; // of which this many for what lies in front of the bin
+constexpr int LIST = 16384;
 constexpr int BLOCK = 64, BLOCKS = 65536 / BLOCK; // 16-bit values are summed up by blocks
 static_assert(MOST_VOCAB <= int64_t(BINS) * STEP, "a bin for a step");
 constexpr uint64_t ONE = uint64_t(1) << 43, MARK = uint64_t(1) << 53;
@@ -38,9 +39,9 @@ struct SampleShared {
     uint64_t block_mass[BLOCKS];
     uint64_t few_place[FEW], few_value[FEW];
     uint64_t scratch[WAVES + 2], other_scratch[WAVES];
-    double pow2[32];
+    uint64_t pow2[32]; // 2^43 2^(i / 32), less i in the place to which scaled_weight adds it
     float top[WAVES];
-    uint32_t where[WAVES], few, front, inside;
+    uint32_t where[WAVES], few, inside;
     union {
         uint64_t list[LIST];
         uint32_t counts[32768]; // two values to a word
@@ -131,6 +132,7 @@ template <int P> __device__ __forceinline__ uint64_t sums_of_many(uint64_t (&v)[
 }
 template <int N, class F, int... I> __device__ __forceinline__ void unrolled_as(F f, std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>{}), ...); }
 template <int N, class F> __device__ __forceinline__ void unrolled(F f) { unrolled_as<N>(f, std::make_integer_sequence<int, N>{}); }
+__device__ __forceinline__ uint32_t lanes_in_front(uint64_t mask) { return __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0)); }
 // A counter's old value; lane by lane (the compiler makes a sum over the wavefront of additions to one address, which is the longer way for the few lanes that come here)
 __device__ __forceinline__ uint32_t take_from(uint32_t &counter, uint32_t n) {
     uint32_t offset = 0;
@@ -182,9 +184,11 @@ template <int DT> struct Row {
     double rate = 0.0;     // log2(e) / temperature
     float floor = 0.0f;    // from here on weights may be more than nothing
     float lowest = 0.0f, highest = 0.0f; // finite bounds of what powers are formed of
-    const double *pow2 = nullptr; // 2^43 2^(i / 32)
-    uint64_t last = ~0ull; // kept: up to this one in the order,
-    double least = 0.0;    // and with at least this weight
+    const uint64_t *pow2 = nullptr;
+    uint64_t last = ~0ull; // kept: up to this one in the order (the one of last_index among the logits that equal last_logit),
+    float last_logit = -__builtin_inff();
+    uint32_t last_index = 0;
+    double least = 0.0; // and with at least this weight
 
     __device__ __forceinline__ Step<DT> load(int step) const {
         constexpr int ES = DT == AXHIP_DTYPE_F32 ? 4 : 2;
@@ -217,7 +221,7 @@ template <int DT> struct Row {
         constexpr double SPLIT = 211106232532992.0; // 1.5 * 2^47: its last bit is 1/32
         const double t = z + SPLIT, r = z - (t - SPLIT);
         const uint32_t i = static_cast<uint32_t>(__double_as_longlong(t));
-        const uint64_t power_of_two = static_cast<uint64_t>(__double_as_longlong(pow2[i & 31])) + (static_cast<uint64_t>((i & ~31u) << 15) << 32);
+        const uint64_t power_of_two = pow2[i & 31] + (static_cast<uint64_t>(i << 15) << 32);
         double p = 0.0013333558146428443;
         p = __builtin_fma(r, p, 0.009618129107628477);
         p = __builtin_fma(r, p, 0.05550410866482158);
@@ -237,9 +241,10 @@ template <int DT> struct Row {
         return static_cast<uint64_t>(hi) << 32 | lo;
     }
     __device__ __forceinline__ uint64_t mass(float v) const { return integer(scaled_weight(power(v))); }
-    __device__ __forceinline__ uint64_t mass_of_least(float v) const { // ... 0 below min_p
+    // ... 0 below min_p, and of what is not kept
+    __device__ __forceinline__ uint64_t mass_of_least(float v, bool kept = true) const {
         const double w = scaled_weight(power(v));
-        return w >= least ? integer(w) : 0;
+        return integer(kept && w >= least ? w : 0.0);
     }
     // bins of the power, BINS to REACH temperatures; the last one holds everything from there on
     __device__ __forceinline__ uint32_t bin_of_power(double z) const {
@@ -253,7 +258,30 @@ template <int DT> struct Row {
         const float low = static_cast<float>(edge) - fabsf(static_cast<float>(edge)) * 1e-6f;
         return low > -3e38f ? low : -3.402823466e38f;
     }
-    __device__ __forceinline__ bool counts(float v, uint32_t i) const { return v >= floor && (last == ~0ull || order_of(v, i) <= last); }
+    // The smallest float of bins up to `bin`, not below `from` (by a whole wavefront: in each round its lanes look at 64 places of what is left)
+    __device__ __forceinline__ float smallest_up_to(int bin, float from) const {
+        auto key_of = [](float v) { return __float_as_uint(v) ^ (__float_as_uint(v) & 0x80000000u ? ~0u : 0x80000000u); };
+        auto float_of = [](uint32_t key) { return __uint_as_float(key ^ (key & 0x80000000u ? 0x80000000u : ~0u)); };
+        uint32_t lo = key_of(from), hi = key_of(top); // (the largest logit's bin is the first)
+        while (lo < hi) {
+            const uint32_t at = lo + static_cast<uint32_t>(static_cast<uint64_t>(hi - lo) * (threadIdx.x % WAVE) / WAVE);
+            const uint64_t reached = __ballot(static_cast<int>(bin_of(float_of(at))) <= bin);
+            const int first = reached ? __builtin_ctzll(reached) : WAVE; // (they are in order: from this one on)
+            const uint32_t at_first = __builtin_amdgcn_readlane(at, first % WAVE), in_front = __builtin_amdgcn_readlane(at, (first + WAVE - 1) % WAVE);
+            if (first == 0) hi = lo;
+            else {
+                lo = in_front + 1;
+                if (first < WAVE) hi = at_first;
+            }
+        }
+        return float_of(lo);
+    }
+    __device__ __forceinline__ void keep_up_to(uint64_t order) {
+        last = order;
+        last_logit = logit_of(order);
+        last_index = index_of(order);
+    }
+    __device__ __forceinline__ bool counts(float v, uint32_t i) const { return v >= floor && (v > last_logit || (v == last_logit && i <= last_index)); }
 };
 
 // ---- All of these are called by the whole work-group, and their answers are every thread's.
@@ -494,8 +522,8 @@ template <int DT, int IT> __global__ __launch_bounds__(THREADS) void sample_kern
     temperature = temperature > 1e30f ? 1e30f : temperature;
     const float p = a.top_p ? a.top_p[row] : 1.0f, m = a.min_p ? a.min_p[row] : 0.0f, u = a.u[row];
     const int32_t k = a.top_k && a.top_k[row] > 0 && a.top_k[row] < a.vocab ? a.top_k[row] : 0;
-    if (t == 0) sh.front = sh.inside = 0;
-    if (t < 32) sh.pow2[t] = exp2(43.0 + t * (1.0 / 32.0)); // (a barrier before they are used)
+    if (t == 0) sh.inside = 0;
+    if (t < 32) sh.pow2[t] = static_cast<uint64_t>(__double_as_longlong(exp2(43.0 + t * (1.0 / 32.0)))) - (uint64_t(t) << 47); // (a barrier before they are used)
     r.pow2 = sh.pow2;
     sh.bins[t] = 0;
     sh.bins[t + THREADS] = 0;
@@ -547,38 +575,32 @@ template <int DT, int IT> __global__ __launch_bounds__(THREADS) void sample_kern
     const double least = m > 0.0f ? (m < 1.0f ? static_cast<double>(m) : 1.0) * static_cast<double>(ONE) : 0.0;
     r.least = least;
 
-    // Those that `taken(logit, index)` gives a kind, 1 or 2, to the list: the first kind from its start, the second from FRONT on.
-    auto gather = [&](auto steps_of, int front_room, auto taken) __attribute__((always_inline)) {
-        steps_of([&](const Step<DT> &s, uint32_t at, int) __attribute__((always_inline)) {
-            uint32_t kinds = 0; // two bits an element
+    // Those for which `taken(logit, index)` holds to the list (as many as it has room for); how many there are.
+    auto gather = [&](auto taken) __attribute__((always_inline)) {
+        each_step_of_memory([&](const Step<DT> &s, uint32_t at, int) __attribute__((always_inline)) {
+            uint64_t lanes[E];
+            uint32_t n = 0, before = 0;
 #pragma unroll
-            for (int e = 0; e < E; ++e) kinds |= taken(element<DT>(s, e), at + e) << (2 * e);
-            if (__ballot(kinds != 0) == 0) return;
-            // places: one addition for the wavefront, and what the lanes in front have of either kind
-            const uint32_t own = __builtin_popcount(kinds & 0x5555u) | static_cast<uint32_t>(__builtin_popcount(kinds & 0xAAAAu)) << 16;
-            const uint32_t upto = wave_upto32(own), all = __builtin_amdgcn_readlane(upto, WAVE - 1);
-            uint32_t f0 = 0, i0 = 0;
-            if (lane == 0) {
-                if (all & 0xFFFFu) f0 = take_from(sh.front, all & 0xFFFFu);
-                if (all >> 16) i0 = take_from(sh.inside, all >> 16);
+            for (int e = 0; e < E; ++e) {
+                lanes[e] = __ballot(taken(element<DT>(s, e), at + e));
+                n += __builtin_popcountll(lanes[e]);
             }
-            uint32_t f = __builtin_amdgcn_readfirstlane(f0) + ((upto - own) & 0xFFFFu), i = FRONT + __builtin_amdgcn_readfirstlane(i0) + ((upto - own) >> 16);
-            if (kinds) {
+            if (n == 0) return;
+            if (lane == 0) before = take_from(sh.inside, n);
+            before = __builtin_amdgcn_readfirstlane(before);
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const uint32_t kind = (kinds >> (2 * e)) & 3u, to = kind == 1 ? f : i;
-                    f += kind == 1;
-                    i += kind == 2;
-                    if (kind && to < static_cast<uint32_t>(kind == 1 ? front_room : LIST)) sh.list[to] = order_of(element<DT>(s, e), at + e);
-                }
+            for (int e = 0; e < E; ++e) {
+                const uint32_t to = before + lanes_in_front(lanes[e]);
+                if ((lanes[e] >> lane & 1) && to < LIST) sh.list[to] = order_of(element<DT>(s, e), at + e);
+                before += __builtin_popcountll(lanes[e]);
             }
         });
         __syncthreads();
+        const int n = static_cast<int>(sh.inside);
+        __syncthreads();
+        if (t == 0) sh.inside = 0;
+        return n;
     };
-
-    // `listed`: the list holds all that is kept: `listed_front` from its start, `listed_inside` from FRONT on.
-    bool listed = false;
-    int listed_front = 0, listed_inside = 0;
 
     // ================ top_k of a few, short rows: a list of little more than what is kept
     if ((k && k <= SMALL_K) || a.vocab <= FEW_LOGITS) {
@@ -612,7 +634,7 @@ template <int DT, int IT> __global__ __launch_bounds__(THREADS) void sample_kern
                     const float v = element<DT>(s, e);
                     const uint64_t taken = __ballot(v >= low);
                     if (taken == 0) continue;
-                    const uint32_t to = own + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(taken >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(taken), 0));
+                    const uint32_t to = own + lanes_in_front(taken);
                     if (v >= low && to < PART) sh.list[wave * PART + to] = order_of(v, at + e);
                     own += __builtin_popcountll(taken);
                 }
@@ -648,17 +670,7 @@ template <int DT, int IT> __global__ __launch_bounds__(THREADS) void sample_kern
                 if (front <= than && front + x > than) answer(static_cast<uint32_t>(drawn >> 44), x, total);
                 return;
             }
-            // many equal ones: a longer list, searched as those of the third way are
-            gather(each_step_of_memory, FRONT, [&](float v, uint32_t) { return v >= low ? 1u : 0u; });
-            const int listed_here = static_cast<int>(sh.front);
-            __syncthreads();
-            if (t == 0) sh.front = 0;
-            __syncthreads();
-            if (listed_here <= FRONT) {
-                listed = true;
-                listed_front = listed_here;
-                r.last = order_of(low, 0xFFFFFu);
-            }
+            __syncthreads(); // (many equal ones: the other ways)
         }
     }
 
@@ -745,7 +757,7 @@ template <int DT, int IT> __global__ __launch_bounds__(THREADS) void sample_kern
     };
 
     // ================ 16-bit logits: counts of their values
-    if (DT != AXHIP_DTYPE_F32 && !listed) {
+    if (DT != AXHIP_DTYPE_F32) {
         const bool filtered = k || p < 1.0f; // (else there is nothing to count)
         // The count of order o is a half of word o % 32768 (values next to each other lie in different banks).
         auto count_at = [&](uint32_t order) { return (sh.counts[order & 0x7FFFu] >> (order >> 15 << 4)) & 0xFFFFu; };
@@ -924,8 +936,9 @@ template <int DT, int IT> __global__ __launch_bounds__(THREADS) void sample_kern
                     for (int e = 0; e < E; ++e) {
                         const uint32_t i = place_of(s.v[0][e / 2])[e % 2];
                         const float v = element<DT>(s, e);
-                        const uint64_t mass = r.formed(r.mass_of_least(v));
-                        x[e] = v >= r.floor && i < values ? in_part && i == values - 1 ? MARK : mass : 0;
+                        const bool marked = in_part && i == values - 1;
+                        x[e] = r.formed(r.mass_of_least(v, v >= r.floor && i < values && !marked));
+                        if (marked) x[e] = MARK;
                     }
                 });
             }
@@ -934,17 +947,10 @@ template <int DT, int IT> __global__ __launch_bounds__(THREADS) void sample_kern
         __syncthreads(); // (the list takes the counts' place)
     }
 
-    // ================ lists, other fp32 rows, and 16-bit ones with more than 65535 equal logits
-    auto each_listed = [&](auto f) __attribute__((always_inline)) {
-        for (int i = t; i < listed_front + listed_inside; i += THREADS) f(sh.list[i < listed_front ? i : FRONT + i - listed_front]);
-    };
+    // ================ other fp32 rows, and 16-bit ones with more than 65535 equal logits
     // Keeps what is kept up to where the running sum of value(logit, power) exceeds than(sum of all).
     auto cut = [&](auto value, auto than_of) __attribute__((always_inline)) {
         auto value_of = [&](float v) __attribute__((always_inline)) { return value(r.power(v)); };
-        if (listed) {
-            r.last = find_place(sh, order_of(r.top, 0), r.last, 0, listed_front + listed_inside, than_of, [&](auto f) __attribute__((always_inline)) { each_listed([&](uint64_t o) { f(o, [&] { return value_of(logit_of(o)); }); }); });
-            return;
-        }
         clear_bins(sh);
         each_step_of_memory([&](const Step<DT> &s, uint32_t at, int) __attribute__((always_inline)) {
             uint64_t x[E];
@@ -965,58 +971,40 @@ template <int DT, int IT> __global__ __launch_bounds__(THREADS) void sample_kern
         uint64_t before;
         const int bin = find_bin(sh, 0, than, before);
         if (bin < 0 || bin == BINS - 1) return; // (all are kept, or all that weigh anything)
-        const float low = fmaxf(r.floor, r.below(bin));
-        gather(each_step_of_memory, FRONT, [&](float v, uint32_t i) {
-            uint32_t kind = 0;
-            if (v >= low) {
-                const uint32_t b = r.bin_of(v);
-                if (b <= static_cast<uint32_t>(bin) && r.counts(v, i)) kind = b == static_cast<uint32_t>(bin) ? 2u : 1u;
-            }
-            return kind;
-        });
-        const int front = static_cast<int>(sh.front), inside = static_cast<int>(sh.inside);
+        // where the bins up to this one end, and those in front of it: two comparisons for each logit instead of its bin
+        if (wave < 2) {
+            const float edge = r.smallest_up_to(bin - wave, r.floor);
+            if (lane == 0) sh.top[wave] = edge;
+        }
         __syncthreads();
-        if (t == 0) sh.front = sh.inside = 0;
-        listed = front <= FRONT && inside <= LIST - FRONT;
-        listed_front = front;
-        listed_inside = inside;
+        const float inside_from = sh.top[0], front_from = bin ? sh.top[1] : __builtin_nanf("");
+        auto inside = [&](float v, uint32_t i) __attribute__((always_inline)) { return v >= inside_from && !(v >= front_from) && r.counts(v, i); };
+        const int n = gather(inside);
         const uint64_t first = order_of(r.top, 0), behind = r.last < (uint64_t(1) << 52) ? r.last : (uint64_t(1) << 52) - 1;
         auto known = [&](auto) { return than; };
-        if (inside <= LIST - FRONT) {
-            const int n = inside;
-            r.last = find_place(sh, first, behind, before, n, known, [&](auto f) __attribute__((always_inline)) {
+        if (n <= LIST) {
+            r.keep_up_to(find_place(sh, first, behind, before, n, known, [&](auto f) __attribute__((always_inline)) {
                 for (int i = t; i < n; i += THREADS) {
-                    const uint64_t o = sh.list[FRONT + i];
+                    const uint64_t o = sh.list[i];
                     f(o, [&] { return value_of(logit_of(o)); });
                 }
-            });
+            }));
         } else {
-            r.last = find_place(sh, first, behind, before, inside, known, [&](auto f) __attribute__((always_inline)) {
+            r.keep_up_to(find_place(sh, first, behind, before, n, known, [&](auto f) __attribute__((always_inline)) {
                 each_of(each_step_of_memory, [&](float v, uint32_t i) {
-                    if (v >= r.floor && r.bin_of(v) == static_cast<uint32_t>(bin)) f(order_of(v, i), [&] { return value_of(v); });
+                    if (inside(v, i)) f(order_of(v, i), [&] { return value_of(v); });
                 });
-            });
+            }));
         }
     };
     if (k) cut([](double) { return uint64_t(1); }, [&](auto) { return static_cast<uint64_t>(k - 1); });
     if (p < 1.0f) cut([&](double z) { return r.integer(r.scaled_weight(z)); }, than_of_p);
 
-    if (listed) {
-        uint64_t total = 0;
-        const uint64_t at = find_place(sh, 0, static_cast<uint64_t>(a.vocab), 0, listed_front + listed_inside, [&](auto sum) { return than_of_u(total = sum()); }, [&](auto f) __attribute__((always_inline)) {
-            each_listed([&](uint64_t o) { f(index_of(o), [&] { return o <= r.last ? r.mass_of_least(logit_of(o)) : uint64_t(0); }); });
-        });
-        each_listed([&](uint64_t o) {
-            if (index_of(o) == at && o <= r.last) answer(static_cast<uint32_t>(at), r.mass_of_least(logit_of(o)), total);
-        });
-        return;
-    }
     draw_by_steps(std::false_type{}, 0, 0, [&](const Step<DT> &s, uint32_t at, uint64_t(&x)[E]) __attribute__((always_inline)) {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             const float v = element<DT>(s, e);
-            const uint64_t mass = r.formed(r.mass_of_least(v));
-            x[e] = r.counts(v, at + e) ? mass : 0;
+            x[e] = r.formed(r.mass_of_least(v, r.counts(v, at + e)));
         }
     });
 }
