@@ -29,7 +29,7 @@ template <int P> __device__ __forceinline__ int q8_lane_sums(int (&v)[P], int la
 
 // A wavefront owns R rows of W and walks k with its 64 lanes side by side, 1 KiB of a row per load; four products and their addition per instruction
 // (v_dot4_i32_i8).  Rows may start anywhere; the chunk that K ends in is fetched as the 16 bytes that end with the row, with those in front of it
-// cleared in x.
+// cleared in x.  1 x 4096 x 4096 3.4 us back to back (16.8 MB from the caches), 4.7 with other weights in between.
 template <int DT, int M, int R>
 __global__ __launch_bounds__(256) void gemm_q8_skinny_kernel(const Q8Args a) {
     const int lane = threadIdx.x % 64;

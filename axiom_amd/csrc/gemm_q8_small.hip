@@ -36,7 +36,7 @@ __device__ __forceinline__ void small_finish(const Q8Args &g, const int4_t (&acc
 // C = A B^T, any alignment: work-group tile 16 MI x 16 NJ, W wavefronts that split k between them (wavefront w takes the pieces of 128 k
 // w, w + W, ...) and meet in LDS once, at the end.  Such products are bound by latency: every wavefront has a stage of LDS of its own and waits for
 // nobody until the sums are added, and the tile is as narrow as it takes to give every CU work.  A piece travels through registers, the next one's loads in flight while one is
-// multiplied; the loads need no alignment, and the last chunk of a row is fetched as the 16 bytes that end with it and shifted into place.
+// multiplied; the loads need no alignment, and the last chunk of a row is fetched as the 16 bytes that end with it and shifted into place.  64 x 4096 x 4096 6.2 us (17 MB: 3.4 at a copy's rate).
 template <int DT, int MI, int NJ, int W>
 __global__ __launch_bounds__(64 * W) void gemm_q8_small_kernel(const Q8Args g) {
     extern __shared__ __attribute__((aligned(1024))) unsigned char small_lds[];
