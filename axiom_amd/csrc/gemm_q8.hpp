@@ -17,8 +17,8 @@ static_assert(sizeof(Q8Args) <= 96, "kernel arguments");
 
 // Work-group tiles (M x N) of the middle-sized and large products.  Q8_128x128_PAIR: on four wavefronts, of which a CU holds two work-groups.
 enum Q8Tile { Q8_256x256, Q8_256x128, Q8_192x128, Q8_128x128, Q8_128x128_PAIR, Q8_64x128, Q8_TILES };
-struct Q8Geometry { int tm, tn, waves; };
-constexpr Q8Geometry Q8_GEOMETRY[Q8_TILES] = {{256, 256, 8}, {256, 128, 8}, {192, 128, 8}, {128, 128, 8}, {128, 128, 4}, {64, 128, 8}};
+struct Q8Geometry { int tm, tn; };
+constexpr Q8Geometry Q8_GEOMETRY[Q8_TILES] = {{256, 256}, {256, 128}, {192, 128}, {128, 128}, {128, 128}, {64, 128}};
 
 // The launchers, K >= 16.  `aligned`: every row of a and b starts on a 16-byte boundary and K is a multiple of 16 (if not: Q8_128x128, through registers).  The small products' tiles are
 // those of the 16-bit ones (SmallShape).

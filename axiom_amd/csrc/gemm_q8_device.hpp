@@ -29,10 +29,10 @@ __device__ __forceinline__ int4_t q8_mfma(const uint4_t &fb, const uint4_t &fa, 
 // have the same bits whichever kernel the other rows lead to.
 __device__ __forceinline__ float q8_scaled(int sum, float sa, float sb, float bias) { return __builtin_fmaf(static_cast<float>(sum), sa * sb, bias); }
 
-// N sums of row `row` from column `col` on, of which columns [first, last) exist, to C: scales (scale_b's in sb, bias in b), residual, activation.
+// N sums of a row, to C from `at` on, of which the first `last` exist: scales (scale_b's in sb, bias in b), residual, activation.
 template <int DT, int N>
-__device__ __forceinline__ void q8_finish(const Q8Args &g, const int (&sum)[N], float sa, const float (&sb)[N], const float (&b)[N], int64_t at, int first, int last) {
-    const bool whole = first == 0 && last == N;
+__device__ __forceinline__ void q8_finish(const Q8Args &g, const int (&sum)[N], float sa, const float (&sb)[N], const float (&b)[N], int64_t at, int last) {
+    const bool whole = last == N;
     float x[N];
 #pragma unroll
     for (int e = 0; e < N; ++e) x[e] = q8_scaled(sum[e], sa, sb[e], b[e]);
@@ -45,7 +45,7 @@ __device__ __forceinline__ void q8_finish(const Q8Args &g, const int (&sum)[N], 
         } else {
 #pragma unroll
             for (int e = 0; e < N; ++e)
-                if (e >= first && e < last) x[e] += Elem<DT>::load(g.residual, at + e);
+                if (e < last) x[e] += Elem<DT>::load(g.residual, at + e);
         }
     }
     gemm_epilogue_all_as<DT != AXHIP_DTYPE_F32>(g.epilogue, x);
@@ -54,7 +54,7 @@ __device__ __forceinline__ void q8_finish(const Q8Args &g, const int (&sum)[N], 
     } else {
 #pragma unroll
         for (int e = 0; e < N; ++e)
-            if (e >= first && e < last) Elem<DT>::store(g.c, at + e, x[e]);
+            if (e < last) Elem<DT>::store(g.c, at + e, x[e]);
     }
 }
 

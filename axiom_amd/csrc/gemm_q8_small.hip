@@ -29,7 +29,7 @@ __device__ __forceinline__ void small_finish(const Q8Args &g, const int4_t (&acc
             sb[e] = e < last ? g.scale_b[col + e] : 0.0f;
             b[e] = g.bias && e < last ? Elem<DT>::load(g.bias, col + e) : 0.0f;
         }
-        q8_finish<DT, 4>(g, sum, g.scale_a[row], sb, b, static_cast<int64_t>(row) * g.ldc + col, 0, last);
+        q8_finish<DT, 4>(g, sum, g.scale_a[row], sb, b, static_cast<int64_t>(row) * g.ldc + col, last);
     }
 }
 

@@ -88,15 +88,6 @@ __device__ __forceinline__ uint64_t wave_upto64(uint64_t v) { // of the lanes up
     v += dpp64<0x142, 0xA>(v); // the row in front, to rows 1 and 3
     return v + dpp64<0x143, 0xC>(v); // the first half, to the second
 }
-template <int CTRL, int ROWS = 0xF> __device__ __forceinline__ uint32_t dpp32(uint32_t v) { return __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xF, false); }
-__device__ __forceinline__ uint32_t wave_upto32(uint32_t v) {
-    v += dpp32<0x111>(v);
-    v += dpp32<0x112>(v);
-    v += dpp32<0x114>(v);
-    v += dpp32<0x118>(v);
-    v += dpp32<0x142, 0xA>(v);
-    return v + dpp32<0x143, 0xC>(v);
-}
 __device__ __forceinline__ uint64_t lane_of(uint64_t v, int lane) {
     return static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(v >> 32)), lane))) << 32 |
            static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(v)), lane));

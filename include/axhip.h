@@ -529,8 +529,8 @@ typedef struct {
     int64_t rows, vocab, ld;
     const float *temperature; /* [rows] or NULL */
     const int32_t *top_k;     /* [rows] or NULL; 0 or less: off for the row */
-    const float *top_p;       /* [rows] or NULL; 1 or more: off for the row */
-    const float *min_p;       /* [rows] or NULL; 0 or less: off for the row */
+    const float *top_p;       /* [rows] or NULL; 1 or more, or NaN: off for the row */
+    const float *min_p;       /* [rows] or NULL; 0 or less, or NaN: off for the row */
     const float *u;           /* [rows] */
 } AxhipSampleParams;
 

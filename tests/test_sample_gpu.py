@@ -212,3 +212,61 @@ def test_masked_halves_and_infinities_under_every_filter(dt):
     for settings in ({}, dict(top_k=3), dict(top_k=700), dict(top_p=0.9), dict(min_p=0.2), dict(top_k=1000, top_p=0.7, min_p=0.01)):
         tokens = check(logits, dt, u, temperature=0.8, **settings)
         assert tokens[0] < 100 and tokens[1] >= 59900 and tokens[2] < 50 and tokens[3] % 2 == 1 and tokens[4] in (7, 50000, 59999)
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("equal", [1, 63, 64, 65, 127, 128, 129, 255, 257, 511, 512, 513, 1023, 1024, 1025, 5000, 19997])
+def test_any_number_of_largest_logits(dt, equal):
+    """`equal` of them, anywhere in the row: all of them reach the bound of a small top_k."""
+    vocab = 20000
+    gen = torch.Generator()
+    gen.manual_seed(equal)
+    logits, u = logits_of(equal, 5, vocab, dt, 1.0)
+    logits = logits.clamp(max=2.0)
+    for row in range(5):
+        logits[row, torch.randperm(vocab, generator=gen)[:equal].cuda()] = 4.0
+    ks = [1, 2, 100, 300, 512]
+    check(logits, dt, u, top_k=ks)
+    check(logits, dt, u, top_k=ks, top_p=[0.5, 0.9, 0.3, 0.75, 0.98], min_p=0.1)
+    check(logits, dt, u, top_p=[0.5, 0.9, 0.3, 0.75, 0.98], temperature=0.5)
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("vocab", [3, 64, 65, 200, 1000, 1023, 1024, 1025, 2000])
+def test_short_rows_under_every_filter(dt, vocab):
+    logits, u = logits_of(vocab, 4, vocab, dt)
+    logits[1] = logits[1].round()
+    logits[2, vocab // 2:] = -float("inf")
+    check(logits, dt, u, top_k=[vocab, vocab // 2, 1 + vocab // 3, 2], top_p=[0.99, 0.9, 0.5, 0.7])
+    check(logits, dt, u, top_p=[0.0, 1e-7, 0.4, 1.0 - 2.0**-24], min_p=[0.0, 0.5, 0.0, 1e-3])
+
+
+def test_settings_that_are_not_numbers():
+    """temperature NaN is 0; of the others NaN is off."""
+    nan = float("nan")
+    logits, u = logits_of(3, 4, 5000, "bf16")
+    largest = logits.float().argmax(1).cpu()
+    tokens, probs = q8.sample(logits, "bf16", u, temperature=[nan, 0.0, -1.0, nan])
+    assert list(tokens) == largest.tolist() and all(p == 1.0 for p in probs)
+    want, _ = q8.sample(logits, "bf16", u)
+    got, _ = q8.sample(logits, "bf16", u, top_p=nan, min_p=nan)
+    assert list(got) == list(want)
+
+
+def test_calls_on_two_streams_at_once():
+    lib = capi.lib()
+    cases, calls = [(1, "f32", dict(top_k=60)), (70, "bf16", dict(top_p=0.9)), (260, "f16", dict(top_k=700, top_p=0.8)), (33, "f32", dict(top_p=0.95))], []
+    for rows, dt, settings in cases:
+        logits, u = logits_of(rows, rows, 40001, dt)
+        want, _ = q8.sample(logits, dt, u, **settings)
+        on = {k: torch.full((rows,), v, dtype=torch.int32 if k == "top_k" else torch.float32, device="cuda") for k, v in settings.items()}
+        u, tokens = u.cuda(), torch.empty(rows, dtype=torch.int64, device="cuda")
+        calls.append((logits, q8.sample_params(logits, dt, u, **on), tokens, want, on, u))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    q8.sync()
+    for _ in range(5):
+        for i, (logits, p, tokens, _, _, _) in enumerate(calls):
+            capi.check(lib.axhip_sample(q8.at(logits), q8.at(tokens), None, C.byref(p), streams[i % 2].cuda_stream))
+    torch.cuda.synchronize()
+    for _, _, tokens, want, _, _ in calls:
+        assert tokens.tolist() == list(want)
