@@ -310,3 +310,37 @@ def test_more_columns_than_one_launch_has_threads_for(m):
     for first in (0, 1 << 20, 1 << 26, n - 5000):
         part = slice(first, first + 5000)
         assert torch.equal(c[:, part].cpu(), (a.cpu().int()[:, None] * b[part].cpu().int()[None]).sum(-1).float())
+
+
+def test_rows_farther_apart_than_32_bits():
+    """Three rows 2^30 elements apart: the last one's bytes, and its elements' number, lie past 2^31."""
+    far, cols = (1 << 30) + 3, 700
+    x = normal(5, 3, cols)
+    apart = torch.empty(3, far, dtype=torch.bfloat16, device="cuda")[:, :cols]
+    apart.copy_(x)
+    want, scales = q8.quantize(x, "bf16")
+    got, more = q8.quantize(apart, "bf16", ld_q=far)
+    assert torch.equal(got, want) and torch.equal(more, scales)
+    weight = normal(6, cols)
+    want = q8.rms_norm(x, x, weight, "bf16")
+    total = torch.empty(3, far, dtype=torch.bfloat16, device="cuda")[:, :cols]
+    got = q8.rms_norm(apart, apart, weight, "bf16", in_place=total)
+    assert all(torch.equal(g, w) for g, w in zip(got, want))
+    u = torch.tensor([0.1, 0.5, 0.9])
+    assert list(q8.sample(apart, "bf16", u, top_p=0.9)[0]) == list(q8.sample(x, "bf16", u, top_p=0.9)[0])
+
+
+@pytest.mark.parametrize("m,k", [(3, 640), (3, 8), (3, 100)])
+def test_products_with_rows_farther_apart_than_32_bits(m, k):
+    far = (1 << 30) + 16
+    a, b, sa, sb = operands(m, 300, k, "f32")
+    residual = normal(1, m, 300, dt="f32")
+    want, _ = q8.gemm(a, b, sa, sb, "f32", None, residual)
+    place = torch.empty(m, far, device="cuda")
+    place[:, :300] = residual
+    got, _ = q8.gemm(a, b, sa, sb, "f32", None, place, ldc=far, out=place)
+    assert torch.equal(got[:, :300], want)
+    apart = torch.empty(m, far, dtype=torch.int8, device="cuda")[:, :k]
+    apart.copy_(a)
+    got, kernel = q8.gemm(apart, b, sa, sb, "f32", None, residual)
+    assert kernel == "generic" and torch.equal(got, want)
