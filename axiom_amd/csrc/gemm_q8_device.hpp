@@ -29,6 +29,17 @@ __device__ __forceinline__ int4_t q8_mfma(const uint4_t &fb, const uint4_t &fa, 
 // have the same bits whichever kernel the other rows lead to.
 __device__ __forceinline__ float q8_scaled(int sum, float sa, float sb, float bias) { return __builtin_fmaf(static_cast<float>(sum), sa * sb, bias); }
 
+// The activation of N values.  What is not a number stays so (v_maximum3_f32, where x > 0 ? x : 0 makes it a zero): a row with an infinity has scale NaN, and is not to
+// leave a layer as zeros.
+template <bool HALF, int N> __device__ __forceinline__ void q8_activation(int op, float (&x)[N]) {
+    if (op == AXHIP_OP_RELU) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[e] = __builtin_elementwise_maximum(x[e], 0.0f);
+    } else {
+        gemm_epilogue_all_as<HALF>(op, x);
+    }
+}
+
 // N sums of a row, to C from `at` on, of which the first `last` exist: scales (scale_b's in sb, bias in b), residual, activation.
 template <int DT, int N>
 __device__ __forceinline__ void q8_finish(const Q8Args &g, const int (&sum)[N], float sa, const float (&sb)[N], const float (&b)[N], int64_t at, int last) {
@@ -48,7 +59,7 @@ __device__ __forceinline__ void q8_finish(const Q8Args &g, const int (&sum)[N], 
                 if (e < last) x[e] += Elem<DT>::load(g.residual, at + e);
         }
     }
-    gemm_epilogue_all_as<DT != AXHIP_DTYPE_F32>(g.epilogue, x);
+    q8_activation<DT != AXHIP_DTYPE_F32>(g.epilogue, x);
     if (whole) {
         store_vec<N, true>(g.c, DT, at, x);
     } else {
@@ -164,7 +175,7 @@ __device__ __forceinline__ void q8_store_blocks(const Q8Args &g, const int4_t (&
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[4 * h + e] = v[e];
         }
-        gemm_epilogue_all_as<DT != AXHIP_DTYPE_F32>(g.epilogue, x);
+        q8_activation<DT != AXHIP_DTYPE_F32>(g.epilogue, x);
         const int64_t to = static_cast<int64_t>(row) * g.ldc + col;
         if (last == 8) {
             store_vec<8, true>(g.c, DT, to, x);
