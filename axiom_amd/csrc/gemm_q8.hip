@@ -36,8 +36,9 @@ __global__ __launch_bounds__(256) void gemm_q8_generic_kernel(const GenericArgs 
     if (m < g.M && n < g.N) {
         float y[1] = {q8_scaled(acc, g.scale_a[m], g.scale_b[n], g.bias ? load_any(g.bias, g.dtype, n) : 0.0f)};
         if (g.residual) y[0] += load_any(g.residual, g.dtype, m * g.ldc + n);
-        if (g.dtype == AXHIP_DTYPE_F32) q8_activation<false>(g.epilogue, y);
-        else q8_activation<true>(g.epilogue, y);
+        if (g.dtype == AXHIP_DTYPE_F32) q8_activation<AXHIP_DTYPE_F32>(g.epilogue, y);
+        else if (g.dtype == AXHIP_DTYPE_F16) q8_activation<AXHIP_DTYPE_F16>(g.epilogue, y);
+        else q8_activation<AXHIP_DTYPE_BF16>(g.epilogue, y);
         store_any(g.c, g.dtype, m * g.ldc + n, y[0]);
     }
 }

@@ -29,12 +29,37 @@ __device__ __forceinline__ int4_t q8_mfma(const uint4_t &fb, const uint4_t &fa, 
 // have the same bits whichever kernel the other rows lead to.
 __device__ __forceinline__ float q8_scaled(int sum, float sa, float sb, float bias) { return __builtin_fmaf(static_cast<float>(sum), sa * sb, bias); }
 
+// x Phi(x) = max(x, 0) - z Phi(-z), z = |x|, for results of 16 bits, with Phi(-z) = 2^P(z): P is fitted to log2 Phi(-z) with all errors of one size, so that the left tail keeps its
+// digits: within 2^-17.5 of itself for f16 (degree 7 up to 5.75, behind which no f16 is left but zero), 2^-12.8 for bf16 (degree 8 up to 13.1, where 2^P is below fp32's normal
+// numbers and zero).  0 at -infinity.
+template <int DT> __device__ __forceinline__ float q8_gelu16(float x) {
+    constexpr float F16[] = {-1.82547734e-06f, 6.14397908e-05f, -0.000929487263f, 0.00850459774f, -0.0539548469f, -0.458468208f, -1.15125004f, -0.999995335f};
+    constexpr float BF16[] = {2.78745644e-08f, -1.76587942e-06f, 4.82301422e-05f, -0.000750397564f, 0.00745485316f, -0.050910629f, -0.462621502f, -1.14912834f, -1.00017551f};
+    const float z = fminf(fabsf(x), DT == AXHIP_DTYPE_F16 ? 5.75f : 13.1f);
+    float p = DT == AXHIP_DTYPE_F16 ? F16[0] : BF16[0];
+#pragma unroll
+    for (int i = 1; i < (DT == AXHIP_DTYPE_F16 ? 8 : 9); ++i) p = __builtin_fmaf(p, z, DT == AXHIP_DTYPE_F16 ? F16[i < 8 ? i : 0] : BF16[i]);
+    return __builtin_fmaf(-z, __builtin_amdgcn_exp2f(p), __builtin_elementwise_maximum(x, 0.0f));
+}
+// ... tanh within 2^-20 of itself: its series up to 1/4 (the next term is 3e-7 of the first), from there on by one exponential
+__device__ __forceinline__ float q8_tanh16(float x) {
+    const float s = x * x, far = 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + __expf(2.0f * x));
+    const float near = x * __builtin_fmaf(s, __builtin_fmaf(s, __builtin_fmaf(s, -0.053968254f, 0.13333333f), -0.33333333f), 1.0f);
+    return s < 0.0625f ? near : far;
+}
 // The activation of N values.  What is not a number stays so (v_maximum3_f32, where x > 0 ? x : 0 makes it a zero): a row with an infinity has scale NaN, and is not to
 // leave a layer as zeros.
-template <bool HALF, int N> __device__ __forceinline__ void q8_activation(int op, float (&x)[N]) {
+template <int DT, int N> __device__ __forceinline__ void q8_activation(int op, float (&x)[N]) {
+    constexpr bool HALF = DT != AXHIP_DTYPE_F32;
     if (op == AXHIP_OP_RELU) {
 #pragma unroll
         for (int e = 0; e < N; ++e) x[e] = __builtin_elementwise_maximum(x[e], 0.0f);
+    } else if (HALF && op == AXHIP_OP_GELU) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[e] = q8_gelu16<DT>(x[e]);
+    } else if (HALF && op == AXHIP_OP_TANH) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[e] = q8_tanh16(x[e]);
     } else {
         gemm_epilogue_all_as<HALF>(op, x);
     }
@@ -59,7 +84,7 @@ __device__ __forceinline__ void q8_finish(const Q8Args &g, const int (&sum)[N], 
                 if (e < last) x[e] += Elem<DT>::load(g.residual, at + e);
         }
     }
-    q8_activation<DT != AXHIP_DTYPE_F32>(g.epilogue, x);
+    q8_activation<DT>(g.epilogue, x);
     if (whole) {
         store_vec<N, true>(g.c, DT, at, x);
     } else {
@@ -175,7 +200,7 @@ __device__ __forceinline__ void q8_store_blocks(const Q8Args &g, const int4_t (&
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[4 * h + e] = v[e];
         }
-        q8_activation<DT != AXHIP_DTYPE_F32>(g.epilogue, x);
+        q8_activation<DT>(g.epilogue, x);
         const int64_t to = static_cast<int64_t>(row) * g.ldc + col;
         if (last == 8) {
             store_vec<8, true>(g.c, DT, to, x);

@@ -77,7 +77,7 @@ __global__ __launch_bounds__(256) void gemm_q8_skinny_kernel(const Q8Args a) {
     for (int i = 0; i < P; ++i) v[i] = acc[i / R][i % R];
     const int sum = q8_lane_sums<P>(v, lane);
     float x[1] = {q8_scaled(sum, sa, sb, bias) + residual};
-    q8_activation<DT != AXHIP_DTYPE_F32>(a.epilogue, x);
+    q8_activation<DT>(a.epilogue, x);
     if (writes) Elem<DT>::store(a.c, at, x[0]);
 }
 

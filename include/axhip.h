@@ -493,7 +493,9 @@ int axhip_rms_norm_q8(const void *x, const void *residual, const void *weight, v
  * nn::Linear (src/nn/linear.cpp:15-27) on rows in 8 bits: C = act(scale_a[m] scale_b[n] sum_k A[m][k] B[n][k] (+ bias[n]) (+ residual)),
  * A (m, k) and B (n, k) int8, row-major, lda / ldb / ldc in elements, any alignment.  The sums are int32 and exact: k up to
  * 131071, beyond which rows of -128 could overflow (AXHIP_ERR_UNSUPPORTED).  scale_a [m] and scale_b [n] are fp32; the rest is fp32 arithmetic (the sum as a
- * float times the scales' product, plus bias, rounded once; plus residual), rounded once to dtype: a row of C has the same bits whatever the other rows are and however many.
+ * float times the scales' product, plus bias, rounded once; plus residual), the activation (of Float32 results within 2e-6 (1 + |y|) of its value y, of 16-bit ones within 2^-15 |y|, GELU
+ * to BFloat16 within 2^-12 |y| and 2^-122), rounded once to dtype: a row of C has the same bits whatever the other rows are and however many (a NaN's own bits
+ * aside).  What is not a number stays so under every activation.
  * residual has C's layout and may be C itself.  No temporary memory. */
 typedef struct {
     int32_t dtype;       /* of C, bias and residual: Float32, Float16 or BFloat16 */
