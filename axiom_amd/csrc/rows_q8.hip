@@ -38,10 +38,14 @@ __device__ __forceinline__ double wave_largest(double v) {
     return v;
 }
 
+// Products of two fp32 numbers may be as small as 2^-298: what a row of them is multiplied by (a power of two, exactly) so that 127 / a is an ordinary number.
+__device__ __forceinline__ double bringing_up(double largest) { return largest > 0.0 ? __builtin_amdgcn_ldexp(1.0, -__builtin_amdgcn_frexp_exp(largest)) : 1.0; }
+
 // E values -> E bytes.  127 y / a rounds to the nearest integer through the sum with 1.5 * 2^23, whose last bit is a one: the low byte of
-// the sum is the integer.  The product with 127 / a is off by less than 3 * 2^-24 * 127 < 4e-5; where it lies that close to a half (4 % of
-// the wavefront's vectors), and where 127 / a would overflow (`tiny`), the quotient is formed in 64 bits, which tell every
-// product of two numbers of up to 24 bits from a half and find the half itself where it is one.
+// the sum is the integer.  The product with 127 / a is off by less than 3 * 2^-24 * 127 < 4e-5; where it lies that close to a half h (4 % of
+// the wavefront's vectors), and where 127 / a would overflow (`tiny`), it is decided exactly.  Of y and a of 24 bits the quotient in 64 bits tells: it is the half itself or
+// 2^-34 from it at least.  Products of two fp32 numbers have 48 bits and quotients as near as 2^-49, where steps are 2^-46: of them the sign of 127 y - h a decides, and where that is
+// nothing the even integer is taken.  With s = h a to 53 bits, 127 y - s and h a - s are multiples of 2^-56 a and below 2^-14 a, so that two fused operations round neither.
 template <int E, class Y> __device__ __forceinline__ void quantize(const Y (&y)[E], float inverse, Y largest, bool tiny, uint32_t (&w)[E / 4]) {
     constexpr float TO_INTEGER = 12582912.0f, NEAR_HALF = 0.49996f;
     uint32_t r[E];
@@ -52,10 +56,22 @@ template <int E, class Y> __device__ __forceinline__ void quantize(const Y (&y)[
         off = fmaxf(off, fabsf(__builtin_fmaf(v, inverse, TO_INTEGER - s)));
         r[e] = __float_as_uint(s);
     }
-    if (off > NEAR_HALF || tiny) {
-        for (int e = 0; e < E; ++e) {
-            const int q = static_cast<int>(__builtin_rint(127.0 * static_cast<double>(y[e]) / static_cast<double>(largest)));
-            r[e] = static_cast<uint32_t>(q);
+    if (off > NEAR_HALF || (tiny && !std::is_same_v<Y, double>)) { // (products of fp32 numbers have been brought up)
+        if constexpr (std::is_same_v<Y, double>) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float n = __uint_as_float(r[e]) - TO_INTEGER, from = __builtin_fmaf(static_cast<float>(y[e]), inverse, -n);
+                const double half = n + __builtin_copysignf(0.5f, from), s = half * largest;
+                const double left = __builtin_fma(127.0, y[e], -s) - __builtin_fma(half, largest, -s);
+                const bool behind = (from > 0.0f) == (left > 0.0); // the half, as seen from n
+                const bool moves = (fabsf(from) > NEAR_HALF) & (((left != 0.0) & behind) | ((left == 0.0) & static_cast<bool>(r[e] & 1u)));
+                r[e] += moves ? (from > 0.0f ? 1u : ~0u) : 0u;
+            }
+        } else {
+            for (int e = 0; e < E; ++e) {
+                const int q = static_cast<int>(__builtin_rint(127.0 * static_cast<double>(y[e]) / static_cast<double>(largest)));
+                r[e] = static_cast<uint32_t>(q);
+            }
         }
     }
 #pragma unroll
@@ -179,7 +195,23 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void rows_q8_kernel(const RowsQ8
         }
         const float top = static_cast<float>(largest);
         const bool finite = __float_as_uint(top) < 0x7F800000u, tiny = top < 1e-30f;
-        const float inverse = tiny ? 0.0f : 127.0f / top;
+        if (lane == 0) { // (here, not behind the integers: nothing of it takes registers there)
+            float scale = top;
+            if constexpr (MODE != QUANTIZE) scale *= 1.0f / sqrtf(squares / static_cast<float>(a.cols) + a.eps);
+            a.scales[row] = !finite ? __uint_as_float(0x7FC00000u) : top > 0.0f ? scale / 127.0f : 0.0f;
+        }
+        float inverse = tiny ? 0.0f : 127.0f / top;
+        if constexpr (std::is_same_v<Y, double>) {
+            if (tiny) {
+                const double up = bringing_up(largest);
+                largest *= up;
+                inverse = 127.0f / static_cast<float>(largest);
+#pragma unroll
+                for (int i = 0; i < IT; ++i)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) y[i][e] *= up;
+            }
+        }
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
             const int64_t at = static_cast<int64_t>(i * G + lane) * E;
@@ -188,11 +220,6 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void rows_q8_kernel(const RowsQ8
                 if (finite && largest > 0) quantize<E, Y>(y[i], inverse, largest, tiny, w);
                 store_bytes<E, UNALIGNED>(a.q + row * a.ld_q, at, a.cols - at, w);
             }
-        }
-        if (lane == 0) {
-            float scale = top;
-            if constexpr (MODE != QUANTIZE) scale *= 1.0f / sqrtf(squares / static_cast<float>(a.cols) + a.eps);
-            a.scales[row] = !finite ? __uint_as_float(0x7FC00000u) : top > 0.0f ? scale / 127.0f : 0.0f;
         }
     }
 }
@@ -236,7 +263,15 @@ __global__ __launch_bounds__(1024) void rows_q8_long_kernel(const RowsQ8Args a) 
         }
         const float top = static_cast<float>(largest);
         const bool finite = __float_as_uint(top) < 0x7F800000u, tiny = top < 1e-30f;
-        const float inverse = tiny ? 0.0f : 127.0f / top;
+        float inverse = tiny ? 0.0f : 127.0f / top;
+        Y up = 1;
+        if constexpr (std::is_same_v<Y, double>) {
+            if (tiny) {
+                up = bringing_up(largest);
+                largest *= up;
+                inverse = 127.0f / static_cast<float>(largest);
+            }
+        }
         RowsQ8Args again = a;
         if (MODE == NORM_RESIDUAL && a.sum) {
             again.x = a.sum;
@@ -249,6 +284,10 @@ __global__ __launch_bounds__(1024) void rows_q8_long_kernel(const RowsQ8Args a) 
             if (MODE == NORM_RESIDUAL && a.sum) make_products<DT, MODE == QUANTIZE ? QUANTIZE : NORM, E, true>(again, row, at, a.cols - at, h, y);
             else make_products<DT, MODE, E, true>(again, row, at, a.cols - at, h, y);
             uint32_t w[E / 4] = {};
+            if constexpr (std::is_same_v<Y, double>) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) y[e] *= up;
+            }
             if (finite && largest > 0) quantize<E, Y>(y, inverse, largest, tiny, w);
             store_bytes<E, true>(a.q + row * a.ld_q, at, a.cols - at, w);
         }

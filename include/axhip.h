@@ -466,7 +466,8 @@ const char *axhip_gemm_last_kernel(void);
 
 /* ------------------------------------------------------------- 8-bit rows
  * Rows of values as int8 with one fp32 scale each: q[r][j] * scales[r] stands for the value.  q lies in [-127, 127]; the nearest
- * integer is taken, halves to the even one, decided on exact products (a value next to a half falls on the right side of it).
+ * integer is taken, halves to the even one, decided on exact products (a value next to a half falls on the right side of it; only of a BFloat16 norm's row whose largest product lies
+ * below 2^-118 the products are those that fp32's subnormal numbers hold).
  * A row of zeros has scale 0; a row that holds an infinity or a NaN (or whose products overflow fp32) has scale NaN and zeros, so
  * that every product with it comes out as NaN.  Rows are contiguous, ld_* elements apart (at least cols; any alignment).
  *
