@@ -14,6 +14,7 @@ struct RowsQ8Args {
     float *scales;
     int64_t rows, ld_x, ld_residual, ld_sum, ld_q;
     int64_t cols;
+    double inverse_cols;
     float eps;
     int blocks;
 };
@@ -32,10 +33,55 @@ __device__ __forceinline__ double larger(double a, double b) { return __longlong
 __device__ __forceinline__ float magnitude(float v) { return fabsf(v); }
 __device__ __forceinline__ double magnitude(double v) { return fabs(v); }
 __device__ __forceinline__ float wave_largest(float v) { return wave_all(v, [](float a, float b) { return larger(a, b); }); }
-__device__ __forceinline__ double wave_largest(double v) {
-#pragma unroll
-    for (int d = 32; d; d /= 2) v = larger(v, __shfl_xor(v, d, WAVE));
+// wave_all of common.hpp in 64 bits
+template <class F> __device__ __forceinline__ double wave_all64(double v, F combine) {
+    auto low = [](double x) { return static_cast<uint32_t>(__double_as_longlong(x)); };
+    auto high = [](double x) { return static_cast<uint32_t>(static_cast<uint64_t>(__double_as_longlong(x)) >> 32); };
+    auto whole = [](uint32_t lo, uint32_t hi) { return __longlong_as_double(static_cast<long long>(static_cast<uint64_t>(hi) << 32 | lo)); };
+    const auto lo32 = __builtin_amdgcn_permlane32_swap(low(v), low(v), false, false), hi32 = __builtin_amdgcn_permlane32_swap(high(v), high(v), false, false);
+    v = combine(whole(lo32[0], hi32[0]), whole(lo32[1], hi32[1]));
+    const auto lo16 = __builtin_amdgcn_permlane16_swap(low(v), low(v), false, false), hi16 = __builtin_amdgcn_permlane16_swap(high(v), high(v), false, false);
+    v = combine(whole(lo16[0], hi16[0]), whole(lo16[1], hi16[1]));
+    auto across = [&](auto control) __attribute__((always_inline)) { // (row_ror)
+        const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(low(v)), decltype(control)::value, 0xF, 0xF, false);
+        const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(high(v)), decltype(control)::value, 0xF, 0xF, false);
+        v = combine(v, whole(lo, hi));
+    };
+    across(std::integral_constant<int, 0x128>{});
+    across(std::integral_constant<int, 0x124>{});
+    across(std::integral_constant<int, 0x122>{});
+    across(std::integral_constant<int, 0x121>{});
     return v;
+}
+__device__ __forceinline__ double wave_largest(double v) { return wave_all64(v, [](double a, double b) { return larger(a, b); }); }
+__device__ __forceinline__ float sum_of_wave(float v) { return wave_sum(v); }
+__device__ __forceinline__ double sum_of_wave(double v) { return wave_all64(v, [](double a, double b) { return a + b; }); }
+
+// The sum of squares: those of f16 numbers lie within fp32's range, those of bf16 and fp32 ones from 2^-298 to 2^256.
+__device__ __forceinline__ float add_square(float h, float sum) { return __builtin_fmaf(h, h, sum); }
+__device__ __forceinline__ double add_square(float h, double sum) { return __builtin_fma(static_cast<double>(h), static_cast<double>(h), sum); }
+template <int DT> using Squares = std::conditional_t<DT == AXHIP_DTYPE_F16, float, double>;
+
+__device__ __forceinline__ float mantissa(float v, int &exponent) {
+    exponent = __builtin_amdgcn_frexp_expf(v);
+    return __builtin_amdgcn_frexp_mantf(v);
+}
+__device__ __forceinline__ float mantissa(double v, int &exponent) {
+    exponent = __builtin_amdgcn_frexp_exp(v);
+    return static_cast<float>(__builtin_amdgcn_frexp_mant(v));
+}
+// The row's scale: largest / 127, over the root of mean(h^2) + eps for a norm.  Mantissas in fp32, with their powers of two by themselves: neither the mean nor the largest need be an fp32 number,
+// the scale alone.
+template <int MODE, class Y, class S> __device__ __forceinline__ float scale_of(const RowsQ8Args &a, Y largest, S squares) {
+    const float top = static_cast<float>(largest);
+    if (!(__float_as_uint(top) < 0x7F800000u)) return __uint_as_float(0x7FC00000u);
+    if (!(largest > 0)) return 0.0f;
+    if constexpr (MODE == QUANTIZE) return top / 127.0f;
+    const double mean = static_cast<double>(squares) * a.inverse_cols + static_cast<double>(a.eps);
+    const int even = (__builtin_amdgcn_frexp_exp(mean) - 1) & ~1;
+    int exponent;
+    const float m = mantissa(largest, exponent);
+    return __builtin_amdgcn_ldexpf(m * (1.0f / sqrtf(static_cast<float>(__builtin_amdgcn_ldexp(mean, -even)))) / 127.0f, exponent - even / 2);
 }
 
 // Products of two fp32 numbers may be as small as 2^-298: what a row of them is multiplied by (a power of two, exactly) so that 127 / a is an ordinary number.
@@ -156,14 +202,15 @@ __device__ __forceinline__ void make_products(const RowsQ8Args &a, int64_t row, 
 template <int DT, int MODE, int G, int IT, bool UNALIGNED>
 __global__ __launch_bounds__(G < 256 ? 256 : G) void rows_q8_kernel(const RowsQ8Args a) {
     using Y = Product<DT, MODE>;
+    using S = Squares<DT>;
     constexpr int E = DT == AXHIP_DTYPE_F32 ? 4 : 8, ROWS = G < 256 ? 256 / G : 1, WAVES = G / WAVE;
     __shared__ Y s_largest[2][WAVES > 1 ? WAVES : 1];
-    __shared__ float s_squares[2][WAVES > 1 ? WAVES : 1];
+    __shared__ S s_squares[2][WAVES > 1 ? WAVES : 1];
     const int lane = threadIdx.x % G, wave = threadIdx.x / WAVE;
     int turn = 0;
     for (int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / G; row < a.rows; row += static_cast<int64_t>(a.blocks) * ROWS, turn ^= 1) {
         Y y[IT][E], largest = 0;
-        float squares = 0.0f;
+        S squares = 0;
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
             const int64_t at = static_cast<int64_t>(i * G + lane) * E;
@@ -173,32 +220,28 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void rows_q8_kernel(const RowsQ8
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     largest = larger(largest, magnitude(y[i][e]));
-                    if constexpr (MODE != QUANTIZE) squares = __builtin_fmaf(h[e], h[e], squares);
+                    if constexpr (MODE != QUANTIZE) squares = add_square(h[e], squares);
                 }
             }
         }
         largest = wave_largest(largest);
-        if constexpr (MODE != QUANTIZE) squares = wave_sum(squares);
+        if constexpr (MODE != QUANTIZE) squares = sum_of_wave(squares);
         if constexpr (WAVES > 1) {
             if (threadIdx.x % WAVE == 0) {
                 s_largest[turn][wave] = largest;
-                s_squares[turn][wave] = squares;
+                if constexpr (MODE != QUANTIZE) s_squares[turn][wave] = squares;
             }
             __syncthreads(); // (the next row uses the other set, and meets here before this one is written again)
             largest = s_largest[turn][0];
-            squares = s_squares[turn][0];
 #pragma unroll
-            for (int w = 1; w < WAVES; ++w) {
-                largest = larger(largest, s_largest[turn][w]);
-                squares += s_squares[turn][w];
-            }
+            for (int w = 1; w < WAVES; ++w) largest = larger(largest, s_largest[turn][w]);
         }
         const float top = static_cast<float>(largest);
         const bool finite = __float_as_uint(top) < 0x7F800000u, tiny = top < 1e-30f;
         if (lane == 0) { // (here, not behind the integers: nothing of it takes registers there)
-            float scale = top;
-            if constexpr (MODE != QUANTIZE) scale *= 1.0f / sqrtf(squares / static_cast<float>(a.cols) + a.eps);
-            a.scales[row] = !finite ? __uint_as_float(0x7FC00000u) : top > 0.0f ? scale / 127.0f : 0.0f;
+            if constexpr (MODE != QUANTIZE && WAVES > 1)
+                for (int w = 1; w < WAVES; ++w) squares += s_squares[turn][w]; // (lane 0 is of wavefront 0)
+            a.scales[row] = scale_of<MODE>(a, largest, squares);
         }
         float inverse = tiny ? 0.0f : 127.0f / top;
         if constexpr (std::is_same_v<Y, double>) {
@@ -229,26 +272,27 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void rows_q8_kernel(const RowsQ8
 template <int DT, int MODE>
 __global__ __launch_bounds__(1024) void rows_q8_long_kernel(const RowsQ8Args a) {
     using Y = Product<DT, MODE>;
+    using S = Squares<DT>;
     constexpr int E = DT == AXHIP_DTYPE_F32 ? 4 : 8;
     __shared__ Y s_largest[16];
-    __shared__ float s_squares[16];
+    __shared__ S s_squares[16];
     for (int64_t row = blockIdx.x; row < a.rows; row += a.blocks) {
         Y largest = 0;
-        float squares = 0.0f;
+        S squares = 0;
         for (int64_t at = threadIdx.x * E; at < a.cols; at += 1024 * E) {
             float h[E];
             Y y[E];
             make_products<DT, MODE, E, true>(a, row, at, a.cols - at, h, y);
-            float part = 0.0f;
+            S part = 0;
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 largest = larger(largest, magnitude(y[e]));
-                part = __builtin_fmaf(h[e], h[e], part);
+                if constexpr (MODE != QUANTIZE) part = add_square(h[e], part);
             }
             squares += part;
         }
         largest = wave_largest(largest);
-        squares = wave_sum(squares);
+        if constexpr (MODE != QUANTIZE) squares = sum_of_wave(squares);
         __syncthreads();
         if (threadIdx.x % WAVE == 0) {
             s_largest[threadIdx.x / WAVE] = largest;
@@ -261,6 +305,7 @@ __global__ __launch_bounds__(1024) void rows_q8_long_kernel(const RowsQ8Args a) 
             largest = larger(largest, s_largest[w]);
             squares += s_squares[w];
         }
+        if (threadIdx.x == 0) a.scales[row] = scale_of<MODE>(a, largest, squares);
         const float top = static_cast<float>(largest);
         const bool finite = __float_as_uint(top) < 0x7F800000u, tiny = top < 1e-30f;
         float inverse = tiny ? 0.0f : 127.0f / top;
@@ -290,11 +335,6 @@ __global__ __launch_bounds__(1024) void rows_q8_long_kernel(const RowsQ8Args a) 
             }
             if (finite && largest > 0) quantize<E, Y>(y, inverse, largest, tiny, w);
             store_bytes<E, true>(a.q + row * a.ld_q, at, a.cols - at, w);
-        }
-        if (threadIdx.x == 0) {
-            float scale = top;
-            if constexpr (MODE != QUANTIZE) scale *= 1.0f / sqrtf(squares / static_cast<float>(a.cols) + a.eps);
-            a.scales[row] = !finite ? __uint_as_float(0x7FC00000u) : top > 0.0f ? scale / 127.0f : 0.0f;
         }
     }
 }
@@ -347,7 +387,7 @@ int rows_q8(const char *who, int mode, const void *x, const void *residual, cons
     const int64_t e = p.dtype == AXHIP_DTYPE_F32 ? 4 : 8;
     const bool aligned = ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(residual) | reinterpret_cast<uintptr_t>(weight) | reinterpret_cast<uintptr_t>(sum)) & 15u) == 0 &&
                          reinterpret_cast<uintptr_t>(q) % e == 0 && (p.ld_x | p.ld_q | (residual ? p.ld_residual : 0) | (sum ? p.ld_sum : 0)) % e == 0;
-    const RowsQ8Args a{x, residual, weight, sum, q, scales, p.rows, p.ld_x, p.ld_residual, p.ld_sum, p.ld_q, p.cols, p.eps, 0};
+    const RowsQ8Args a{x, residual, weight, sum, q, scales, p.rows, p.ld_x, p.ld_residual, p.ld_sum, p.ld_q, p.cols, 1.0 / static_cast<double>(p.cols), p.eps, 0};
     hipStream_t s = resolve_stream(stream);
     if (mode == QUANTIZE) launch_dtype<QUANTIZE>(a, p.dtype, aligned, s);
     else if (!residual) launch_dtype<NORM>(a, p.dtype, aligned, s);

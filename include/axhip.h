@@ -466,8 +466,8 @@ const char *axhip_gemm_last_kernel(void);
 
 /* ------------------------------------------------------------- 8-bit rows
  * Rows of values as int8 with one fp32 scale each: q[r][j] * scales[r] stands for the value.  q lies in [-127, 127]; the nearest
- * integer is taken, halves to the even one, decided on exact products (a value next to a half falls on the right side of it; only of a BFloat16 norm's row whose largest product lies
- * below 2^-118 the products are those that fp32's subnormal numbers hold).
+ * integer is taken, halves to the even one, decided on exact products (a value next to a half falls on the right side of it; only of
+ * a BFloat16 norm's row whose largest product lies below 2^-118 the products are those that fp32's subnormal numbers hold).
  * A row of zeros has scale 0; a row that holds an infinity or a NaN (or whose products overflow fp32) has scale NaN and zeros, so
  * that every product with it comes out as NaN.  Rows are contiguous, ld_* elements apart (at least cols; any alignment).
  *
@@ -476,9 +476,10 @@ const char *axhip_gemm_last_kernel(void);
  * axhip_rms_norm_q8: the residual's addition and the RMS norm of a pre-norm block (ops::add, then ops::rms_norm,
  * include/axiom/operations.hpp and src/nn/normalization.cpp), out in 8 bits for the product that follows: with
  *     h = x + residual, rounded to dtype (residual NULL: h = x),   y = h / sqrt(mean(h^2) + eps) * weight
- * q and scales stand for y, which is rounded nowhere else; the statistics are fp32.  sum: NULL, or where h goes for the
- * next residual addition (x or residual itself, with the same ld, is allowed; needs a residual).  x, residual, weight (NULL: ones) and sum are of
- * `dtype`.  No temporary memory; axhip_quantize_q8 reads dtype, rows, cols, ld_x and ld_q only. */
+ * q and scales stand for y, which is rounded nowhere else; the squares are summed up in 64 bits (of Float16 rows in 32), so that
+ * rows whose squares are beyond fp32 have their scale too.  sum: NULL, or where h goes for the next residual addition (x or residual
+ * itself, with the same ld, is allowed; needs a residual).  x, residual, weight (NULL: ones) and sum are of `dtype`.  No temporary
+ * memory; axhip_quantize_q8 reads dtype, rows, cols, ld_x and ld_q only. */
 typedef struct {
     int32_t dtype; /* of x, residual, weight and sum */
     float eps;
