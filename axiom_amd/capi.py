@@ -95,9 +95,10 @@ class GemmQ8Params(C.Structure):
 
 class SampleParams(C.Structure):
     _fields_ = [
-        ("dtype", C.c_int32),
+        ("dtype", C.c_int32), ("uniform", C.c_int32),
         ("rows", C.c_int64), ("vocab", C.c_int64), ("ld", C.c_int64),
         ("temperature", C.c_void_p), ("top_k", C.c_void_p), ("top_p", C.c_void_p), ("min_p", C.c_void_p), ("u", C.c_void_p),
+        ("all_temperature", C.c_float), ("all_top_k", C.c_int32), ("all_top_p", C.c_float), ("all_min_p", C.c_float),
     ]
 
 

@@ -13,6 +13,8 @@ struct SampleArgs {
     const float *top_p, *min_p, *u;
     int64_t ld;
     int vocab;
+    int32_t all_top_k; // where there is no array
+    float all_temperature, all_top_p, all_min_p;
 };
 
 constexpr int64_t MOST_VOCAB = 1 << 20;

@@ -509,10 +509,10 @@ template <int DT, int IT> __global__ __launch_bounds__(THREADS) void sample_kern
         });
     };
 
-    float temperature = a.temperature ? a.temperature[row] : 1.0f;
+    float temperature = a.temperature ? a.temperature[row] : a.all_temperature;
     temperature = temperature > 1e30f ? 1e30f : temperature;
-    const float p = a.top_p ? a.top_p[row] : 1.0f, m = a.min_p ? a.min_p[row] : 0.0f, u = a.u[row];
-    const int32_t k = a.top_k && a.top_k[row] > 0 && a.top_k[row] < a.vocab ? a.top_k[row] : 0;
+    const float p = a.top_p ? a.top_p[row] : a.all_top_p, m = a.min_p ? a.min_p[row] : a.all_min_p, u = a.u[row];
+    const int32_t asked = a.top_k ? a.top_k[row] : a.all_top_k, k = asked > 0 && asked < a.vocab ? asked : 0;
     if (t == 0) sh.inside = 0;
     if (t < 32) sh.pow2[t] = static_cast<uint64_t>(__double_as_longlong(exp2(43.0 + t * (1.0 / 32.0)))) - (uint64_t(t) << 47); // (a barrier before they are used)
     r.pow2 = sh.pow2;

@@ -42,7 +42,7 @@ struct Sampled {
 };
 // Tokens by given random numbers u in [0, 1) (Float32, one for each row): see axhip_sample for what the settings keep and which token u falls on.
 Sampled sample(const Tensor &logits, const Tensor &u, const SampleSettings &settings);
-// the same settings for every row: temperature 0 is greedy; top_k 0, top_p 1 and min_p 0 are off
+// the same settings for every row (they go with the launch: nothing is copied or waited for): temperature 0 is greedy; top_k 0, top_p 1 and min_p 0 are off
 Sampled sample(const Tensor &logits, const Tensor &u, float temperature = 1.0f, int top_k = 0, float top_p = 1.0f, float min_p = 0.0f);
 
 } // namespace ops

@@ -117,14 +117,16 @@ Tensor linear_int8(const Quantized &x, const Quantized &weight, const Tensor &bi
 }
 Tensor linear_int8(const Quantized &x, const Quantized &weight, DType dtype) { return linear_int8(x, weight, Tensor(), Tensor(), "none", dtype); }
 
-Sampled sample(const Tensor &logits, const Tensor &u, const SampleSettings &settings) {
+namespace {
+// The checks of both forms; `settings` puts the settings of so many rows into the parameters and keeps the tensors they lie in.
+template <class F> Sampled draw(const Tensor &logits, const Tensor &u, F settings) {
     const char *who = "sample";
     need_gpu(who, logits);
     need_floating(who, logits);
     if (logits.ndim() == 0 || logits.shape().back() == 0) throw ShapeError("sample: logits (..., vocabulary)");
     const Shape out_shape = without_last(logits.shape());
     const size_t rows = ShapeUtils::size(out_shape);
-    auto setting = [&](const char *what, const Tensor &t, DType want) {
+    auto of_rows = [&](const char *what, const Tensor &t, DType want) {
         if (t.empty()) return Tensor();
         need_gpu(who, t);
         need_type(who, what, t, want);
@@ -132,32 +134,40 @@ Sampled sample(const Tensor &logits, const Tensor &u, const SampleSettings &sett
         return settled(t);
     };
     if (u.empty()) throw ValueError("sample: a random number for each row");
-    const Tensor src = settled(logits), un = setting("u", u, DType::Float32), temperature = setting("temperature", settings.temperature, DType::Float32),
-                 top_k = setting("top_k", settings.top_k, DType::Int32), top_p = setting("top_p", settings.top_p, DType::Float32), min_p = setting("min_p", settings.min_p, DType::Float32);
+    const Tensor src = settled(logits), un = of_rows("u", u, DType::Float32);
     AxhipSampleParams p{};
     p.dtype = ::axiom::detail::to_axhip_dtype(src.dtype());
     p.rows = static_cast<int64_t>(rows);
     p.vocab = p.ld = static_cast<int64_t>(logits.shape().back());
-    p.temperature = reinterpret_cast<const float *>(at(temperature));
-    p.top_k = reinterpret_cast<const int32_t *>(at(top_k));
-    p.top_p = reinterpret_cast<const float *>(at(top_p));
-    p.min_p = reinterpret_cast<const float *>(at(min_p));
     p.u = reinterpret_cast<const float *>(at(un));
+    [[maybe_unused]] const auto kept = settings(p, of_rows);
     Sampled out{Tensor(out_shape, DType::Int64, Device::GPU), Tensor(out_shape, DType::Float32, Device::GPU)};
     AXHIP_CALL(axhip_sample(at(src), reinterpret_cast<int64_t *>(out_at(out.tokens)), reinterpret_cast<float *>(out_at(out.probabilities)), &p, nullptr));
     return out;
 }
+} // namespace
+
+Sampled sample(const Tensor &logits, const Tensor &u, const SampleSettings &settings) {
+    return draw(logits, u, [&](AxhipSampleParams &p, auto of_rows) {
+        SampleSettings s{of_rows("temperature", settings.temperature, DType::Float32), of_rows("top_k", settings.top_k, DType::Int32), of_rows("top_p", settings.top_p, DType::Float32),
+                         of_rows("min_p", settings.min_p, DType::Float32)};
+        p.temperature = reinterpret_cast<const float *>(at(s.temperature));
+        p.top_k = reinterpret_cast<const int32_t *>(at(s.top_k));
+        p.top_p = reinterpret_cast<const float *>(at(s.top_p));
+        p.min_p = reinterpret_cast<const float *>(at(s.min_p));
+        return s;
+    });
+}
 
 Sampled sample(const Tensor &logits, const Tensor &u, float temperature, int top_k, float top_p, float min_p) {
-    need_gpu("sample", logits);
-    if (logits.ndim() == 0) throw ShapeError("sample: logits (..., vocabulary)");
-    const Shape rows = without_last(logits.shape());
-    SampleSettings s;
-    if (temperature != 1.0f) s.temperature = Tensor::full<float>(rows, temperature, Device::GPU);
-    if (top_k > 0) s.top_k = Tensor::full<int32_t>(rows, top_k, Device::GPU);
-    if (top_p < 1.0f) s.top_p = Tensor::full<float>(rows, top_p, Device::GPU);
-    if (min_p > 0.0f) s.min_p = Tensor::full<float>(rows, min_p, Device::GPU);
-    return sample(logits, u, s);
+    return draw(logits, u, [&](AxhipSampleParams &p, auto) {
+        p.uniform = 1;
+        p.all_temperature = temperature;
+        p.all_top_k = top_k;
+        p.all_top_p = top_p;
+        p.all_min_p = min_p;
+        return 0;
+    });
 }
 
 } // namespace axiom::ops

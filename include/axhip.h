@@ -516,7 +516,8 @@ const char *axhip_gemm_q8_last_kernel(void);
 
 /* ---------------------------------------------------------------- sampling
  * A token from each row of logits [rows, vocab]: what axhip_argreduce does for greedy decoding, for the rest.  It has no
- * counterpart in the reference.  Each setting is an array of `rows` values on the device, or NULL (off).  With
+ * counterpart in the reference.  Each setting is an array of `rows` values on the device, or NULL (off); with `uniform` 1 the arrays are
+ * NULL and the four values all_* hold for every row (nothing is allocated, copied or waited for on their behalf).  With
  * w_i = exp((l_i - max l) / temperature) and the order "larger logit first, equal ones by index":
  *     top_k  (k > 0)      keeps the first k;
  *     top_p  (p < 1)      of those, keeps the ones in front of which less than p of their sum of w lies (always the first);
@@ -530,12 +531,16 @@ const char *axhip_gemm_q8_last_kernel(void);
  * vocab up to 2^20 (AXHIP_ERR_UNSUPPORTED beyond), rows ld elements apart, any alignment. */
 typedef struct {
     int32_t dtype;
+    int32_t uniform; /* 0: the arrays; 1: the values at the end */
     int64_t rows, vocab, ld;
     const float *temperature; /* [rows] or NULL */
     const int32_t *top_k;     /* [rows] or NULL; 0 or less: off for the row */
     const float *top_p;       /* [rows] or NULL; 1 or more, or NaN: off for the row */
     const float *min_p;       /* [rows] or NULL; 0 or less, or NaN: off for the row */
     const float *u;           /* [rows] */
+    float all_temperature;    /* read with uniform 1 only; off as in the arrays, temperature 1 being off */
+    int32_t all_top_k;
+    float all_top_p, all_min_p;
 } AxhipSampleParams;
 
 int axhip_sample(const void *logits, int64_t *tokens, float *probs, const AxhipSampleParams *params_host, void *stream);
