@@ -596,8 +596,7 @@ template <int DT, int IT> __global__ __launch_bounds__(THREADS) void sample_kern
     // ================ top_k of a few, short rows: a list of little more than what is kept
     if ((k && k <= SMALL_K) || a.vocab <= FEW_LOGITS) {
         float low = r.floor;
-        bool bounded = a.vocab <= FEW_LOGITS;
-        if (!bounded) { // (the bins are clear: a barrier ago)
+        if (a.vocab > FEW_LOGITS) { // (the bins are clear: a barrier ago)
             if (a.vocab >= THREADS * E) {
                 if (mine >= r.floor) add_to_bin(sh.bins[r.bin_of(mine)], 1);
             } else { // (too few threads have any: all logits)
@@ -608,61 +607,58 @@ template <int DT, int IT> __global__ __launch_bounds__(THREADS) void sample_kern
             __syncthreads();
             uint64_t in_front;
             const int bin = find_bin(sh, 0, static_cast<uint64_t>(k - 1), in_front);
-            bounded = bin >= 0 && bin < BINS - 1;
-            if (bounded) low = fmaxf(low, r.below(bin));
+            if (bin >= 0 && bin < BINS - 1) low = fmaxf(low, r.below(bin)); // (or there are fewer than k that weigh anything: all of them)
         }
-        if (bounded) {
-            // each wavefront's to a part of the list of its own
-            constexpr uint32_t PART = LIST / WAVES;
-            uint32_t own = 0;
-            each_step([&](const Step<DT> &s, uint32_t at, int) __attribute__((always_inline)) {
-                float largest = element<DT>(s, 0);
+        // each wavefront's to a part of the list of its own
+        constexpr uint32_t PART = LIST / WAVES;
+        uint32_t own = 0;
+        each_step([&](const Step<DT> &s, uint32_t at, int) __attribute__((always_inline)) {
+            float largest = element<DT>(s, 0);
 #pragma unroll
-                for (int e = 1; e < E; ++e) largest = fmaxf(largest, element<DT>(s, e));
-                if (__ballot(largest >= low) == 0) return;
+            for (int e = 1; e < E; ++e) largest = fmaxf(largest, element<DT>(s, e));
+            if (__ballot(largest >= low) == 0) return;
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const float v = element<DT>(s, e);
-                    const uint64_t taken = __ballot(v >= low);
-                    if (taken == 0) continue;
-                    const uint32_t to = own + lanes_in_front(taken);
-                    if (v >= low && to < PART) sh.list[wave * PART + to] = order_of(v, at + e);
-                    own += __builtin_popcountll(taken);
-                }
-            });
-            if (lane == 0) sh.where[wave] = own;
+            for (int e = 0; e < E; ++e) {
+                const float v = element<DT>(s, e);
+                const uint64_t taken = __ballot(v >= low);
+                if (taken == 0) continue;
+                const uint32_t to = own + lanes_in_front(taken);
+                if (v >= low && to < PART) sh.list[wave * PART + to] = order_of(v, at + e);
+                own += __builtin_popcountll(taken);
+            }
+        });
+        if (lane == 0) sh.where[wave] = own;
+        __syncthreads();
+        uint32_t in_front = 0, n = 0;
+        for (int w = 0; w < WAVES; ++w) {
+            in_front += w < wave ? sh.where[w] : 0;
+            n += sh.where[w];
+        }
+        if (n <= THREADS) { // an entry to a thread
+            uint64_t *const entries = sh.bins;
+            for (uint32_t i = lane; i < own; i += WAVE) entries[in_front + i] = sh.list[wave * PART + i];
             __syncthreads();
-            uint32_t in_front = 0, n = 0;
-            for (int w = 0; w < WAVES; ++w) {
-                in_front += w < wave ? sh.where[w] : 0;
-                n += sh.where[w];
+            uint64_t o = static_cast<uint32_t>(t) < n ? entries[t] : ~0ull, total;
+            int waves = 1;
+            while (waves * WAVE < static_cast<int>(n)) waves *= 2;
+            if (k || p < 1.0f) o = sorted(sh.list, o, waves);
+            // (in their order: what lies in front of an entry is what the threads in front hold)
+            bool kept = static_cast<uint32_t>(t) < n && (k == 0 || t < k);
+            const float v = logit_of(o);
+            if (p < 1.0f) {
+                const uint64_t front = sum_in_front(sh, kept ? r.mass(v) : 0, total);
+                kept = kept && front <= than_of_p([&] { return total; });
             }
-            if (n <= THREADS) { // an entry to a thread
-                uint64_t *const entries = sh.bins;
-                for (uint32_t i = lane; i < own; i += WAVE) entries[in_front + i] = sh.list[wave * PART + i];
-                __syncthreads();
-                uint64_t o = static_cast<uint32_t>(t) < n ? entries[t] : ~0ull, total;
-                int waves = 1;
-                while (waves * WAVE < static_cast<int>(n)) waves *= 2;
-                if (k || p < 1.0f) o = sorted(sh.list, o, waves);
-                // (in their order: what lies in front of an entry is what the threads in front hold)
-                bool kept = static_cast<uint32_t>(t) < n && (k == 0 || t < k);
-                const float v = logit_of(o);
-                if (p < 1.0f) {
-                    const uint64_t front = sum_in_front(sh, kept ? r.mass(v) : 0, total);
-                    kept = kept && front <= than_of_p([&] { return total; });
-                }
-                // by index, with their weights: 20 and 44 bits
-                static_assert(MOST_VOCAB <= int64_t(1) << 20 && ONE < uint64_t(1) << 44, "one number for both");
-                const uint64_t mass = kept ? r.mass_of_least(v) : 0;
-                const uint64_t drawn = sorted(sh.list, mass ? static_cast<uint64_t>(index_of(o)) << 44 | mass : ~0ull, waves);
-                const uint64_t x = drawn != ~0ull ? drawn & ((uint64_t(1) << 44) - 1) : 0;
-                const uint64_t front = sum_in_front(sh, x, total), than = than_of_u(total);
-                if (front <= than && front + x > than) answer(static_cast<uint32_t>(drawn >> 44), x, total);
-                return;
-            }
-            __syncthreads(); // (many equal ones: the other ways)
+            // by index, with their weights: 20 and 44 bits
+            static_assert(MOST_VOCAB <= int64_t(1) << 20 && ONE < uint64_t(1) << 44, "one number for both");
+            const uint64_t mass = kept ? r.mass_of_least(v) : 0;
+            const uint64_t drawn = sorted(sh.list, mass ? static_cast<uint64_t>(index_of(o)) << 44 | mass : ~0ull, waves);
+            const uint64_t x = drawn != ~0ull ? drawn & ((uint64_t(1) << 44) - 1) : 0;
+            const uint64_t front = sum_in_front(sh, x, total), than = than_of_u(total);
+            if (front <= than && front + x > than) answer(static_cast<uint32_t>(drawn >> 44), x, total);
+            return;
         }
+        __syncthreads(); // (many equal ones: the other ways)
     }
 
     // The draw by the sums of the wavefronts' steps, and then within one.  masses(vectors, index of the first, sums): of a lane's eight, MARK for a logit of which only the first
