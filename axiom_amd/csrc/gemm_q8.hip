@@ -53,6 +53,7 @@ bool takes_q8_kernels(const AxhipGemmQ8Params &p) {
 // take on the 256 CUs (whole rounds of the tile kernels, of which a CU holds one, or two of a pair; the small ones share a CU, and a part of a round costs
 // about half of what is missing from a whole one) and u how full the first is.  Fitted to 460 products of m 9 .. 8192, n and k 64 .. 8192, results in bfloat16, every
 // candidate timed (mean error 5 - 12 %); the one picked takes 1.022 of the fastest one's time on average, 1.26 at worst (303 x 883 x 6416, 14.0 us instead of 11.1).
+// The same numbers serve fp32 results, residuals, activations and n beyond 8192, of which none were in the fit.
 struct Q8Kernel {
     bool small;
     int tile, waves; // a Q8Tile, or a SmallShape and its wavefronts

@@ -13,7 +13,7 @@
 // shifted into place.
 // What bounds it: 8192 x 4096 x 4096 + residual 118 - 133 us (2.07 - 2.33 POP/s, as the vendor's library): of a 256 x 256 tile's 3100 cycles per k-tile of 128 the matrix pipe is busy
 // for 2048 and LDS as long.  Two work-groups per CU, deeper rings, 64-byte k-tiles, priorities of wavefronts and a residual fetched into L2 ahead changed nothing or cost 10 %.
-// 1500 x 5120 x 1280 + GELU 19.0 us: one round of 240 work-groups, of which launch, first loads and epilogue are about 9.
+// 1500 x 5120 x 1280 + GELU 17.6 - 18.9 us by card: one round of 240 work-groups, of which launch, first loads and epilogue are about 9 (0.6 of them the exponentials of GELU).
 #pragma once
 #include "gemm_q8_device.hpp"
 

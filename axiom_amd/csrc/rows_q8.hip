@@ -194,8 +194,8 @@ __device__ __forceinline__ void make_products(const RowsQ8Args &a, int64_t row, 
     }
 }
 
-// Bound by memory: one read of x (and the residual), one write of the integers (and the sum).  bf16 8192 x 4096 with a residual and the sum 47.2 us (235 MB, 5.0 TB/s, 97 % of what a
-// copy reaches), fp32 4096 x 4096 14.7 (84 MB, partly from the caches); one row of 1280 takes 3.2 us, a launch.
+// Bound by memory: one read of x (and the residual), one write of the integers (and the sum).  bf16 8192 x 4096 with a residual and the sum 47.8 us (235 MB, 4.9 TB/s, 96 % of what a
+// copy reaches; squares in 64 bits take 0.6 of them), fp32 4096 x 4096 14.6 (84 MB, partly from the caches); one row of 1280 takes 3.1 - 3.6 us, a launch.
 // A row to G threads, in their registers (IT chunks of 16 bytes each), so that x is read once.  1 / sqrt(mean(h^2) + eps) is the same factor in y
 // and in max |y|: it cancels in the integers and shows in the scale alone, so the integers wait for one maximum, not for a norm and then
 // a maximum.

@@ -13,7 +13,8 @@ namespace {
 // the order of the indexes.  Weights are integers, multiples of 2^-43 of the largest, of which 2^20 fit 64 bits: sums do not depend on the order in which
 // atomics arrive.  Three ways, by what is asked of the row:
 //   * top_k up to SMALL_K (and short rows): of the threads' 1024 largest logits the k-th largest is a bound that at least k logits reach, and hardly more do (of k = 512, 1024 ln 2 = 710 where
-//     they lie anywhere; a larger k would often leave more than there are threads).  An entry to a thread, they are sorted by the order, and then those that are kept by index.
+//     they lie anywhere; a larger k would often leave more than there are threads).  On a steep row, where fewer than k weigh anything, the list is all that do.  An entry to a thread, they are
+//     sorted by the order, and then those that are kept by index (a list of more than there are threads, of equal logits or near ones, goes the other ways).
 //   * other 16-bit rows: all 65535 values are counted in LDS (128 KiB), and every filter is answered by the counts: one weight for each value that occurs
 //     instead of one for each logit.  The draw takes weights from a table of the values that are kept.  Counts are 16 bits wide; if one overflows, the sum of all shows
 //     it and the row goes the third way.
@@ -22,7 +23,8 @@ namespace {
 //     in LDS if they fit, where the cut is found.  (Lists of all that is kept, for the draw, and weights formed of what is kept alone took as long as a pass over the row.)
 // What bounds it: few rows the chain of dependent passes and barriers (fp32 1 x 51865, top_k: 8.9 us, of which 3 are the launch; bf16 64 x 51865, top_k, top_p and min_p: 15.2);
 // 256 rows a CU's own work on its row.  bf16 256 x 128256, top_p, 49 us: 8 loading (at HBM's rate), 2 the largest, 11 counting (LDS atomics: a wavefront's 64 random banks take 12
-// cycles), 5 the blocks' weights (64-bit operations), 3 the cut, 8 the draw's table look-ups, 3 the step it falls in.  fp32, the same rows: without filters 61, top_k 45, top_p 129: a pass over the row takes
+// cycles), 5 the blocks' weights (64-bit operations), 3 the cut, 8 the draw's table look-ups, 3 the step it falls in.  (Rows of more than 65536 are held in 64 registers of a thread's 128, and a thread spills 44 bytes,
+// f16 36.)  fp32, the same rows: without filters 61, top_k 45, top_p 129: a pass over the row takes
 // 35 to 45, 200 cycles of a SIMD for each vector of 64 weights, half of them 64-bit operations.
 constexpr int THREADS = 1024, WAVES = THREADS / WAVE, E = 8; // elements of a lane's vector
 constexpr int STEP = WAVE * E;                               // consecutive elements of a wavefront's step
@@ -885,7 +887,8 @@ template <int DT, int IT> __global__ __launch_bounds__(THREADS) void sample_kern
             const bool in_part = of_last != 0; // (those that weigh nothing need no marks)
             const uint32_t values = last - first + 1;
             __syncthreads(); // (the counts make room for the weights)
-            // (weights of logits between two small ones of either sign are the same integer: one entry of the table for all of them, which lets it reach negative bfloat16 logits)
+            // (weights of logits between two small ones of either sign are the same to an eighth of an integer, and are taken as one: one entry of the table for all of them, which lets it
+            // reach negative bfloat16 logits)
             uint32_t zone = values, gap = 0; // entries zone .. zone + gap are one
             if (DT == AXHIP_DTYPE_BF16 && values >= LIST) {
                 const uint32_t small = order_of16(f32_to_bf16_bits(temperature * 7.105427357601002e-15f)); // 2^-47 temperatures
