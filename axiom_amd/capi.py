@@ -102,6 +102,73 @@ class SampleParams(C.Structure):
     ]
 
 
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_BANDS = 0, 1, 2, 3
+
+
+class RopeScaling(C.Structure):
+    _fields_ = [
+        ("rot_dim", C.c_int32), ("kind", C.c_int32),
+        ("theta", C.c_double), ("factor", C.c_double), ("low", C.c_double), ("high", C.c_double), ("length", C.c_double),
+    ]
+
+
+class RopeParams(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("heads", C.c_int32), ("head_dim", C.c_int32), ("rot_dim", C.c_int32),
+        ("interleaved", C.c_int32), ("inverse", C.c_int32), ("amplitude", C.c_float), ("position_bytes", C.c_int32),
+        ("tokens", C.c_int64), ("x_strides", C.c_int64 * 2), ("y_strides", C.c_int64 * 2),
+        ("positions", C.c_void_p), ("turns", C.c_void_p),
+    ]
+
+
+class KvPages(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p),
+        ("dtype", C.c_int32), ("page_size", C.c_int32), ("heads", C.c_int32), ("head_dim", C.c_int32),
+        ("n_pages", C.c_int64), ("k_strides", C.c_int64 * 3), ("v_strides", C.c_int64 * 3),
+    ]
+
+
+class KvAppendParams(C.Structure):
+    _fields_ = [
+        ("pages", KvPages),
+        ("heads", C.c_int32), ("rot_dim", C.c_int32), ("interleaved", C.c_int32), ("amplitude", C.c_float), ("position_bytes", C.c_int32),
+        ("tokens", C.c_int64),
+        ("q_strides", C.c_int64 * 2), ("k_strides", C.c_int64 * 2), ("v_strides", C.c_int64 * 2), ("q_out_strides", C.c_int64 * 2),
+        ("positions", C.c_void_p), ("turns", C.c_void_p), ("slots", C.c_void_p),
+    ]
+
+
+class KvCopyParams(C.Structure):
+    _fields_ = [
+        ("pages", KvPages),
+        ("layers", C.c_int32), ("pairs", C.c_int32), ("k_layer_stride", C.c_int64), ("v_layer_stride", C.c_int64),
+        ("src", C.c_void_p), ("dst", C.c_void_p), ("rows", C.c_void_p),
+    ]
+
+
+class SdpaPackedParams(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32),
+        ("n_seqs", C.c_int32), ("is_causal", C.c_int32), ("scale", C.c_float), ("max_kv", C.c_int32),
+        ("total_q", C.c_int64), ("total_kv", C.c_int64),
+        ("q_strides", C.c_int64 * 2), ("k_strides", C.c_int64 * 2), ("v_strides", C.c_int64 * 2), ("o_strides", C.c_int64 * 2),
+        ("cu_q", C.c_void_p), ("cu_kv", C.c_void_p), ("page_table", C.c_void_p), ("kv_lengths", C.c_void_p),
+        ("table_ld", C.c_int64), ("pages", KvPages),
+    ]
+
+
+class SdpaPagedParams(C.Structure):
+    _fields_ = [
+        ("pages", KvPages),
+        ("heads", C.c_int32), ("n_seqs", C.c_int32), ("new_tokens", C.c_int32), ("max_kv", C.c_int32), ("scale", C.c_float),
+        ("n_groups", C.c_int32), ("max_prefix", C.c_int32), ("reserved", C.c_int32),
+        ("q_strides", C.c_int64 * 3), ("o_strides", C.c_int64 * 3),
+        ("page_table", C.c_void_p), ("kv_lengths", C.c_void_p), ("table_ld", C.c_int64),
+        ("group_starts", C.c_void_p), ("prefix_table", C.c_void_p), ("prefix_lengths", C.c_void_p), ("prefix_ld", C.c_int64),
+    ]
+
+
 _lib = None
 
 
@@ -174,6 +241,19 @@ def lib() -> C.CDLL:
         l.axhip_sample_workspace_bytes.restype = C.c_size_t
         l.axhip_sample_workspace_bytes.argtypes = [C.POINTER(SampleParams)]
         l.axhip_sample_ws.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.POINTER(SampleParams), C.c_void_p, C.c_size_t, C.c_void_p]
+        l.axhip_rope_turns.argtypes = [C.POINTER(RopeScaling), C.POINTER(C.c_uint64)]
+        l.axhip_rope.argtypes = [C.c_void_p, C.c_void_p, C.POINTER(RopeParams), C.c_void_p]
+        l.axhip_kv_append.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.POINTER(KvAppendParams), C.c_void_p]
+        l.axhip_kv_copy_pages.argtypes = [C.POINTER(KvCopyParams), C.c_void_p]
+        l.axhip_sdpa_packed.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.POINTER(SdpaPackedParams), C.c_void_p]
+        l.axhip_sdpa_packed_workspace_bytes.restype = C.c_size_t
+        l.axhip_sdpa_packed_workspace_bytes.argtypes = [C.POINTER(SdpaPackedParams)]
+        l.axhip_sdpa_packed_ws.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.POINTER(SdpaPackedParams), C.c_void_p, C.c_size_t, C.c_void_p]
+        l.axhip_sdpa_paged.argtypes = [C.c_void_p, C.c_void_p, C.POINTER(SdpaPagedParams), C.c_void_p]
+        l.axhip_sdpa_paged_workspace_bytes.restype = C.c_size_t
+        l.axhip_sdpa_paged_workspace_bytes.argtypes = [C.POINTER(SdpaPagedParams)]
+        l.axhip_sdpa_paged_ws.argtypes = [C.c_void_p, C.c_void_p, C.POINTER(SdpaPagedParams), C.c_void_p, C.c_size_t, C.c_void_p]
+        l.axhip_sdpa_cache_last_kernel.restype = C.c_char_p
         _lib = l
     return _lib
 

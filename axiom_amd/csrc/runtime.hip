@@ -56,6 +56,13 @@ size_t axhip_sizeof(int which) {
     case 5: return sizeof(AxhipRowsQ8Params);
     case 6: return sizeof(AxhipGemmQ8Params);
     case 7: return sizeof(AxhipSampleParams);
+    case 8: return sizeof(AxhipRopeScaling);
+    case 9: return sizeof(AxhipRopeParams);
+    case 10: return sizeof(AxhipKvPages);
+    case 11: return sizeof(AxhipKvAppendParams);
+    case 12: return sizeof(AxhipKvCopyParams);
+    case 13: return sizeof(AxhipSdpaPackedParams);
+    case 14: return sizeof(AxhipSdpaPagedParams);
     default: return 0;
     }
 }

@@ -1,0 +1,327 @@
+// Attention of sequences of different lengths, packed or over the pages of a cache: axhip_sdpa_packed, axhip_sdpa_paged.
+#include "sdpa_cache.hpp"
+
+#include <algorithm>
+#include <cmath>
+
+namespace axhip {
+
+// ------------------------------------------------------------- generic kernel
+// Every type, head size up to 256, stride and alignment, in fp32: 16 rows of 16 lanes, keys 32 at a time through LDS.  Lane c of a row
+// computes the scores of keys c and c + 16 and the dims c, c + 16, ...
+constexpr int CM = 16, CN = 32, CMAXD = 256;
+
+__global__ __launch_bounds__(256) void sdpa_cache_generic_kernel(const CacheArgs a) {
+    extern __shared__ float smem[];
+    const int D = a.D, ksd = D + 1;
+    float *Qs = smem;           // [CM][D]
+    float *Ksm = Qs + CM * D;   // [CN][D + 1]
+    float *Vs = Ksm + CN * ksd; // [CN][D]
+    float *Ps = Vs + CN * D;    // [CM][CN]
+    __shared__ int bad_page;
+    const int tid = threadIdx.x, r = tid / 16, c = tid % 16;
+    const int kvh = blockIdx.x % a.kv_heads;
+    int64_t block = blockIdx.x / a.kv_heads;
+    // which entry: with cu_q entry s gets the blocks from cu_q[s] * each / CM + s on, one more than it needs at most
+    int s;
+    if (a.new_tokens) {
+        const int per = (a.new_tokens * a.each + CM - 1) / CM;
+        s = static_cast<int>(block / per);
+        block %= per;
+    } else {
+        auto first = [&](int e) { return static_cast<int64_t>(clamped(a.cu_q[e], 0, a.total_q)) * a.each / CM + e; };
+        int lo = 0, hi = a.entries - 1; // first(lo) <= block
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) / 2;
+            if (first(mid) <= block) lo = mid;
+            else hi = mid - 1;
+        }
+        s = lo;
+        block -= first(s);
+    }
+    const TokenRun t = tokens_of(a, s);
+    const int64_t rows = static_cast<int64_t>(t.n) * a.each, row0 = block * CM;
+    if (block < 0 || row0 >= rows) return;
+    const int64_t row = row0 + r;
+    const bool row_ok = row < rows;
+    const int token = static_cast<int>(row / a.each), head = kvh * a.each + static_cast<int>(row % a.each);
+    auto q_at = [&](int64_t rr) {
+        const int64_t tok = rr / a.each, h = kvh * a.each + rr % a.each;
+        return s * a.qs[0] + (t.from + tok) * a.qs[1] + h * a.qs[2];
+    };
+    for (int i = tid; i < CM * D; i += 256) {
+        const int rr = i / D, d = i % D;
+        Qs[i] = row0 + rr < rows ? load_any(a.q, a.dtype, q_at(row0 + rr) + d) : 0.0f;
+    }
+    if (tid == 0) bad_page = 0;
+
+    float acc[CMAXD / 16];
+#pragma unroll
+    for (int i = 0; i < CMAXD / 16; ++i) acc[i] = 0.0f;
+    float m_run = NEG_INF_F, l_run = 0.0f;
+
+    auto walk = [&](const KeyRun &run, bool causal) {
+        const int limit = causal ? run.n - t.n + token : run.n - 1; // last key that this row sees
+        const int last_token = static_cast<int>(min(row0 + CM - 1, rows - 1) / a.each);
+        const int end = causal ? min(run.n, run.n - t.n + last_token + 1) : run.n;
+        for (int kv0 = 0; kv0 < end; kv0 += CN) {
+            __syncthreads();
+            for (int i = tid; i < CN * D; i += 256) {
+                const int rr = i / D, d = i % D, key = kv0 + rr;
+                float kx = 0.0f, vx = 0.0f;
+                if (key < run.n) {
+                    int64_t page = 0, in_page = run.base + key;
+                    if (run.table) {
+                        page = run.table[key >> a.page_shift];
+                        in_page = key & ((1 << a.page_shift) - 1);
+                        if (page < 0 || page >= a.n_pages) {
+                            bad_page = 1;
+                            page = -1;
+                        }
+                    }
+                    if (page >= 0) {
+                        kx = load_any(a.k, a.dtype, page * a.ks[0] + in_page * a.ks[1] + kvh * a.ks[2] + d);
+                        vx = load_any(a.v, a.dtype, page * a.vs[0] + in_page * a.vs[1] + kvh * a.vs[2] + d);
+                    }
+                }
+                Ksm[rr * ksd + d] = kx;
+                Vs[rr * D + d] = vx;
+            }
+            __syncthreads();
+            float sc[CN / 16];
+#pragma unroll
+            for (int jj = 0; jj < CN / 16; ++jj) {
+                const int j = c + 16 * jj;
+                float dot = 0.0f;
+                for (int d = 0; d < D; ++d) dot = __builtin_fmaf(Qs[r * D + d], Ksm[j * ksd + d], dot);
+                sc[jj] = kv0 + j > limit || kv0 + j >= run.n ? NEG_INF_F : dot * a.scale_log2e;
+            }
+            float mloc = fmaxf(sc[0], sc[1]);
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) mloc = fmaxf(mloc, __shfl_xor(mloc, o, WAVE));
+            const float m_new = fmaxf(m_run, mloc), m_use = m_new == NEG_INF_F ? 0.0f : m_new;
+            const float alpha = exp2f(m_run - m_use);
+            m_run = m_new;
+            float lsum = 0.0f;
+#pragma unroll
+            for (int jj = 0; jj < CN / 16; ++jj) {
+                const float p = exp2f(sc[jj] - m_use);
+                Ps[r * CN + c + 16 * jj] = p;
+                lsum += p;
+            }
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) lsum += __shfl_xor(lsum, o, WAVE);
+            l_run = l_run * alpha + lsum;
+            __syncthreads();
+#pragma unroll
+            for (int dd = 0; dd < CMAXD / 16; ++dd) {
+                const int d = c + 16 * dd;
+                if (d < D) {
+                    float x = acc[dd] * alpha;
+                    for (int j = 0; j < CN; ++j) x = __builtin_fmaf(Ps[r * CN + j], Vs[j * D + d], x);
+                    acc[dd] = x;
+                }
+            }
+        }
+    };
+    if (a.groups > 0) {
+        const int g = group_of(a, s);
+        if (g >= 0) walk(prefix_of(a, g), false);
+    }
+    walk(keys_of(a, s), a.causal != 0);
+    __syncthreads();
+    const float inv = bad_page ? __builtin_nanf("") : l_run > 0.0f ? 1.0f / l_run : 0.0f;
+    if (row_ok) {
+        const int64_t at = s * a.os[0] + (t.from + token) * a.os[1] + head * a.os[2];
+#pragma unroll
+        for (int dd = 0; dd < CMAXD / 16; ++dd) {
+            const int d = c + 16 * dd;
+            if (d < D) store_any(a.o, a.dtype, at + d, acc[dd] * inv);
+        }
+    }
+}
+
+// ------------------------------------------------------------------ host side
+namespace {
+
+thread_local const char *last_kernel = "none";
+
+bool sane(const int64_t *s, int n) {
+    for (int i = 0; i < n; ++i)
+        if (s[i] < 0 || s[i] >= (int64_t(1) << 40)) return false;
+    return true;
+}
+bool int_aligned(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+
+int launch_generic(const CacheArgs &a, hipStream_t s, const char *who) {
+    const int64_t blocks = (a.new_tokens ? (static_cast<int64_t>(a.new_tokens) * a.each + CM - 1) / CM * a.entries : a.total_q * a.each / CM + a.entries) * a.kv_heads;
+    AXHIP_REQUIRE(launch_fits(blocks, 256), AXHIP_ERR_UNSUPPORTED, "%s: grid too large", who);
+    const size_t lds = sizeof(float) * (static_cast<size_t>(CM) * a.D + static_cast<size_t>(CN) * (a.D + 1) + static_cast<size_t>(CN) * a.D + CM * CN);
+    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(sdpa_cache_generic_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024);
+    AXHIP_CHECK_HIP(attr);
+    last_kernel = "generic";
+    hipLaunchKernelGGL(sdpa_cache_generic_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), lds, s, a);
+    AXHIP_CHECK_HIP(hipGetLastError());
+    return AXHIP_OK;
+}
+
+// What both entry points check alike, and the arguments that follow from it.
+int common_args(const char *who, CacheArgs &a, int dtype, int heads, int kv_heads, int head_dim, float scale) {
+    AXHIP_REQUIRE(valid_dtype(dtype), AXHIP_ERR_INVALID_ARG, "%s: bad dtype %d", who, dtype);
+    AXHIP_REQUIRE(heads > 0 && kv_heads > 0 && heads < (1 << 20) && heads % kv_heads == 0, AXHIP_ERR_INVALID_ARG, "%s: %d heads over %d key heads", who, heads, kv_heads);
+    AXHIP_REQUIRE(head_dim > 0, AXHIP_ERR_INVALID_ARG, "%s: head_dim %d", who, head_dim);
+    AXHIP_REQUIRE(head_dim <= CMAXD, AXHIP_ERR_UNSUPPORTED, "%s: head_dim %d > %d is not supported", who, head_dim, CMAXD);
+    AXHIP_REQUIRE(!std::isnan(scale) && !std::isinf(scale), AXHIP_ERR_INVALID_ARG, "%s: scale must be a finite number", who);
+    a.dtype = dtype;
+    a.heads = heads;
+    a.kv_heads = kv_heads;
+    a.each = heads / kv_heads;
+    a.D = head_dim;
+    a.scale_log2e = static_cast<float>((scale > 0.0f ? static_cast<double>(scale) : 1.0 / std::sqrt(static_cast<double>(head_dim))) * 1.44269504088896340736);
+    return AXHIP_OK;
+}
+int page_args(const char *who, CacheArgs &a, const AxhipKvPages &g, const int32_t *table, int64_t table_ld, const int32_t *lengths) {
+    const int rc = check_pages(who, g);
+    if (rc) return rc;
+    AXHIP_REQUIRE(table_ld > 0 && table_ld < (int64_t(1) << 31), AXHIP_ERR_INVALID_ARG, "%s: bad table_ld", who);
+    AXHIP_REQUIRE(table && lengths && int_aligned(table) && int_aligned(lengths), AXHIP_ERR_INVALID_ARG, "%s: NULL or unaligned page_table or kv_lengths", who);
+    a.k = g.k;
+    a.v = g.v;
+    a.table = table;
+    a.lengths = lengths;
+    a.table_ld = table_ld;
+    a.n_pages = g.n_pages;
+    a.page_shift = __builtin_ctz(static_cast<unsigned>(g.page_size));
+    for (int i = 0; i < 3; ++i) {
+        a.ks[i] = g.k_strides[i];
+        a.vs[i] = g.v_strides[i];
+    }
+    return AXHIP_OK;
+}
+
+int packed_args(CacheArgs &a, const AxhipSdpaPackedParams *params) {
+    const char *who = "axhip_sdpa_packed";
+    AXHIP_REQUIRE(params != nullptr, AXHIP_ERR_INVALID_ARG, "axhip_sdpa_packed: params is NULL");
+    const AxhipSdpaPackedParams &p = *params;
+    int rc = common_args(who, a, p.dtype, p.heads, p.kv_heads, p.head_dim, p.scale);
+    if (rc) return rc;
+    AXHIP_REQUIRE(p.n_seqs >= 0 && p.n_seqs < (1 << 24) && p.total_q >= 0 && p.total_q < (int64_t(1) << 31), AXHIP_ERR_INVALID_ARG, "axhip_sdpa_packed: bad extent");
+    AXHIP_REQUIRE(p.is_causal == 0 || p.is_causal == 1, AXHIP_ERR_INVALID_ARG, "axhip_sdpa_packed: is_causal is %d, neither 0 nor 1", p.is_causal);
+    AXHIP_REQUIRE(sane(p.q_strides, 2) && sane(p.o_strides, 2), AXHIP_ERR_INVALID_ARG, "axhip_sdpa_packed: bad stride");
+    a.entries = p.n_seqs;
+    a.causal = p.is_causal;
+    a.total_q = p.total_q;
+    a.cu_q = p.cu_q;
+    for (int i = 0; i < 2; ++i) {
+        a.qs[i + 1] = p.q_strides[i];
+        a.os[i + 1] = p.o_strides[i];
+    }
+    if (p.n_seqs == 0 || p.total_q == 0) return AXHIP_OK;
+    AXHIP_REQUIRE(p.cu_q && int_aligned(p.cu_q), AXHIP_ERR_INVALID_ARG, "axhip_sdpa_packed: NULL or unaligned cu_q");
+    if (p.page_table) {
+        rc = page_args(who, a, p.pages, p.page_table, p.table_ld, p.kv_lengths);
+        if (rc) return rc;
+        AXHIP_REQUIRE(p.pages.dtype == p.dtype && p.pages.heads == p.kv_heads && p.pages.head_dim == p.head_dim, AXHIP_ERR_INVALID_ARG,
+                      "axhip_sdpa_packed: pages of another type, other heads or another head_dim");
+        return AXHIP_OK;
+    }
+    AXHIP_REQUIRE(p.total_kv >= 0 && p.total_kv < (int64_t(1) << 31), AXHIP_ERR_INVALID_ARG, "axhip_sdpa_packed: bad extent");
+    AXHIP_REQUIRE(sane(p.k_strides, 2) && sane(p.v_strides, 2), AXHIP_ERR_INVALID_ARG, "axhip_sdpa_packed: bad stride");
+    AXHIP_REQUIRE(p.cu_kv && int_aligned(p.cu_kv), AXHIP_ERR_INVALID_ARG, "axhip_sdpa_packed: NULL or unaligned cu_kv");
+    a.cu_kv = p.cu_kv;
+    a.total_kv = p.total_kv;
+    for (int i = 0; i < 2; ++i) {
+        a.ks[i + 1] = p.k_strides[i];
+        a.vs[i + 1] = p.v_strides[i];
+    }
+    return AXHIP_OK;
+}
+
+int paged_args(CacheArgs &a, const AxhipSdpaPagedParams *params) {
+    const char *who = "axhip_sdpa_paged";
+    AXHIP_REQUIRE(params != nullptr, AXHIP_ERR_INVALID_ARG, "axhip_sdpa_paged: params is NULL");
+    const AxhipSdpaPagedParams &p = *params;
+    int rc = common_args(who, a, p.pages.dtype, p.heads, p.pages.heads, p.pages.head_dim, p.scale);
+    if (rc) return rc;
+    AXHIP_REQUIRE(p.n_seqs >= 0 && p.n_seqs < (1 << 24) && p.new_tokens > 0 && p.new_tokens < (1 << 20) && static_cast<int64_t>(p.new_tokens) * p.heads < (1 << 30), AXHIP_ERR_INVALID_ARG, "axhip_sdpa_paged: %d sequences of %d new tokens", p.n_seqs,
+                  p.new_tokens);
+    AXHIP_REQUIRE(p.n_groups >= 0 && p.n_groups < (1 << 24) && p.reserved == 0, AXHIP_ERR_INVALID_ARG, "axhip_sdpa_paged: bad number of groups, or reserved is not 0");
+    AXHIP_REQUIRE(sane(p.q_strides, 3) && sane(p.o_strides, 3), AXHIP_ERR_INVALID_ARG, "axhip_sdpa_paged: bad stride");
+    a.entries = p.n_seqs;
+    a.causal = 1;
+    a.new_tokens = p.new_tokens;
+    for (int i = 0; i < 3; ++i) {
+        a.qs[i] = p.q_strides[i];
+        a.os[i] = p.o_strides[i];
+    }
+    if (p.n_seqs == 0) return AXHIP_OK;
+    rc = page_args(who, a, p.pages, p.page_table, p.table_ld, p.kv_lengths);
+    if (rc) return rc;
+    if (p.n_groups > 0) {
+        AXHIP_REQUIRE(p.prefix_ld > 0 && p.prefix_ld < (int64_t(1) << 31), AXHIP_ERR_INVALID_ARG, "axhip_sdpa_paged: bad prefix_ld");
+        AXHIP_REQUIRE(p.group_starts && p.prefix_table && p.prefix_lengths && int_aligned(p.group_starts) && int_aligned(p.prefix_table) && int_aligned(p.prefix_lengths),
+                      AXHIP_ERR_INVALID_ARG, "axhip_sdpa_paged: NULL or unaligned group_starts, prefix_table or prefix_lengths");
+        a.groups = p.n_groups;
+        a.group_starts = p.group_starts;
+        a.prefix_table = p.prefix_table;
+        a.prefix_lengths = p.prefix_lengths;
+        a.prefix_ld = p.prefix_ld;
+    }
+    return AXHIP_OK;
+}
+bool tensor_ok(const void *p, int dtype) { return p && (reinterpret_cast<uintptr_t>(p) & (dtype_size(dtype) - 1)) == 0; }
+
+} // namespace
+} // namespace axhip
+using namespace axhip;
+
+extern "C" {
+
+const char *axhip_sdpa_cache_last_kernel(void) { return last_kernel; }
+
+size_t axhip_sdpa_packed_workspace_bytes(const AxhipSdpaPackedParams *) { return 0; }
+
+int axhip_sdpa_packed(const void *q, const void *k, const void *v, void *o, const AxhipSdpaPackedParams *params, void *stream) {
+    return axhip_sdpa_packed_ws(q, k, v, o, params, nullptr, 0, stream);
+}
+
+int axhip_sdpa_packed_ws(const void *q, const void *k, const void *v, void *o, const AxhipSdpaPackedParams *params, void *, size_t, void *stream) {
+    CacheArgs a{};
+    int rc = packed_args(a, params);
+    if (rc) return rc;
+    last_kernel = "empty";
+    if (a.entries == 0 || a.total_q == 0) return AXHIP_OK;
+    AXHIP_REQUIRE(tensor_ok(q, a.dtype) && tensor_ok(o, a.dtype), AXHIP_ERR_INVALID_ARG, "axhip_sdpa_packed: q or o is NULL or not aligned to its elements");
+    if (a.table) {
+        AXHIP_REQUIRE(!k && !v, AXHIP_ERR_INVALID_ARG, "axhip_sdpa_packed: k or v beside a page_table");
+    } else {
+        AXHIP_REQUIRE(a.total_kv == 0 || (tensor_ok(k, a.dtype) && tensor_ok(v, a.dtype)), AXHIP_ERR_INVALID_ARG, "axhip_sdpa_packed: k or v is NULL or not aligned to its elements");
+        a.k = k;
+        a.v = v;
+    }
+    a.q = q;
+    a.o = o;
+    rc = ensure_init();
+    if (rc) return rc;
+    return launch_generic(a, resolve_stream(stream), "axhip_sdpa_packed");
+}
+
+size_t axhip_sdpa_paged_workspace_bytes(const AxhipSdpaPagedParams *) { return 0; }
+
+int axhip_sdpa_paged(const void *q, void *o, const AxhipSdpaPagedParams *params, void *stream) { return axhip_sdpa_paged_ws(q, o, params, nullptr, 0, stream); }
+
+int axhip_sdpa_paged_ws(const void *q, void *o, const AxhipSdpaPagedParams *params, void *, size_t, void *stream) {
+    CacheArgs a{};
+    int rc = paged_args(a, params);
+    if (rc) return rc;
+    last_kernel = "empty";
+    if (a.entries == 0) return AXHIP_OK;
+    AXHIP_REQUIRE(tensor_ok(q, a.dtype) && tensor_ok(o, a.dtype), AXHIP_ERR_INVALID_ARG, "axhip_sdpa_paged: q or o is NULL or not aligned to its elements");
+    a.q = q;
+    a.o = o;
+    rc = ensure_init();
+    if (rc) return rc;
+    return launch_generic(a, resolve_stream(stream), "axhip_sdpa_paged");
+}
+
+} // extern "C"

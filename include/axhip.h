@@ -8,9 +8,10 @@
  *     hipError_t, a negative value is one of AXHIP_ERR_*.  A human-readable
  *     message for the calling thread's last failure is at axhip_last_error().
  *   - the caller owns every buffer; kernels never allocate.  Pointers are
- *     device pointers unless a parameter says "host".  Four entry points need
+ *     device pointers unless a parameter says "host".  Six entry points need
  *     temporary device memory for some argument values (axhip_sdpa_fwd,
- *     axhip_gemm, axhip_argreduce, axhip_reduce_axis: each says when).  Their
+ *     axhip_sdpa_packed, axhip_sdpa_paged, axhip_gemm, axhip_argreduce,
+ *     axhip_reduce_axis: each says when).  Their
  *     *_ws forms take it from the caller -- `workspace` of at least
  *     *_workspace_bytes(...) bytes, 256-byte aligned -- and allocate nothing;
  *     the plain forms (and a *_ws call with workspace == NULL) take it from the
@@ -549,11 +550,166 @@ size_t axhip_sample_workspace_bytes(const AxhipSampleParams *params_host);
 int axhip_sample_ws(const void *logits, int64_t *tokens, float *probs, const AxhipSampleParams *params_host,
                     void *workspace, size_t workspace_bytes, void *stream);
 
+/* -------------------------------------------- rotary positions and a cache
+ * What a decoder does with positions and with the keys and values of its earlier tokens.  It has no counterpart in the reference,
+ * whose attention takes keys that lie in one piece per (batch, head), of one length for the batch.
+ *
+ * Angles are fractions of a full turn in 64 bits: turns[i] = 2^64 f_i / (2 pi), f_i radians a position.  position * turns[i] modulo
+ * 2^64 is then the angle of any position, a negative one too, to position * 2^-65 turns: what 64 bits keep of position 2^31, a
+ * product of 32-bit numbers loses at position 2^10.
+ * axhip_rope_turns fills such a table on the host (rot_dim / 2 values; no device is needed); copy it to the device once.  f_i =
+ * theta^(-2 i / rot_dim), and for contexts longer than the trained `length`:
+ *     LINEAR  f_i / factor
+ *     BASE    theta * factor^(rot_dim / (rot_dim - 2)) in theta's place: the slowest angle is divided by factor, the fastest is kept
+ *     BANDS   f_i (k + (1 - k) / factor), k = clamp((t - low) / (high - low), 0, 1), t = length f_i / (2 pi) the turns over `length`
+ * theta >= 1; factor > 0; 0 <= low < high; length > 0.  What a kind does not name is not read. */
+#define AXHIP_ROPE_PLAIN 0
+#define AXHIP_ROPE_LINEAR 1
+#define AXHIP_ROPE_BASE 2
+#define AXHIP_ROPE_BANDS 3
+typedef struct {
+    int32_t rot_dim; /* even, up to 1024 */
+    int32_t kind;    /* AXHIP_ROPE_* */
+    double theta, factor, low, high, length;
+} AxhipRopeScaling;
+int axhip_rope_turns(const AxhipRopeScaling *scaling_host, uint64_t *turns_host);
+
+/* y = x with the first rot_dim dims of every head rotated by its token's position, the other dims copied:
+ *     y_a = amplitude (x_a cos t - x_b sin t),  y_b = amplitude (x_b cos t + x_a sin t)
+ * over the pairs (a, b) = (i, i + rot_dim / 2), or (2 i, 2 i + 1) with `interleaved`.  `inverse` rotates back: with the same
+ * amplitude it is the gradient of the call without it.  x, y: [tokens, heads, head_dim], the last dimension contiguous, element
+ * strides of tokens and heads; y may be x itself (then with the same strides).  fp32 arithmetic (sines within 2^-22), rounded once. */
+typedef struct {
+    int32_t dtype;
+    int32_t heads, head_dim, rot_dim; /* rot_dim: even, 2 .. head_dim */
+    int32_t interleaved, inverse;     /* 0 or 1 */
+    float amplitude;                  /* 0 means 1 */
+    int32_t position_bytes;           /* 4 (int32) or 8 (int64) */
+    int64_t tokens;
+    int64_t x_strides[2], y_strides[2]; /* token, head (elements) */
+    const void *positions;              /* [tokens] */
+    const uint64_t *turns;              /* [rot_dim / 2], on the device */
+} AxhipRopeParams;
+int axhip_rope(const void *x, void *y, const AxhipRopeParams *params_host, void *stream);
+
+/* The pages of a cache (of one layer): k and v are [n_pages, page_size rows, heads, head_dim] by element strides, in any order of
+ * rows and heads, the last dimension contiguous.  Row j of a sequence lies in row j % page_size of page table[j / page_size], where
+ * table is the sequence's row of a page table (int32, on the device).  page_size is a power of two up to 65536.  Offsets are 64 bits. */
+typedef struct {
+    void *k, *v;
+    int32_t dtype;
+    int32_t page_size;
+    int32_t heads, head_dim;
+    int64_t n_pages; /* below 2^31 */
+    int64_t k_strides[3], v_strides[3]; /* page, row, head (elements) */
+} AxhipKvPages;
+
+/* New tokens into the cache, in one launch: q rotated to q_out as by axhip_rope (heads = 0: no q, q and q_out NULL; q_out may be q),
+ * k rotated and v as it is written to row slots[t] % page_size of page slots[t] / page_size.  A slot that is negative or behind the
+ * last page is not written (the padded end of a batch: q_out is written for it).  Two tokens must not have the same slot.  q, k, v,
+ * q_out: [tokens, heads or pages.heads, head_dim] by token and head strides, such as views of one product's output.  rot_dim 0:
+ * nothing is rotated, turns and positions may be NULL. */
+typedef struct {
+    AxhipKvPages pages;
+    int32_t heads; /* of q: 0, or any number */
+    int32_t rot_dim, interleaved;
+    float amplitude;        /* of q and of k; 0 means 1 */
+    int32_t position_bytes; /* 4 or 8 */
+    int64_t tokens;
+    int64_t q_strides[2], k_strides[2], v_strides[2], q_out_strides[2]; /* token, head (elements) */
+    const void *positions;  /* [tokens] */
+    const uint64_t *turns;  /* [rot_dim / 2], on the device */
+    const int64_t *slots;   /* [tokens] */
+} AxhipKvAppendParams;
+int axhip_kv_append(const void *q, const void *k, const void *v, void *q_out, const AxhipKvAppendParams *params_host, void *stream);
+
+/* Page dst[i] = page src[i], K and V of every layer: a fork's last page, a pool that is compacted.  With `rows`, the first rows[i]
+ * rows only (values are clamped to 0 .. page_size).  A pair with a page that does not exist is left out; a page that one pair writes
+ * may not be read or written by another one (a pair of a page and itself changes nothing). */
+typedef struct {
+    AxhipKvPages pages; /* of the first layer */
+    int32_t layers;
+    int32_t pairs;
+    int64_t k_layer_stride, v_layer_stride; /* elements */
+    const int32_t *src, *dst;               /* [pairs], on the device */
+    const int32_t *rows;                    /* [pairs], on the device, or NULL: whole pages */
+} AxhipKvCopyParams;
+int axhip_kv_copy_pages(const AxhipKvCopyParams *params_host, void *stream);
+
+/* Attention of packed sequences of different lengths.  q and o: [total_q, heads, head_dim] by token and head strides; sequence s owns
+ * the rows cu_q[s] .. cu_q[s + 1] - 1 (rows of o that no sequence owns are left as they are).  Its keys are
+ *   - the rows cu_kv[s] .. cu_kv[s + 1] - 1 of k and v, [total_kv, kv_heads, head_dim] by strides, or
+ *   - with page_table (then k and v are NULL, cu_kv is not read): kv_lengths[s] rows of its pages, page_table[s * table_ld + ..].
+ * heads is a multiple of kv_heads: head h reads key head h / (heads / kv_heads).  is_causal: the last query sees every key, the one in
+ * front of it one less: query i of n sees key j <= i + keys - n, so that a sequence's next chunk of tokens can be computed behind what
+ * the cache holds already.  A query that sees nothing yields zeros.  scale <= 0 means 1 / sqrt(head_dim).  fp32 sums and softmax, exponentials
+ * rounded to dtype before the second product, results rounded once to dtype.
+ * Keys outside a sequence are neither read nor can what lies there matter; a key that a causal query does not see meets a weight of zero and has to be finite in V.
+ * Numbers in cu_q, cu_kv and kv_lengths that lie outside the tensors are clamped to them; a sequence with a page that does not exist among
+ * those of its keys yields NaN.  max_kv: about how many keys the longest sequence has, which the division of the work goes by and nothing else.
+ * 16 bits with head_dim a multiple of 8 up to 256 and pages of 8 rows or more, 16-byte aligned, on the matrix cores; fp32 with head_dim a multiple of 4 up to 128
+ * likewise; everything else up to 256 dims on the generic kernel. */
+typedef struct {
+    int32_t dtype;
+    int32_t heads, kv_heads, head_dim;
+    int32_t n_seqs;
+    int32_t is_causal;
+    float scale;
+    int32_t max_kv;
+    int64_t total_q, total_kv;
+    int64_t q_strides[2], k_strides[2], v_strides[2], o_strides[2]; /* token, head (elements) */
+    const int32_t *cu_q;       /* [n_seqs + 1], on the device */
+    const int32_t *cu_kv;      /* [n_seqs + 1] */
+    const int32_t *page_table; /* [n_seqs, table_ld] or NULL */
+    const int32_t *kv_lengths; /* [n_seqs] */
+    int64_t table_ld;
+    AxhipKvPages pages;        /* read with page_table only */
+} AxhipSdpaPackedParams;
+int axhip_sdpa_packed(const void *q, const void *k, const void *v, void *o, const AxhipSdpaPackedParams *params_host, void *stream);
+size_t axhip_sdpa_packed_workspace_bytes(const AxhipSdpaPackedParams *params_host);
+int axhip_sdpa_packed_ws(const void *q, const void *k, const void *v, void *o, const AxhipSdpaPackedParams *params_host,
+                         void *workspace, size_t workspace_bytes, void *stream);
+
+/* A decoding step: the last new_tokens tokens of each of n_seqs sequences against what the cache holds of it (theirs among it).  q and
+ * o: [n_seqs, new_tokens, heads, head_dim] by strides; kv_lengths[s] keys in pages page_table[s * table_ld + ..]; token i sees key j <=
+ * kv_lengths[s] - new_tokens + i.
+ * Shared prefixes: the sequences group_starts[g] .. group_starts[g + 1] - 1 have the prefix_lengths[g] keys in pages
+ * prefix_table[g * prefix_ld + ..] in front of their own, all of which every token sees.  They are read once for the group, not once
+ * for each of its sequences.  Sequences in front of the first group and behind the last have no prefix; groups may be empty.
+ * Everything else as in axhip_sdpa_packed; max_kv and max_prefix are hints alike (own keys, prefix).  Lengths, tables and groups are
+ * read on the device when the kernels run: a captured step replays with what the arrays hold then. */
+typedef struct {
+    AxhipKvPages pages;
+    int32_t heads;
+    int32_t n_seqs, new_tokens;
+    int32_t max_kv;
+    float scale;
+    int32_t n_groups; /* 0: no prefixes */
+    int32_t max_prefix;
+    int32_t reserved; /* 0 */
+    int64_t q_strides[3], o_strides[3]; /* sequence, token, head (elements) */
+    const int32_t *page_table;          /* [n_seqs, table_ld], on the device */
+    const int32_t *kv_lengths;          /* [n_seqs] */
+    int64_t table_ld;
+    const int32_t *group_starts;        /* [n_groups + 1] */
+    const int32_t *prefix_table;        /* [n_groups, prefix_ld] */
+    const int32_t *prefix_lengths;      /* [n_groups] */
+    int64_t prefix_ld;
+} AxhipSdpaPagedParams;
+int axhip_sdpa_paged(const void *q, void *o, const AxhipSdpaPagedParams *params_host, void *stream);
+size_t axhip_sdpa_paged_workspace_bytes(const AxhipSdpaPagedParams *params_host);
+int axhip_sdpa_paged_ws(const void *q, void *o, const AxhipSdpaPagedParams *params_host, void *workspace, size_t workspace_bytes,
+                        void *stream);
+/* diagnostic: the kernels of the calling thread's last axhip_sdpa_packed or axhip_sdpa_paged ("tile", "rows", "f32", "generic", "empty"). */
+const char *axhip_sdpa_cache_last_kernel(void);
+
 /* sizeof() of the parameter structs as this library was compiled, so that a
  * foreign-language binding can verify its own struct layout at load time:
  * which = 0 AxhipSdpaParams, 1 AxhipRowsProgram, 2 AxhipGemmParams,
  * 3 AxhipOperand, 4 AxhipChainOp, 5 AxhipRowsQ8Params, 6 AxhipGemmQ8Params,
- * 7 AxhipSampleParams; anything else returns 0. */
+ * 7 AxhipSampleParams, 8 AxhipRopeScaling, 9 AxhipRopeParams, 10 AxhipKvPages,
+ * 11 AxhipKvAppendParams, 12 AxhipKvCopyParams, 13 AxhipSdpaPackedParams,
+ * 14 AxhipSdpaPagedParams; anything else returns 0. */
 size_t axhip_sizeof(int which);
 
 #ifdef __cplusplus
