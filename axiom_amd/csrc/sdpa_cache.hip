@@ -3,6 +3,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstdlib>
 
 namespace axhip {
 
@@ -269,6 +270,21 @@ int paged_args(CacheArgs &a, const AxhipSdpaPagedParams *params) {
     }
     return AXHIP_OK;
 }
+// Whether rows can be moved 16 bytes at a time and the matrix-core kernels take the head size.
+bool for_matrix_cores(const CacheArgs &a) {
+    const int es = static_cast<int>(dtype_size(a.dtype)), v = 16 / es;
+    if (a.D % v != 0 || a.D > (es == 2 ? 256 : 128) || (a.table && a.page_shift < 3)) return false;
+    uint64_t seen = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) | reinterpret_cast<uintptr_t>(a.o);
+    for (int i = 0; i < 3; ++i) seen |= static_cast<uint64_t>(a.qs[i] | a.ks[i] | a.vs[i] | a.os[i]) * es;
+    // (offsets inside a piece of 8 rows, and numbers of rows with one more block for each entry, are 32-bit ones)
+    const int64_t rows = (a.new_tokens ? static_cast<int64_t>(a.entries) * a.new_tokens : a.total_q) * a.each;
+    return (seen & 15) == 0 && a.ks[1] < (1 << 26) && a.vs[1] < (1 << 26) && rows + int64_t(256) * a.entries < (int64_t(1) << 30);
+}
+// AXHIP_SDPA_TILE_WAVES=4|8: waves of a work-group of the tile kernel (measurements only)
+const int tile_waves = [] {
+    const char *e = getenv("AXHIP_SDPA_TILE_WAVES");
+    return e ? atoi(e) : 0;
+}();
 bool tensor_ok(const void *p, int dtype) { return p && (reinterpret_cast<uintptr_t>(p) & (dtype_size(dtype) - 1)) == 0; }
 
 } // namespace
@@ -303,7 +319,14 @@ int axhip_sdpa_packed_ws(const void *q, const void *k, const void *v, void *o, c
     a.o = o;
     rc = ensure_init();
     if (rc) return rc;
-    return launch_generic(a, resolve_stream(stream), "axhip_sdpa_packed");
+    hipStream_t s = resolve_stream(stream);
+    if (a.dtype != AXHIP_DTYPE_F32 && for_matrix_cores(a)) {
+        const int64_t blocks = (a.total_q * a.each + 255) / 256 * a.kv_heads;
+        const int waves = tile_waves ? tile_waves : blocks >= 192 ? 8 : 4;
+        last_kernel = "tile";
+        return a.dtype == AXHIP_DTYPE_BF16 ? launch_tile_bf16(a, waves, s) : launch_tile_f16(a, waves, s);
+    }
+    return launch_generic(a, s, "axhip_sdpa_packed");
 }
 
 size_t axhip_sdpa_paged_workspace_bytes(const AxhipSdpaPagedParams *) { return 0; }

@@ -67,4 +67,8 @@ __device__ __forceinline__ int group_of(const CacheArgs &a, int s) {
     return lo > 0 && a.group_starts[lo] > s ? lo - 1 : -1;
 }
 
+// The matrix-core kernels (16 bits) of rows found by cu_q: sdpa_tile.hpp; 4 or 8 waves of 32 rows
+int launch_tile_bf16(const CacheArgs &a, int waves, hipStream_t s);
+int launch_tile_f16(const CacheArgs &a, int waves, hipStream_t s);
+
 } // namespace axhip

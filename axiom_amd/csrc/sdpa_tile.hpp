@@ -1,0 +1,415 @@
+// Ragged attention on the matrix cores, 16 bits: the kernel of whole prompts, of chunks of them, and of prefixes that many sequences share.
+//
+// A work-group owns 32 * NW rows of one entry and key head and walks its keys in tiles of 64.  It computes S^T = K Q^T on v_mfma_f32_32x32x16, so that a
+// lane owns one query and its softmax needs one exchange with lane ^ 32, and the exponentiated scores are the B operand of O^T += V^T P^T as they lie.  K and V go
+// from memory straight into swizzled LDS, K a tile ahead of V; the MFMAs of a step -- the output of tile j, the scores of tile j + 1 -- are issued back to back in
+// alternation, the softmax follows.  With eight waves the upper four (one of each SIMD's two) do that in the other order, so that one of the two is
+// in its matrix phase while the other one is in its vector phase.
+//
+// What the ragged form asks for:
+//  * rows are tokens times the heads that share a key head: one tile of keys serves them all, and a short sequence fills the work-group.
+//  * a piece of a tile that one load instruction fetches (2 to 8 rows) lies in one page, so that its address is wave-uniform: a scalar load of the page's number
+//    a step ahead and scalar arithmetic, no vector instruction a piece.  Only the piece with the last key has lanes to aim elsewhere (at that key: what lies behind it is not read).
+//  * work-groups find their rows in the lengths on the device, longest walks first (see tile_item).
+//  * scores are scaled in fp32, in the FMA that subtracts the maximum: q rounded after its scaling, which would save nothing here, adds as much error as the output's rounding does.
+#pragma once
+
+#include "sdpa_cache.hpp"
+
+#include <type_traits>
+
+namespace axhip {
+
+constexpr int TK = 64; // keys of a tile
+
+typedef int tile_int4_t __attribute__((ext_vector_type(4)));
+typedef const __attribute__((address_space(4))) int32_t *scalar_ints; // read by scalar loads
+
+template <bool BF16> __device__ __forceinline__ float16_t tile_mfma(uint4_t a, uint4_t b, float16_t c) {
+    if constexpr (BF16) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
+}
+// 4 consecutive keys of one dim out of [key][dim] rows: within a group of 16 lanes, lane i receives element i & 3 of the 8-byte pieces that lanes (i >> 2) + 4 j address
+__device__ __forceinline__ uint2_t tile_transposed(const unsigned char *p) {
+    typedef short short4_t __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) short4_t lds_short4_t;
+    return __builtin_bit_cast(uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_t *)(p)));
+}
+// 16 bytes a lane from base + offset straight into LDS: lane i's land at lds_base + 16 i; a lane that is switched off leaves its place as it is
+__device__ __forceinline__ void tile_fetch(uint64_t base_uniform, uint32_t offset, uint32_t lds_base_uniform) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_base_uniform), "v"(offset), "s"(base_uniform) : "memory");
+}
+// XOR of the 16-byte chunk's place in a row, so that neither 16 rows of one chunk nor the 4 rows of a transposing read meet on a bank
+template <int D> __device__ __forceinline__ int tile_swizzle_k(int row) { return D >= 128 ? (((row & 3) << 2) | ((row >> 2) & 3)) : ((row >> 1) & 7); }
+template <int D> __device__ __forceinline__ int tile_swizzle_v(int row) { return D >= 128 ? (((row & 3) << 2) | ((row >> 2) & 3)) : (((row >> 1) & 1) << 2); }
+
+__device__ __forceinline__ uint64_t uniform64(uint64_t v) {
+    return (static_cast<uint64_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(v >> 32))) << 32) | static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(v)));
+}
+
+// Block `index` of all blocks of BM rows, those that walk the most tiles of keys first: a long sequence's last blocks, started last, would keep a few CUs busy
+// after all others are done.  Up to 256 entries: the number of blocks that walk c tiles or more is a sum over the entries, four to a lane, and c is searched for.
+// More: in the order of the entries.  index: uniform.  entry < 0: no such block.
+struct TileItem { int entry, block; };
+template <int BM> __device__ __forceinline__ TileItem tile_item(const CacheArgs &a, int index) {
+    const int lane = threadIdx.x % WAVE;
+    if (a.entries > 256) {
+        auto first = [&](int e) { return static_cast<int>(static_cast<int64_t>(clamped(a.cu_q[e], 0, a.total_q)) * a.each / BM + e); };
+        int lo = 0, hi = a.entries; // first(lo) <= index; first(hi) is beyond it
+        while (hi - lo > 1) { // 64 candidates at a time
+            const int step = (hi - lo + WAVE - 1) / WAVE, e = lo + lane * step;
+            const uint64_t below = __builtin_amdgcn_ballot_w64(e < hi && first(e) <= index);
+            const int n = below ? 64 - __builtin_clzll(below) : 1;
+            hi = min(hi, lo + n * step);
+            lo = lo + (n - 1) * step;
+        }
+        return {lo, index - first(lo)};
+    }
+    int blocks[4], past[4], last[4], tiles[4]; // of this lane's entries: blocks, keys in front of the first token, last token, tiles of keys
+    float most = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int e = lane + WAVE * i;
+        blocks[i] = past[i] = last[i] = tiles[i] = 0;
+        if (WAVE * i < a.entries && e < a.entries) {
+            const TokenRun t = tokens_of(a, e);
+            const int keys = keys_of(a, e).n;
+            blocks[i] = (t.n * a.each + BM - 1) / BM;
+            past[i] = keys - t.n;
+            last[i] = t.n - 1;
+            tiles[i] = (keys + TK - 1) / TK;
+            if (blocks[i] > 0) most = fmaxf(most, static_cast<float>(tiles[i]));
+        }
+    }
+    auto with = [&](int i, int c) { // blocks of entry i that walk c tiles or more
+        if (c <= 0) return blocks[i];
+        if (tiles[i] < c) return 0;
+        if (!a.causal) return blocks[i];
+        const int token = TK * (c - 1) - past[i]; // the first one that sees so far
+        if (token <= 0) return blocks[i];
+        return token > last[i] ? 0 : blocks[i] - token * a.each / BM;
+    };
+    auto all_with = [&](int c) {
+        float n = 0.0f; // (below 2^24: exact)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (WAVE * i < a.entries) n += static_cast<float>(with(i, c));
+        return static_cast<int>(wave_sum(n));
+    };
+    int lo = 0, hi = static_cast<int>(wave_max(most)) + 1; // all_with(lo) > index >= all_with(hi)
+    if (index >= all_with(0)) return {-1, 0};
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (all_with(mid) > index) lo = mid;
+        else hi = mid;
+    }
+    int left = index - all_with(lo + 1); // among those that walk `lo` tiles exactly
+    TileItem item{-1, 0};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (WAVE * i >= a.entries || item.entry >= 0) continue;
+        const int mine = with(i, lo) - with(i, lo + 1);
+        int upto = mine;
+#pragma unroll
+        for (int d = 1; d < WAVE; d *= 2) {
+            const int other = __shfl_up(upto, d, WAVE);
+            if (lane >= d) upto += other;
+        }
+        const uint64_t reached = __builtin_amdgcn_ballot_w64(upto > left);
+        if (reached) {
+            const int at = __builtin_ctzll(reached);
+            item.entry = at + WAVE * i;
+            item.block = __builtin_amdgcn_readlane(blocks[i] - with(i, lo) + left - (upto - mine), at);
+        } else {
+            left -= __builtin_amdgcn_readlane(upto, WAVE - 1);
+        }
+    }
+    return item;
+}
+
+// D: the LDS row in dims; DE: the dims that are computed; the head size in memory, a multiple of 8, may be less (zeros in its place)
+template <bool BF16, int D, int DE, int NW, bool PAGED>
+__global__ __launch_bounds__(64 * NW, NW == 8 || D > 128 ? 1 : 2) void sdpa_tile_kernel(const CacheArgs a) {
+    static_assert(DE % 32 == 0 && DE <= D, "dims");
+    constexpr int PF = 3, RING = PF + 1; // LDS reads run this many MFMAs ahead
+    constexpr int KT = DE / 16, DT = DE / 32, BM = 32 * NW, ROWB = 2 * D, CHUNKS = ROWB / 16, RPL = WAVE / CHUNKS;
+    constexpr int NLOAD = TK / (RPL * NW), TILEB = TK * ROWB, NM = DE / 4;
+    constexpr int NV = RPL * NW < 16 ? 2 : 1; // (the swizzles see row & 15)
+    static_assert(NLOAD >= 1, "every wave fetches");
+    extern __shared__ __attribute__((aligned(1024))) unsigned char tile_lds[]; // K0 K1 V0 V1
+
+    const int tid = threadIdx.x, lane = tid % WAVE, wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
+    const int ql = lane % 32, g = lane / 32;
+    const bool second = NW == 8 && wave >= 4;
+    const int kvh = blockIdx.x % a.kv_heads;
+    const TileItem item = tile_item<BM>(a, blockIdx.x / a.kv_heads);
+    const int entry = __builtin_amdgcn_readfirstlane(item.entry), block = __builtin_amdgcn_readfirstlane(item.block);
+    if (entry < 0) return;
+    const TokenRun tokens = tokens_of(a, entry);
+    const KeyRun run = keys_of(a, entry);
+    const int rows = __builtin_amdgcn_readfirstlane(tokens.n * a.each), nk = __builtin_amdgcn_readfirstlane(run.n);
+    const int row0 = block * BM;
+    if (block < 0 || row0 >= rows) return;
+    const int dv = a.D;
+    const int past = nk - tokens.n;
+
+    // this lane's query, and the last key that it sees; rows behind the last one see what that one does and are not stored
+    const int row = row0 + 32 * wave + ql;
+    const bool row_ok = row < rows;
+    auto sees = [&](int r) { return a.causal ? past + min(r, rows - 1) / a.each : nk - 1; };
+    const int token = min(row, rows - 1) / a.each, head = kvh * a.each + min(row, rows - 1) % a.each;
+    const int limit = a.causal ? past + token : nk - 1;
+    const int wave_row = row0 + 32 * wave;
+    const int least = __builtin_amdgcn_readfirstlane(sees(wave_row)), farthest = __builtin_amdgcn_readfirstlane(wave_row < rows ? sees(wave_row + 31) : -1);
+    const int ntiles = __builtin_amdgcn_readfirstlane((sees(row0 + BM - 1) + TK) / TK); // (sees -1: none)
+    const int64_t at_q = (tokens.from + token) * a.qs[1] + head * a.qs[2];
+    uint16_t *const orow = static_cast<uint16_t *>(a.o) + (tokens.from + token) * a.os[1] + head * a.os[2];
+
+    uint4_t qf[KT];
+    {
+        const uint16_t *q = static_cast<const uint16_t *>(a.q) + at_q;
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+            qf[t] = uint4_t{0, 0, 0, 0};
+            if (row_ok && 16 * t + 8 * g < dv) qf[t] = *reinterpret_cast<const uint4_t *>(q + 16 * t + 8 * g);
+        }
+    }
+
+    // ---- memory -> LDS
+    const uint64_t k_base = uniform64(reinterpret_cast<uint64_t>(a.k) + static_cast<uint64_t>(kvh * a.ks[2]) * 2), v_base = uniform64(reinterpret_cast<uint64_t>(a.v) + static_cast<uint64_t>(kvh * a.vs[2]) * 2);
+    const uint32_t k_row = static_cast<uint32_t>(a.ks[1]) * 2, v_row = static_cast<uint32_t>(a.vs[1]) * 2;
+    const scalar_ints table = (scalar_ints)(uniform64(reinterpret_cast<uint64_t>(run.table)));
+    const int my = lane / CHUNKS; // row of a piece
+    uint32_t k_off[NV], v_off[NV];
+    int k_chunk[NV], v_chunk[NV];
+#pragma unroll
+    for (int o = 0; o < NV; ++o) {
+        const int r = RPL * wave + my + 8 * o;
+        k_chunk[o] = (lane % CHUNKS) ^ tile_swizzle_k<D>(r);
+        v_chunk[o] = (lane % CHUNKS) ^ tile_swizzle_v<D>(r);
+        k_off[o] = my * k_row + k_chunk[o] * 16;
+        v_off[o] = my * v_row + v_chunk[o] * 16;
+    }
+    const uint32_t lds_base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(tile_lds));
+    const uint32_t lds_wave = __builtin_amdgcn_readfirstlane(lds_base + RPL * wave * ROWB);
+    const int last_piece = __builtin_amdgcn_readfirstlane((nk - 1) / RPL * RPL);
+    bool bad = false;
+    auto piece_of = [&](int tile, int n) { return min(tile * TK + RPL * NW * n + RPL * wave, last_piece); };
+    struct Pages { int id[NLOAD]; };
+    auto pages_at = [&](int tile) { // the pages of this wave's pieces of a tile
+        Pages p;
+#pragma unroll
+        for (int n = 0; n < NLOAD; ++n) p.id[n] = PAGED ? table[piece_of(tile, n) >> a.page_shift] : 0;
+        return p;
+    };
+    auto fetch = [&](uint64_t base, const int64_t (&strides)[3], uint32_t row_bytes, const uint32_t (&off)[NV], const int (&chunk)[NV], int tile, const Pages &p, uint32_t to) __attribute__((always_inline)) {
+#pragma unroll
+        for (int n = 0; n < NLOAD; ++n) {
+            const int piece = piece_of(tile, n);
+            int64_t at;
+            if constexpr (PAGED) {
+                int id = p.id[n];
+                if (static_cast<uint32_t>(id) >= static_cast<uint32_t>(a.n_pages)) {
+                    bad = true;
+                    id = 0;
+                }
+                at = id * strides[0] * 2 + static_cast<int64_t>(piece & ((1 << a.page_shift) - 1)) * row_bytes;
+            } else {
+                at = (run.base + piece) * static_cast<int64_t>(row_bytes);
+            }
+            uint32_t offset = off[n % NV];
+            if (piece == last_piece) offset -= (my - min(my, nk - 1 - last_piece)) * row_bytes;
+            if (chunk[n % NV] * 8 < dv) tile_fetch(uniform64(base + static_cast<uint64_t>(at)), offset, to + n * RPL * NW * ROWB);
+        }
+    };
+    auto load_k = [&](int tile, int buf, const Pages &p) __attribute__((always_inline)) { fetch(k_base, a.ks, k_row, k_off, k_chunk, tile, p, lds_wave + buf * TILEB); };
+    auto load_v = [&](int tile, int buf, const Pages &p) __attribute__((always_inline)) { fetch(v_base, a.vs, v_row, v_off, v_chunk, tile, p, lds_wave + (2 + buf) * TILEB); };
+
+    // ---- LDS fragments (bytes)
+    int k_at[KT]; // row ql (+ 32), chunk 2 t + g
+#pragma unroll
+    for (int t = 0; t < KT; ++t) k_at[t] = ql * ROWB + (((2 * t + g) ^ tile_swizzle_k<D>(ql)) * 16);
+    int v_at[2][DT]; // rows 4 g + s (+ 8), dims 32 dt + lane % 32
+    {
+        const int s = (lane & 15) >> 2, c = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1), part = lane & 1;
+#pragma unroll
+        for (int hi = 0; hi < 2; ++hi)
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                const int r = 4 * g + s + 8 * hi;
+                v_at[hi][dt] = r * ROWB + (((dt * 4 + c) ^ tile_swizzle_v<D>(r)) * 16) + part * 8;
+            }
+    }
+    auto barrier = [] { asm volatile("s_barrier" ::: "memory"); };
+    auto landed = [] { __builtin_amdgcn_s_waitcnt(0x0F70); }; // vmcnt(0)
+
+    if (dv < DE) { // the dims that no load fills: zeros, whatever K and V hold there
+        for (int i = tid; i < 4 * TILEB / 16; i += 64 * NW) reinterpret_cast<uint4_t *>(tile_lds)[i] = uint4_t{0, 0, 0, 0};
+        __syncthreads();
+    }
+
+    float16_t oacc[DT], s[2];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) oacc[dt][i] = 0.0f;
+    float m_run = NEG_INF_F, l0 = 0.0f, l1 = 0.0f; // the reference that exponentials are taken against (base 2, scaled), may lag the maximum
+    uint32_t w[16];
+    auto larger = [](float x, float y) { return __builtin_elementwise_maximum(x, y); }; // (needs no canonical input; hands a NaN on)
+
+    auto softmax_phase = [&](int j) __attribute__((always_inline)) {
+        if (j * TK + TK - 1 > least) {
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (j * TK + kt * 32 + (i / 4) * 8 + g * 4 + i % 4 > limit) s[kt][i] = NEG_INF_F;
+        }
+        float m[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            m[c] = larger(s[c / 2][8 * (c % 2)], s[c / 2][8 * (c % 2) + 1]);
+#pragma unroll
+            for (int i = 2; i < 8; i += 2) m[c] = larger(larger(m[c], s[c / 2][8 * (c % 2) + i]), s[c / 2][8 * (c % 2) + i + 1]);
+        }
+        float top = larger(larger(m[0], m[1]), larger(m[2], m[3]));
+        top = across32(top, [&](float x, float y) { return larger(x, y); });
+        const float m_new = larger(m_run, top * a.scale_log2e);
+        if (__builtin_amdgcn_ballot_w64(m_new - m_run > RESCALE_THRESHOLD) != 0) { // (rare; -inf - -inf compares false)
+            const float alpha = m_new == NEG_INF_F ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
+            m_run = m_new;
+            l0 *= alpha;
+            l1 *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) oacc[dt][i] *= alpha;
+        }
+        const float minus = m_run == NEG_INF_F ? 0.0f : -m_run;
+#pragma unroll
+        for (int pr = 0; pr < 16; ++pr) {
+            const int kt = pr / 8, i = (pr % 8) * 2;
+            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][i], a.scale_log2e, minus));
+            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][i + 1], a.scale_log2e, minus));
+            w[pr] = pack2<BF16>(p0, p1);
+            l0 += p0; // (sums of pairs by the dot instruction wait for the matrix pipe)
+            l1 += p1;
+        }
+    };
+    // O^T += V^T P^T of tile j and S^T = K Q^T of tile j + 1 in turn, so that neighbours never share an accumulator
+    auto matrix_phase = [&](const unsigned char *Kn, const unsigned char *Vb) __attribute__((always_inline)) {
+        uint4_t fr[RING];
+        auto read = [&](int m) __attribute__((always_inline)) {
+            const int i = m / 2;
+            if (m % 2 == 0) {
+                fr[m % RING] = *reinterpret_cast<const uint4_t *>(Kn + (i & 1) * 32 * ROWB + k_at[i >> 1]);
+            } else {
+                const uint2_t lo = tile_transposed(Vb + (i / DT) * 16 * ROWB + v_at[0][i % DT]), hi = tile_transposed(Vb + (i / DT) * 16 * ROWB + v_at[1][i % DT]);
+                fr[m % RING] = uint4_t{lo.x, lo.y, hi.x, hi.y};
+            }
+        };
+#pragma unroll
+        for (int m = 0; m < PF; ++m) read(m);
+#pragma unroll
+        for (int m = 0; m < NM; ++m) {
+            if (m + PF < NM) read(m + PF);
+            const int i = m / 2;
+            if (m % 2 == 0) {
+                const float16_t zero{};
+                s[i & 1] = tile_mfma<BF16>(fr[m % RING], qf[i >> 1], i < 2 ? zero : s[i & 1]);
+            } else {
+                const uint4_t p = {w[4 * (i / DT)], w[4 * (i / DT) + 1], w[4 * (i / DT) + 2], w[4 * (i / DT) + 3]};
+                oacc[i % DT] = tile_mfma<BF16>(fr[m % RING], p, oacc[i % DT]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+
+    if (ntiles > 0) {
+        Pages here = pages_at(0), next = pages_at(1); // of the tile that V is fetched of next, of the one that K is
+        load_k(0, 0, here);
+        load_v(0, 0, here);
+        if (ntiles > 1) load_k(1, 1, next);
+        here = next;
+        next = pages_at(2);
+        landed();
+        barrier();
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+            for (int t = 0; t < KT; ++t) {
+                const float16_t zero{};
+                s[kt] = tile_mfma<BF16>(*reinterpret_cast<const uint4_t *>(tile_lds + kt * 32 * ROWB + k_at[t]), qf[t], t == 0 ? zero : s[kt]);
+            }
+        }
+        __builtin_amdgcn_s_waitcnt(0xC07F); // lgkmcnt(0): K buffer 0 is read
+        auto active = [&](int j) { return j * TK <= farthest; };
+        // one barrier a tile: behind it tile j + 1 of K and j of V have landed, and every wave is done with the buffers that K(j + 2) and V(j + 1) go to
+        auto step = [&](int j, auto parity) __attribute__((always_inline)) {
+            constexpr int PAR = decltype(parity)::value;
+            landed();
+            barrier();
+            if (j + 2 < ntiles) load_k(j + 2, PAR, next);
+            if (j + 1 < ntiles) load_v(j + 1, 1 - PAR, here);
+            here = next;
+            next = pages_at(j + 3);
+            if (second && active(j)) softmax_phase(j);
+            if (active(j)) matrix_phase(tile_lds + (1 - PAR) * TILEB, tile_lds + (2 + PAR) * TILEB);
+            if (!second && j + 1 < ntiles && active(j + 1)) softmax_phase(j + 1);
+        };
+        if (!second && active(0)) softmax_phase(0);
+        for (int j = 0; j < ntiles; j += 2) {
+            step(j, std::integral_constant<int, 0>{});
+            if (j + 1 < ntiles) step(j + 1, std::integral_constant<int, 1>{});
+        }
+    }
+
+    float l = across32(l0 + l1, lanes_add);
+    if constexpr (PAGED) { // a page that does not exist, seen by any wave
+        __syncthreads();
+        uint32_t *flags = reinterpret_cast<uint32_t *>(tile_lds);
+        if (lane == 0) flags[wave] = bad;
+        __syncthreads();
+        uint32_t any = 0;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) any |= flags[i];
+        if (any) l = __builtin_nanf("");
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    // a lane holds 4 consecutive dims of each group of 8; the halves trade every second group: 16 bytes a store
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int ip = 0; ip < 2; ++ip) {
+            const int ia = 8 * ip, ib = 8 * ip + 4;
+            const uint32_t x0 = pack2<BF16>(oacc[dt][ia] * inv, oacc[dt][ia + 1] * inv), x1 = pack2<BF16>(oacc[dt][ia + 2] * inv, oacc[dt][ia + 3] * inv);
+            const uint32_t y0 = pack2<BF16>(oacc[dt][ib] * inv, oacc[dt][ib + 1] * inv), y1 = pack2<BF16>(oacc[dt][ib + 2] * inv, oacc[dt][ib + 3] * inv);
+            const auto r0 = __builtin_amdgcn_permlane32_swap(x0, y0, false, false);
+            const auto r1 = __builtin_amdgcn_permlane32_swap(x1, y1, false, false);
+            const int d = dt * 32 + (2 * ip + g) * 8;
+            if (row_ok && d < dv) *reinterpret_cast<uint4_t *>(orow + d) = uint4_t{r0[0], r1[0], r0[1], r1[1]};
+        }
+}
+
+// Blocks of BM rows, at most; 0: more than a launch takes
+template <bool BF16, int D, int DE, int NW, bool PAGED> int launch_tile_as(const CacheArgs &a, hipStream_t s) {
+    constexpr int lds = 4 * TK * 2 * D;
+    if constexpr (lds > 65536) {
+        static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(&sdpa_tile_kernel<BF16, D, DE, NW, PAGED>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        AXHIP_CHECK_HIP(attr);
+    }
+    const int64_t blocks = (a.total_q * a.each / (32 * NW) + a.entries) * a.kv_heads;
+    AXHIP_REQUIRE(launch_fits(blocks, 64 * NW), AXHIP_ERR_UNSUPPORTED, "axhip_sdpa_packed: grid too large");
+    hipLaunchKernelGGL((sdpa_tile_kernel<BF16, D, DE, NW, PAGED>), dim3(static_cast<unsigned>(blocks)), dim3(64 * NW), lds, s, a);
+    AXHIP_CHECK_HIP(hipGetLastError());
+    return AXHIP_OK;
+}
+template <bool BF16, bool PAGED> int launch_tile_paged(const CacheArgs &a, int waves, hipStream_t s) {
+    if (a.D > 128) return launch_tile_as<BF16, 256, 256, 4, PAGED>(a, s);
+    if (a.D > 96) return waves == 8 ? launch_tile_as<BF16, 128, 128, 8, PAGED>(a, s) : launch_tile_as<BF16, 128, 128, 4, PAGED>(a, s);
+    if (a.D > 64) return waves == 8 ? launch_tile_as<BF16, 128, 96, 8, PAGED>(a, s) : launch_tile_as<BF16, 128, 96, 4, PAGED>(a, s);
+    return waves == 8 ? launch_tile_as<BF16, 64, 64, 8, PAGED>(a, s) : launch_tile_as<BF16, 64, 64, 4, PAGED>(a, s);
+}
+template <bool BF16> int launch_tile(const CacheArgs &a, int waves, hipStream_t s) { return a.table ? launch_tile_paged<BF16, true>(a, waves, s) : launch_tile_paged<BF16, false>(a, waves, s); }
+
+} // namespace axhip
