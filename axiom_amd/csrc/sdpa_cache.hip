@@ -206,7 +206,7 @@ int packed_args(CacheArgs &a, const AxhipSdpaPackedParams *params) {
     const AxhipSdpaPackedParams &p = *params;
     int rc = common_args(who, a, p.dtype, p.heads, p.kv_heads, p.head_dim, p.scale);
     if (rc) return rc;
-    AXHIP_REQUIRE(p.n_seqs >= 0 && p.n_seqs < (1 << 24) && p.total_q >= 0 && p.total_q < (int64_t(1) << 31), AXHIP_ERR_INVALID_ARG, "axhip_sdpa_packed: bad extent");
+    AXHIP_REQUIRE(p.n_seqs >= 0 && p.n_seqs < (1 << 24) && p.total_q >= 0 && p.total_q < MOST_KEYS, AXHIP_ERR_INVALID_ARG, "axhip_sdpa_packed: bad extent");
     AXHIP_REQUIRE(p.is_causal == 0 || p.is_causal == 1, AXHIP_ERR_INVALID_ARG, "axhip_sdpa_packed: is_causal is %d, neither 0 nor 1", p.is_causal);
     AXHIP_REQUIRE(sane(p.q_strides, 2) && sane(p.o_strides, 2), AXHIP_ERR_INVALID_ARG, "axhip_sdpa_packed: bad stride");
     a.entries = p.n_seqs;
@@ -226,7 +226,7 @@ int packed_args(CacheArgs &a, const AxhipSdpaPackedParams *params) {
                       "axhip_sdpa_packed: pages of another type, other heads or another head_dim");
         return AXHIP_OK;
     }
-    AXHIP_REQUIRE(p.total_kv >= 0 && p.total_kv < (int64_t(1) << 31), AXHIP_ERR_INVALID_ARG, "axhip_sdpa_packed: bad extent");
+    AXHIP_REQUIRE(p.total_kv >= 0 && p.total_kv < MOST_KEYS, AXHIP_ERR_INVALID_ARG, "axhip_sdpa_packed: bad extent");
     AXHIP_REQUIRE(sane(p.k_strides, 2) && sane(p.v_strides, 2), AXHIP_ERR_INVALID_ARG, "axhip_sdpa_packed: bad stride");
     AXHIP_REQUIRE(p.cu_kv && int_aligned(p.cu_kv), AXHIP_ERR_INVALID_ARG, "axhip_sdpa_packed: NULL or unaligned cu_kv");
     a.cu_kv = p.cu_kv;
@@ -276,15 +276,42 @@ bool for_matrix_cores(const CacheArgs &a) {
     if (a.D % v != 0 || a.D > (es == 2 ? 256 : 128) || (a.table && a.page_shift < 3)) return false;
     uint64_t seen = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) | reinterpret_cast<uintptr_t>(a.o);
     for (int i = 0; i < 3; ++i) seen |= static_cast<uint64_t>(a.qs[i] | a.ks[i] | a.vs[i] | a.os[i]) * es;
-    // (offsets inside a piece of 8 rows, and numbers of rows with one more block for each entry, are 32-bit ones)
+    // (offsets inside a piece of 8 rows, and numbers of rows with one more block for each entry, are 32-bit ones; numbers of blocks are added up as floats, exactly below 2^24)
     const int64_t rows = (a.new_tokens ? static_cast<int64_t>(a.entries) * a.new_tokens : a.total_q) * a.each;
-    return (seen & 15) == 0 && a.ks[1] < (1 << 26) && a.vs[1] < (1 << 26) && rows + int64_t(256) * a.entries < (int64_t(1) << 30);
+    return (seen & 15) == 0 && a.ks[1] < (1 << 26) && a.vs[1] < (1 << 26) && rows + int64_t(256) * a.entries < (int64_t(1) << (es == 4 ? 27 : 30));
 }
 // AXHIP_SDPA_TILE_WAVES=4|8: waves of a work-group of the tile kernel (measurements only)
 const int tile_waves = [] {
     const char *e = getenv("AXHIP_SDPA_TILE_WAVES");
     return e ? atoi(e) : 0;
 }();
+
+// How a decoding step is divided, and its temporary memory: what the parts leave for the join.  Nothing of it depends on addresses.
+struct StepPlan {
+    int want, prefix;
+    size_t own_out, own_lse, prefix_out, prefix_lse, bytes; // places; all of it (0: nothing can have two parts)
+};
+StepPlan step_plan(const CacheArgs &a) {
+    StepPlan p{};
+    const int64_t rows = static_cast<int64_t>(a.new_tokens) * a.each, tiles = (rows + 15) / 16, most = std::min(a.table_ld << a.page_shift, MOST_KEYS);
+    // parts of the own keys: four work-groups of four waves for each CU
+    p.want = static_cast<int>(std::max<int64_t>(1, 1024 / (a.kv_heads * tiles)));
+    if (a.groups == 0 && most <= 128) return p;
+    // parts of a prefix: one work-group of 128 rows for each CU
+    const int64_t blocks = (a.entries * rows + 127) / 128 * a.kv_heads;
+    p.prefix = a.groups == 0 ? 0 : static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({64, 256 / blocks, (std::min(a.prefix_ld << a.page_shift, MOST_KEYS) + 63) / 64})));
+    CacheArgs with = a;
+    with.want_parts = p.want;
+    const size_t own = static_cast<size_t>(own_capacity(with)) * a.kv_heads * rows, pre = static_cast<size_t>(a.entries) * a.kv_heads * rows * p.prefix;
+    size_t at = CallScratch::rounded(sizeof(int2_t) * a.entries);
+    auto place = [&](size_t floats) { const size_t here = at; at = CallScratch::rounded(at + floats * sizeof(float)); return here; };
+    p.own_out = place(own * a.D);
+    p.own_lse = place(own);
+    p.prefix_out = place(pre * a.D);
+    p.prefix_lse = place(pre);
+    p.bytes = at;
+    return p;
+}
 bool tensor_ok(const void *p, int dtype) { return p && (reinterpret_cast<uintptr_t>(p) & (dtype_size(dtype) - 1)) == 0; }
 
 } // namespace
@@ -320,7 +347,11 @@ int axhip_sdpa_packed_ws(const void *q, const void *k, const void *v, void *o, c
     rc = ensure_init();
     if (rc) return rc;
     hipStream_t s = resolve_stream(stream);
-    if (a.dtype != AXHIP_DTYPE_F32 && for_matrix_cores(a)) {
+    if (a.dtype == AXHIP_DTYPE_F32 && for_matrix_cores(a)) {
+        last_kernel = "f32";
+        return launch_rows_packed_f32(a, s);
+    }
+    if (for_matrix_cores(a)) {
         const int64_t blocks = (a.total_q * a.each + 255) / 256 * a.kv_heads;
         const int waves = tile_waves ? tile_waves : blocks >= 192 ? 8 : 4;
         last_kernel = "tile";
@@ -329,11 +360,15 @@ int axhip_sdpa_packed_ws(const void *q, const void *k, const void *v, void *o, c
     return launch_generic(a, s, "axhip_sdpa_packed");
 }
 
-size_t axhip_sdpa_paged_workspace_bytes(const AxhipSdpaPagedParams *) { return 0; }
+size_t axhip_sdpa_paged_workspace_bytes(const AxhipSdpaPagedParams *params) {
+    CacheArgs a{};
+    if (paged_args(a, params) != AXHIP_OK || a.entries == 0) return 0;
+    return step_plan(a).bytes;
+}
 
 int axhip_sdpa_paged(const void *q, void *o, const AxhipSdpaPagedParams *params, void *stream) { return axhip_sdpa_paged_ws(q, o, params, nullptr, 0, stream); }
 
-int axhip_sdpa_paged_ws(const void *q, void *o, const AxhipSdpaPagedParams *params, void *, size_t, void *stream) {
+int axhip_sdpa_paged_ws(const void *q, void *o, const AxhipSdpaPagedParams *params, void *workspace, size_t workspace_bytes, void *stream) {
     CacheArgs a{};
     int rc = paged_args(a, params);
     if (rc) return rc;
@@ -344,7 +379,37 @@ int axhip_sdpa_paged_ws(const void *q, void *o, const AxhipSdpaPagedParams *para
     a.o = o;
     rc = ensure_init();
     if (rc) return rc;
-    return launch_generic(a, resolve_stream(stream), "axhip_sdpa_paged");
+    hipStream_t s = resolve_stream(stream);
+    if (!for_matrix_cores(a)) return launch_generic(a, s, "axhip_sdpa_paged");
+    const StepPlan plan = step_plan(a);
+    a.want_parts = plan.want;
+    a.prefix_parts = plan.prefix;
+    CallScratch scratch(workspace, workspace_bytes, s);
+    if (plan.bytes > 0) {
+        void *at = nullptr;
+        rc = scratch.take(&at, plan.bytes, "axhip_sdpa_paged");
+        if (rc) return rc;
+        char *p = static_cast<char *>(at);
+        a.parts_of = reinterpret_cast<int2_t *>(p);
+        a.own_out = reinterpret_cast<float *>(p + plan.own_out);
+        a.own_lse = reinterpret_cast<float *>(p + plan.own_lse);
+        a.prefix_out = reinterpret_cast<float *>(p + plan.prefix_out);
+        a.prefix_lse = reinterpret_cast<float *>(p + plan.prefix_lse);
+    }
+    last_kernel = "rows";
+    const bool f32 = a.dtype == AXHIP_DTYPE_F32, bf16 = a.dtype == AXHIP_DTYPE_BF16;
+    if (a.groups > 0) {
+        last_kernel = "rows, prefix";
+        rc = f32 ? launch_prefix_f32(a, s) : bf16 ? launch_prefix_bf16(a, s) : launch_prefix_f16(a, s);
+        if (rc) return rc;
+    }
+    rc = f32 ? launch_rows_own_f32(a, s) : bf16 ? launch_rows_own_bf16(a, s) : launch_rows_own_f16(a, s);
+    if (rc) return rc;
+    if (plan.bytes > 0) {
+        rc = f32 ? launch_join_f32(a, s) : bf16 ? launch_join_bf16(a, s) : launch_join_f16(a, s);
+        if (rc) return rc;
+    }
+    return scratch.release();
 }
 
 } // extern "C"

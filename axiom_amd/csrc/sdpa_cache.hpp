@@ -29,7 +29,16 @@ struct CacheArgs {
     int groups;
     const int32_t *group_starts, *prefix_table, *prefix_lengths;
     int64_t prefix_ld;
+    // decoding in parts: how many of the own keys are wanted, how many a prefix has at most; what they leave for the join, by part, key head and row, or by
+    // sequence, key head, row and part; for each sequence where its parts begin and how many there are to join (0: it is finished)
+    int want_parts, prefix_parts;
+    float *own_out, *own_lse, *prefix_out, *prefix_lse;
+    int2_t *parts_of;
 };
+// Parts of the own keys there can be: see own_part
+inline int64_t own_capacity(const CacheArgs &a) { return static_cast<int64_t>(a.want_parts) + a.entries + 2; }
+
+constexpr int64_t MOST_KEYS = int64_t(1) << 30; // of a sequence
 
 // The keys of an entry
 struct KeyRun {
@@ -41,14 +50,14 @@ __device__ __forceinline__ int clamped(int64_t v, int64_t lo, int64_t hi) { retu
 __device__ __forceinline__ KeyRun keys_of(const CacheArgs &a, int s) {
     if (a.table) {
         const int64_t most = a.table_ld << a.page_shift;
-        return {a.table + s * a.table_ld, 0, clamped(a.lengths[s], 0, most < 0x7FFFFFFF ? most : 0x7FFFFFFF)};
+        return {a.table + s * a.table_ld, 0, clamped(a.lengths[s], 0, most < MOST_KEYS ? most : MOST_KEYS)};
     }
     const int from = clamped(a.cu_kv[s], 0, a.total_kv);
     return {nullptr, from, clamped(a.cu_kv[s + 1], from, a.total_kv) - from};
 }
 __device__ __forceinline__ KeyRun prefix_of(const CacheArgs &a, int group) {
     const int64_t most = a.prefix_ld << a.page_shift;
-    return {a.prefix_table + group * a.prefix_ld, 0, clamped(a.prefix_lengths[group], 0, most < 0x7FFFFFFF ? most : 0x7FFFFFFF)};
+    return {a.prefix_table + group * a.prefix_ld, 0, clamped(a.prefix_lengths[group], 0, most < MOST_KEYS ? most : MOST_KEYS)};
 }
 struct TokenRun { int from, n; };
 __device__ __forceinline__ TokenRun tokens_of(const CacheArgs &a, int s) {
@@ -70,5 +79,17 @@ __device__ __forceinline__ int group_of(const CacheArgs &a, int s) {
 // The matrix-core kernels (16 bits) of rows found by cu_q: sdpa_tile.hpp; 4 or 8 waves of 32 rows
 int launch_tile_bf16(const CacheArgs &a, int waves, hipStream_t s);
 int launch_tile_f16(const CacheArgs &a, int waves, hipStream_t s);
+// .. of a group's rows against the parts of its prefix
+int launch_prefix_bf16(const CacheArgs &a, hipStream_t s);
+int launch_prefix_f16(const CacheArgs &a, hipStream_t s);
+int launch_prefix_f32(const CacheArgs &a, hipStream_t s);
+// Few rows and fp32: sdpa_rows.hpp
+int launch_rows_own_bf16(const CacheArgs &a, hipStream_t s);
+int launch_rows_own_f16(const CacheArgs &a, hipStream_t s);
+int launch_rows_own_f32(const CacheArgs &a, hipStream_t s);
+int launch_rows_packed_f32(const CacheArgs &a, hipStream_t s);
+int launch_join_bf16(const CacheArgs &a, hipStream_t s);
+int launch_join_f16(const CacheArgs &a, hipStream_t s);
+int launch_join_f32(const CacheArgs &a, hipStream_t s);
 
 } // namespace axhip

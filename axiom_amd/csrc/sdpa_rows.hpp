@@ -1,0 +1,504 @@
+// Ragged attention of few rows against many keys, and of fp32: 16 rows of one entry and key head, four waves that take 16 or 32 keys in turn and meet once, at the end, through LDS.
+//
+// Nothing is shared before that: K and V go from memory straight into the operands of the matrix instructions.  In what order keys and dims run through an MFMA is free as
+// long as both operands agree, so:
+//   S^T = K Q^T    leaves lane (l16, g) with row l16 and keys 4 g + i of a 16-key sub-tile;
+//   O^T = V^T P^T  takes those keys as its k-slots (the probabilities are its B operand as they stand), and the lane needs, of V, rows of its own keys: in 16 bits 16-byte runs
+//                  whose transpose is byte permutes between its registers, in fp32 the elements as they come.
+// Bound by one read of K and V (decoding): a step's 16 loads are requested a step ahead, the page numbers they need a step earlier.
+//
+// A decoding step divides all its own keys into parts of one size, found from the lengths on the device, so that the chip is filled whatever they are: Parts below.  A sequence of
+// one part and no prefix is finished here; the others leave fp32 results and the base-2 logarithm of their denominators for sdpa_join_kernel.
+#pragma once
+
+#include "sdpa_cache.hpp"
+#include "sdpa_tile_item.hpp"
+
+#include <type_traits>
+
+namespace axhip {
+
+typedef float rows_f32x4 __attribute__((ext_vector_type(4)));
+template <int DT> __device__ __forceinline__ rows_f32x4 rows_mfma(uint4_t a, uint4_t b, rows_f32x4 c) {
+    if constexpr (DT == AXHIP_DTYPE_BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
+}
+
+constexpr int ROWS_WAVES = 4, ROWS = 16;
+template <int D> constexpr int rows_lds_bytes() { return ROWS_WAVES * ROWS * (D + 4 + 2) * 4; }
+
+// Which keys of which sequence: part `part` of `parts`, of `chunk` keys each, at place `slot` among all parts
+struct Part { int entry, part, parts, chunk, slot; };
+// Part `index` of a decoding step's own keys, by all 256 threads of a work-group.  Lengths count in units of UNIT keys; with a sum of U units a part is ceil(U / want) units, at least
+// one, which makes want + entries parts at most (every sequence has one, an empty one too); two more for the rounding of the sum, which is one of floats.
+constexpr int UNIT = 128;
+__device__ inline Part own_part(const CacheArgs &a, int index) {
+    __shared__ float sums[ROWS_WAVES];
+    __shared__ int totals[ROWS_WAVES];
+    __shared__ Part found;
+    const int tid = threadIdx.x, lane = tid % WAVE, wave = tid / WAVE;
+    const int n = a.entries, per = (n + 255) / 256, from = min(tid * per, n), to = min(from + per, n);
+    auto units = [&](int e) { return (keys_of(a, e).n + UNIT - 1) / UNIT; };
+    float u = 0.0f;
+    for (int e = from; e < to; ++e) u += static_cast<float>(units(e));
+    u = wave_sum(u);
+    if (lane == 0) sums[wave] = u;
+    if (tid == 0) found.entry = -1;
+    __syncthreads();
+    u = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+    const int size = max(1, static_cast<int>(fminf(ceilf(u / static_cast<float>(a.want_parts)), 8388608.0f)));
+    int mine = 0;
+    for (int e = from; e < to; ++e) mine += max(1, (units(e) + size - 1) / size);
+    int upto = mine;
+#pragma unroll
+    for (int d = 1; d < WAVE; d *= 2) {
+        const int other = __shfl_up(upto, d, WAVE);
+        if (lane >= d) upto += other;
+    }
+    if (lane == WAVE - 1) totals[wave] = upto;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) upto += totals[w];
+    int at = upto - mine;
+    if (index >= at && index < upto) {
+        for (int e = from; e < to; ++e) {
+            const int parts = max(1, (units(e) + size - 1) / size);
+            if (index < at + parts) {
+                found = Part{e, index - at, parts, size * UNIT, at};
+                break;
+            }
+            at += parts;
+        }
+    }
+    __syncthreads();
+    return found;
+}
+
+// What a work-group does: OWN, a part of a sequence's own keys (decoding); PACKED, whole sequences by cu_q (fp32 prompts); PREFIX, a part of a group's prefix for 16 of its rows (fp32)
+enum RowsMode { ROWS_OWN = 0, ROWS_PACKED = 1, ROWS_PREFIX = 2 };
+
+template <int DT, int D, bool PAD, int MODE>
+__global__ __launch_bounds__(64 * ROWS_WAVES, D > 128 ? 1 : 2) void sdpa_rows_kernel(const CacheArgs a) {
+    constexpr bool F32 = DT == AXHIP_DTYPE_F32;
+    constexpr int ES = F32 ? 4 : 2;
+    constexpr int SUB = F32 && D > 64 ? 1 : 2, KEYS = 16 * SUB, STRIDE = KEYS * ROWS_WAVES;
+    constexpr int KJ = F32 ? D / 16 : D / 32; // 16-byte pieces of a K row that a lane holds
+    constexpr int NT = D / 16;                // 16 bits: output tiles, and elements of V that a lane holds of a key
+    constexpr int VH = F32 ? D / 64 : (NT * 2 + 15) / 16; // 16-byte pieces of a V row that a lane holds (D = 64 in 16 bits: half of one)
+    static_assert(!F32 || D <= 128, "fp32 head sizes");
+    extern __shared__ __attribute__((aligned(16))) float rows_lds[];
+    const int tid = threadIdx.x, lane = tid % WAVE, wave = __builtin_amdgcn_readfirstlane(tid / WAVE), l16 = lane % 16, g = lane / 16;
+    const int dv = a.D;
+    const int kvh = blockIdx.x % a.kv_heads;
+    int rest = blockIdx.x / a.kv_heads;
+
+    // ---- which rows and keys
+    int entry, row0, rows, begin = 0, end, n_keys, tokens, q_from = 0, part = 0, parts = 1, slot = 0;
+    KeyRun run;
+    if constexpr (MODE == ROWS_OWN) {
+        const int tiles = (a.new_tokens * a.each + ROWS - 1) / ROWS;
+        const int tile = rest % tiles;
+        const Part p = own_part(a, rest / tiles);
+        entry = __builtin_amdgcn_readfirstlane(p.entry);
+        if (entry < 0) return;
+        row0 = tile * ROWS;
+        tokens = a.new_tokens;
+        rows = tokens * a.each;
+        run = keys_of(a, entry);
+        begin = __builtin_amdgcn_readfirstlane(p.part * p.chunk);
+        end = __builtin_amdgcn_readfirstlane(min(run.n, begin + p.chunk));
+        part = p.part;
+        parts = p.parts;
+        slot = p.slot;
+    } else if constexpr (MODE == ROWS_PACKED) {
+        const TileItem item = tile_item<ROWS>(a, rest);
+        entry = __builtin_amdgcn_readfirstlane(item.entry);
+        if (entry < 0) return;
+        const TokenRun t = tokens_of(a, entry);
+        tokens = t.n;
+        q_from = t.from;
+        rows = tokens * a.each;
+        row0 = __builtin_amdgcn_readfirstlane(item.block) * ROWS;
+        if (row0 < 0 || row0 >= rows) return;
+        run = keys_of(a, entry);
+        const int last = min(row0 + ROWS, rows) - 1;
+        end = __builtin_amdgcn_readfirstlane(a.causal ? run.n - tokens + last / a.each + 1 : run.n);
+    } else {
+        part = rest % a.prefix_parts;
+        const GroupItem item = group_item<ROWS>(a, rest / a.prefix_parts);
+        entry = __builtin_amdgcn_readfirstlane(item.group);
+        if (entry < 0) return;
+        rows = item.rows;
+        row0 = item.row0;
+        q_from = item.first;
+        tokens = 0;
+        run = prefix_of(a, entry);
+        const int chunk = prefix_chunk(a, run.n);
+        begin = __builtin_amdgcn_readfirstlane(part * chunk);
+        end = __builtin_amdgcn_readfirstlane(min(run.n, begin + chunk));
+        if (begin >= run.n) return; // (as many parts as that are there for the join)
+    }
+    n_keys = __builtin_amdgcn_readfirstlane(run.n);
+
+    // ---- this lane's row
+    const int row = min(row0 + l16, rows - 1);
+    const bool row_ok = row0 + l16 < rows;
+    auto q_place = [&](int r) { // of the element strides
+        const int token = r / a.each, head = kvh * a.each + r % a.each;
+        struct { int64_t q, o; } at;
+        if constexpr (MODE == ROWS_PACKED) {
+            at.q = (q_from + token) * a.qs[1] + head * a.qs[2];
+            at.o = (q_from + token) * a.os[1] + head * a.os[2];
+        } else {
+            const int seq = MODE == ROWS_OWN ? entry : q_from + token / a.new_tokens, t = MODE == ROWS_OWN ? token : token % a.new_tokens;
+            at.q = seq * a.qs[0] + t * a.qs[1] + head * a.qs[2];
+            at.o = seq * a.os[0] + t * a.os[1] + head * a.os[2];
+        }
+        return at;
+    };
+    const int limit = MODE == ROWS_PREFIX || !a.causal ? end - 1 : min(end - 1, n_keys - tokens + row / a.each); // last key that this row sees
+    const int least = MODE == ROWS_PREFIX || !a.causal ? end - 1 : min(end - 1, n_keys - tokens + row0 / a.each); // .. that every row of the tile sees
+
+    uint4_t qf[KJ];
+    {
+        const unsigned char *q = static_cast<const unsigned char *>(a.q) + q_place(row).q * ES;
+#pragma unroll
+        for (int j = 0; j < KJ; ++j) {
+            const int d = F32 ? 16 * j + 4 * g : 32 * j + 8 * g;
+            qf[j] = row_ok && d < dv ? *reinterpret_cast<const uint4_t *>(q + d * ES) : uint4_t{0, 0, 0, 0};
+        }
+    }
+
+    // ---- K and V from memory.  Rows behind the last key are that key again; dims behind the head size of K are zeros, of V the last ones again.
+    const unsigned char *kb = static_cast<const unsigned char *>(a.k) + kvh * a.ks[2] * ES, *vb = static_cast<const unsigned char *>(a.v) + kvh * a.vs[2] * ES;
+    const int64_t k_page = a.ks[0] * ES, v_page = a.vs[0] * ES, k_row = a.ks[1] * ES, v_row = a.vs[1] * ES;
+    int k_dim[KJ], v_dim[VH]; // bytes into a row
+    bool k_in[KJ];
+#pragma unroll
+    for (int j = 0; j < KJ; ++j) {
+        const int d = F32 ? 16 * j + 4 * g : 32 * j + 8 * g;
+        k_in[j] = d < dv;
+        k_dim[j] = (PAD && d >= dv ? 0 : d) * ES;
+    }
+#pragma unroll
+    for (int h = 0; h < VH; ++h) {
+        const int d = F32 ? 64 * h + 4 * l16 : NT * l16 + 8 * h;
+        v_dim[h] = (PAD && d >= dv ? 0 : d) * ES;
+    }
+    struct Ids { int k[SUB], v[SUB]; };
+    const int mask = (1 << a.page_shift) - 1;
+    auto ids_at = [&](int at) __attribute__((always_inline)) {
+        Ids p;
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) {
+            p.k[u] = run.table ? run.table[min(at + 16 * u + l16, n_keys - 1) >> a.page_shift] : 0;
+            p.v[u] = run.table ? run.table[min(at + 16 * u + 4 * g, n_keys - 1) >> a.page_shift] : 0;
+        }
+        return p;
+    };
+    bool bad = false;
+    uint4_t kf[SUB][KJ];
+    uint32_t vf[SUB][4][F32 ? 4 * VH : NT / 2];
+    auto load = [&](int at, Ids p) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) {
+            const int key = min(at + 16 * u + l16, n_keys - 1), vkey = min(at + 16 * u + 4 * g, n_keys - 1);
+            const unsigned char *k = kb, *v = vb;
+            if (run.table) {
+                if (static_cast<uint32_t>(p.k[u]) >= static_cast<uint32_t>(a.n_pages) || static_cast<uint32_t>(p.v[u]) >= static_cast<uint32_t>(a.n_pages)) {
+                    bad = true;
+                    p.k[u] = p.v[u] = 0;
+                }
+                k += p.k[u] * k_page + (key & mask) * k_row;
+                v += p.v[u] * v_page + (vkey & mask) * v_row;
+            } else {
+                k += (run.base + key) * k_row;
+                v += (run.base + vkey) * v_row;
+            }
+#pragma unroll
+            for (int j = 0; j < KJ; ++j) {
+                kf[u][j] = *reinterpret_cast<const uint4_t *>(k + k_dim[j]);
+                if (PAD && !k_in[j]) kf[u][j] = uint4_t{0, 0, 0, 0};
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const unsigned char *vi = v + min(i, n_keys - 1 - vkey) * v_row;
+                if constexpr (!F32 && D == 64) {
+                    const uint2_t t = *reinterpret_cast<const uint2_t *>(vi + v_dim[0]);
+                    vf[u][i][0] = t.x;
+                    vf[u][i][1] = t.y;
+                } else {
+#pragma unroll
+                    for (int h = 0; h < VH; ++h) {
+                        const uint4_t t = *reinterpret_cast<const uint4_t *>(vi + v_dim[h]);
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) vf[u][i][4 * h + c] = t[c];
+                    }
+                }
+            }
+        }
+    };
+
+    constexpr int NACC = F32 ? 4 * VH : NT; // fp32: tile 4 h + c holds dims 64 h + 4 (4 g + i) + c; 16 bits: tile t dims (4 g + i) NT + t
+    rows_f32x4 oacc[NACC];
+#pragma unroll
+    for (int t = 0; t < NACC; ++t) oacc[t] = rows_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    float m_run = NEG_INF_F, l_run = 0.0f;
+    int at = begin + KEYS * wave;
+    Ids ids{};
+    if (at < end) {
+        load(at, ids_at(at));
+        if (at + STRIDE < end) ids = ids_at(at + STRIDE);
+    }
+    while (at < end) {
+        uint4_t kc[SUB][KJ];
+        uint32_t vc[SUB][4][F32 ? 4 * VH : NT / 2];
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) {
+#pragma unroll
+            for (int j = 0; j < KJ; ++j) kc[u][j] = kf[u][j];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int c = 0; c < (F32 ? 4 * VH : NT / 2); ++c) vc[u][i][c] = vf[u][i][c];
+        }
+        const int now = at;
+        at += STRIDE;
+        if (at < end) {
+            load(at, ids);
+            if (at + STRIDE < end) ids = ids_at(at + STRIDE);
+        }
+
+        rows_f32x4 s[SUB];
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) s[u] = rows_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < KJ; ++j)
+#pragma unroll
+            for (int u = 0; u < SUB; ++u) {
+                if constexpr (F32) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kc[u][j][c]), __uint_as_float(qf[j][c]), s[u], 0, 0, 0);
+                } else {
+                    s[u] = rows_mfma<DT>(kc[u][j], qf[j], s[u]);
+                }
+            }
+        if (now + KEYS - 1 > least) {
+#pragma unroll
+            for (int u = 0; u < SUB; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (now + 16 * u + 4 * g + i > limit) s[u][i] = NEG_INF_F;
+        }
+        float top = NEG_INF_F;
+#pragma unroll
+        for (int u = 0; u < SUB; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = fmaxf(top, s[u][i]);
+        top = across32(across16(top, lanes_max), lanes_max);
+        const float m_new = fmaxf(m_run, top * a.scale_log2e);
+        if (__builtin_amdgcn_ballot_w64(m_new - m_run > RESCALE_THRESHOLD) != 0) {
+            const float alpha = m_new == NEG_INF_F ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
+            m_run = m_new;
+            l_run *= alpha;
+#pragma unroll
+            for (int t = 0; t < NACC; ++t) oacc[t] *= alpha;
+        }
+        const float minus = m_run == NEG_INF_F ? 0.0f : -m_run;
+        float p[SUB][4];
+#pragma unroll
+        for (int u = 0; u < SUB; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                p[u][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], a.scale_log2e, minus));
+                l_run += p[u][i];
+            }
+        if constexpr (F32) {
+#pragma unroll
+            for (int u = 0; u < SUB; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int t = 0; t < NACC; ++t) oacc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vc[u][i][t]), p[u][i], oacc[t], 0, 0, 0);
+        } else {
+            uint4_t pf; // slot 8 g + e of the second product is key 4 g + e % 4 of sub-tile e / 4
+#pragma unroll
+            for (int e = 0; e < 4; ++e) pf[e] = pack2<DT == AXHIP_DTYPE_BF16>(p[e / 2][2 * (e % 2)], p[e / 2][2 * (e % 2) + 1]);
+#pragma unroll
+            for (int t = 0; t < NACC; ++t) {
+                uint4_t vt;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    vt[e] = __builtin_amdgcn_perm(vc[e / 2][2 * (e % 2) + 1][t / 2], vc[e / 2][2 * (e % 2)][t / 2], t % 2 ? 0x07060302u : 0x05040100u);
+                oacc[t] = rows_mfma<DT>(vt, pf, oacc[t]);
+            }
+        }
+    }
+
+    // ---- the four waves' states meet: [wave][row][D + 4], then maxima and denominators
+    const float l_tot = across32(across16(l_run, lanes_add), lanes_add);
+    float *const tops = rows_lds + ROWS_WAVES * ROWS * (D + 4), *const dens = tops + ROWS_WAVES * ROWS;
+    {
+        float *mine = rows_lds + (wave * ROWS + l16) * (D + 4);
+        if constexpr (F32) {
+#pragma unroll
+            for (int h = 0; h < VH; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    *reinterpret_cast<rows_f32x4 *>(mine + 64 * h + 16 * g + 4 * i) = rows_f32x4{oacc[4 * h][i], oacc[4 * h + 1][i], oacc[4 * h + 2][i], oacc[4 * h + 3][i]};
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int t = 0; t < NT; t += 4)
+                    *reinterpret_cast<rows_f32x4 *>(mine + (4 * g + i) * NT + t) = rows_f32x4{oacc[t][i], oacc[t + 1][i], oacc[t + 2][i], oacc[t + 3][i]};
+        }
+        if (g == 0) {
+            tops[wave * ROWS + l16] = m_run;
+            dens[wave * ROWS + l16] = l_tot;
+        }
+    }
+    const int any_bad = __syncthreads_or(bad);
+
+    // finished here, or left for the join: own parts by their place among all parts, prefix parts by row
+    bool leave = MODE == ROWS_PREFIX || parts > 1;
+    if constexpr (MODE == ROWS_OWN) {
+        if (a.groups > 0 && !leave) {
+            const int group = group_of(a, entry);
+            leave = group >= 0 && prefix_of(a, group).n > 0;
+        }
+        if (a.parts_of && part == 0 && kvh == 0 && row0 == 0 && tid == 0) a.parts_of[entry] = int2_t{slot, leave ? parts : 0};
+    }
+    for (int item = tid; item < ROWS * (D / 4); item += 64 * ROWS_WAVES) {
+        const int r = item / (D / 4), d = item % (D / 4) * 4;
+        if (row0 + r >= rows || d >= dv) continue;
+        float top = NEG_INF_F, den = 0.0f;
+        rows_f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < ROWS_WAVES; ++w) top = fmaxf(top, tops[w * ROWS + r]);
+        if (top != NEG_INF_F) {
+#pragma unroll
+            for (int w = 0; w < ROWS_WAVES; ++w) {
+                const float scale = __builtin_amdgcn_exp2f(tops[w * ROWS + r] - top);
+                o += scale * *reinterpret_cast<const rows_f32x4 *>(rows_lds + (w * ROWS + r) * (D + 4) + d);
+                den += scale * dens[w * ROWS + r];
+            }
+        } else { // no key of this row, or no number among its scores
+#pragma unroll
+            for (int w = 0; w < ROWS_WAVES; ++w) den += dens[w * ROWS + r];
+        }
+        if (any_bad) den = __builtin_nanf("");
+        o *= den == 0.0f ? 0.0f : 1.0f / den;
+        if (leave) {
+            int64_t place;
+            if constexpr (MODE == ROWS_PREFIX) {
+                const int64_t of = static_cast<int64_t>(q_from) * a.new_tokens * a.each + row0 + r; // sequence, token, head of the key head
+                const int64_t per = static_cast<int64_t>(a.new_tokens) * a.each;
+                place = ((of / per * a.kv_heads + kvh) * per + of % per) * a.prefix_parts + part;
+                *reinterpret_cast<rows_f32x4 *>(a.prefix_out + place * dv + d) = o;
+            } else {
+                place = (static_cast<int64_t>(slot + part) * a.kv_heads + kvh) * rows + row0 + r;
+                *reinterpret_cast<rows_f32x4 *>(a.own_out + place * dv + d) = o;
+            }
+            // (what is no number makes the joined row none: +inf minus itself)
+            if (d == 0) (MODE == ROWS_PREFIX ? a.prefix_lse : a.own_lse)[place] = den == 0.0f ? NEG_INF_F : den == den ? top + __builtin_amdgcn_logf(den) : -NEG_INF_F;
+        } else {
+            unsigned char *out = static_cast<unsigned char *>(a.o) + (q_place(row0 + r).o + d) * ES;
+            if constexpr (F32) *reinterpret_cast<rows_f32x4 *>(out) = o;
+            else *reinterpret_cast<uint2_t *>(out) = uint2_t{pack2<DT == AXHIP_DTYPE_BF16>(o[0], o[1]), pack2<DT == AXHIP_DTYPE_BF16>(o[2], o[3])};
+        }
+    }
+}
+
+// out = sum_s 2^(lse_s - max lse) O_s / sum_s 2^(lse_s - max lse) over a row's prefix parts and own parts, in that order.  A wave per row; D / 4 lanes a partial result.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void sdpa_join_kernel(const CacheArgs a) {
+    constexpr int LANES = D / 4, TAKE = WAVE / LANES, AHEAD = 4;
+    const int lane = threadIdx.x % WAVE, d = lane % LANES * 4, first = lane / LANES;
+    const int64_t id = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / WAVE; // sequence, token, head
+    const int per = a.new_tokens * a.heads;
+    if (id >= static_cast<int64_t>(a.entries) * per) return;
+    const int seq = static_cast<int>(id / per), token = static_cast<int>(id % per) / a.heads, head = static_cast<int>(id % per) % a.heads;
+    const int kvh = head / a.each, row = token * a.each + head % a.each, rows = a.new_tokens * a.each;
+    const int2_t own = a.parts_of[seq];
+    if (own.y == 0) return; // finished already
+    int prefix = 0;
+    if (a.groups > 0) {
+        const int group = group_of(a, seq);
+        if (group >= 0) {
+            const int n = prefix_of(a, group).n, chunk = prefix_chunk(a, n);
+            prefix = (n + chunk - 1) / chunk;
+        }
+    }
+    const int n = prefix + own.y;
+    const int64_t pre = ((static_cast<int64_t>(seq) * a.kv_heads + kvh) * rows + row) * a.prefix_parts;
+    auto place = [&](int i) { return i < prefix ? pre + i : (static_cast<int64_t>(own.x + i - prefix) * a.kv_heads + kvh) * rows + row; };
+    auto lse = [&](int i) { return (i < prefix ? a.prefix_lse : a.own_lse)[place(i)]; };
+    float top = NEG_INF_F;
+    for (int i = lane; i < n; i += WAVE) top = fmaxf(top, lse(i));
+    top = wave_max(top);
+    float den = 0.0f;
+    rows_f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i0 = first; i0 < n && top != NEG_INF_F; i0 += TAKE * AHEAD) {
+        rows_f32x4 o[AHEAD];
+        float w[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            const int i = min(i0 + TAKE * k, n - 1);
+            w[k] = i0 + TAKE * k < n ? lse(i) : NEG_INF_F;
+            o[k] = d < a.D ? *reinterpret_cast<const rows_f32x4 *>((i < prefix ? a.prefix_out : a.own_out) + place(i) * a.D + d) : rows_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            const float e = w[k] == NEG_INF_F ? 0.0f : __builtin_amdgcn_exp2f(w[k] - top);
+            den += e;
+            acc += e == 0.0f ? rows_f32x4{0.0f, 0.0f, 0.0f, 0.0f} : e * o[k];
+        }
+    }
+#pragma unroll
+    for (int o = LANES; o < WAVE; o *= 2) {
+        den += __shfl_xor(den, o, WAVE);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[c] += __shfl_xor(acc[c], o, WAVE);
+    }
+    if (first != 0 || d >= a.D) return;
+    acc *= den == 0.0f ? 0.0f : 1.0f / den;
+    const int64_t at = seq * a.os[0] + token * a.os[1] + head * a.os[2] + d;
+    if constexpr (DT == AXHIP_DTYPE_F32) *reinterpret_cast<rows_f32x4 *>(static_cast<float *>(a.o) + at) = acc;
+    else *reinterpret_cast<uint2_t *>(static_cast<uint16_t *>(a.o) + at) = uint2_t{pack2<DT == AXHIP_DTYPE_BF16>(acc[0], acc[1]), pack2<DT == AXHIP_DTYPE_BF16>(acc[2], acc[3])};
+}
+
+template <int DT, int D, bool PAD, int MODE> int launch_rows_as(const CacheArgs &a, int64_t blocks, hipStream_t s) {
+    constexpr int lds = rows_lds_bytes<D>();
+    if constexpr (lds > 65536) {
+        static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(&sdpa_rows_kernel<DT, D, PAD, MODE>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        AXHIP_CHECK_HIP(attr);
+    }
+    AXHIP_REQUIRE(launch_fits(blocks, 64 * ROWS_WAVES), AXHIP_ERR_UNSUPPORTED, "attention over pages: grid too large");
+    hipLaunchKernelGGL((sdpa_rows_kernel<DT, D, PAD, MODE>), dim3(static_cast<unsigned>(blocks)), dim3(64 * ROWS_WAVES), lds, s, a);
+    AXHIP_CHECK_HIP(hipGetLastError());
+    return AXHIP_OK;
+}
+template <int DT, int MODE> int launch_rows_mode(const CacheArgs &a, int64_t blocks, hipStream_t s) {
+    if (a.D == 64) return launch_rows_as<DT, 64, false, MODE>(a, blocks, s);
+    if (a.D == 128) return launch_rows_as<DT, 128, false, MODE>(a, blocks, s);
+    if (a.D < 64) return launch_rows_as<DT, 64, true, MODE>(a, blocks, s);
+    if (a.D < 128) return launch_rows_as<DT, 128, true, MODE>(a, blocks, s);
+    if constexpr (DT != AXHIP_DTYPE_F32) return launch_rows_as<DT, 256, true, MODE>(a, blocks, s);
+    return AXHIP_ERR_UNSUPPORTED;
+}
+// the parts of a decoding step's own keys
+template <int DT> int launch_rows_own(const CacheArgs &a, hipStream_t s) {
+    const int64_t tiles = (static_cast<int64_t>(a.new_tokens) * a.each + ROWS - 1) / ROWS;
+    return launch_rows_mode<DT, ROWS_OWN>(a, own_capacity(a) * tiles * a.kv_heads, s);
+}
+template <int DT> int launch_join(const CacheArgs &a, hipStream_t s) {
+    const int64_t blocks = (static_cast<int64_t>(a.entries) * a.new_tokens * a.heads + 3) / 4;
+    AXHIP_REQUIRE(launch_fits(blocks, 256), AXHIP_ERR_UNSUPPORTED, "axhip_sdpa_paged: grid too large");
+    if (a.D <= 64) hipLaunchKernelGGL((sdpa_join_kernel<DT, 64>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, a);
+    else if (a.D <= 128) hipLaunchKernelGGL((sdpa_join_kernel<DT, 128>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((sdpa_join_kernel<DT, 256>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, a);
+    AXHIP_CHECK_HIP(hipGetLastError());
+    return AXHIP_OK;
+}
+
+} // namespace axhip

@@ -14,13 +14,11 @@
 //  * scores are scaled in fp32, in the FMA that subtracts the maximum: q rounded after its scaling, which would save nothing here, adds as much error as the output's rounding does.
 #pragma once
 
-#include "sdpa_cache.hpp"
+#include "sdpa_tile_item.hpp"
 
 #include <type_traits>
 
 namespace axhip {
-
-constexpr int TK = 64; // keys of a tile
 
 typedef int tile_int4_t __attribute__((ext_vector_type(4)));
 typedef const __attribute__((address_space(4))) int32_t *scalar_ints; // read by scalar loads
@@ -47,88 +45,10 @@ __device__ __forceinline__ uint64_t uniform64(uint64_t v) {
     return (static_cast<uint64_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(v >> 32))) << 32) | static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(v)));
 }
 
-// Block `index` of all blocks of BM rows, those that walk the most tiles of keys first: a long sequence's last blocks, started last, would keep a few CUs busy
-// after all others are done.  Up to 256 entries: the number of blocks that walk c tiles or more is a sum over the entries, four to a lane, and c is searched for.
-// More: in the order of the entries.  index: uniform.  entry < 0: no such block.
-struct TileItem { int entry, block; };
-template <int BM> __device__ __forceinline__ TileItem tile_item(const CacheArgs &a, int index) {
-    const int lane = threadIdx.x % WAVE;
-    if (a.entries > 256) {
-        auto first = [&](int e) { return static_cast<int>(static_cast<int64_t>(clamped(a.cu_q[e], 0, a.total_q)) * a.each / BM + e); };
-        int lo = 0, hi = a.entries; // first(lo) <= index; first(hi) is beyond it
-        while (hi - lo > 1) { // 64 candidates at a time
-            const int step = (hi - lo + WAVE - 1) / WAVE, e = lo + lane * step;
-            const uint64_t below = __builtin_amdgcn_ballot_w64(e < hi && first(e) <= index);
-            const int n = below ? 64 - __builtin_clzll(below) : 1;
-            hi = min(hi, lo + n * step);
-            lo = lo + (n - 1) * step;
-        }
-        return {lo, index - first(lo)};
-    }
-    int blocks[4], past[4], last[4], tiles[4]; // of this lane's entries: blocks, keys in front of the first token, last token, tiles of keys
-    float most = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int e = lane + WAVE * i;
-        blocks[i] = past[i] = last[i] = tiles[i] = 0;
-        if (WAVE * i < a.entries && e < a.entries) {
-            const TokenRun t = tokens_of(a, e);
-            const int keys = keys_of(a, e).n;
-            blocks[i] = (t.n * a.each + BM - 1) / BM;
-            past[i] = keys - t.n;
-            last[i] = t.n - 1;
-            tiles[i] = (keys + TK - 1) / TK;
-            if (blocks[i] > 0) most = fmaxf(most, static_cast<float>(tiles[i]));
-        }
-    }
-    auto with = [&](int i, int c) { // blocks of entry i that walk c tiles or more
-        if (c <= 0) return blocks[i];
-        if (tiles[i] < c) return 0;
-        if (!a.causal) return blocks[i];
-        const int token = TK * (c - 1) - past[i]; // the first one that sees so far
-        if (token <= 0) return blocks[i];
-        return token > last[i] ? 0 : blocks[i] - token * a.each / BM;
-    };
-    auto all_with = [&](int c) {
-        float n = 0.0f; // (below 2^24: exact)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (WAVE * i < a.entries) n += static_cast<float>(with(i, c));
-        return static_cast<int>(wave_sum(n));
-    };
-    int lo = 0, hi = static_cast<int>(wave_max(most)) + 1; // all_with(lo) > index >= all_with(hi)
-    if (index >= all_with(0)) return {-1, 0};
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (all_with(mid) > index) lo = mid;
-        else hi = mid;
-    }
-    int left = index - all_with(lo + 1); // among those that walk `lo` tiles exactly
-    TileItem item{-1, 0};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (WAVE * i >= a.entries || item.entry >= 0) continue;
-        const int mine = with(i, lo) - with(i, lo + 1);
-        int upto = mine;
-#pragma unroll
-        for (int d = 1; d < WAVE; d *= 2) {
-            const int other = __shfl_up(upto, d, WAVE);
-            if (lane >= d) upto += other;
-        }
-        const uint64_t reached = __builtin_amdgcn_ballot_w64(upto > left);
-        if (reached) {
-            const int at = __builtin_ctzll(reached);
-            item.entry = at + WAVE * i;
-            item.block = __builtin_amdgcn_readlane(blocks[i] - with(i, lo) + left - (upto - mine), at);
-        } else {
-            left -= __builtin_amdgcn_readlane(upto, WAVE - 1);
-        }
-    }
-    return item;
-}
-
 // D: the LDS row in dims; DE: the dims that are computed; the head size in memory, a multiple of 8, may be less (zeros in its place)
-template <bool BF16, int D, int DE, int NW, bool PAGED>
+// PREFIX: the rows of a group of sequences against a part of their prefix (decoding): fp32 results and the base-2 logarithm of their denominators, for sdpa_join_kernel
+enum TileKeys { TILE_PACKED = 0, TILE_PAGED = 1, TILE_PREFIX = 2 };
+template <bool BF16, int D, int DE, int NW, int KEYS>
 __global__ __launch_bounds__(64 * NW, NW == 8 || D > 128 ? 1 : 2) void sdpa_tile_kernel(const CacheArgs a) {
     static_assert(DE % 32 == 0 && DE <= D, "dims");
     constexpr int PF = 3, RING = PF + 1; // LDS reads run this many MFMAs ahead
@@ -142,28 +62,53 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || D > 128 ? 1 : 2) void sdpa_tile
     const int ql = lane % 32, g = lane / 32;
     const bool second = NW == 8 && wave >= 4;
     const int kvh = blockIdx.x % a.kv_heads;
-    const TileItem item = tile_item<BM>(a, blockIdx.x / a.kv_heads);
-    const int entry = __builtin_amdgcn_readfirstlane(item.entry), block = __builtin_amdgcn_readfirstlane(item.block);
-    if (entry < 0) return;
-    const TokenRun tokens = tokens_of(a, entry);
-    const KeyRun run = keys_of(a, entry);
-    const int rows = __builtin_amdgcn_readfirstlane(tokens.n * a.each), nk = __builtin_amdgcn_readfirstlane(run.n);
-    const int row0 = block * BM;
-    if (block < 0 || row0 >= rows) return;
+    // entry, its rows from row0 on, its keys [begin, nk)
+    int entry, rows, row0, nk, begin = 0, part = 0, from;
+    KeyRun run;
+    if constexpr (KEYS == TILE_PREFIX) {
+        const int rest = blockIdx.x / a.kv_heads;
+        part = rest % a.prefix_parts;
+        const GroupItem item = group_item<BM>(a, rest / a.prefix_parts);
+        entry = __builtin_amdgcn_readfirstlane(item.group);
+        if (entry < 0) return;
+        rows = __builtin_amdgcn_readfirstlane(item.rows);
+        row0 = __builtin_amdgcn_readfirstlane(item.row0);
+        from = item.first;
+        run = prefix_of(a, entry);
+        const int chunk = prefix_chunk(a, run.n);
+        begin = __builtin_amdgcn_readfirstlane(part * chunk);
+        nk = __builtin_amdgcn_readfirstlane(min(run.n, begin + chunk));
+        if (begin >= nk) return; // (as many parts as that are there for the join)
+    } else {
+        const TileItem item = tile_item<BM>(a, blockIdx.x / a.kv_heads);
+        entry = __builtin_amdgcn_readfirstlane(item.entry);
+        const int block = __builtin_amdgcn_readfirstlane(item.block);
+        if (entry < 0) return;
+        const TokenRun t = tokens_of(a, entry);
+        run = keys_of(a, entry);
+        rows = __builtin_amdgcn_readfirstlane(t.n * a.each);
+        nk = __builtin_amdgcn_readfirstlane(run.n);
+        row0 = block * BM;
+        from = t.from;
+        if (block < 0 || row0 >= rows) return;
+    }
+    constexpr bool PAGED = KEYS != TILE_PACKED;
+    const bool causal = KEYS != TILE_PREFIX && a.causal;
     const int dv = a.D;
-    const int past = nk - tokens.n;
+    const int past = nk - rows / a.each; // keys in front of the first token
 
     // this lane's query, and the last key that it sees; rows behind the last one see what that one does and are not stored
     const int row = row0 + 32 * wave + ql;
     const bool row_ok = row < rows;
-    auto sees = [&](int r) { return a.causal ? past + min(r, rows - 1) / a.each : nk - 1; };
+    auto sees = [&](int r) { return causal ? past + min(r, rows - 1) / a.each : nk - 1; };
     const int token = min(row, rows - 1) / a.each, head = kvh * a.each + min(row, rows - 1) % a.each;
-    const int limit = a.causal ? past + token : nk - 1;
+    const int limit = causal ? past + token : nk - 1;
     const int wave_row = row0 + 32 * wave;
     const int least = __builtin_amdgcn_readfirstlane(sees(wave_row)), farthest = __builtin_amdgcn_readfirstlane(wave_row < rows ? sees(wave_row + 31) : -1);
-    const int ntiles = __builtin_amdgcn_readfirstlane((sees(row0 + BM - 1) + TK) / TK); // (sees -1: none)
-    const int64_t at_q = (tokens.from + token) * a.qs[1] + head * a.qs[2];
-    uint16_t *const orow = static_cast<uint16_t *>(a.o) + (tokens.from + token) * a.os[1] + head * a.os[2];
+    const int ntiles = __builtin_amdgcn_readfirstlane((sees(row0 + BM - 1) - begin + TK) / TK); // (sees -1: none)
+    int64_t at_q;
+    if constexpr (KEYS == TILE_PREFIX) at_q = (from + token / a.new_tokens) * a.qs[0] + token % a.new_tokens * a.qs[1] + head * a.qs[2];
+    else at_q = (from + token) * a.qs[1] + head * a.qs[2];
 
     uint4_t qf[KT];
     {
@@ -194,7 +139,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || D > 128 ? 1 : 2) void sdpa_tile
     const uint32_t lds_wave = __builtin_amdgcn_readfirstlane(lds_base + RPL * wave * ROWB);
     const int last_piece = __builtin_amdgcn_readfirstlane((nk - 1) / RPL * RPL);
     bool bad = false;
-    auto piece_of = [&](int tile, int n) { return min(tile * TK + RPL * NW * n + RPL * wave, last_piece); };
+    auto piece_of = [&](int tile, int n) { return min(begin + tile * TK + RPL * NW * n + RPL * wave, last_piece); };
     struct Pages { int id[NLOAD]; };
     auto pages_at = [&](int tile) { // the pages of this wave's pieces of a tile
         Pages p;
@@ -258,12 +203,12 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || D > 128 ? 1 : 2) void sdpa_tile
     auto larger = [](float x, float y) { return __builtin_elementwise_maximum(x, y); }; // (needs no canonical input; hands a NaN on)
 
     auto softmax_phase = [&](int j) __attribute__((always_inline)) {
-        if (j * TK + TK - 1 > least) {
+        if (begin + j * TK + TK - 1 > least) {
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    if (j * TK + kt * 32 + (i / 4) * 8 + g * 4 + i % 4 > limit) s[kt][i] = NEG_INF_F;
+                    if (begin + j * TK + kt * 32 + (i / 4) * 8 + g * 4 + i % 4 > limit) s[kt][i] = NEG_INF_F;
         }
         float m[4];
 #pragma unroll
@@ -343,7 +288,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || D > 128 ? 1 : 2) void sdpa_tile
             }
         }
         __builtin_amdgcn_s_waitcnt(0xC07F); // lgkmcnt(0): K buffer 0 is read
-        auto active = [&](int j) { return j * TK <= farthest; };
+        auto active = [&](int j) { return begin + j * TK <= farthest; };
         // one barrier a tile: behind it tile j + 1 of K and j of V have landed, and every wave is done with the buffers that K(j + 2) and V(j + 1) go to
         auto step = [&](int j, auto parity) __attribute__((always_inline)) {
             constexpr int PAR = decltype(parity)::value;
@@ -376,6 +321,22 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || D > 128 ? 1 : 2) void sdpa_tile
         if (any) l = __builtin_nanf("");
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    if constexpr (KEYS == TILE_PREFIX) {
+        if (!row_ok) return;
+        const int64_t per = static_cast<int64_t>(a.new_tokens) * a.each, of = from * per + row; // sequence, token, head of the key head
+        const int64_t place = ((of / per * a.kv_heads + kvh) * per + of % per) * a.prefix_parts + part;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const int d = dt * 32 + i * 2 + 4 * g;
+                if (d < dv) *reinterpret_cast<float4_t *>(a.prefix_out + place * dv + d) = float4_t{oacc[dt][i] * inv, oacc[dt][i + 1] * inv, oacc[dt][i + 2] * inv, oacc[dt][i + 3] * inv};
+            }
+        // (what is no number makes the joined row none: +inf minus itself)
+        if (g == 0) a.prefix_lse[place] = l == 0.0f ? NEG_INF_F : l == l ? m_run + __builtin_amdgcn_logf(l) : -NEG_INF_F;
+        return;
+    }
+    uint16_t *const orow = static_cast<uint16_t *>(a.o) + (from + token) * a.os[1] + head * a.os[2];
     // a lane holds 4 consecutive dims of each group of 8; the halves trade every second group: 16 bytes a store
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
@@ -391,25 +352,28 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || D > 128 ? 1 : 2) void sdpa_tile
         }
 }
 
-// Blocks of BM rows, at most; 0: more than a launch takes
-template <bool BF16, int D, int DE, int NW, bool PAGED> int launch_tile_as(const CacheArgs &a, hipStream_t s) {
-    constexpr int lds = 4 * TK * 2 * D;
+template <bool BF16, int D, int DE, int NW, int KEYS> int launch_tile_as(const CacheArgs &a, hipStream_t s) {
+    constexpr int lds = 4 * TK * 2 * D, BM = 32 * NW;
     if constexpr (lds > 65536) {
-        static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(&sdpa_tile_kernel<BF16, D, DE, NW, PAGED>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(&sdpa_tile_kernel<BF16, D, DE, NW, KEYS>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         AXHIP_CHECK_HIP(attr);
     }
-    const int64_t blocks = (a.total_q * a.each / (32 * NW) + a.entries) * a.kv_heads;
-    AXHIP_REQUIRE(launch_fits(blocks, 64 * NW), AXHIP_ERR_UNSUPPORTED, "axhip_sdpa_packed: grid too large");
-    hipLaunchKernelGGL((sdpa_tile_kernel<BF16, D, DE, NW, PAGED>), dim3(static_cast<unsigned>(blocks)), dim3(64 * NW), lds, s, a);
+    // blocks of BM rows, at most
+    int64_t blocks = a.kv_heads;
+    if (KEYS == TILE_PREFIX) blocks *= (static_cast<int64_t>(a.entries) * a.new_tokens * a.each / BM + a.groups) * a.prefix_parts;
+    else blocks *= a.total_q * a.each / BM + a.entries;
+    AXHIP_REQUIRE(launch_fits(blocks, 64 * NW), AXHIP_ERR_UNSUPPORTED, "attention of ragged sequences: grid too large");
+    hipLaunchKernelGGL((sdpa_tile_kernel<BF16, D, DE, NW, KEYS>), dim3(static_cast<unsigned>(blocks)), dim3(64 * NW), lds, s, a);
     AXHIP_CHECK_HIP(hipGetLastError());
     return AXHIP_OK;
 }
-template <bool BF16, bool PAGED> int launch_tile_paged(const CacheArgs &a, int waves, hipStream_t s) {
-    if (a.D > 128) return launch_tile_as<BF16, 256, 256, 4, PAGED>(a, s);
-    if (a.D > 96) return waves == 8 ? launch_tile_as<BF16, 128, 128, 8, PAGED>(a, s) : launch_tile_as<BF16, 128, 128, 4, PAGED>(a, s);
-    if (a.D > 64) return waves == 8 ? launch_tile_as<BF16, 128, 96, 8, PAGED>(a, s) : launch_tile_as<BF16, 128, 96, 4, PAGED>(a, s);
-    return waves == 8 ? launch_tile_as<BF16, 64, 64, 8, PAGED>(a, s) : launch_tile_as<BF16, 64, 64, 4, PAGED>(a, s);
+template <bool BF16, int KEYS> int launch_tile_keys(const CacheArgs &a, int waves, hipStream_t s) {
+    if (a.D > 128) return launch_tile_as<BF16, 256, 256, 4, KEYS>(a, s);
+    if (a.D > 96) return waves == 8 ? launch_tile_as<BF16, 128, 128, 8, KEYS>(a, s) : launch_tile_as<BF16, 128, 128, 4, KEYS>(a, s);
+    if (a.D > 64) return waves == 8 ? launch_tile_as<BF16, 128, 96, 8, KEYS>(a, s) : launch_tile_as<BF16, 128, 96, 4, KEYS>(a, s);
+    return waves == 8 ? launch_tile_as<BF16, 64, 64, 8, KEYS>(a, s) : launch_tile_as<BF16, 64, 64, 4, KEYS>(a, s);
 }
-template <bool BF16> int launch_tile(const CacheArgs &a, int waves, hipStream_t s) { return a.table ? launch_tile_paged<BF16, true>(a, waves, s) : launch_tile_paged<BF16, false>(a, waves, s); }
+template <bool BF16> int launch_tile(const CacheArgs &a, int waves, hipStream_t s) { return a.table ? launch_tile_keys<BF16, TILE_PAGED>(a, waves, s) : launch_tile_keys<BF16, TILE_PACKED>(a, waves, s); }
+template <bool BF16> int launch_prefix(const CacheArgs &a, hipStream_t s) { return launch_tile_keys<BF16, TILE_PREFIX>(a, 4, s); }
 
 } // namespace axhip

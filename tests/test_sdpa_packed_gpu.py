@@ -64,7 +64,7 @@ class Problem:
 def test_prompts(dt, lengths, heads, kv_heads, dim):
     p = Problem(LENGTHS[lengths], heads, kv_heads, dim, dt, seed=dim)
     o, kernel = p.run()
-    assert kernel
+    assert kernel != "generic"
     p.check(o)
 
 
@@ -76,7 +76,7 @@ def test_chunks_over_pages(dt, causal, heads, kv_heads, dim, page, by_head):
     lengths, keys = [1, 70, 130, 5, 0, 9, 64], [200, 70, 700, 3, 50, 0, 129]
     p = Problem(lengths, heads, kv_heads, dim, dt, keys, page, by_head, seed=page)
     o, kernel = p.run(causal)
-    assert kernel
+    assert kernel != "generic"
     p.check(o, causal)
 
 
@@ -86,7 +86,7 @@ def test_head_sizes(dt, dim):
     for page in (0, 16):
         p = Problem([40, 100, 3], 4, 2, dim, dt, page=page, seed=dim)
         o, kernel = p.run()
-        assert kernel
+        assert (kernel == "generic") == (dim % 8 != 0 if dt == "bf16" else dim > 128)
         p.check(o)
 
 
@@ -186,7 +186,7 @@ def test_keys_behind_four_gigabytes():
         x[-20:] = torch.randn(20, page, heads, dim, generator=ch.generator(i)).bfloat16().cuda()
     q = torch.randn(50, 4, dim, generator=ch.generator(9)).bfloat16().cuda()
     o, kernel = ch.packed(q, None, None, ints([0, 50]), "bf16", kp=kp, vp=vp, table=table.cuda(), lengths=ints([313]))
-    assert kernel
+    assert kernel != "generic"
     k, v = (x[-20:].cpu().double().flip(0).reshape(-1, heads, dim)[:313] for x in (kp, vp))
     want, around, big = ch.attention(q, k, v, 263)
     assert float(((o.cpu().double() - want).abs() - ch.attention_tolerance(want, around, big, 313, dim, "bf16")).max()) <= 0

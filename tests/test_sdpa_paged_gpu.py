@@ -54,7 +54,7 @@ class Step:
 def test_steps(dt, by_head, lengths, new, heads, kv_heads, dim, page):
     s = Step(lengths, new, heads, kv_heads, dim, page, dt, by_head)
     o, kernel = s.run()
-    assert kernel
+    assert kernel != "generic"
     s.check(o)
 
 
@@ -65,7 +65,7 @@ def test_steps(dt, by_head, lengths, new, heads, kv_heads, dim, page):
 def test_shared_prefixes(dt, lengths, new, heads, kv_heads, dim, page, starts, prefixes):
     s = Step(lengths, new, heads, kv_heads, dim, page, dt, starts=starts, prefixes=prefixes)
     o, kernel = s.run()
-    assert kernel
+    assert kernel != "generic"
     s.check(o)
 
 
