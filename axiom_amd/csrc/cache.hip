@@ -85,16 +85,6 @@ __global__ __launch_bounds__(256) void move_heads_kernel(const MoveArgs a) {
     // where the unit lies in a head: of halves, V dims and those rot / 2 behind; else V dims
     const int d0 = turns ? static_cast<int>(unit) * a.step : a.rot + (static_cast<int>(unit) - a.turning) * V;
     const bool two = !PAIRS && turns;
-    constexpr int ANGLES = PAIRS ? V / 2 : V;
-    CosSin t[ANGLES];
-    if (turns) {
-        const int64_t position = a.position_bytes == 8 ? static_cast<const int64_t *>(a.positions)[token] : static_cast<const int32_t *>(a.positions)[token];
-#pragma unroll
-        for (int i = 0; i < ANGLES; ++i) {
-            t[i] = turned(position, a.turns[static_cast<int>(unit) * ANGLES + i], a.amplitude);
-            t[i].s *= a.direction;
-        }
-    }
     int64_t page = -1, row = 0;
     if (a.slots) {
         const int64_t slot = a.slots[token];
@@ -106,28 +96,35 @@ __global__ __launch_bounds__(256) void move_heads_kernel(const MoveArgs a) {
     const int all = a.heads + 2 * a.kv_heads;
     Pack<DT, V> x[PER], y[PER];
     E *to[PER];
-    // (every load of the thread is on its way before the first is waited for)
+    // (every load of the thread is on its way before the angles are formed; a thread's head behind the last one is the last one again, and not stored)
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        const int head = static_cast<int>(group + i * a.groups.d);
-        to[i] = nullptr;
-        const E *from = nullptr;
+        const int wanted = static_cast<int>(group + i * a.groups.d), head = min(wanted, all - 1);
+        const E *from;
         if (head < a.heads) {
             from = static_cast<const E *>(a.q) + token * a.qs[0] + head * a.qs[1];
             to[i] = static_cast<E *>(a.q_out) + token * a.os[0] + head * a.os[1];
-        } else if (head < all && page >= 0) {
-            const int h = head - a.heads;
-            if (h < a.kv_heads) {
-                from = static_cast<const E *>(a.k) + token * a.ks[0] + h * a.ks[1];
-                to[i] = static_cast<E *>(a.k_pages) + page * a.kp[0] + row * a.kp[1] + h * a.kp[2];
-            } else {
-                from = static_cast<const E *>(a.v) + token * a.vs[0] + (h - a.kv_heads) * a.vs[1];
-                to[i] = static_cast<E *>(a.v_pages) + page * a.vp[0] + row * a.vp[1] + (h - a.kv_heads) * a.vp[2];
-            }
+        } else {
+            int h = head - a.heads;
+            const bool is_k = h < a.kv_heads;
+            if (!is_k) h -= a.kv_heads;
+            from = is_k ? static_cast<const E *>(a.k) + token * a.ks[0] + h * a.ks[1] : static_cast<const E *>(a.v) + token * a.vs[0] + h * a.vs[1];
+            to[i] = is_k ? static_cast<E *>(a.k_pages) + page * a.kp[0] + row * a.kp[1] + h * a.kp[2] : static_cast<E *>(a.v_pages) + page * a.vp[0] + row * a.vp[1] + h * a.vp[2];
+            if (page < 0) to[i] = nullptr;
         }
-        if (from) {
-            x[i] = *reinterpret_cast<const Pack<DT, V> *>(from + d0);
-            if (two) y[i] = *reinterpret_cast<const Pack<DT, V> *>(from + d0 + a.apart);
+        if (wanted >= all) to[i] = nullptr;
+        x[i] = *reinterpret_cast<const Pack<DT, V> *>(from + d0);
+        if (two) y[i] = *reinterpret_cast<const Pack<DT, V> *>(from + d0 + a.apart);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    constexpr int ANGLES = PAIRS ? V / 2 : V;
+    CosSin t[ANGLES];
+    if (turns) {
+        const int64_t position = a.position_bytes == 8 ? static_cast<const int64_t *>(a.positions)[token] : static_cast<const int32_t *>(a.positions)[token];
+#pragma unroll
+        for (int i = 0; i < ANGLES; ++i) {
+            t[i] = turned(position, a.turns[static_cast<int>(unit) * ANGLES + i], a.amplitude);
+            t[i].s *= a.direction;
         }
     }
 #pragma unroll
@@ -180,19 +177,25 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(const CopyArgs a) {
     const unsigned char *from = base + src * a.page_bytes[which];
     unsigned char *to = base + dst * a.page_bytes[which];
     Piece p[COPY_DEEP];
+    const uint32_t v0 = slice * (COPY_DEEP * 256u) + threadIdx.x;
+    if (DENSE && rows == a.page_size && (slice + 1) * (COPY_DEEP * 256u) <= a.vectors) { // nothing to leave out
+#pragma unroll
+        for (int i = 0; i < COPY_DEEP; ++i) p[i] = *reinterpret_cast<const Piece *>(from + static_cast<int64_t>(v0 + i * 256u) * V);
+#pragma unroll
+        for (int i = 0; i < COPY_DEEP; ++i) *reinterpret_cast<Piece *>(to + static_cast<int64_t>(v0 + i * 256u) * V) = p[i];
+        return;
+    }
     int64_t at[COPY_DEEP];
 #pragma unroll
     for (int i = 0; i < COPY_DEEP; ++i) {
-        const uint32_t v = (slice * COPY_DEEP + i) * 256u + threadIdx.x;
+        const uint32_t v = v0 + i * 256u;
         at[i] = -1;
         if (v >= a.vectors) continue;
-        int row;
         if constexpr (DENSE) {
-            row = static_cast<int>(a.row_div.of(v) & static_cast<uint32_t>(a.page_size - 1));
-            if (row < rows) at[i] = static_cast<int64_t>(v) * V;
+            if (static_cast<int>(a.row_div.of(v) & static_cast<uint32_t>(a.page_size - 1)) < rows) at[i] = static_cast<int64_t>(v) * V;
         } else { // piece of a head, head, row
             const uint32_t line = a.dim_div.of(v), r = a.head_div.of(line);
-            row = static_cast<int>(r);
+            const int row = static_cast<int>(r);
             if (row < rows) at[i] = row * a.row_bytes[which] + static_cast<int64_t>(line - r * a.head_div.d) * a.head_bytes[which] + static_cast<int64_t>(v - line * a.dim_div.d) * V;
         }
         if (at[i] >= 0) p[i] = *reinterpret_cast<const Piece *>(from + at[i]);

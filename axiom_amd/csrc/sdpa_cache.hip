@@ -288,21 +288,25 @@ const int tile_waves = [] {
 
 // How a decoding step is divided, and its temporary memory: what the parts leave for the join.  Nothing of it depends on addresses.
 struct StepPlan {
-    int want, prefix;
+    int shares, prefix;
     size_t own_out, own_lse, prefix_out, prefix_lse, bytes; // places; all of it (0: nothing can have two parts)
 };
+// AXHIP_SDPA_STEP_GROUPS: work-groups of a step's own keys (measurements only)
+const int step_groups = [] {
+    const char *e = getenv("AXHIP_SDPA_STEP_GROUPS");
+    return e ? atoi(e) : 512;
+}();
 StepPlan step_plan(const CacheArgs &a) {
     StepPlan p{};
     const int64_t rows = static_cast<int64_t>(a.new_tokens) * a.each, tiles = (rows + 15) / 16, most = std::min(a.table_ld << a.page_shift, MOST_KEYS);
-    // parts of the own keys: four work-groups of four waves for each CU
-    p.want = static_cast<int>(std::max<int64_t>(1, 1024 / (a.kv_heads * tiles)));
+    const int64_t units = (most + 127) / 128 * a.entries; // at most
+    // shares of the own keys: two work-groups of four waves on each CU
+    p.shares = static_cast<int>(std::min<int64_t>(std::max<int64_t>(1, step_groups / (a.kv_heads * tiles)), units));
     if (a.groups == 0 && most <= 128) return p;
     // parts of a prefix: one work-group of 128 rows for each CU
     const int64_t blocks = (a.entries * rows + 127) / 128 * a.kv_heads;
     p.prefix = a.groups == 0 ? 0 : static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({64, 256 / blocks, (std::min(a.prefix_ld << a.page_shift, MOST_KEYS) + 63) / 64})));
-    CacheArgs with = a;
-    with.want_parts = p.want;
-    const size_t own = static_cast<size_t>(own_capacity(with)) * a.kv_heads * rows, pre = static_cast<size_t>(a.entries) * a.kv_heads * rows * p.prefix;
+    const size_t own = (static_cast<size_t>(2 * p.shares) + (a.groups > 0 ? a.entries : 0)) * a.kv_heads * rows, pre = static_cast<size_t>(a.entries) * a.kv_heads * rows * p.prefix;
     size_t at = CallScratch::rounded(sizeof(int2_t) * a.entries);
     auto place = [&](size_t floats) { const size_t here = at; at = CallScratch::rounded(at + floats * sizeof(float)); return here; };
     p.own_out = place(own * a.D);
@@ -380,9 +384,10 @@ int axhip_sdpa_paged_ws(const void *q, void *o, const AxhipSdpaPagedParams *para
     rc = ensure_init();
     if (rc) return rc;
     hipStream_t s = resolve_stream(stream);
-    if (!for_matrix_cores(a)) return launch_generic(a, s, "axhip_sdpa_paged");
+    // (units of 128 keys are counted in 32 bits)
+    if (!for_matrix_cores(a) || (std::min(a.table_ld << a.page_shift, MOST_KEYS) / 128 + 1) * a.entries >= (int64_t(1) << 31)) return launch_generic(a, s, "axhip_sdpa_paged");
     const StepPlan plan = step_plan(a);
-    a.want_parts = plan.want;
+    a.shares = plan.shares;
     a.prefix_parts = plan.prefix;
     CallScratch scratch(workspace, workspace_bytes, s);
     if (plan.bytes > 0) {
@@ -398,12 +403,13 @@ int axhip_sdpa_paged_ws(const void *q, void *o, const AxhipSdpaPagedParams *para
     }
     last_kernel = "rows";
     const bool f32 = a.dtype == AXHIP_DTYPE_F32, bf16 = a.dtype == AXHIP_DTYPE_BF16;
-    if (a.groups > 0) {
-        last_kernel = "rows, prefix";
-        rc = f32 ? launch_prefix_f32(a, s) : bf16 ? launch_prefix_bf16(a, s) : launch_prefix_f16(a, s);
+    if (a.groups > 0) last_kernel = "rows, prefix";
+    if (a.groups > 0 && f32) {
+        rc = launch_prefix_f32(a, s);
         if (rc) return rc;
     }
-    rc = f32 ? launch_rows_own_f32(a, s) : bf16 ? launch_rows_own_bf16(a, s) : launch_rows_own_f16(a, s);
+    if (a.groups > 0 && !f32) rc = bf16 ? launch_step_bf16(a, s) : launch_step_f16(a, s);
+    else rc = f32 ? launch_rows_own_f32(a, s) : bf16 ? launch_rows_own_bf16(a, s) : launch_rows_own_f16(a, s);
     if (rc) return rc;
     if (plan.bytes > 0) {
         rc = f32 ? launch_join_f32(a, s) : bf16 ? launch_join_bf16(a, s) : launch_join_f16(a, s);

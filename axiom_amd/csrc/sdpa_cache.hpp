@@ -29,14 +29,14 @@ struct CacheArgs {
     int groups;
     const int32_t *group_starts, *prefix_table, *prefix_lengths;
     int64_t prefix_ld;
-    // decoding in parts: how many of the own keys are wanted, how many a prefix has at most; what they leave for the join, by part, key head and row, or by
-    // sequence, key head, row and part; for each sequence where its parts begin and how many there are to join (0: it is finished)
-    int want_parts, prefix_parts;
+    // decoding in parts: the shares that the own keys are dealt out in, the parts that a prefix has at most; what they leave for the join, by slot (two to a share, then one to a sequence), key head and row, or by
+    // sequence, key head, row and part; for each sequence the first of its slots and how many there are to join (0: it is finished)
+    int shares, prefix_parts;
     float *own_out, *own_lse, *prefix_out, *prefix_lse;
     int2_t *parts_of;
 };
-// Parts of the own keys there can be: see own_part
-inline int64_t own_capacity(const CacheArgs &a) { return static_cast<int64_t>(a.want_parts) + a.entries + 2; }
+// Work-groups of a step's own keys
+inline int64_t own_blocks(const CacheArgs &a) { return (static_cast<int64_t>(a.new_tokens) * a.each + 15) / 16 * a.kv_heads * a.shares; }
 
 constexpr int64_t MOST_KEYS = int64_t(1) << 30; // of a sequence
 
@@ -79,9 +79,9 @@ __device__ __forceinline__ int group_of(const CacheArgs &a, int s) {
 // The matrix-core kernels (16 bits) of rows found by cu_q: sdpa_tile.hpp; 4 or 8 waves of 32 rows
 int launch_tile_bf16(const CacheArgs &a, int waves, hipStream_t s);
 int launch_tile_f16(const CacheArgs &a, int waves, hipStream_t s);
-// .. of a group's rows against the parts of its prefix
-int launch_prefix_bf16(const CacheArgs &a, hipStream_t s);
-int launch_prefix_f16(const CacheArgs &a, hipStream_t s);
+// A decoding step with prefixes: sdpa_step.hpp; of fp32 the prefixes alone
+int launch_step_bf16(const CacheArgs &a, hipStream_t s);
+int launch_step_f16(const CacheArgs &a, hipStream_t s);
 int launch_prefix_f32(const CacheArgs &a, hipStream_t s);
 // Few rows and fp32: sdpa_rows.hpp
 int launch_rows_own_bf16(const CacheArgs &a, hipStream_t s);

@@ -7,8 +7,9 @@
 //                  whose transpose is byte permutes between its registers, in fp32 the elements as they come.
 // Bound by one read of K and V (decoding): a step's 16 loads are requested a step ahead, the page numbers they need a step earlier.
 //
-// A decoding step divides all its own keys into parts of one size, found from the lengths on the device, so that the chip is filled whatever they are: Parts below.  A sequence of
-// one part and no prefix is finished here; the others leave fp32 results and the base-2 logarithm of their denominators for sdpa_join_kernel.
+// A decoding step deals all its own keys out to its work-groups in equal shares, found from the lengths on the device, so that every CU has as much to do whatever they are: own_share
+// below.  A share may be a part of one sequence or several whole ones.  A sequence within one share and without a prefix is finished there; the others leave fp32 results and the
+// base-2 logarithm of their denominators for sdpa_join_kernel.
 #pragma once
 
 #include "sdpa_cache.hpp"
@@ -27,57 +28,82 @@ template <int DT> __device__ __forceinline__ rows_f32x4 rows_mfma(uint4_t a, uin
 constexpr int ROWS_WAVES = 4, ROWS = 16;
 template <int D> constexpr int rows_lds_bytes() { return ROWS_WAVES * ROWS * (D + 4 + 2) * 4; }
 
-// Which keys of which sequence: part `part` of `parts`, of `chunk` keys each, at place `slot` among all parts
-struct Part { int entry, part, parts, chunk, slot; };
-// Part `index` of a decoding step's own keys, by all 256 threads of a work-group.  Lengths count in units of UNIT keys; with a sum of U units a part is ceil(U / want) units, at least
-// one, which makes want + entries parts at most (every sequence has one, an empty one too); two more for the rounding of the sum, which is one of floats.
+// Keys are dealt out in units of UNIT; a sequence has one at least, so that somebody writes its rows.  With U units in all and W <= U shares, share i begins at unit i U / W, and unit u
+// lies in share ((u + 1) W - 1) / U.  What a share leaves of a sequence that others have parts of goes to slot 2 i where the sequence began at the share's first unit or in front of it, else
+// (it is the share's last one then) to slot 2 i + 1; of a whole sequence s that has a prefix, to slot 2 W + s.
 constexpr int UNIT = 128;
-__device__ inline Part own_part(const CacheArgs &a, int index) {
-    __shared__ float sums[ROWS_WAVES];
-    __shared__ int totals[ROWS_WAVES];
-    __shared__ Part found;
-    const int tid = threadIdx.x, lane = tid % WAVE, wave = tid / WAVE;
-    const int n = a.entries, per = (n + 255) / 256, from = min(tid * per, n), to = min(from + per, n);
-    auto units = [&](int e) { return (keys_of(a, e).n + UNIT - 1) / UNIT; };
-    float u = 0.0f;
-    for (int e = from; e < to; ++e) u += static_cast<float>(units(e));
-    u = wave_sum(u);
-    if (lane == 0) sums[wave] = u;
-    if (tid == 0) found.entry = -1;
-    __syncthreads();
-    u = (sums[0] + sums[1]) + (sums[2] + sums[3]);
-    const int size = max(1, static_cast<int>(fminf(ceilf(u / static_cast<float>(a.want_parts)), 8388608.0f)));
-    int mine = 0;
-    for (int e = from; e < to; ++e) mine += max(1, (units(e) + size - 1) / size);
-    int upto = mine;
+__device__ __forceinline__ int units_of(int keys) { return max(1, (keys + UNIT - 1) / UNIT); }
+struct Share { int units, shares, from, to, entry, entry_at; }; // of all; how many shares; this one's units; the sequence that the first one lies in, and its first unit
+// By a wavefront; up to 256 sequences four to a lane, more in runs, one to a lane.
+__device__ inline Share own_share(const CacheArgs &a, int index) {
+    const int lane = threadIdx.x % WAVE, n = a.entries;
+    auto scan = [&](int v) {
 #pragma unroll
-    for (int d = 1; d < WAVE; d *= 2) {
-        const int other = __shfl_up(upto, d, WAVE);
-        if (lane >= d) upto += other;
+        for (int d = 1; d < WAVE; d *= 2) {
+            const int other = __shfl_up(v, d, WAVE);
+            if (lane >= d) v += other;
+        }
+        return v;
+    };
+    const bool few = n <= 4 * WAVE;
+    const int run = (n + WAVE - 1) / WAVE, run_from = min(lane * run, n), run_to = min(run_from + run, n);
+    int u[4] = {0, 0, 0, 0}, upto[4], total = 0;
+    if (few) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (WAVE * i < n && lane + WAVE * i < n) u[i] = units_of(keys_of(a, lane + WAVE * i).n);
+    } else {
+        for (int e = run_from; e < run_to; ++e) u[0] += units_of(keys_of(a, e).n);
     }
-    if (lane == WAVE - 1) totals[wave] = upto;
-    __syncthreads();
-    for (int w = 0; w < wave; ++w) upto += totals[w];
-    int at = upto - mine;
-    if (index >= at && index < upto) {
-        for (int e = from; e < to; ++e) {
-            const int parts = max(1, (units(e) + size - 1) / size);
-            if (index < at + parts) {
-                found = Part{e, index - at, parts, size * UNIT, at};
-                break;
-            }
-            at += parts;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        upto[i] = 0;
+        if (i > 0 && (!few || WAVE * i >= n)) continue;
+        upto[i] = total + scan(u[i]);
+        total = __builtin_amdgcn_readlane(upto[i], WAVE - 1);
+    }
+    Share s;
+    s.units = total;
+    s.shares = min(a.shares, total); // (none is empty)
+    s.from = s.to = s.entry = s.entry_at = 0;
+    if (index >= s.shares) return s;
+    s.from = static_cast<int>(static_cast<int64_t>(index) * total / s.shares);
+    s.to = static_cast<int>(static_cast<int64_t>(index + 1) * total / s.shares);
+    bool found = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (found || (i > 0 && (!few || WAVE * i >= n))) continue;
+        const uint64_t beyond = __builtin_amdgcn_ballot_w64(upto[i] > s.from);
+        if (beyond) {
+            const int at = __builtin_ctzll(beyond);
+            s.entry = at + WAVE * i;
+            s.entry_at = __builtin_amdgcn_readlane(upto[i] - u[i], at);
+            found = true;
         }
     }
-    __syncthreads();
-    return found;
+    if (!few) { // within that lane's run
+        int e = s.entry * run;
+        for (; e < n - 1; ++e) {
+            const int more = units_of(keys_of(a, e).n);
+            if (s.entry_at + more > s.from) break;
+            s.entry_at += more;
+        }
+        s.entry = e;
+    }
+    return s;
 }
 
 // What a work-group does: OWN, a part of a sequence's own keys (decoding); PACKED, whole sequences by cu_q (fp32 prompts); PREFIX, a part of a group's prefix for 16 of its rows (fp32)
 enum RowsMode { ROWS_OWN = 0, ROWS_PACKED = 1, ROWS_PREFIX = 2 };
 
-template <int DT, int D, bool PAD, int MODE>
-__global__ __launch_bounds__(64 * ROWS_WAVES, D > 128 ? 1 : 2) void sdpa_rows_kernel(const CacheArgs a) {
+// 16 rows, from row0 on of `rows`, against the keys [begin, end) of a run.  slot < 0: finished here; else where the results go for the join.
+struct Segment {
+    KeyRun run;
+    int entry, row0, rows, begin, end, tokens, q_from; // tokens: of the entry, the last of which sees the last key; q_from: its first token, or a group's first sequence
+    int64_t slot;                                      // own parts: their place; prefix: the part's number
+};
+
+template <int DT, int D, bool PAD, int MODE> __device__ __forceinline__ void rows_segment(const CacheArgs &a, int kvh, const Segment &seg) {
     constexpr bool F32 = DT == AXHIP_DTYPE_F32;
     constexpr int ES = F32 ? 4 : 2;
     constexpr int SUB = F32 && D > 64 ? 1 : 2, KEYS = 16 * SUB, STRIDE = KEYS * ROWS_WAVES;
@@ -85,59 +111,13 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, D > 128 ? 1 : 2) void sdpa_rows_ke
     constexpr int NT = D / 16;                // 16 bits: output tiles, and elements of V that a lane holds of a key
     constexpr int VH = F32 ? D / 64 : (NT * 2 + 15) / 16; // 16-byte pieces of a V row that a lane holds (D = 64 in 16 bits: half of one)
     static_assert(!F32 || D <= 128, "fp32 head sizes");
-    extern __shared__ __attribute__((aligned(16))) float rows_lds[];
+    extern __shared__ __attribute__((aligned(1024))) unsigned char tile_lds[];
+    float *const rows_lds = reinterpret_cast<float *>(tile_lds);
     const int tid = threadIdx.x, lane = tid % WAVE, wave = __builtin_amdgcn_readfirstlane(tid / WAVE), l16 = lane % 16, g = lane / 16;
     const int dv = a.D;
-    const int kvh = blockIdx.x % a.kv_heads;
-    int rest = blockIdx.x / a.kv_heads;
-
-    // ---- which rows and keys
-    int entry, row0, rows, begin = 0, end, n_keys, tokens, q_from = 0, part = 0, parts = 1, slot = 0;
-    KeyRun run;
-    if constexpr (MODE == ROWS_OWN) {
-        const int tiles = (a.new_tokens * a.each + ROWS - 1) / ROWS;
-        const int tile = rest % tiles;
-        const Part p = own_part(a, rest / tiles);
-        entry = __builtin_amdgcn_readfirstlane(p.entry);
-        if (entry < 0) return;
-        row0 = tile * ROWS;
-        tokens = a.new_tokens;
-        rows = tokens * a.each;
-        run = keys_of(a, entry);
-        begin = __builtin_amdgcn_readfirstlane(p.part * p.chunk);
-        end = __builtin_amdgcn_readfirstlane(min(run.n, begin + p.chunk));
-        part = p.part;
-        parts = p.parts;
-        slot = p.slot;
-    } else if constexpr (MODE == ROWS_PACKED) {
-        const TileItem item = tile_item<ROWS>(a, rest);
-        entry = __builtin_amdgcn_readfirstlane(item.entry);
-        if (entry < 0) return;
-        const TokenRun t = tokens_of(a, entry);
-        tokens = t.n;
-        q_from = t.from;
-        rows = tokens * a.each;
-        row0 = __builtin_amdgcn_readfirstlane(item.block) * ROWS;
-        if (row0 < 0 || row0 >= rows) return;
-        run = keys_of(a, entry);
-        const int last = min(row0 + ROWS, rows) - 1;
-        end = __builtin_amdgcn_readfirstlane(a.causal ? run.n - tokens + last / a.each + 1 : run.n);
-    } else {
-        part = rest % a.prefix_parts;
-        const GroupItem item = group_item<ROWS>(a, rest / a.prefix_parts);
-        entry = __builtin_amdgcn_readfirstlane(item.group);
-        if (entry < 0) return;
-        rows = item.rows;
-        row0 = item.row0;
-        q_from = item.first;
-        tokens = 0;
-        run = prefix_of(a, entry);
-        const int chunk = prefix_chunk(a, run.n);
-        begin = __builtin_amdgcn_readfirstlane(part * chunk);
-        end = __builtin_amdgcn_readfirstlane(min(run.n, begin + chunk));
-        if (begin >= run.n) return; // (as many parts as that are there for the join)
-    }
-    n_keys = __builtin_amdgcn_readfirstlane(run.n);
+    const KeyRun run = seg.run;
+    const int entry = seg.entry, row0 = seg.row0, rows = seg.rows, begin = seg.begin, end = seg.end, tokens = seg.tokens, q_from = seg.q_from;
+    const int n_keys = __builtin_amdgcn_readfirstlane(run.n);
 
     // ---- this lane's row
     const int row = min(row0 + l16, rows - 1);
@@ -359,15 +339,7 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, D > 128 ? 1 : 2) void sdpa_rows_ke
     }
     const int any_bad = __syncthreads_or(bad);
 
-    // finished here, or left for the join: own parts by their place among all parts, prefix parts by row
-    bool leave = MODE == ROWS_PREFIX || parts > 1;
-    if constexpr (MODE == ROWS_OWN) {
-        if (a.groups > 0 && !leave) {
-            const int group = group_of(a, entry);
-            leave = group >= 0 && prefix_of(a, group).n > 0;
-        }
-        if (a.parts_of && part == 0 && kvh == 0 && row0 == 0 && tid == 0) a.parts_of[entry] = int2_t{slot, leave ? parts : 0};
-    }
+    const bool leave = seg.slot >= 0;
     for (int item = tid; item < ROWS * (D / 4); item += 64 * ROWS_WAVES) {
         const int r = item / (D / 4), d = item % (D / 4) * 4;
         if (row0 + r >= rows || d >= dv) continue;
@@ -393,10 +365,10 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, D > 128 ? 1 : 2) void sdpa_rows_ke
             if constexpr (MODE == ROWS_PREFIX) {
                 const int64_t of = static_cast<int64_t>(q_from) * a.new_tokens * a.each + row0 + r; // sequence, token, head of the key head
                 const int64_t per = static_cast<int64_t>(a.new_tokens) * a.each;
-                place = ((of / per * a.kv_heads + kvh) * per + of % per) * a.prefix_parts + part;
+                place = ((of / per * a.kv_heads + kvh) * per + of % per) * a.prefix_parts + seg.slot;
                 *reinterpret_cast<rows_f32x4 *>(a.prefix_out + place * dv + d) = o;
             } else {
-                place = (static_cast<int64_t>(slot + part) * a.kv_heads + kvh) * rows + row0 + r;
+                place = (seg.slot * a.kv_heads + kvh) * rows + row0 + r;
                 *reinterpret_cast<rows_f32x4 *>(a.own_out + place * dv + d) = o;
             }
             // (what is no number makes the joined row none: +inf minus itself)
@@ -409,14 +381,83 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, D > 128 ? 1 : 2) void sdpa_rows_ke
     }
 }
 
-// out = sum_s 2^(lse_s - max lse) O_s / sum_s 2^(lse_s - max lse) over a row's prefix parts and own parts, in that order.  A wave per row; D / 4 lanes a partial result.
-template <int DT, int D>
+template <int DT, int D, bool PAD, int MODE> __device__ __forceinline__ void rows_body(const CacheArgs &a, int index_of_all) {
+    const int kvh = index_of_all % a.kv_heads, rest = index_of_all / a.kv_heads;
+    Segment seg{};
+    seg.slot = -1;
+    if constexpr (MODE == ROWS_OWN) {
+        seg.tokens = a.new_tokens;
+        seg.rows = a.new_tokens * a.each;
+        const int tiles = (seg.rows + ROWS - 1) / ROWS, share = rest / tiles;
+        seg.row0 = rest % tiles * ROWS;
+        const Share s = own_share(a, share);
+        int entry = __builtin_amdgcn_readfirstlane(s.entry), entry_at = __builtin_amdgcn_readfirstlane(s.entry_at);
+        const int from = __builtin_amdgcn_readfirstlane(s.from), to = __builtin_amdgcn_readfirstlane(s.to);
+        for (int at = from; at < to; ++entry) {
+            seg.run = keys_of(a, entry);
+            seg.entry = entry;
+            const int n = __builtin_amdgcn_readfirstlane(seg.run.n), entry_to = entry_at + units_of(n);
+            seg.begin = (at - entry_at) * UNIT;
+            seg.end = min(n, (min(to, entry_to) - entry_at) * UNIT);
+            const bool whole = entry_at >= from && entry_to <= to;
+            seg.slot = 2 * share + (entry_at <= from ? 0 : 1);
+            if (whole) {
+                const int group = a.groups > 0 ? group_of(a, entry) : -1;
+                seg.slot = group >= 0 && prefix_of(a, group).n > 0 ? 2 * a.shares + entry : -1;
+            }
+            if (a.parts_of && entry_at >= from && kvh == 0 && seg.row0 == 0 && threadIdx.x == 0) {
+                const int last = static_cast<int>((static_cast<int64_t>(entry_to) * s.shares - 1) / s.units);
+                a.parts_of[entry] = int2_t{static_cast<int>(seg.slot), seg.slot < 0 ? 0 : last - share + 1};
+            }
+            rows_segment<DT, D, PAD, MODE>(a, kvh, seg);
+            at = entry_at = entry_to;
+            if (at < to) __syncthreads(); // (the states in LDS are read)
+        }
+    } else if constexpr (MODE == ROWS_PACKED) {
+        const TileItem item = tile_item<ROWS>(a, rest);
+        seg.entry = __builtin_amdgcn_readfirstlane(item.entry);
+        if (seg.entry < 0) return;
+        const TokenRun t = tokens_of(a, seg.entry);
+        seg.tokens = t.n;
+        seg.q_from = t.from;
+        seg.rows = t.n * a.each;
+        seg.row0 = __builtin_amdgcn_readfirstlane(item.block) * ROWS;
+        if (seg.row0 < 0 || seg.row0 >= seg.rows) return;
+        seg.run = keys_of(a, seg.entry);
+        seg.end = __builtin_amdgcn_readfirstlane(a.causal ? seg.run.n - t.n + (min(seg.row0 + ROWS, seg.rows) - 1) / a.each + 1 : seg.run.n);
+        rows_segment<DT, D, PAD, MODE>(a, kvh, seg);
+    } else {
+        const int part = rest % a.prefix_parts;
+        const GroupItem item = group_item<ROWS>(a, rest / a.prefix_parts);
+        seg.entry = __builtin_amdgcn_readfirstlane(item.group);
+        if (seg.entry < 0) return;
+        seg.rows = item.rows;
+        seg.row0 = item.row0;
+        seg.q_from = item.first;
+        seg.run = prefix_of(a, seg.entry);
+        const int chunk = prefix_chunk(a, seg.run.n);
+        seg.begin = __builtin_amdgcn_readfirstlane(part * chunk);
+        seg.end = __builtin_amdgcn_readfirstlane(min(seg.run.n, seg.begin + chunk));
+        if (seg.begin >= seg.run.n) return; // (as many parts as that are there for the join)
+        seg.slot = part;
+        rows_segment<DT, D, PAD, MODE>(a, kvh, seg);
+    }
+}
+template <int DT, int D, bool PAD, int MODE>
+__global__ __launch_bounds__(64 * ROWS_WAVES, D > 128 ? 1 : 2) void sdpa_rows_kernel(const CacheArgs a) {
+    rows_body<DT, D, PAD, MODE>(a, blockIdx.x);
+}
+
+// out = sum_s 2^(lse_s - max lse) O_s / sum_s 2^(lse_s - max lse) over a row's prefix parts and own parts, in that order.  WAVES wavefronts to a row take them in turn, D / 4 lanes a
+// result, and everything that fits the first trip to memory is requested before the weights are known.
+template <int DT, int D, int WAVES>
 __global__ __launch_bounds__(256) void sdpa_join_kernel(const CacheArgs a) {
-    constexpr int LANES = D / 4, TAKE = WAVE / LANES, AHEAD = 4;
-    const int lane = threadIdx.x % WAVE, d = lane % LANES * 4, first = lane / LANES;
-    const int64_t id = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / WAVE; // sequence, token, head
+    constexpr int LANES = D / 4, TAKE = WAVE / LANES * WAVES, AHEAD = 8;
+    __shared__ __attribute__((aligned(16))) float sums[4][D + 4];
+    const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE, d = lane % LANES * 4, first = wave % WAVES * (WAVE / LANES) + lane / LANES;
+    const int64_t id = static_cast<int64_t>(blockIdx.x) * (4 / WAVES) + wave / WAVES; // sequence, token, head
     const int per = a.new_tokens * a.heads;
-    if (id >= static_cast<int64_t>(a.entries) * per) return;
+    if (id >= static_cast<int64_t>(a.entries) * per) return; // (whole work-groups with WAVES = 4)
     const int seq = static_cast<int>(id / per), token = static_cast<int>(id % per) / a.heads, head = static_cast<int>(id % per) % a.heads;
     const int kvh = head / a.each, row = token * a.each + head % a.each, rows = a.new_tokens * a.each;
     const int2_t own = a.parts_of[seq];
@@ -431,36 +472,59 @@ __global__ __launch_bounds__(256) void sdpa_join_kernel(const CacheArgs a) {
     }
     const int n = prefix + own.y;
     const int64_t pre = ((static_cast<int64_t>(seq) * a.kv_heads + kvh) * rows + row) * a.prefix_parts;
-    auto place = [&](int i) { return i < prefix ? pre + i : (static_cast<int64_t>(own.x + i - prefix) * a.kv_heads + kvh) * rows + row; };
+    // (own parts: the first share's slot, then the first slots of the shares behind it)
+    auto place = [&](int i) { return i < prefix ? pre + i : (static_cast<int64_t>(i == prefix ? own.x : own.x / 2 * 2 + 2 * (i - prefix)) * a.kv_heads + kvh) * rows + row; };
     auto lse = [&](int i) { return (i < prefix ? a.prefix_lse : a.own_lse)[place(i)]; };
-    float top = NEG_INF_F;
-    for (int i = lane; i < n; i += WAVE) top = fmaxf(top, lse(i));
-    top = wave_max(top);
-    float den = 0.0f;
-    rows_f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int i0 = first; i0 < n && top != NEG_INF_F; i0 += TAKE * AHEAD) {
-        rows_f32x4 o[AHEAD];
-        float w[AHEAD];
+    rows_f32x4 o[AHEAD];
+    float w[AHEAD];
+    auto fetch = [&](int i0) __attribute__((always_inline)) {
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k) {
             const int i = min(i0 + TAKE * k, n - 1);
             w[k] = i0 + TAKE * k < n ? lse(i) : NEG_INF_F;
-            o[k] = d < a.D ? *reinterpret_cast<const rows_f32x4 *>((i < prefix ? a.prefix_out : a.own_out) + place(i) * a.D + d) : rows_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            o[k] = *reinterpret_cast<const rows_f32x4 *>((i < prefix ? a.prefix_out : a.own_out) + place(i) * a.D + (d < a.D ? d : 0));
         }
+    };
+    float top = NEG_INF_F;
+    for (int i = lane; i < n; i += WAVE) top = fmaxf(top, lse(i));
+    fetch(first);
+    __builtin_amdgcn_sched_barrier(0);
+    top = wave_max(top);
+    float den = 0.0f;
+    rows_f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (top != NEG_INF_F) {
+        for (int i0 = first;;) {
 #pragma unroll
-        for (int k = 0; k < AHEAD; ++k) {
-            const float e = w[k] == NEG_INF_F ? 0.0f : __builtin_amdgcn_exp2f(w[k] - top);
-            den += e;
-            acc += e == 0.0f ? rows_f32x4{0.0f, 0.0f, 0.0f, 0.0f} : e * o[k];
+            for (int k = 0; k < AHEAD; ++k) {
+                const float e = w[k] == NEG_INF_F ? 0.0f : __builtin_amdgcn_exp2f(w[k] - top);
+                den += e;
+                acc += e == 0.0f ? rows_f32x4{0.0f, 0.0f, 0.0f, 0.0f} : e * o[k];
+            }
+            i0 += TAKE * AHEAD;
+            if (i0 >= n) break;
+            fetch(i0);
         }
     }
 #pragma unroll
-    for (int o = LANES; o < WAVE; o *= 2) {
-        den += __shfl_xor(den, o, WAVE);
+    for (int x = LANES; x < WAVE; x *= 2) {
+        den += __shfl_xor(den, x, WAVE);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) acc[c] += __shfl_xor(acc[c], o, WAVE);
+        for (int c = 0; c < 4; ++c) acc[c] += __shfl_xor(acc[c], x, WAVE);
     }
-    if (first != 0 || d >= a.D) return;
+    if constexpr (WAVES == 4) {
+        if (lane < LANES) *reinterpret_cast<rows_f32x4 *>(&sums[wave][d]) = acc;
+        if (lane == 0) sums[wave][D] = den;
+        __syncthreads();
+        if (wave != 0) return;
+        acc = *reinterpret_cast<const rows_f32x4 *>(&sums[0][d]);
+        den = sums[0][D];
+#pragma unroll
+        for (int i = 1; i < 4; ++i) {
+            acc += *reinterpret_cast<const rows_f32x4 *>(&sums[i][d]);
+            den += sums[i][D];
+        }
+    }
+    if (lane >= LANES || d >= a.D) return;
     acc *= den == 0.0f ? 0.0f : 1.0f / den;
     const int64_t at = seq * a.os[0] + token * a.os[1] + head * a.os[2] + d;
     if constexpr (DT == AXHIP_DTYPE_F32) *reinterpret_cast<rows_f32x4 *>(static_cast<float *>(a.o) + at) = acc;
@@ -486,17 +550,19 @@ template <int DT, int MODE> int launch_rows_mode(const CacheArgs &a, int64_t blo
     if constexpr (DT != AXHIP_DTYPE_F32) return launch_rows_as<DT, 256, true, MODE>(a, blocks, s);
     return AXHIP_ERR_UNSUPPORTED;
 }
-// the parts of a decoding step's own keys
-template <int DT> int launch_rows_own(const CacheArgs &a, hipStream_t s) {
-    const int64_t tiles = (static_cast<int64_t>(a.new_tokens) * a.each + ROWS - 1) / ROWS;
-    return launch_rows_mode<DT, ROWS_OWN>(a, own_capacity(a) * tiles * a.kv_heads, s);
+// the shares of a decoding step's own keys
+template <int DT> int launch_rows_own(const CacheArgs &a, hipStream_t s) { return launch_rows_mode<DT, ROWS_OWN>(a, own_blocks(a), s); }
+template <int DT, int D> void launch_join_as(const CacheArgs &a, int64_t rows, hipStream_t s) {
+    // a work-group to a row where those are few (up to 128 results in the first trip), else a wavefront
+    if (rows <= 1024) hipLaunchKernelGGL((sdpa_join_kernel<DT, D, 4>), dim3(static_cast<unsigned>(rows)), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((sdpa_join_kernel<DT, D, 1>), dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), 0, s, a);
 }
 template <int DT> int launch_join(const CacheArgs &a, hipStream_t s) {
-    const int64_t blocks = (static_cast<int64_t>(a.entries) * a.new_tokens * a.heads + 3) / 4;
-    AXHIP_REQUIRE(launch_fits(blocks, 256), AXHIP_ERR_UNSUPPORTED, "axhip_sdpa_paged: grid too large");
-    if (a.D <= 64) hipLaunchKernelGGL((sdpa_join_kernel<DT, 64>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, a);
-    else if (a.D <= 128) hipLaunchKernelGGL((sdpa_join_kernel<DT, 128>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((sdpa_join_kernel<DT, 256>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, a);
+    const int64_t rows = static_cast<int64_t>(a.entries) * a.new_tokens * a.heads;
+    AXHIP_REQUIRE(launch_fits((rows + 3) / 4, 256), AXHIP_ERR_UNSUPPORTED, "axhip_sdpa_paged: grid too large");
+    if (a.D <= 64) launch_join_as<DT, 64>(a, rows, s);
+    else if (a.D <= 128) launch_join_as<DT, 128>(a, rows, s);
+    else launch_join_as<DT, 256>(a, rows, s);
     AXHIP_CHECK_HIP(hipGetLastError());
     return AXHIP_OK;
 }

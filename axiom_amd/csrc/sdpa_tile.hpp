@@ -49,7 +49,7 @@ __device__ __forceinline__ uint64_t uniform64(uint64_t v) {
 // PREFIX: the rows of a group of sequences against a part of their prefix (decoding): fp32 results and the base-2 logarithm of their denominators, for sdpa_join_kernel
 enum TileKeys { TILE_PACKED = 0, TILE_PAGED = 1, TILE_PREFIX = 2 };
 template <bool BF16, int D, int DE, int NW, int KEYS>
-__global__ __launch_bounds__(64 * NW, NW == 8 || D > 128 ? 1 : 2) void sdpa_tile_kernel(const CacheArgs a) {
+__device__ __forceinline__ void tile_body(const CacheArgs &a, int index_of_all) {
     static_assert(DE % 32 == 0 && DE <= D, "dims");
     constexpr int PF = 3, RING = PF + 1; // LDS reads run this many MFMAs ahead
     constexpr int KT = DE / 16, DT = DE / 32, BM = 32 * NW, ROWB = 2 * D, CHUNKS = ROWB / 16, RPL = WAVE / CHUNKS;
@@ -61,12 +61,12 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || D > 128 ? 1 : 2) void sdpa_tile
     const int tid = threadIdx.x, lane = tid % WAVE, wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
     const int ql = lane % 32, g = lane / 32;
     const bool second = NW == 8 && wave >= 4;
-    const int kvh = blockIdx.x % a.kv_heads;
+    const int kvh = index_of_all % a.kv_heads;
     // entry, its rows from row0 on, its keys [begin, nk)
     int entry, rows, row0, nk, begin = 0, part = 0, from;
     KeyRun run;
     if constexpr (KEYS == TILE_PREFIX) {
-        const int rest = blockIdx.x / a.kv_heads;
+        const int rest = index_of_all / a.kv_heads;
         part = rest % a.prefix_parts;
         const GroupItem item = group_item<BM>(a, rest / a.prefix_parts);
         entry = __builtin_amdgcn_readfirstlane(item.group);
@@ -80,7 +80,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || D > 128 ? 1 : 2) void sdpa_tile
         nk = __builtin_amdgcn_readfirstlane(min(run.n, begin + chunk));
         if (begin >= nk) return; // (as many parts as that are there for the join)
     } else {
-        const TileItem item = tile_item<BM>(a, blockIdx.x / a.kv_heads);
+        const TileItem item = tile_item<BM>(a, index_of_all / a.kv_heads);
         entry = __builtin_amdgcn_readfirstlane(item.entry);
         const int block = __builtin_amdgcn_readfirstlane(item.block);
         if (entry < 0) return;
@@ -352,16 +352,18 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || D > 128 ? 1 : 2) void sdpa_tile
         }
 }
 
+template <bool BF16, int D, int DE, int NW, int KEYS>
+__global__ __launch_bounds__(64 * NW, NW == 8 || D > 128 ? 1 : 2) void sdpa_tile_kernel(const CacheArgs a) {
+    tile_body<BF16, D, DE, NW, KEYS>(a, blockIdx.x);
+}
+
 template <bool BF16, int D, int DE, int NW, int KEYS> int launch_tile_as(const CacheArgs &a, hipStream_t s) {
     constexpr int lds = 4 * TK * 2 * D, BM = 32 * NW;
     if constexpr (lds > 65536) {
         static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(&sdpa_tile_kernel<BF16, D, DE, NW, KEYS>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         AXHIP_CHECK_HIP(attr);
     }
-    // blocks of BM rows, at most
-    int64_t blocks = a.kv_heads;
-    if (KEYS == TILE_PREFIX) blocks *= (static_cast<int64_t>(a.entries) * a.new_tokens * a.each / BM + a.groups) * a.prefix_parts;
-    else blocks *= a.total_q * a.each / BM + a.entries;
+    const int64_t blocks = (a.total_q * a.each / BM + a.entries) * a.kv_heads; // at most
     AXHIP_REQUIRE(launch_fits(blocks, 64 * NW), AXHIP_ERR_UNSUPPORTED, "attention of ragged sequences: grid too large");
     hipLaunchKernelGGL((sdpa_tile_kernel<BF16, D, DE, NW, KEYS>), dim3(static_cast<unsigned>(blocks)), dim3(64 * NW), lds, s, a);
     AXHIP_CHECK_HIP(hipGetLastError());
@@ -374,6 +376,5 @@ template <bool BF16, int KEYS> int launch_tile_keys(const CacheArgs &a, int wave
     return waves == 8 ? launch_tile_as<BF16, 64, 64, 8, KEYS>(a, s) : launch_tile_as<BF16, 64, 64, 4, KEYS>(a, s);
 }
 template <bool BF16> int launch_tile(const CacheArgs &a, int waves, hipStream_t s) { return a.table ? launch_tile_keys<BF16, TILE_PAGED>(a, waves, s) : launch_tile_keys<BF16, TILE_PACKED>(a, waves, s); }
-template <bool BF16> int launch_prefix(const CacheArgs &a, hipStream_t s) { return launch_tile_keys<BF16, TILE_PREFIX>(a, 4, s); }
 
 } // namespace axhip

@@ -1,5 +1,4 @@
 #include "sdpa_tile.hpp"
 namespace axhip {
 int launch_tile_bf16(const CacheArgs &a, int waves, hipStream_t s) { return launch_tile<true>(a, waves, s); }
-int launch_prefix_bf16(const CacheArgs &a, hipStream_t s) { return launch_prefix<true>(a, s); }
 } // namespace axhip

@@ -1,5 +1,4 @@
 #include "sdpa_tile.hpp"
 namespace axhip {
 int launch_tile_f16(const CacheArgs &a, int waves, hipStream_t s) { return launch_tile<false>(a, waves, s); }
-int launch_prefix_f16(const CacheArgs &a, hipStream_t s) { return launch_prefix<false>(a, s); }
 } // namespace axhip
