@@ -58,6 +58,13 @@ template <int DT, int V> __device__ __forceinline__ void put(Pack<DT, V> &p, int
     else p.w[i] = static_cast<uint16_t>(pack_bf16x2(v, v));
 }
 
+// STREAM: past the caches.  Outputs of 64 MiB and more (STREAMING_OUTPUT_BYTES) are gone from them before anyone reads them, and stores that take a line in there first cost a third of the
+// rate: 8192 tokens of 48 heads of 128, 100 MB each way, 51.2 -> 35.2 us; 300 pages of 32 KiB in 8 layers, 157 MB each way, 85 -> 62.
+template <bool STREAM, class T> __device__ __forceinline__ void put_down(void *to, const T &v) {
+    if constexpr (STREAM && sizeof(T) == 16) __builtin_nontemporal_store(__builtin_bit_cast(uint4_t, v), static_cast<uint4_t *>(to));
+    else *static_cast<T *>(to) = v;
+}
+
 // Heads of a token in this order: those of q, of k, of v.  A unit is V elements of a head, whole pairs with PAIRS, else two such groups
 // `apart` (rot / 2 dims; 1 where pairs lie side by side but are not aligned to two elements); a thread takes one unit of `per` heads of a token, so that an angle's sine is formed once for all of them.
 struct MoveArgs {
@@ -74,7 +81,7 @@ struct MoveArgs {
     float amplitude, direction;
 };
 
-template <int DT, int V, bool PAIRS, int PER>
+template <int DT, int V, bool PAIRS, int PER, bool STREAM>
 __global__ __launch_bounds__(256) void move_heads_kernel(const MoveArgs a) {
     using E = typename Elem<DT>::type;
     const uint32_t id = blockIdx.x * 256u + threadIdx.x;
@@ -147,8 +154,8 @@ __global__ __launch_bounds__(256) void move_heads_kernel(const MoveArgs a) {
                 }
             }
         }
-        *reinterpret_cast<Pack<DT, V> *>(to[i] + d0) = x[i];
-        if (two) *reinterpret_cast<Pack<DT, V> *>(to[i] + d0 + a.apart) = y[i];
+        put_down<STREAM>(to[i] + d0, x[i]);
+        if (two) put_down<STREAM>(to[i] + d0 + a.apart, y[i]);
     }
 }
 
@@ -165,7 +172,7 @@ struct CopyArgs {
 };
 constexpr int COPY_DEEP = 8; // pieces of a thread, all requested before the first is stored
 
-template <int V, bool DENSE>
+template <int V, bool DENSE, bool STREAM>
 __global__ __launch_bounds__(256) void copy_pages_kernel(const CopyArgs a) {
     struct alignas(V) Piece { unsigned char b[V]; };
     const uint32_t rest = a.slices.of(blockIdx.x), slice = blockIdx.x - rest * a.slices.d;
@@ -180,9 +187,13 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(const CopyArgs a) {
     const uint32_t v0 = slice * (COPY_DEEP * 256u) + threadIdx.x;
     if (DENSE && rows == a.page_size && (slice + 1) * (COPY_DEEP * 256u) <= a.vectors) { // nothing to leave out
 #pragma unroll
-        for (int i = 0; i < COPY_DEEP; ++i) p[i] = *reinterpret_cast<const Piece *>(from + static_cast<int64_t>(v0 + i * 256u) * V);
+        for (int i = 0; i < COPY_DEEP; ++i) {
+            const unsigned char *at = from + static_cast<int64_t>(v0 + i * 256u) * V;
+            if constexpr (STREAM && V == 16) p[i] = __builtin_bit_cast(Piece, __builtin_nontemporal_load(reinterpret_cast<const uint4_t *>(at)));
+            else p[i] = *reinterpret_cast<const Piece *>(at);
+        }
 #pragma unroll
-        for (int i = 0; i < COPY_DEEP; ++i) *reinterpret_cast<Piece *>(to + static_cast<int64_t>(v0 + i * 256u) * V) = p[i];
+        for (int i = 0; i < COPY_DEEP; ++i) put_down<STREAM>(to + static_cast<int64_t>(v0 + i * 256u) * V, p[i]);
         return;
     }
     int64_t at[COPY_DEEP];
@@ -202,7 +213,7 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(const CopyArgs a) {
     }
 #pragma unroll
     for (int i = 0; i < COPY_DEEP; ++i)
-        if (at[i] >= 0) *reinterpret_cast<Piece *>(to + at[i]) = p[i];
+        if (at[i] >= 0) put_down<STREAM>(to + at[i], p[i]);
 }
 
 // ------------------------------------------------------------------ host side
@@ -217,22 +228,27 @@ int launch_moves(MoveArgs &a, int dtype, bool pairs, int dim, int64_t tokens, in
     a.apart = loose ? 1 : a.rot / 2;
     const int units = a.turning + (dim - a.rot) / v;
     const int all = a.heads + 2 * a.kv_heads;
-    // Heads of a thread: four share an angle's sines and 64 or 128 bytes are requested at once; one where that would leave the chip's 1024 SIMDs
-    // without two wavefronts each.  (8192 tokens of 48 heads of 128: 41.7 us with four, 50.8 with one.)
-    const bool four = all >= 4 && tokens * all * units >= int64_t(4) * 2 * 64 * 1024;
-    const int per = four ? 4 : 1, groups = (all + per - 1) / per;
+    // Heads of a thread: two share an angle's sines, one where that would leave the chip's 1024 SIMDs without two wavefronts each.  (8192 tokens of 48 heads of 128: two 35.2 us, four 36.4;
+    // stores through the caches: one 48.7, two 48.2, four 51.2, eight 52.1.)
+    const bool many = all >= 2 && tokens * all * units >= int64_t(2) * 2 * 64 * 1024;
+    const bool stream = many && tokens * all * dim * static_cast<int64_t>(dtype_size(dtype)) >= STREAMING_OUTPUT_BYTES;
+    const int per = many ? 2 : 1, groups = (all + per - 1) / per;
     const int64_t total = tokens * groups * units;
     AXHIP_REQUIRE(total < (int64_t(1) << 31), AXHIP_ERR_UNSUPPORTED, "%s: %lld tokens of %d heads are too many for one launch", who, static_cast<long long>(tokens), all);
     a.units = Divisor(static_cast<uint32_t>(units));
     a.groups = Divisor(static_cast<uint32_t>(groups));
     a.total = static_cast<uint32_t>(total);
     const dim3 grid(static_cast<unsigned>((total + 255) / 256)), block(256);
-#define AXHIP_MOVE(DT, V)                                                                                        \
-    do {                                                                                                         \
-        if (pairs && four) hipLaunchKernelGGL((move_heads_kernel<DT, (V) < 2 ? 2 : (V), true, 4>), grid, block, 0, s, a); \
-        else if (pairs) hipLaunchKernelGGL((move_heads_kernel<DT, (V) < 2 ? 2 : (V), true, 1>), grid, block, 0, s, a);    \
-        else if (four) hipLaunchKernelGGL((move_heads_kernel<DT, V, false, 4>), grid, block, 0, s, a);           \
-        else hipLaunchKernelGGL((move_heads_kernel<DT, V, false, 1>), grid, block, 0, s, a);                     \
+#define AXHIP_MOVE_AS(DT, V, PAIRS)                                                                                             \
+    do {                                                                                                                        \
+        if (stream) hipLaunchKernelGGL((move_heads_kernel<DT, V, PAIRS, 2, true>), grid, block, 0, s, a);                       \
+        else if (many) hipLaunchKernelGGL((move_heads_kernel<DT, V, PAIRS, 2, false>), grid, block, 0, s, a);                   \
+        else hipLaunchKernelGGL((move_heads_kernel<DT, V, PAIRS, 1, false>), grid, block, 0, s, a);                             \
+    } while (0)
+#define AXHIP_MOVE(DT, V)                                      \
+    do {                                                       \
+        if (pairs) AXHIP_MOVE_AS(DT, ((V) < 2 ? 2 : (V)), true); \
+        else AXHIP_MOVE_AS(DT, V, false);                      \
     } while (0)
 #define AXHIP_MOVE16(DT)                   \
     do {                                   \
@@ -248,6 +264,7 @@ int launch_moves(MoveArgs &a, int dtype, bool pairs, int dim, int64_t tokens, in
     else AXHIP_MOVE(AXHIP_DTYPE_F32, 1);
 #undef AXHIP_MOVE16
 #undef AXHIP_MOVE
+#undef AXHIP_MOVE_AS
     AXHIP_CHECK_HIP(hipGetLastError());
     return AXHIP_OK;
 }
@@ -461,10 +478,12 @@ int axhip_kv_copy_pages(const AxhipKvCopyParams *params, void *stream) {
     const bool dense = row_major || head_major;
     const dim3 grid(static_cast<unsigned>(blocks)), block(256);
     hipStream_t s = resolve_stream(stream);
-#define AXHIP_COPY(V)                                                                                \
-    do {                                                                                             \
-        if (dense) hipLaunchKernelGGL((copy_pages_kernel<V, true>), grid, block, 0, s, a);           \
-        else hipLaunchKernelGGL((copy_pages_kernel<V, false>), grid, block, 0, s, a);                \
+    const bool past_caches = vectors * v * p.layers * 2 * p.pairs >= STREAMING_OUTPUT_BYTES;
+#define AXHIP_COPY(V)                                                                                              \
+    do {                                                                                                           \
+        if (dense && past_caches) hipLaunchKernelGGL((copy_pages_kernel<V, true, true>), grid, block, 0, s, a);         \
+        else if (dense) hipLaunchKernelGGL((copy_pages_kernel<V, true, false>), grid, block, 0, s, a);             \
+        else hipLaunchKernelGGL((copy_pages_kernel<V, false, false>), grid, block, 0, s, a);                       \
     } while (0)
     if (v == 16) AXHIP_COPY(16);
     else if (v == 8) AXHIP_COPY(8);
