@@ -270,15 +270,20 @@ int paged_args(CacheArgs &a, const AxhipSdpaPagedParams *params) {
     }
     return AXHIP_OK;
 }
-// Whether rows can be moved 16 bytes at a time and the matrix-core kernels take the head size.
-bool for_matrix_cores(const CacheArgs &a) {
+// Whether the matrix-core kernels take the head size and the numbers of rows
+bool form_for_matrix_cores(const CacheArgs &a) {
     const int es = static_cast<int>(dtype_size(a.dtype)), v = 16 / es;
     if (a.D % v != 0 || a.D > (es == 2 ? 256 : 128) || (a.table && a.page_shift < 3)) return false;
+    // (numbers of rows with one more block for each entry are 32-bit ones; numbers of blocks are added up as floats, exactly below 2^24)
+    const int64_t rows = (a.new_tokens ? static_cast<int64_t>(a.entries) * a.new_tokens : a.total_q) * a.each;
+    return rows + int64_t(256) * a.entries < (int64_t(1) << (es == 4 ? 27 : 30));
+}
+// .. and rows can be moved 16 bytes at a time (and offsets inside a piece of 8 rows are 32-bit ones)
+bool for_matrix_cores(const CacheArgs &a) {
+    const int es = static_cast<int>(dtype_size(a.dtype));
     uint64_t seen = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) | reinterpret_cast<uintptr_t>(a.o);
     for (int i = 0; i < 3; ++i) seen |= static_cast<uint64_t>(a.qs[i] | a.ks[i] | a.vs[i] | a.os[i]) * es;
-    // (offsets inside a piece of 8 rows, and numbers of rows with one more block for each entry, are 32-bit ones; numbers of blocks are added up as floats, exactly below 2^24)
-    const int64_t rows = (a.new_tokens ? static_cast<int64_t>(a.entries) * a.new_tokens : a.total_q) * a.each;
-    return (seen & 15) == 0 && a.ks[1] < (1 << 26) && a.vs[1] < (1 << 26) && rows + int64_t(256) * a.entries < (int64_t(1) << (es == 4 ? 27 : 30));
+    return form_for_matrix_cores(a) && (seen & 15) == 0 && a.ks[1] < (1 << 26) && a.vs[1] < (1 << 26);
 }
 // AXHIP_SDPA_TILE_WAVES=4|8: waves of a work-group of the tile kernel (measurements only)
 const int tile_waves = [] {
@@ -286,36 +291,85 @@ const int tile_waves = [] {
     return e ? atoi(e) : 0;
 }();
 
-// How a decoding step is divided, and its temporary memory: what the parts leave for the join.  Nothing of it depends on addresses.
-struct StepPlan {
-    int shares, prefix;
-    size_t own_out, own_lse, prefix_out, prefix_lse, bytes; // places; all of it (0: nothing can have two parts)
+// How a call is divided, and its temporary memory: what the parts leave for the join.  By the numbers in the arguments and the hints alone: nothing of it depends on addresses or on what the
+// device holds.
+struct CachePlan {
+    int shares, parts;
+    bool whole;                                         // decoding: one launch, nothing is divided
+    size_t own_out, own_lse, part_out, part_lse, bytes; // places; all of it
 };
+void place_parts(CachePlan &p, const CacheArgs &a, size_t rows) {
+    auto place = [&](size_t floats) { const size_t here = p.bytes; p.bytes = CallScratch::rounded(p.bytes + floats * sizeof(float)); return here; };
+    p.part_out = place(rows * p.parts * a.D);
+    p.part_lse = place(rows * p.parts);
+}
 // AXHIP_SDPA_STEP_GROUPS: work-groups of a step's own keys (measurements only)
 const int step_groups = [] {
     const char *e = getenv("AXHIP_SDPA_STEP_GROUPS");
-    return e ? atoi(e) : 512;
+    return e ? atoi(e) : 0;
 }();
-StepPlan step_plan(const CacheArgs &a) {
-    StepPlan p{};
+CachePlan step_plan(const CacheArgs &a, int max_kv, int max_prefix) {
+    CachePlan p{};
+    p.parts = 1;
     const int64_t rows = static_cast<int64_t>(a.new_tokens) * a.each, tiles = (rows + 15) / 16, most = std::min(a.table_ld << a.page_shift, MOST_KEYS);
-    const int64_t units = (most + 127) / 128 * a.entries; // at most
-    // shares of the own keys: two work-groups of four waves on each CU
-    p.shares = static_cast<int>(std::min<int64_t>(std::max<int64_t>(1, step_groups / (a.kv_heads * tiles)), units));
-    if (a.groups == 0 && most <= 128) return p;
+    const int64_t most_prefix = a.groups > 0 ? std::min(a.prefix_ld << a.page_shift, MOST_KEYS) : 0;
+    // Short sequences stay whole: the join is a launch, 4 - 5 us, and a work-group walks 128 keys a microsecond
+    const int64_t walk = std::min<int64_t>(std::max(max_kv, 0), most) + std::min<int64_t>(std::max(max_prefix, 0), most_prefix);
+    p.whole = walk <= 640 && (a.groups == 0 || a.entries * tiles * a.kv_heads <= 512);
+    if (p.whole) return p;
+    // shares of the own keys: two work-groups of four waves on each CU; beside prefixes one
+    const int64_t groups = step_groups ? step_groups : a.groups > 0 ? 256 : 512;
+    p.shares = static_cast<int>(std::min<int64_t>(std::max<int64_t>(1, groups / (a.kv_heads * tiles)), (most + 127) / 128 * a.entries));
     // parts of a prefix: one work-group of 128 rows for each CU
     const int64_t blocks = (a.entries * rows + 127) / 128 * a.kv_heads;
-    p.prefix = a.groups == 0 ? 0 : static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({64, 256 / blocks, (std::min(a.prefix_ld << a.page_shift, MOST_KEYS) + 63) / 64})));
-    const size_t own = (static_cast<size_t>(2 * p.shares) + (a.groups > 0 ? a.entries : 0)) * a.kv_heads * rows, pre = static_cast<size_t>(a.entries) * a.kv_heads * rows * p.prefix;
-    size_t at = CallScratch::rounded(sizeof(int2_t) * a.entries);
-    auto place = [&](size_t floats) { const size_t here = at; at = CallScratch::rounded(at + floats * sizeof(float)); return here; };
+    p.parts = a.groups == 0 ? 0 : static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({64, 256 / blocks, (most_prefix + 63) / 64})));
+    const size_t own = (static_cast<size_t>(2 * p.shares) + (a.groups > 0 ? a.entries : 0)) * a.kv_heads * rows;
+    p.bytes = CallScratch::rounded(sizeof(int2_t) * a.entries);
+    auto place = [&](size_t floats) { const size_t here = p.bytes; p.bytes = CallScratch::rounded(p.bytes + floats * sizeof(float)); return here; };
     p.own_out = place(own * a.D);
     p.own_lse = place(own);
-    p.prefix_out = place(pre * a.D);
-    p.prefix_lse = place(pre);
-    p.bytes = at;
+    place_parts(p, a, static_cast<size_t>(a.entries) * a.kv_heads * rows);
     return p;
 }
+// Prompts: the keys of a block of rows in parts where there are few blocks for the chip, or a few that are long.  In tiles of 64 keys at 1.1 us (16 rows of fp32: 0.9), the time is that of the
+// longest walk or of all walks over the 512 work-groups that the chip holds, and with parts the join's: a launch and one write and one read of the partial results.
+CachePlan prompt_plan(const CacheArgs &a, int max_kv) {
+    CachePlan p{};
+    p.parts = 1;
+    const int rows = a.dtype == AXHIP_DTYPE_F32 ? 16 : 128;
+    const double blocks = static_cast<double>(a.total_q * a.each / rows + (a.entries + 1) / 2) * a.kv_heads, tile = a.dtype == AXHIP_DTYPE_F32 ? 0.9 : 1.1;
+    const int64_t most = std::min(a.table ? a.table_ld << a.page_shift : a.total_kv, MOST_KEYS), longest = std::min<int64_t>(std::max(max_kv, 1), std::max<int64_t>(most, 1));
+    const double tokens = static_cast<double>(std::min<int64_t>(longest, a.total_q / std::max(a.entries, 1))), average = a.causal ? static_cast<double>(longest) - tokens / 2 : static_cast<double>(longest);
+    const double traffic = static_cast<double>(a.total_q) * a.heads * a.D * 8 / 4e6;
+    double best = 0;
+    for (int parts = 1; parts <= 32 && (parts == 1 || longest >= 128 * parts); ++parts) {
+        const double time = tile / 64 * std::max(static_cast<double>(longest) / parts, blocks * average / 512) + (parts > 1 ? 4.5 + traffic * parts : 0.0);
+        if (parts == 1 || time < 0.93 * best) {
+            best = time;
+            p.parts = parts;
+        }
+    }
+    if (p.parts > 1) place_parts(p, a, static_cast<size_t>(a.total_q) * a.heads);
+    return p;
+}
+// The plan's places in temporary memory
+int take_parts(const char *who, CacheArgs &a, const CachePlan &plan, CallScratch &scratch) {
+    a.shares = plan.shares;
+    a.parts = plan.parts;
+    if (plan.bytes == 0) return AXHIP_OK;
+    void *at = nullptr;
+    const int rc = scratch.take(&at, plan.bytes, who);
+    if (rc) return rc;
+    char *p = static_cast<char *>(at);
+    a.parts_of = reinterpret_cast<int2_t *>(p);
+    a.own_out = reinterpret_cast<float *>(p + plan.own_out);
+    a.own_lse = reinterpret_cast<float *>(p + plan.own_lse);
+    a.part_out = reinterpret_cast<float *>(p + plan.part_out);
+    a.part_lse = reinterpret_cast<float *>(p + plan.part_lse);
+    return AXHIP_OK;
+}
+// (units of 128 keys are counted in 32 bits)
+bool step_fits(const CacheArgs &a) { return (std::min(a.table_ld << a.page_shift, MOST_KEYS) / 128 + 1) * a.entries < (int64_t(1) << 31); }
 bool tensor_ok(const void *p, int dtype) { return p && (reinterpret_cast<uintptr_t>(p) & (dtype_size(dtype) - 1)) == 0; }
 
 } // namespace
@@ -326,13 +380,18 @@ extern "C" {
 
 const char *axhip_sdpa_cache_last_kernel(void) { return last_kernel; }
 
-size_t axhip_sdpa_packed_workspace_bytes(const AxhipSdpaPackedParams *) { return 0; }
+// (asked for by form: a call whose addresses or strides send it to the generic kernel leaves it alone)
+size_t axhip_sdpa_packed_workspace_bytes(const AxhipSdpaPackedParams *params) {
+    CacheArgs a{};
+    if (packed_args(a, params) != AXHIP_OK || a.entries == 0 || a.total_q == 0 || !form_for_matrix_cores(a)) return 0;
+    return prompt_plan(a, params->max_kv).bytes;
+}
 
 int axhip_sdpa_packed(const void *q, const void *k, const void *v, void *o, const AxhipSdpaPackedParams *params, void *stream) {
     return axhip_sdpa_packed_ws(q, k, v, o, params, nullptr, 0, stream);
 }
 
-int axhip_sdpa_packed_ws(const void *q, const void *k, const void *v, void *o, const AxhipSdpaPackedParams *params, void *, size_t, void *stream) {
+int axhip_sdpa_packed_ws(const void *q, const void *k, const void *v, void *o, const AxhipSdpaPackedParams *params, void *workspace, size_t workspace_bytes, void *stream) {
     CacheArgs a{};
     int rc = packed_args(a, params);
     if (rc) return rc;
@@ -351,23 +410,29 @@ int axhip_sdpa_packed_ws(const void *q, const void *k, const void *v, void *o, c
     rc = ensure_init();
     if (rc) return rc;
     hipStream_t s = resolve_stream(stream);
-    if (a.dtype == AXHIP_DTYPE_F32 && for_matrix_cores(a)) {
-        last_kernel = "f32";
-        return launch_rows_packed_f32(a, s);
-    }
-    if (for_matrix_cores(a)) {
+    if (!for_matrix_cores(a)) return launch_generic(a, s, "axhip_sdpa_packed");
+    const CachePlan plan = prompt_plan(a, params->max_kv);
+    CallScratch scratch(workspace, workspace_bytes, s);
+    rc = take_parts("axhip_sdpa_packed", a, plan, scratch);
+    if (rc) return rc;
+    const bool f32 = a.dtype == AXHIP_DTYPE_F32, bf16 = a.dtype == AXHIP_DTYPE_BF16;
+    if (f32) {
+        last_kernel = plan.parts > 1 ? "f32, parts" : "f32";
+        rc = launch_rows_packed_f32(a, s);
+    } else {
         const int64_t blocks = (a.total_q * a.each + 255) / 256 * a.kv_heads;
-        const int waves = tile_waves ? tile_waves : blocks >= 192 ? 8 : 4;
-        last_kernel = "tile";
-        return a.dtype == AXHIP_DTYPE_BF16 ? launch_tile_bf16(a, waves, s) : launch_tile_f16(a, waves, s);
+        const int waves = tile_waves ? tile_waves : blocks >= 192 && plan.parts == 1 ? 8 : 4;
+        last_kernel = plan.parts > 1 ? "tile, parts" : "tile";
+        rc = bf16 ? launch_tile_bf16(a, waves, s) : launch_tile_f16(a, waves, s);
     }
-    return launch_generic(a, s, "axhip_sdpa_packed");
+    if (!rc && plan.parts > 1) rc = f32 ? launch_join_f32(a, s) : bf16 ? launch_join_bf16(a, s) : launch_join_f16(a, s);
+    return rc ? rc : scratch.release();
 }
 
 size_t axhip_sdpa_paged_workspace_bytes(const AxhipSdpaPagedParams *params) {
     CacheArgs a{};
-    if (paged_args(a, params) != AXHIP_OK || a.entries == 0) return 0;
-    return step_plan(a).bytes;
+    if (paged_args(a, params) != AXHIP_OK || a.entries == 0 || !form_for_matrix_cores(a) || !step_fits(a)) return 0;
+    return step_plan(a, params->max_kv, params->max_prefix).bytes;
 }
 
 int axhip_sdpa_paged(const void *q, void *o, const AxhipSdpaPagedParams *params, void *stream) { return axhip_sdpa_paged_ws(q, o, params, nullptr, 0, stream); }
@@ -384,38 +449,28 @@ int axhip_sdpa_paged_ws(const void *q, void *o, const AxhipSdpaPagedParams *para
     rc = ensure_init();
     if (rc) return rc;
     hipStream_t s = resolve_stream(stream);
-    // (units of 128 keys are counted in 32 bits)
-    if (!for_matrix_cores(a) || (std::min(a.table_ld << a.page_shift, MOST_KEYS) / 128 + 1) * a.entries >= (int64_t(1) << 31)) return launch_generic(a, s, "axhip_sdpa_paged");
-    const StepPlan plan = step_plan(a);
-    a.shares = plan.shares;
-    a.prefix_parts = plan.prefix;
+    if (!for_matrix_cores(a) || !step_fits(a)) return launch_generic(a, s, "axhip_sdpa_paged");
+    const CachePlan plan = step_plan(a, params->max_kv, params->max_prefix);
     CallScratch scratch(workspace, workspace_bytes, s);
-    if (plan.bytes > 0) {
-        void *at = nullptr;
-        rc = scratch.take(&at, plan.bytes, "axhip_sdpa_paged");
-        if (rc) return rc;
-        char *p = static_cast<char *>(at);
-        a.parts_of = reinterpret_cast<int2_t *>(p);
-        a.own_out = reinterpret_cast<float *>(p + plan.own_out);
-        a.own_lse = reinterpret_cast<float *>(p + plan.own_lse);
-        a.prefix_out = reinterpret_cast<float *>(p + plan.prefix_out);
-        a.prefix_lse = reinterpret_cast<float *>(p + plan.prefix_lse);
-    }
-    last_kernel = "rows";
-    const bool f32 = a.dtype == AXHIP_DTYPE_F32, bf16 = a.dtype == AXHIP_DTYPE_BF16;
-    if (a.groups > 0) last_kernel = "rows, prefix";
-    if (a.groups > 0 && f32) {
-        rc = launch_prefix_f32(a, s);
-        if (rc) return rc;
-    }
-    if (a.groups > 0 && !f32) rc = bf16 ? launch_step_bf16(a, s) : launch_step_f16(a, s);
-    else rc = f32 ? launch_rows_own_f32(a, s) : bf16 ? launch_rows_own_bf16(a, s) : launch_rows_own_f16(a, s);
+    rc = take_parts("axhip_sdpa_paged", a, plan, scratch);
     if (rc) return rc;
-    if (plan.bytes > 0) {
-        rc = f32 ? launch_join_f32(a, s) : bf16 ? launch_join_bf16(a, s) : launch_join_f16(a, s);
-        if (rc) return rc;
+    const bool f32 = a.dtype == AXHIP_DTYPE_F32, bf16 = a.dtype == AXHIP_DTYPE_BF16;
+    if (plan.whole) {
+        last_kernel = "whole";
+        return f32 ? launch_rows_whole_f32(a, s) : bf16 ? launch_rows_whole_bf16(a, s) : launch_rows_whole_f16(a, s);
     }
-    return scratch.release();
+    last_kernel = a.groups > 0 ? "shares, prefix" : "shares";
+    if (a.groups > 0 && !f32) {
+        rc = bf16 ? launch_step_bf16(a, s) : launch_step_f16(a, s);
+    } else {
+        if (a.groups > 0) {
+            rc = launch_prefix_f32(a, s);
+            if (rc) return rc;
+        }
+        rc = f32 ? launch_rows_own_f32(a, s) : bf16 ? launch_rows_own_bf16(a, s) : launch_rows_own_f16(a, s);
+    }
+    if (!rc) rc = f32 ? launch_join_f32(a, s) : bf16 ? launch_join_bf16(a, s) : launch_join_f16(a, s);
+    return rc ? rc : scratch.release();
 }
 
 } // extern "C"

@@ -29,10 +29,11 @@ struct CacheArgs {
     int groups;
     const int32_t *group_starts, *prefix_table, *prefix_lengths;
     int64_t prefix_ld;
-    // decoding in parts: the shares that the own keys are dealt out in, the parts that a prefix has at most; what they leave for the join, by slot (two to a share, then one to a sequence), key head and row, or by
-    // sequence, key head, row and part; for each sequence the first of its slots and how many there are to join (0: it is finished)
-    int shares, prefix_parts;
-    float *own_out, *own_lse, *prefix_out, *prefix_lse;
+    // in parts: how many a prefix (decoding) or the keys of a block of rows (prompts) have, at most, and what they leave for the join, by row -- sequence, key head, row of it (decoding),
+    // or token, head -- and part; the shares that a step's own keys are dealt out in, what they leave by slot (two to a share, then one to a sequence), key head and row, and for each
+    // sequence the first of its slots and how many there are to join (0: it is finished)
+    int parts, shares;
+    float *part_out, *part_lse, *own_out, *own_lse;
     int2_t *parts_of;
 };
 // Work-groups of a step's own keys
@@ -88,6 +89,10 @@ int launch_rows_own_bf16(const CacheArgs &a, hipStream_t s);
 int launch_rows_own_f16(const CacheArgs &a, hipStream_t s);
 int launch_rows_own_f32(const CacheArgs &a, hipStream_t s);
 int launch_rows_packed_f32(const CacheArgs &a, hipStream_t s);
+// .. whole sequences, prefix and own keys one behind the other: a step that is not divided
+int launch_rows_whole_bf16(const CacheArgs &a, hipStream_t s);
+int launch_rows_whole_f16(const CacheArgs &a, hipStream_t s);
+int launch_rows_whole_f32(const CacheArgs &a, hipStream_t s);
 int launch_join_bf16(const CacheArgs &a, hipStream_t s);
 int launch_join_f16(const CacheArgs &a, hipStream_t s);
 int launch_join_f32(const CacheArgs &a, hipStream_t s);

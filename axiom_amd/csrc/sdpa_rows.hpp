@@ -67,8 +67,13 @@ __device__ inline Share own_share(const CacheArgs &a, int index) {
     s.shares = min(a.shares, total); // (none is empty)
     s.from = s.to = s.entry = s.entry_at = 0;
     if (index >= s.shares) return s;
-    s.from = static_cast<int>(static_cast<int64_t>(index) * total / s.shares);
-    s.to = static_cast<int>(static_cast<int64_t>(index + 1) * total / s.shares);
+    if (total < (1 << 20) && s.shares < (1 << 11)) { // (a division of 64 bits is a hundred instructions)
+        s.from = static_cast<int>(static_cast<uint32_t>(index * total) / static_cast<uint32_t>(s.shares));
+        s.to = static_cast<int>(static_cast<uint32_t>((index + 1) * total) / static_cast<uint32_t>(s.shares));
+    } else {
+        s.from = static_cast<int>(static_cast<int64_t>(index) * total / s.shares);
+        s.to = static_cast<int>(static_cast<int64_t>(index + 1) * total / s.shares);
+    }
     bool found = false;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -93,14 +98,16 @@ __device__ inline Share own_share(const CacheArgs &a, int index) {
     return s;
 }
 
-// What a work-group does: OWN, a part of a sequence's own keys (decoding); PACKED, whole sequences by cu_q (fp32 prompts); PREFIX, a part of a group's prefix for 16 of its rows (fp32)
-enum RowsMode { ROWS_OWN = 0, ROWS_PACKED = 1, ROWS_PREFIX = 2 };
+// What a work-group does: OWN, a share of all own keys (decoding); PACKED, 16 rows of a sequence by cu_q, or a part of their keys (fp32 prompts); PREFIX, a part of a group's prefix for 16 of its
+// rows (fp32); WHOLE, all keys of 16 rows, prefix and own (decoding, not divided)
+enum RowsMode { ROWS_OWN = 0, ROWS_PACKED = 1, ROWS_PREFIX = 2, ROWS_WHOLE = 3 };
 
 // 16 rows, from row0 on of `rows`, against the keys [begin, end) of a run.  slot < 0: finished here; else where the results go for the join.
 struct Segment {
     KeyRun run;
     int entry, row0, rows, begin, end, tokens, q_from; // tokens: of the entry, the last of which sees the last key; q_from: its first token, or a group's first sequence
-    int64_t slot;                                      // own parts: their place; prefix: the part's number
+    int64_t slot;                                      // own parts: their place; else the part's number
+    KeyRun prefix;                                     // WHOLE: these keys first
 };
 
 template <int DT, int D, bool PAD, int MODE> __device__ __forceinline__ void rows_segment(const CacheArgs &a, int kvh, const Segment &seg) {
@@ -115,9 +122,9 @@ template <int DT, int D, bool PAD, int MODE> __device__ __forceinline__ void row
     float *const rows_lds = reinterpret_cast<float *>(tile_lds);
     const int tid = threadIdx.x, lane = tid % WAVE, wave = __builtin_amdgcn_readfirstlane(tid / WAVE), l16 = lane % 16, g = lane / 16;
     const int dv = a.D;
-    const KeyRun run = seg.run;
-    const int entry = seg.entry, row0 = seg.row0, rows = seg.rows, begin = seg.begin, end = seg.end, tokens = seg.tokens, q_from = seg.q_from;
-    const int n_keys = __builtin_amdgcn_readfirstlane(run.n);
+    KeyRun run = seg.run;
+    const int entry = seg.entry, row0 = seg.row0, rows = seg.rows, tokens = seg.tokens, q_from = seg.q_from;
+    int begin = seg.begin, end = seg.end, n_keys = __builtin_amdgcn_readfirstlane(run.n);
 
     // ---- this lane's row
     const int row = min(row0 + l16, rows - 1);
@@ -129,14 +136,15 @@ template <int DT, int D, bool PAD, int MODE> __device__ __forceinline__ void row
             at.q = (q_from + token) * a.qs[1] + head * a.qs[2];
             at.o = (q_from + token) * a.os[1] + head * a.os[2];
         } else {
-            const int seq = MODE == ROWS_OWN ? entry : q_from + token / a.new_tokens, t = MODE == ROWS_OWN ? token : token % a.new_tokens;
+            constexpr bool OF_GROUP = MODE == ROWS_PREFIX;
+            const int seq = OF_GROUP ? q_from + token / a.new_tokens : entry, t = OF_GROUP ? token % a.new_tokens : token;
             at.q = seq * a.qs[0] + t * a.qs[1] + head * a.qs[2];
             at.o = seq * a.os[0] + t * a.os[1] + head * a.os[2];
         }
         return at;
     };
-    const int limit = MODE == ROWS_PREFIX || !a.causal ? end - 1 : min(end - 1, n_keys - tokens + row / a.each); // last key that this row sees
-    const int least = MODE == ROWS_PREFIX || !a.causal ? end - 1 : min(end - 1, n_keys - tokens + row0 / a.each); // .. that every row of the tile sees
+    int limit = MODE == ROWS_PREFIX || !a.causal ? end - 1 : min(end - 1, n_keys - tokens + row / a.each); // last key that this row sees
+    int least = MODE == ROWS_PREFIX || !a.causal ? end - 1 : min(end - 1, n_keys - tokens + row0 / a.each); // .. that every row of the tile sees
 
     uint4_t qf[KJ];
     {
@@ -223,6 +231,16 @@ template <int DT, int D, bool PAD, int MODE> __device__ __forceinline__ void row
 #pragma unroll
     for (int t = 0; t < NACC; ++t) oacc[t] = rows_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     float m_run = NEG_INF_F, l_run = 0.0f;
+    for (int pass = MODE == ROWS_WHOLE && seg.prefix.n > 0 ? 0 : 1; pass < 2; ++pass) {
+    if constexpr (MODE == ROWS_WHOLE) {
+        if (seg.prefix.n > 0) { // the prefix, which every row sees, then the sequence's own keys
+            run = pass == 0 ? seg.prefix : seg.run;
+            n_keys = __builtin_amdgcn_readfirstlane(run.n);
+            end = pass == 0 ? n_keys : seg.end;
+            limit = pass == 0 ? end - 1 : min(end - 1, n_keys - tokens + row / a.each);
+            least = pass == 0 ? end - 1 : min(end - 1, n_keys - tokens + row0 / a.each);
+        }
+    }
     int at = begin + KEYS * wave;
     Ids ids{};
     if (at < end) {
@@ -314,6 +332,8 @@ template <int DT, int D, bool PAD, int MODE> __device__ __forceinline__ void row
         }
     }
 
+    }
+
     // ---- the four waves' states meet: [wave][row][D + 4], then maxima and denominators
     const float l_tot = across32(across16(l_run, lanes_add), lanes_add);
     float *const tops = rows_lds + ROWS_WAVES * ROWS * (D + 4), *const dens = tops + ROWS_WAVES * ROWS;
@@ -361,18 +381,22 @@ template <int DT, int D, bool PAD, int MODE> __device__ __forceinline__ void row
         if (any_bad) den = __builtin_nanf("");
         o *= den == 0.0f ? 0.0f : 1.0f / den;
         if (leave) {
+            float *outs = a.part_out, *lses = a.part_lse;
             int64_t place;
             if constexpr (MODE == ROWS_PREFIX) {
                 const int64_t of = static_cast<int64_t>(q_from) * a.new_tokens * a.each + row0 + r; // sequence, token, head of the key head
                 const int64_t per = static_cast<int64_t>(a.new_tokens) * a.each;
-                place = ((of / per * a.kv_heads + kvh) * per + of % per) * a.prefix_parts + seg.slot;
-                *reinterpret_cast<rows_f32x4 *>(a.prefix_out + place * dv + d) = o;
+                place = ((of / per * a.kv_heads + kvh) * per + of % per) * a.parts + seg.slot;
+            } else if constexpr (MODE == ROWS_PACKED) {
+                place = (static_cast<int64_t>(q_from + (row0 + r) / a.each) * a.heads + kvh * a.each + (row0 + r) % a.each) * a.parts + seg.slot;
             } else {
                 place = (seg.slot * a.kv_heads + kvh) * rows + row0 + r;
-                *reinterpret_cast<rows_f32x4 *>(a.own_out + place * dv + d) = o;
+                outs = a.own_out;
+                lses = a.own_lse;
             }
+            *reinterpret_cast<rows_f32x4 *>(outs + place * dv + d) = o;
             // (what is no number makes the joined row none: +inf minus itself)
-            if (d == 0) (MODE == ROWS_PREFIX ? a.prefix_lse : a.own_lse)[place] = den == 0.0f ? NEG_INF_F : den == den ? top + __builtin_amdgcn_logf(den) : -NEG_INF_F;
+            if (d == 0) lses[place] = den == 0.0f ? NEG_INF_F : den == den ? top + __builtin_amdgcn_logf(den) : -NEG_INF_F;
         } else {
             unsigned char *out = static_cast<unsigned char *>(a.o) + (q_place(row0 + r).o + d) * ES;
             if constexpr (F32) *reinterpret_cast<rows_f32x4 *>(out) = o;
@@ -382,7 +406,8 @@ template <int DT, int D, bool PAD, int MODE> __device__ __forceinline__ void row
 }
 
 template <int DT, int D, bool PAD, int MODE> __device__ __forceinline__ void rows_body(const CacheArgs &a, int index_of_all) {
-    const int kvh = index_of_all % a.kv_heads, rest = index_of_all / a.kv_heads;
+    const int kvh = index_of_all % a.kv_heads;
+    int rest = index_of_all / a.kv_heads;
     Segment seg{};
     seg.slot = -1;
     if constexpr (MODE == ROWS_OWN) {
@@ -413,7 +438,23 @@ template <int DT, int D, bool PAD, int MODE> __device__ __forceinline__ void row
             at = entry_at = entry_to;
             if (at < to) __syncthreads(); // (the states in LDS are read)
         }
+    } else if constexpr (MODE == ROWS_WHOLE) {
+        seg.tokens = a.new_tokens;
+        seg.rows = a.new_tokens * a.each;
+        const int tiles = (seg.rows + ROWS - 1) / ROWS;
+        seg.entry = rest / tiles;
+        seg.row0 = rest % tiles * ROWS;
+        seg.run = keys_of(a, seg.entry);
+        seg.end = seg.run.n = __builtin_amdgcn_readfirstlane(seg.run.n);
+        const int group = a.groups > 0 ? group_of(a, seg.entry) : -1;
+        if (group >= 0) seg.prefix = prefix_of(a, group);
+        rows_segment<DT, D, PAD, MODE>(a, kvh, seg);
     } else if constexpr (MODE == ROWS_PACKED) {
+        int part = 0;
+        if (a.parts > 1) {
+            part = rest % a.parts;
+            rest /= a.parts;
+        }
         const TileItem item = tile_item<ROWS>(a, rest);
         seg.entry = __builtin_amdgcn_readfirstlane(item.entry);
         if (seg.entry < 0) return;
@@ -425,17 +466,23 @@ template <int DT, int D, bool PAD, int MODE> __device__ __forceinline__ void row
         if (seg.row0 < 0 || seg.row0 >= seg.rows) return;
         seg.run = keys_of(a, seg.entry);
         seg.end = __builtin_amdgcn_readfirstlane(a.causal ? seg.run.n - t.n + (min(seg.row0 + ROWS, seg.rows) - 1) / a.each + 1 : seg.run.n);
+        if (a.parts > 1) {
+            const int chunk = part_keys(a, max(0, seg.end));
+            seg.begin = part * chunk;
+            seg.end = min(seg.end, seg.begin + chunk);
+            seg.slot = part;
+        }
         rows_segment<DT, D, PAD, MODE>(a, kvh, seg);
     } else {
-        const int part = rest % a.prefix_parts;
-        const GroupItem item = group_item<ROWS>(a, rest / a.prefix_parts);
+        const int part = rest % a.parts;
+        const GroupItem item = group_item<ROWS>(a, rest / a.parts);
         seg.entry = __builtin_amdgcn_readfirstlane(item.group);
         if (seg.entry < 0) return;
         seg.rows = item.rows;
         seg.row0 = item.row0;
         seg.q_from = item.first;
         seg.run = prefix_of(a, seg.entry);
-        const int chunk = prefix_chunk(a, seg.run.n);
+        const int chunk = part_keys(a, seg.run.n);
         seg.begin = __builtin_amdgcn_readfirstlane(part * chunk);
         seg.end = __builtin_amdgcn_readfirstlane(min(seg.run.n, seg.begin + chunk));
         if (seg.begin >= seg.run.n) return; // (as many parts as that are there for the join)
@@ -450,31 +497,47 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, D > 128 ? 1 : 2) void sdpa_rows_ke
 
 // out = sum_s 2^(lse_s - max lse) O_s / sum_s 2^(lse_s - max lse) over a row's prefix parts and own parts, in that order.  WAVES wavefronts to a row take them in turn, D / 4 lanes a
 // result, and everything that fits the first trip to memory is requested before the weights are known.
-template <int DT, int D, int WAVES>
+// PACKED: of prompts, whose rows are token and head and which have a.parts each; rows that no sequence owns are left as they are.
+template <int DT, int D, int WAVES, bool PACKED>
 __global__ __launch_bounds__(256) void sdpa_join_kernel(const CacheArgs a) {
     constexpr int LANES = D / 4, TAKE = WAVE / LANES * WAVES, AHEAD = 8;
     __shared__ __attribute__((aligned(16))) float sums[4][D + 4];
     const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE, d = lane % LANES * 4, first = wave % WAVES * (WAVE / LANES) + lane / LANES;
     const int64_t id = static_cast<int64_t>(blockIdx.x) * (4 / WAVES) + wave / WAVES; // sequence, token, head
-    const int per = a.new_tokens * a.heads;
-    if (id >= static_cast<int64_t>(a.entries) * per) return; // (whole work-groups with WAVES = 4)
-    const int seq = static_cast<int>(id / per), token = static_cast<int>(id % per) / a.heads, head = static_cast<int>(id % per) % a.heads;
-    const int kvh = head / a.each, row = token * a.each + head % a.each, rows = a.new_tokens * a.each;
-    const int2_t own = a.parts_of[seq];
-    if (own.y == 0) return; // finished already
-    int prefix = 0;
-    if (a.groups > 0) {
-        const int group = group_of(a, seq);
-        if (group >= 0) {
-            const int n = prefix_of(a, group).n, chunk = prefix_chunk(a, n);
-            prefix = (n + chunk - 1) / chunk;
+    int64_t pre, at;
+    int prefix = 0, n, kvh = 0, row = 0, rows = 0;
+    int2_t own = {0, 0};
+    if constexpr (PACKED) {
+        if (id >= a.total_q * a.heads) return; // (whole work-groups with WAVES = 4)
+        const int token = static_cast<int>(id / a.heads), head = static_cast<int>(id % a.heads);
+        const int e = last_not_beyond(a.entries, token, [&](int i) { return a.cu_q[i]; });
+        if (a.cu_q[e] > token || a.cu_q[e + 1] <= token) return;
+        prefix = n = a.parts;
+        pre = id * a.parts;
+        at = token * a.os[1] + head * a.os[2] + d;
+    } else {
+        const int per = a.new_tokens * a.heads;
+        if (id >= static_cast<int64_t>(a.entries) * per) return;
+        const int seq = static_cast<int>(id / per), token = static_cast<int>(id % per) / a.heads, head = static_cast<int>(id % per) % a.heads;
+        kvh = head / a.each;
+        row = token * a.each + head % a.each;
+        rows = a.new_tokens * a.each;
+        own = a.parts_of[seq];
+        if (own.y == 0) return; // finished already
+        if (a.groups > 0) {
+            const int group = group_of(a, seq);
+            if (group >= 0) {
+                const int keys = prefix_of(a, group).n, chunk = part_keys(a, keys);
+                prefix = (keys + chunk - 1) / chunk;
+            }
         }
+        n = prefix + own.y;
+        pre = ((static_cast<int64_t>(seq) * a.kv_heads + kvh) * rows + row) * a.parts;
+        at = seq * a.os[0] + token * a.os[1] + head * a.os[2] + d;
     }
-    const int n = prefix + own.y;
-    const int64_t pre = ((static_cast<int64_t>(seq) * a.kv_heads + kvh) * rows + row) * a.prefix_parts;
     // (own parts: the first share's slot, then the first slots of the shares behind it)
-    auto place = [&](int i) { return i < prefix ? pre + i : (static_cast<int64_t>(i == prefix ? own.x : own.x / 2 * 2 + 2 * (i - prefix)) * a.kv_heads + kvh) * rows + row; };
-    auto lse = [&](int i) { return (i < prefix ? a.prefix_lse : a.own_lse)[place(i)]; };
+    auto place = [&](int i) { return PACKED || i < prefix ? pre + i : (static_cast<int64_t>(i == prefix ? own.x : own.x / 2 * 2 + 2 * (i - prefix)) * a.kv_heads + kvh) * rows + row; };
+    auto lse = [&](int i) { return (PACKED || i < prefix ? a.part_lse : a.own_lse)[place(i)]; };
     rows_f32x4 o[AHEAD];
     float w[AHEAD];
     auto fetch = [&](int i0) __attribute__((always_inline)) {
@@ -482,7 +545,7 @@ __global__ __launch_bounds__(256) void sdpa_join_kernel(const CacheArgs a) {
         for (int k = 0; k < AHEAD; ++k) {
             const int i = min(i0 + TAKE * k, n - 1);
             w[k] = i0 + TAKE * k < n ? lse(i) : NEG_INF_F;
-            o[k] = *reinterpret_cast<const rows_f32x4 *>((i < prefix ? a.prefix_out : a.own_out) + place(i) * a.D + (d < a.D ? d : 0));
+            o[k] = *reinterpret_cast<const rows_f32x4 *>((PACKED || i < prefix ? a.part_out : a.own_out) + place(i) * a.D + (d < a.D ? d : 0));
         }
     };
     float top = NEG_INF_F;
@@ -526,7 +589,6 @@ __global__ __launch_bounds__(256) void sdpa_join_kernel(const CacheArgs a) {
     }
     if (lane >= LANES || d >= a.D) return;
     acc *= den == 0.0f ? 0.0f : 1.0f / den;
-    const int64_t at = seq * a.os[0] + token * a.os[1] + head * a.os[2] + d;
     if constexpr (DT == AXHIP_DTYPE_F32) *reinterpret_cast<rows_f32x4 *>(static_cast<float *>(a.o) + at) = acc;
     else *reinterpret_cast<uint2_t *>(static_cast<uint16_t *>(a.o) + at) = uint2_t{pack2<DT == AXHIP_DTYPE_BF16>(acc[0], acc[1]), pack2<DT == AXHIP_DTYPE_BF16>(acc[2], acc[3])};
 }
@@ -552,19 +614,21 @@ template <int DT, int MODE> int launch_rows_mode(const CacheArgs &a, int64_t blo
 }
 // the shares of a decoding step's own keys
 template <int DT> int launch_rows_own(const CacheArgs &a, hipStream_t s) { return launch_rows_mode<DT, ROWS_OWN>(a, own_blocks(a), s); }
-template <int DT, int D> void launch_join_as(const CacheArgs &a, int64_t rows, hipStream_t s) {
+template <int DT> int launch_rows_whole(const CacheArgs &a, hipStream_t s) { return launch_rows_mode<DT, ROWS_WHOLE>(a, (static_cast<int64_t>(a.new_tokens) * a.each + ROWS - 1) / ROWS * a.kv_heads * a.entries, s); }
+template <int DT, int D, bool PACKED> void launch_join_as(const CacheArgs &a, int64_t rows, hipStream_t s) {
     // a work-group to a row where those are few (up to 128 results in the first trip), else a wavefront
-    if (rows <= 1024) hipLaunchKernelGGL((sdpa_join_kernel<DT, D, 4>), dim3(static_cast<unsigned>(rows)), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((sdpa_join_kernel<DT, D, 1>), dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), 0, s, a);
+    if (rows <= 1024) hipLaunchKernelGGL((sdpa_join_kernel<DT, D, 4, PACKED>), dim3(static_cast<unsigned>(rows)), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((sdpa_join_kernel<DT, D, 1, PACKED>), dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), 0, s, a);
 }
-template <int DT> int launch_join(const CacheArgs &a, hipStream_t s) {
-    const int64_t rows = static_cast<int64_t>(a.entries) * a.new_tokens * a.heads;
-    AXHIP_REQUIRE(launch_fits((rows + 3) / 4, 256), AXHIP_ERR_UNSUPPORTED, "axhip_sdpa_paged: grid too large");
-    if (a.D <= 64) launch_join_as<DT, 64>(a, rows, s);
-    else if (a.D <= 128) launch_join_as<DT, 128>(a, rows, s);
-    else launch_join_as<DT, 256>(a, rows, s);
+template <int DT, bool PACKED> int launch_join_of(const CacheArgs &a, hipStream_t s) {
+    const int64_t rows = PACKED ? a.total_q * a.heads : static_cast<int64_t>(a.entries) * a.new_tokens * a.heads;
+    AXHIP_REQUIRE(launch_fits((rows + 3) / 4, 256), AXHIP_ERR_UNSUPPORTED, "attention of ragged sequences: grid too large");
+    if (a.D <= 64) launch_join_as<DT, 64, PACKED>(a, rows, s);
+    else if (a.D <= 128) launch_join_as<DT, 128, PACKED>(a, rows, s);
+    else launch_join_as<DT, 256, PACKED>(a, rows, s);
     AXHIP_CHECK_HIP(hipGetLastError());
     return AXHIP_OK;
 }
+template <int DT> int launch_join(const CacheArgs &a, hipStream_t s) { return a.new_tokens ? launch_join_of<DT, false>(a, s) : launch_join_of<DT, true>(a, s); }
 
 } // namespace axhip

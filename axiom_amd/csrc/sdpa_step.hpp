@@ -19,7 +19,7 @@ template <bool BF16, int D, int DE, bool PAD> int launch_step_as(const CacheArgs
         static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(&sdpa_step_kernel<BF16, D, DE, PAD>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         AXHIP_CHECK_HIP(attr);
     }
-    const int64_t prefix = (static_cast<int64_t>(a.entries) * a.new_tokens * a.each / 128 + a.groups) * a.prefix_parts * a.kv_heads, all = prefix + own_blocks(a); // at most
+    const int64_t prefix = (static_cast<int64_t>(a.entries) * a.new_tokens * a.each / 128 + a.groups) * a.parts * a.kv_heads, all = prefix + own_blocks(a); // at most
     AXHIP_REQUIRE(launch_fits(all, 256), AXHIP_ERR_UNSUPPORTED, "axhip_sdpa_paged: grid too large");
     hipLaunchKernelGGL((sdpa_step_kernel<BF16, D, DE, PAD>), dim3(static_cast<unsigned>(all)), dim3(256), lds, s, a, static_cast<int>(prefix));
     AXHIP_CHECK_HIP(hipGetLastError());

@@ -62,50 +62,55 @@ __device__ __forceinline__ void tile_body(const CacheArgs &a, int index_of_all) 
     const int ql = lane % 32, g = lane / 32;
     const bool second = NW == 8 && wave >= 4;
     const int kvh = index_of_all % a.kv_heads;
-    // entry, its rows from row0 on, its keys [begin, nk)
-    int entry, rows, row0, nk, begin = 0, part = 0, from;
+    // entry, its rows from row0 on; its keys: n_all, of which [begin, nk) are this work-group's
+    int rest = index_of_all / a.kv_heads, part = 0, entry, rows, row0, n_all, from;
+    if (a.parts > 1) {
+        part = rest % a.parts;
+        rest /= a.parts;
+    }
     KeyRun run;
     if constexpr (KEYS == TILE_PREFIX) {
-        const int rest = index_of_all / a.kv_heads;
-        part = rest % a.prefix_parts;
-        const GroupItem item = group_item<BM>(a, rest / a.prefix_parts);
+        const GroupItem item = group_item<BM>(a, rest);
         entry = __builtin_amdgcn_readfirstlane(item.group);
         if (entry < 0) return;
         rows = __builtin_amdgcn_readfirstlane(item.rows);
         row0 = __builtin_amdgcn_readfirstlane(item.row0);
         from = item.first;
         run = prefix_of(a, entry);
-        const int chunk = prefix_chunk(a, run.n);
-        begin = __builtin_amdgcn_readfirstlane(part * chunk);
-        nk = __builtin_amdgcn_readfirstlane(min(run.n, begin + chunk));
-        if (begin >= nk) return; // (as many parts as that are there for the join)
     } else {
-        const TileItem item = tile_item<BM>(a, index_of_all / a.kv_heads);
+        const TileItem item = tile_item<BM>(a, rest);
         entry = __builtin_amdgcn_readfirstlane(item.entry);
         const int block = __builtin_amdgcn_readfirstlane(item.block);
         if (entry < 0) return;
         const TokenRun t = tokens_of(a, entry);
         run = keys_of(a, entry);
         rows = __builtin_amdgcn_readfirstlane(t.n * a.each);
-        nk = __builtin_amdgcn_readfirstlane(run.n);
         row0 = block * BM;
         from = t.from;
         if (block < 0 || row0 >= rows) return;
     }
+    n_all = __builtin_amdgcn_readfirstlane(run.n);
     constexpr bool PAGED = KEYS != TILE_PACKED;
     const bool causal = KEYS != TILE_PREFIX && a.causal;
     const int dv = a.D;
-    const int past = nk - rows / a.each; // keys in front of the first token
+    const int past = n_all - rows / a.each; // keys in front of the first token
+    auto sees = [&](int r) { return causal ? past + min(r, rows - 1) / a.each : n_all - 1; }; // the last key that a row sees
+    int begin = 0, nk = max(0, __builtin_amdgcn_readfirstlane(sees(row0 + BM - 1) + 1));
+    if (a.parts > 1) {
+        const int chunk = part_keys(a, nk);
+        begin = part * chunk;
+        nk = min(nk, begin + chunk);
+        if (KEYS == TILE_PREFIX && begin >= nk) return; // (as many parts as that are there for the join)
+    }
 
     // this lane's query, and the last key that it sees; rows behind the last one see what that one does and are not stored
     const int row = row0 + 32 * wave + ql;
     const bool row_ok = row < rows;
-    auto sees = [&](int r) { return causal ? past + min(r, rows - 1) / a.each : nk - 1; };
     const int token = min(row, rows - 1) / a.each, head = kvh * a.each + min(row, rows - 1) % a.each;
-    const int limit = causal ? past + token : nk - 1;
+    const int limit = min(causal ? past + token : n_all - 1, nk - 1);
     const int wave_row = row0 + 32 * wave;
-    const int least = __builtin_amdgcn_readfirstlane(sees(wave_row)), farthest = __builtin_amdgcn_readfirstlane(wave_row < rows ? sees(wave_row + 31) : -1);
-    const int ntiles = __builtin_amdgcn_readfirstlane((sees(row0 + BM - 1) - begin + TK) / TK); // (sees -1: none)
+    const int least = __builtin_amdgcn_readfirstlane(min(sees(wave_row), nk - 1)), farthest = __builtin_amdgcn_readfirstlane(wave_row < rows ? min(sees(wave_row + 31), nk - 1) : -1);
+    const int ntiles = (nk - begin + TK - 1) / TK; // (0 or less: none)
     int64_t at_q;
     if constexpr (KEYS == TILE_PREFIX) at_q = (from + token / a.new_tokens) * a.qs[0] + token % a.new_tokens * a.qs[1] + head * a.qs[2];
     else at_q = (from + token) * a.qs[1] + head * a.qs[2];
@@ -137,7 +142,7 @@ __device__ __forceinline__ void tile_body(const CacheArgs &a, int index_of_all) 
     }
     const uint32_t lds_base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(tile_lds));
     const uint32_t lds_wave = __builtin_amdgcn_readfirstlane(lds_base + RPL * wave * ROWB);
-    const int last_piece = __builtin_amdgcn_readfirstlane((nk - 1) / RPL * RPL);
+    const int last_piece = (nk - 1) / RPL * RPL;
     bool bad = false;
     auto piece_of = [&](int tile, int n) { return min(begin + tile * TK + RPL * NW * n + RPL * wave, last_piece); };
     struct Pages { int id[NLOAD]; };
@@ -321,19 +326,27 @@ __device__ __forceinline__ void tile_body(const CacheArgs &a, int index_of_all) 
         if (any) l = __builtin_nanf("");
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    if constexpr (KEYS == TILE_PREFIX) {
+    if (KEYS == TILE_PREFIX || a.parts > 1) {
         if (!row_ok) return;
-        const int64_t per = static_cast<int64_t>(a.new_tokens) * a.each, of = from * per + row; // sequence, token, head of the key head
-        const int64_t place = ((of / per * a.kv_heads + kvh) * per + of % per) * a.prefix_parts + part;
+        int64_t place;
+        if constexpr (KEYS == TILE_PREFIX) { // sequence, key head, token, head of the key head
+            const int64_t per = static_cast<int64_t>(a.new_tokens) * a.each, of = from * per + row;
+            place = (of / per * a.kv_heads + kvh) * per + of % per;
+        } else { // token, head
+            place = static_cast<int64_t>(from + token) * a.heads + head;
+        }
+        place = place * a.parts + part;
+        if (ntiles > 0) {
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
+            for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                const int d = dt * 32 + i * 2 + 4 * g;
-                if (d < dv) *reinterpret_cast<float4_t *>(a.prefix_out + place * dv + d) = float4_t{oacc[dt][i] * inv, oacc[dt][i + 1] * inv, oacc[dt][i + 2] * inv, oacc[dt][i + 3] * inv};
-            }
+                for (int i = 0; i < 16; i += 4) {
+                    const int d = dt * 32 + i * 2 + 4 * g;
+                    if (d < dv) *reinterpret_cast<float4_t *>(a.part_out + place * dv + d) = float4_t{oacc[dt][i] * inv, oacc[dt][i + 1] * inv, oacc[dt][i + 2] * inv, oacc[dt][i + 3] * inv};
+                }
+        }
         // (what is no number makes the joined row none: +inf minus itself)
-        if (g == 0) a.prefix_lse[place] = l == 0.0f ? NEG_INF_F : l == l ? m_run + __builtin_amdgcn_logf(l) : -NEG_INF_F;
+        if (g == 0) a.part_lse[place] = l == 0.0f ? NEG_INF_F : l == l ? m_run + __builtin_amdgcn_logf(l) : -NEG_INF_F;
         return;
     }
     uint16_t *const orow = static_cast<uint16_t *>(a.o) + (from + token) * a.os[1] + head * a.os[2];
@@ -363,7 +376,7 @@ template <bool BF16, int D, int DE, int NW, int KEYS> int launch_tile_as(const C
         static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(&sdpa_tile_kernel<BF16, D, DE, NW, KEYS>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         AXHIP_CHECK_HIP(attr);
     }
-    const int64_t blocks = (a.total_q * a.each / BM + a.entries) * a.kv_heads; // at most
+    const int64_t blocks = (a.total_q * a.each / BM + a.entries) * a.kv_heads * a.parts; // at most
     AXHIP_REQUIRE(launch_fits(blocks, 64 * NW), AXHIP_ERR_UNSUPPORTED, "attention of ragged sequences: grid too large");
     hipLaunchKernelGGL((sdpa_tile_kernel<BF16, D, DE, NW, KEYS>), dim3(static_cast<unsigned>(blocks)), dim3(64 * NW), lds, s, a);
     AXHIP_CHECK_HIP(hipGetLastError());

@@ -33,8 +33,8 @@ template <int BM> __device__ __forceinline__ GroupItem group_item(const CacheArg
     if (block < 0 || block > rows / BM || block * BM >= rows) return {-1, 0, 0, 0};
     return {e, block * BM, rows, from};
 }
-// Keys of a part of a prefix of n: whole tiles, prefix_parts parts at most
-__device__ __forceinline__ int prefix_chunk(const CacheArgs &a, int n) { return max(1, ((n + a.prefix_parts - 1) / a.prefix_parts + TK - 1) / TK) * TK; }
+// Keys of a part of n: whole tiles, a.parts parts at most
+__device__ __forceinline__ int part_keys(const CacheArgs &a, int n) { return max(1, ((n + a.parts - 1) / a.parts + TK - 1) / TK) * TK; }
 
 // Block `index` of all blocks of BM rows, those that walk the most tiles of keys first: a long sequence's last blocks, started last, would keep a few CUs busy
 // after all others are done.  Up to 256 entries: the number of blocks that walk c tiles or more is a sum over the entries, four to a lane, and c is searched for.

@@ -168,6 +168,26 @@ def test_pages_that_do_not_exist_and_numbers_out_of_range(dt):
     q.check(o)
 
 
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("page", [0, 16])
+@pytest.mark.parametrize("hint", [0, 1, 128, 700, 10**6])
+def test_hints_are_hints(dt, page, hint):
+    """Keys undivided and in as many parts as there may be: sequences longer and shorter than the hint says, and rows that no sequence owns."""
+    p = Problem([40, 0, 3, 150], 4, 2, 96, dt, keys=[900, 5, 0, 1500] if page else None, page=page)
+    o, kernel = p.run(max_kv=hint)
+    assert ("parts" in kernel) == (page > 0 and hint > 128)
+    p.check(o)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_every_run_gives_the_same_bits(dt):
+    p = Problem([50, 700, 3], 8, 2, 128, dt, keys=[3000, 700, 1000], page=16)
+    first = p.run(max_kv=3000)[0].clone()
+    p.check(first)
+    for _ in range(5):
+        assert torch.equal(p.run(max_kv=3000)[0], first)
+
+
 @pytest.mark.parametrize("dt", ["bf16", "f32"])
 def test_more_sequences_than_a_wavefront_has_lanes(dt):
     for n in (64, 65, 300, 1100):

@@ -72,8 +72,20 @@ def test_shared_prefixes(dt, lengths, new, heads, kv_heads, dim, page, starts, p
 @pytest.mark.parametrize("dt", ["bf16", "f32"])
 @pytest.mark.parametrize("hint", [0, 1, 10**6])
 def test_hints_are_hints(dt, hint):
-    s = Step([1500, 7, 300], 1, 8, 2, 64, 16, dt, starts=[0, 2], prefixes=[900])
-    o, _ = s.run(max_kv=hint, max_prefix=hint)
+    for starts in ([0, 2], None):
+        s = Step([1500, 7, 300], 1, 8, 2, 64, 16, dt, starts=starts, prefixes=[900] if starts else None)
+        o, kernel = s.run(max_kv=hint, max_prefix=hint)
+        assert (kernel == "whole") == (hint < 10)
+        s.check(o)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("starts,prefixes", [(None, None), ([0, 3], [100]), ([1, 3, 3, 5], [33, 40, 130])])
+@pytest.mark.parametrize("heads,kv_heads,dim,new", [(8, 2, 128, 1), (4, 4, 64, 3), (12, 1, 80, 2), (2, 2, 128, 20)])
+def test_short_sequences_undivided(dt, starts, prefixes, heads, kv_heads, dim, new):
+    s = Step([5, 0, 130, 64, 1], new, heads, kv_heads, dim, 16, dt, starts=starts, prefixes=prefixes)
+    o, kernel = s.run(max_kv=130, max_prefix=130)
+    assert kernel == "whole"
     s.check(o)
 
 
