@@ -1,24 +1,12 @@
 // Rotary positions, new tokens into the pages of a cache, and pages copied: axhip_rope, axhip_kv_append, axhip_kv_copy_pages.
 //
 // All three move every element once and compute next to nothing: the bound is HBM, and for a decoding step the launch.
-#include "common.hpp"
+#include "divisor.hpp"
 
 #include <cmath>
 
 namespace axhip {
 namespace {
-
-// n / d for n < 2^31 by one multiplication (d fixed for a launch): with m = ceil(2^(32 + s) / d), 2^s >= d, the error n / 2^(32 + s) stays
-// below 1 / d.  m - 2^32 is what is kept; (hi + n) / 2^s without an overflow since n < 2^31.
-struct Divisor {
-    uint32_t d = 1, m = 1, s = 0;
-    Divisor() = default;
-    explicit Divisor(uint32_t div) : d(div), m(0), s(0) {
-        while ((uint64_t(1) << s) < d) ++s;
-        m = static_cast<uint32_t>(((uint64_t(1) << 32) * ((uint64_t(1) << s) - d)) / d + 1);
-    }
-    __device__ __forceinline__ uint32_t of(uint32_t n) const { return (__umulhi(n, m) + n) >> s; }
-};
 
 // The angle position * turns modulo 2^64 as (cos, sin): the nearest quarter turn is taken off, which leaves |r| <= pi / 4 for the series of
 // both; the first term left out is r^11 / 11! < 1.8e-9 and r^12 / 12! < 1.2e-10.  (An angle formed in 32 bits is 0.004 radians off at

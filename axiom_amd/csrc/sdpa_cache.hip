@@ -177,6 +177,7 @@ int common_args(const char *who, CacheArgs &a, int dtype, int heads, int kv_head
     a.heads = heads;
     a.kv_heads = kv_heads;
     a.each = heads / kv_heads;
+    a.by_each = Divisor(static_cast<uint32_t>(a.each));
     a.D = head_dim;
     a.scale_log2e = static_cast<float>((scale > 0.0f ? static_cast<double>(scale) : 1.0 / std::sqrt(static_cast<double>(head_dim))) * 1.44269504088896340736);
     return AXHIP_OK;

@@ -1,6 +1,7 @@
 // Attention of sequences of different lengths over packed keys or the pages of a cache: what its kernels share.
 #pragma once
 
+#include "divisor.hpp"
 #include "sdpa.hpp"
 
 namespace axhip {
@@ -15,6 +16,7 @@ struct CacheArgs {
     void *o;
     int dtype, heads, kv_heads, each, D, entries, causal;
     float scale_log2e;
+    Divisor by_each;
     // the tokens of entry s: new_tokens of every sequence (decoding), or cu_q[s] .. cu_q[s + 1] - 1, at most total_q
     int new_tokens; // 0: by cu_q
     const int32_t *cu_q;

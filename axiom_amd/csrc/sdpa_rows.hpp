@@ -102,59 +102,60 @@ __device__ inline Share own_share(const CacheArgs &a, int index) {
 // rows (fp32); WHOLE, all keys of 16 rows, prefix and own (decoding, not divided)
 enum RowsMode { ROWS_OWN = 0, ROWS_PACKED = 1, ROWS_PREFIX = 2, ROWS_WHOLE = 3 };
 
-// 16 rows, from row0 on of `rows`, against the keys [begin, end) of a run.  slot < 0: finished here; else where the results go for the join.
+// The rows of a work-group: ROWS from row0 on of `rows`, of a sequence or a group; and the keys [begin, end) of one run of keys that it takes next.
+struct RowTile { int kvh, row0, rows; };
 struct Segment {
     KeyRun run;
-    int entry, row0, rows, begin, end, tokens, q_from; // tokens: of the entry, the last of which sees the last key; q_from: its first token, or a group's first sequence
-    int64_t slot;                                      // own parts: their place; else the part's number
-    KeyRun prefix;                                     // WHOLE: these keys first
+    int entry, begin, end, tokens, q_from; // tokens: of the entry, the last of which sees the last key (0: every row sees every key); q_from: its first token, or a group's first sequence
+    bool more;                             // the segment behind it is of the same rows: nothing is finished yet
+    int64_t slot;                          // where the results go for the join: own parts: their place; else the part's number; below 0: they are finished here
 };
 
-template <int DT, int D, bool PAD, int MODE> __device__ __forceinline__ void rows_segment(const CacheArgs &a, int kvh, const Segment &seg) {
+// Segments come from next(segment), one behind the other, until it answers false.  Their steps are one stream: while a wave works on a step, the next one's K and V are on their way and
+// the page numbers of the one behind that, whether or not they are of the same segment.
+template <int DT, int D, bool PAD, int MODE, class Next> __device__ __forceinline__ void rows_stream(const CacheArgs &a, const RowTile &tile, Next next) {
     constexpr bool F32 = DT == AXHIP_DTYPE_F32;
     constexpr int ES = F32 ? 4 : 2;
     constexpr int SUB = F32 && D > 64 ? 1 : 2, KEYS = 16 * SUB, STRIDE = KEYS * ROWS_WAVES;
     constexpr int KJ = F32 ? D / 16 : D / 32; // 16-byte pieces of a K row that a lane holds
     constexpr int NT = D / 16;                // 16 bits: output tiles, and elements of V that a lane holds of a key
     constexpr int VH = F32 ? D / 64 : (NT * 2 + 15) / 16; // 16-byte pieces of a V row that a lane holds (D = 64 in 16 bits: half of one)
+    constexpr int VW = F32 ? 4 * VH : NT / 2;             // 32-bit words of that
     static_assert(!F32 || D <= 128, "fp32 head sizes");
     extern __shared__ __attribute__((aligned(1024))) unsigned char tile_lds[];
     float *const rows_lds = reinterpret_cast<float *>(tile_lds);
     const int tid = threadIdx.x, lane = tid % WAVE, wave = __builtin_amdgcn_readfirstlane(tid / WAVE), l16 = lane % 16, g = lane / 16;
-    const int dv = a.D;
-    KeyRun run = seg.run;
-    const int entry = seg.entry, row0 = seg.row0, rows = seg.rows, tokens = seg.tokens, q_from = seg.q_from;
-    int begin = seg.begin, end = seg.end, n_keys = __builtin_amdgcn_readfirstlane(run.n);
+    const int dv = a.D, kvh = tile.kvh, row0 = tile.row0, rows = tile.rows;
 
     // ---- this lane's row
     const int row = min(row0 + l16, rows - 1);
     const bool row_ok = row0 + l16 < rows;
-    auto q_place = [&](int r) { // of the element strides
-        const int token = r / a.each, head = kvh * a.each + r % a.each;
+    const int row_token = static_cast<int>(a.by_each.of(row)), first_token = static_cast<int>(a.by_each.of(row0));
+    auto place_of = [&](const Segment &seg, int r) { // of the element strides
+        const int token = static_cast<int>(a.by_each.of(r)), head = kvh * a.each + r - token * a.each;
         struct { int64_t q, o; } at;
         if constexpr (MODE == ROWS_PACKED) {
-            at.q = (q_from + token) * a.qs[1] + head * a.qs[2];
-            at.o = (q_from + token) * a.os[1] + head * a.os[2];
+            at.q = (seg.q_from + token) * a.qs[1] + head * a.qs[2];
+            at.o = (seg.q_from + token) * a.os[1] + head * a.os[2];
         } else {
             constexpr bool OF_GROUP = MODE == ROWS_PREFIX;
-            const int seq = OF_GROUP ? q_from + token / a.new_tokens : entry, t = OF_GROUP ? token % a.new_tokens : token;
+            const int seq = OF_GROUP ? seg.q_from + token / a.new_tokens : seg.entry, t = OF_GROUP ? token % a.new_tokens : token;
             at.q = seq * a.qs[0] + t * a.qs[1] + head * a.qs[2];
             at.o = seq * a.os[0] + t * a.os[1] + head * a.os[2];
         }
         return at;
     };
-    int limit = MODE == ROWS_PREFIX || !a.causal ? end - 1 : min(end - 1, n_keys - tokens + row / a.each); // last key that this row sees
-    int least = MODE == ROWS_PREFIX || !a.causal ? end - 1 : min(end - 1, n_keys - tokens + row0 / a.each); // .. that every row of the tile sees
-
-    uint4_t qf[KJ];
-    {
-        const unsigned char *q = static_cast<const unsigned char *>(a.q) + q_place(row).q * ES;
+    struct Queries { uint4_t f[KJ]; };
+    auto queries_of = [&](const Segment &seg) __attribute__((always_inline)) {
+        Queries q;
+        const unsigned char *from = static_cast<const unsigned char *>(a.q) + place_of(seg, row).q * ES;
 #pragma unroll
         for (int j = 0; j < KJ; ++j) {
             const int d = F32 ? 16 * j + 4 * g : 32 * j + 8 * g;
-            qf[j] = row_ok && d < dv ? *reinterpret_cast<const uint4_t *>(q + d * ES) : uint4_t{0, 0, 0, 0};
+            q.f[j] = row_ok && d < dv ? *reinterpret_cast<const uint4_t *>(from + d * ES) : uint4_t{0, 0, 0, 0};
         }
-    }
+        return q;
+    };
 
     // ---- K and V from memory.  Rows behind the last key are that key again; dims behind the head size of K are zeros, of V the last ones again.
     const unsigned char *kb = static_cast<const unsigned char *>(a.k) + kvh * a.ks[2] * ES, *vb = static_cast<const unsigned char *>(a.v) + kvh * a.vs[2] * ES;
@@ -174,26 +175,27 @@ template <int DT, int D, bool PAD, int MODE> __device__ __forceinline__ void row
     }
     struct Ids { int k[SUB], v[SUB]; };
     const int mask = (1 << a.page_shift) - 1;
-    auto ids_at = [&](int at) __attribute__((always_inline)) {
+    bool bad = false, bad_next = false; // a page that does not exist, of the segment at hand and of the next one
+    uint4_t kf[SUB][KJ];
+    uint32_t vf[SUB][4][VW];
+    auto ids_at = [&](const KeyRun &run, int at) __attribute__((always_inline)) {
         Ids p;
 #pragma unroll
         for (int u = 0; u < SUB; ++u) {
-            p.k[u] = run.table ? run.table[min(at + 16 * u + l16, n_keys - 1) >> a.page_shift] : 0;
-            p.v[u] = run.table ? run.table[min(at + 16 * u + 4 * g, n_keys - 1) >> a.page_shift] : 0;
+            p.k[u] = run.table ? run.table[min(at + 16 * u + l16, run.n - 1) >> a.page_shift] : 0;
+            p.v[u] = run.table ? run.table[min(at + 16 * u + 4 * g, run.n - 1) >> a.page_shift] : 0;
         }
         return p;
     };
-    bool bad = false;
-    uint4_t kf[SUB][KJ];
-    uint32_t vf[SUB][4][F32 ? 4 * VH : NT / 2];
-    auto load = [&](int at, Ids p) __attribute__((always_inline)) {
+    auto load = [&](const KeyRun &run, int at, Ids p) __attribute__((always_inline)) { // whether all pages exist
+        bool exist = true;
 #pragma unroll
         for (int u = 0; u < SUB; ++u) {
-            const int key = min(at + 16 * u + l16, n_keys - 1), vkey = min(at + 16 * u + 4 * g, n_keys - 1);
+            const int key = min(at + 16 * u + l16, run.n - 1), vkey = min(at + 16 * u + 4 * g, run.n - 1);
             const unsigned char *k = kb, *v = vb;
             if (run.table) {
                 if (static_cast<uint32_t>(p.k[u]) >= static_cast<uint32_t>(a.n_pages) || static_cast<uint32_t>(p.v[u]) >= static_cast<uint32_t>(a.n_pages)) {
-                    bad = true;
+                    exist = false;
                     p.k[u] = p.v[u] = 0;
                 }
                 k += p.k[u] * k_page + (key & mask) * k_row;
@@ -203,13 +205,10 @@ template <int DT, int D, bool PAD, int MODE> __device__ __forceinline__ void row
                 v += (run.base + vkey) * v_row;
             }
 #pragma unroll
-            for (int j = 0; j < KJ; ++j) {
-                kf[u][j] = *reinterpret_cast<const uint4_t *>(k + k_dim[j]);
-                if (PAD && !k_in[j]) kf[u][j] = uint4_t{0, 0, 0, 0};
-            }
+            for (int j = 0; j < KJ; ++j) kf[u][j] = *reinterpret_cast<const uint4_t *>(k + k_dim[j]);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const unsigned char *vi = v + min(i, n_keys - 1 - vkey) * v_row;
+                const unsigned char *vi = v + min(i, run.n - 1 - vkey) * v_row;
                 if constexpr (!F32 && D == 64) {
                     const uint2_t t = *reinterpret_cast<const uint2_t *>(vi + v_dim[0]);
                     vf[u][i][0] = t.x;
@@ -224,47 +223,75 @@ template <int DT, int D, bool PAD, int MODE> __device__ __forceinline__ void row
                 }
             }
         }
+        return exist;
     };
 
     constexpr int NACC = F32 ? 4 * VH : NT; // fp32: tile 4 h + c holds dims 64 h + 4 (4 g + i) + c; 16 bits: tile t dims (4 g + i) NT + t
     rows_f32x4 oacc[NACC];
+    float m_run, l_run;
+    auto fresh = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int t = 0; t < NACC; ++t) oacc[t] = rows_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    float m_run = NEG_INF_F, l_run = 0.0f;
-    for (int pass = MODE == ROWS_WHOLE && seg.prefix.n > 0 ? 0 : 1; pass < 2; ++pass) {
-    if constexpr (MODE == ROWS_WHOLE) {
-        if (seg.prefix.n > 0) { // the prefix, which every row sees, then the sequence's own keys
-            run = pass == 0 ? seg.prefix : seg.run;
-            n_keys = __builtin_amdgcn_readfirstlane(run.n);
-            end = pass == 0 ? n_keys : seg.end;
-            limit = pass == 0 ? end - 1 : min(end - 1, n_keys - tokens + row / a.each);
-            least = pass == 0 ? end - 1 : min(end - 1, n_keys - tokens + row0 / a.each);
+        for (int t = 0; t < NACC; ++t) oacc[t] = rows_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        m_run = NEG_INF_F;
+        l_run = 0.0f;
+    };
+    fresh();
+
+    // The wave's steps: one in registers (loaded), one whose page numbers are on their way (wanted); below 0: none.  *_next: of the segment behind the one at hand.
+    Segment cur{}, nxt{};
+    if (!next(cur)) return;
+    bool has_next = next(nxt);
+    int loaded, wanted;
+    bool loaded_next = false, wanted_next = false;
+    auto first_of = [&](const Segment &seg) { const int at = seg.begin + KEYS * wave; return at < seg.end ? at : -1; };
+    auto behind = [&](int at, bool of_next) { // the step behind one: into `wanted`
+        wanted_next = of_next;
+        wanted = at + STRIDE < (of_next ? nxt.end : cur.end) ? at + STRIDE : -1;
+        if (wanted < 0 && !of_next) {
+            wanted_next = true;
+            wanted = has_next ? first_of(nxt) : -1;
         }
-    }
-    int at = begin + KEYS * wave;
+    };
     Ids ids{};
-    if (at < end) {
-        load(at, ids_at(at));
-        if (at + STRIDE < end) ids = ids_at(at + STRIDE);
-    }
-    while (at < end) {
+    auto want_ids = [&]() __attribute__((always_inline)) { if (wanted >= 0) ids = ids_at(wanted_next ? nxt.run : cur.run, wanted); };
+    auto load_wanted = [&]() __attribute__((always_inline)) {
+        loaded = wanted;
+        loaded_next = wanted_next;
+        if (wanted < 0) return;
+        const bool exist = load(wanted_next ? nxt.run : cur.run, wanted, ids);
+        if (wanted_next) bad_next = bad_next || !exist;
+        else bad = bad || !exist;
+        behind(loaded, loaded_next);
+        want_ids();
+    };
+    auto start = [&]() __attribute__((always_inline)) { // nothing is loaded: from the first step of this segment, or of the next one
+        wanted = first_of(cur);
+        wanted_next = wanted < 0;
+        if (wanted_next) wanted = has_next ? first_of(nxt) : -1;
+        want_ids();
+        load_wanted();
+    };
+    Queries q = queries_of(cur), q_next{};
+    start();
+    if (MODE == ROWS_OWN && has_next) q_next = queries_of(nxt);
+
+    for (;;) {
+    const int limit = cur.tokens ? min(cur.end - 1, cur.run.n - cur.tokens + row_token) : cur.end - 1;   // last key that this row sees
+    const int least = cur.tokens ? min(cur.end - 1, cur.run.n - cur.tokens + first_token) : cur.end - 1; // .. that every row of the tile sees
+    while (loaded >= 0 && !loaded_next) {
         uint4_t kc[SUB][KJ];
-        uint32_t vc[SUB][4][F32 ? 4 * VH : NT / 2];
+        uint32_t vc[SUB][4][VW];
 #pragma unroll
         for (int u = 0; u < SUB; ++u) {
 #pragma unroll
-            for (int j = 0; j < KJ; ++j) kc[u][j] = kf[u][j];
+            for (int j = 0; j < KJ; ++j) kc[u][j] = PAD && !k_in[j] ? uint4_t{0, 0, 0, 0} : kf[u][j];
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int c = 0; c < (F32 ? 4 * VH : NT / 2); ++c) vc[u][i][c] = vf[u][i][c];
+                for (int c = 0; c < VW; ++c) vc[u][i][c] = vf[u][i][c];
         }
-        const int now = at;
-        at += STRIDE;
-        if (at < end) {
-            load(at, ids);
-            if (at + STRIDE < end) ids = ids_at(at + STRIDE);
-        }
+        const int now = loaded;
+        load_wanted();
 
         rows_f32x4 s[SUB];
 #pragma unroll
@@ -275,9 +302,9 @@ template <int DT, int D, bool PAD, int MODE> __device__ __forceinline__ void row
             for (int u = 0; u < SUB; ++u) {
                 if constexpr (F32) {
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kc[u][j][c]), __uint_as_float(qf[j][c]), s[u], 0, 0, 0);
+                    for (int c = 0; c < 4; ++c) s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kc[u][j][c]), __uint_as_float(q.f[j][c]), s[u], 0, 0, 0);
                 } else {
-                    s[u] = rows_mfma<DT>(kc[u][j], qf[j], s[u]);
+                    s[u] = rows_mfma<DT>(kc[u][j], q.f[j], s[u]);
                 }
             }
         if (now + KEYS - 1 > least) {
@@ -332,8 +359,7 @@ template <int DT, int D, bool PAD, int MODE> __device__ __forceinline__ void row
         }
     }
 
-    }
-
+    if (!cur.more) {
     // ---- the four waves' states meet: [wave][row][D + 4], then maxima and denominators
     const float l_tot = across32(across16(l_run, lanes_add), lanes_add);
     float *const tops = rows_lds + ROWS_WAVES * ROWS * (D + 4), *const dens = tops + ROWS_WAVES * ROWS;
@@ -359,7 +385,7 @@ template <int DT, int D, bool PAD, int MODE> __device__ __forceinline__ void row
     }
     const int any_bad = __syncthreads_or(bad);
 
-    const bool leave = seg.slot >= 0;
+    const bool leave = cur.slot >= 0;
     for (int item = tid; item < ROWS * (D / 4); item += 64 * ROWS_WAVES) {
         const int r = item / (D / 4), d = item % (D / 4) * 4;
         if (row0 + r >= rows || d >= dv) continue;
@@ -384,13 +410,13 @@ template <int DT, int D, bool PAD, int MODE> __device__ __forceinline__ void row
             float *outs = a.part_out, *lses = a.part_lse;
             int64_t place;
             if constexpr (MODE == ROWS_PREFIX) {
-                const int64_t of = static_cast<int64_t>(q_from) * a.new_tokens * a.each + row0 + r; // sequence, token, head of the key head
+                const int64_t of = static_cast<int64_t>(cur.q_from) * a.new_tokens * a.each + row0 + r; // sequence, token, head of the key head
                 const int64_t per = static_cast<int64_t>(a.new_tokens) * a.each;
-                place = ((of / per * a.kv_heads + kvh) * per + of % per) * a.parts + seg.slot;
+                place = ((of / per * a.kv_heads + kvh) * per + of % per) * a.parts + cur.slot;
             } else if constexpr (MODE == ROWS_PACKED) {
-                place = (static_cast<int64_t>(q_from + (row0 + r) / a.each) * a.heads + kvh * a.each + (row0 + r) % a.each) * a.parts + seg.slot;
+                place = (static_cast<int64_t>(cur.q_from + (row0 + r) / a.each) * a.heads + kvh * a.each + (row0 + r) % a.each) * a.parts + cur.slot;
             } else {
-                place = (seg.slot * a.kv_heads + kvh) * rows + row0 + r;
+                place = (cur.slot * a.kv_heads + kvh) * rows + row0 + r;
                 outs = a.own_out;
                 lses = a.own_lse;
             }
@@ -398,30 +424,54 @@ template <int DT, int D, bool PAD, int MODE> __device__ __forceinline__ void row
             // (what is no number makes the joined row none: +inf minus itself)
             if (d == 0) lses[place] = den == 0.0f ? NEG_INF_F : den == den ? top + __builtin_amdgcn_logf(den) : -NEG_INF_F;
         } else {
-            unsigned char *out = static_cast<unsigned char *>(a.o) + (q_place(row0 + r).o + d) * ES;
+            unsigned char *out = static_cast<unsigned char *>(a.o) + (place_of(cur, row0 + r).o + d) * ES;
             if constexpr (F32) *reinterpret_cast<rows_f32x4 *>(out) = o;
             else *reinterpret_cast<uint2_t *>(out) = uint2_t{pack2<DT == AXHIP_DTYPE_BF16>(o[0], o[1]), pack2<DT == AXHIP_DTYPE_BF16>(o[2], o[3])};
         }
     }
+    }
+    // ---- on to the next segment
+    if (!has_next) return;
+    if (!cur.more) {
+        fresh();
+        bad = false;
+        __syncthreads(); // (the states in LDS are read)
+    }
+    bad = bad || bad_next;
+    bad_next = false;
+    cur = nxt;
+    if constexpr (MODE == ROWS_OWN) q = q_next;
+    has_next = next(nxt);
+    if (MODE == ROWS_OWN && has_next) q_next = queries_of(nxt);
+    loaded_next = false;
+    wanted_next = false;
+    if (loaded < 0) {
+        start();
+    } else if (wanted < 0) {
+        behind(loaded, false);
+        want_ids();
+    }
+    }
 }
 
 template <int DT, int D, bool PAD, int MODE> __device__ __forceinline__ void rows_body(const CacheArgs &a, int index_of_all) {
-    const int kvh = index_of_all % a.kv_heads;
+    RowTile tile{index_of_all % a.kv_heads, 0, 0};
     int rest = index_of_all / a.kv_heads;
-    Segment seg{};
-    seg.slot = -1;
     if constexpr (MODE == ROWS_OWN) {
-        seg.tokens = a.new_tokens;
-        seg.rows = a.new_tokens * a.each;
-        const int tiles = (seg.rows + ROWS - 1) / ROWS, share = rest / tiles;
-        seg.row0 = rest % tiles * ROWS;
+        tile.rows = a.new_tokens * a.each;
+        const int tiles = (tile.rows + ROWS - 1) / ROWS, share = rest / tiles;
+        tile.row0 = rest % tiles * ROWS;
         const Share s = own_share(a, share);
-        int entry = __builtin_amdgcn_readfirstlane(s.entry), entry_at = __builtin_amdgcn_readfirstlane(s.entry_at);
         const int from = __builtin_amdgcn_readfirstlane(s.from), to = __builtin_amdgcn_readfirstlane(s.to);
-        for (int at = from; at < to; ++entry) {
-            seg.run = keys_of(a, entry);
+        int entry = __builtin_amdgcn_readfirstlane(s.entry), entry_at = __builtin_amdgcn_readfirstlane(s.entry_at), at = from;
+        KeyRun ahead = at < to ? keys_of(a, entry) : KeyRun{}; // (a segment before it is needed)
+        rows_stream<DT, D, PAD, MODE>(a, tile, [&](Segment &seg) {
+            if (at >= to) return false;
+            const int n = __builtin_amdgcn_readfirstlane(ahead.n), entry_to = entry_at + units_of(n);
+            seg.run = ahead;
+            seg.run.n = n;
             seg.entry = entry;
-            const int n = __builtin_amdgcn_readfirstlane(seg.run.n), entry_to = entry_at + units_of(n);
+            seg.tokens = a.new_tokens;
             seg.begin = (at - entry_at) * UNIT;
             seg.end = min(n, (min(to, entry_to) - entry_at) * UNIT);
             const bool whole = entry_at >= from && entry_to <= to;
@@ -430,64 +480,79 @@ template <int DT, int D, bool PAD, int MODE> __device__ __forceinline__ void row
                 const int group = a.groups > 0 ? group_of(a, entry) : -1;
                 seg.slot = group >= 0 && prefix_of(a, group).n > 0 ? 2 * a.shares + entry : -1;
             }
-            if (a.parts_of && entry_at >= from && kvh == 0 && seg.row0 == 0 && threadIdx.x == 0) {
+            if (entry_at >= from && tile.kvh == 0 && tile.row0 == 0 && threadIdx.x == 0) {
                 const int last = static_cast<int>((static_cast<int64_t>(entry_to) * s.shares - 1) / s.units);
                 a.parts_of[entry] = int2_t{static_cast<int>(seg.slot), seg.slot < 0 ? 0 : last - share + 1};
             }
-            rows_segment<DT, D, PAD, MODE>(a, kvh, seg);
             at = entry_at = entry_to;
-            if (at < to) __syncthreads(); // (the states in LDS are read)
-        }
+            ++entry;
+            if (at < to) ahead = keys_of(a, entry);
+            return true;
+        });
     } else if constexpr (MODE == ROWS_WHOLE) {
-        seg.tokens = a.new_tokens;
-        seg.rows = a.new_tokens * a.each;
-        const int tiles = (seg.rows + ROWS - 1) / ROWS;
-        seg.entry = rest / tiles;
-        seg.row0 = rest % tiles * ROWS;
-        seg.run = keys_of(a, seg.entry);
-        seg.end = seg.run.n = __builtin_amdgcn_readfirstlane(seg.run.n);
-        const int group = a.groups > 0 ? group_of(a, seg.entry) : -1;
-        if (group >= 0) seg.prefix = prefix_of(a, group);
-        rows_segment<DT, D, PAD, MODE>(a, kvh, seg);
-    } else if constexpr (MODE == ROWS_PACKED) {
-        int part = 0;
-        if (a.parts > 1) {
-            part = rest % a.parts;
-            rest /= a.parts;
-        }
-        const TileItem item = tile_item<ROWS>(a, rest);
-        seg.entry = __builtin_amdgcn_readfirstlane(item.entry);
-        if (seg.entry < 0) return;
-        const TokenRun t = tokens_of(a, seg.entry);
-        seg.tokens = t.n;
-        seg.q_from = t.from;
-        seg.rows = t.n * a.each;
-        seg.row0 = __builtin_amdgcn_readfirstlane(item.block) * ROWS;
-        if (seg.row0 < 0 || seg.row0 >= seg.rows) return;
-        seg.run = keys_of(a, seg.entry);
-        seg.end = __builtin_amdgcn_readfirstlane(a.causal ? seg.run.n - t.n + (min(seg.row0 + ROWS, seg.rows) - 1) / a.each + 1 : seg.run.n);
-        if (a.parts > 1) {
-            const int chunk = part_keys(a, max(0, seg.end));
-            seg.begin = part * chunk;
-            seg.end = min(seg.end, seg.begin + chunk);
-            seg.slot = part;
-        }
-        rows_segment<DT, D, PAD, MODE>(a, kvh, seg);
+        tile.rows = a.new_tokens * a.each;
+        const int tiles = (tile.rows + ROWS - 1) / ROWS, entry = rest / tiles;
+        tile.row0 = rest % tiles * ROWS;
+        KeyRun own = keys_of(a, entry), prefix{};
+        const int group = a.groups > 0 ? group_of(a, entry) : -1;
+        if (group >= 0) prefix = prefix_of(a, group);
+        own.n = __builtin_amdgcn_readfirstlane(own.n);
+        prefix.n = __builtin_amdgcn_readfirstlane(prefix.n);
+        int count = prefix.n > 0 ? 0 : 1; // the prefix, which every row sees, then the sequence's own keys
+        rows_stream<DT, D, PAD, MODE>(a, tile, [&](Segment &seg) {
+            if (count > 1) return false;
+            const KeyRun &run = count == 0 ? prefix : own;
+            seg = Segment{run, entry, 0, run.n, count == 0 ? 0 : a.new_tokens, 0, count == 0, -1};
+            ++count;
+            return true;
+        });
     } else {
-        const int part = rest % a.parts;
-        const GroupItem item = group_item<ROWS>(a, rest / a.parts);
-        seg.entry = __builtin_amdgcn_readfirstlane(item.group);
-        if (seg.entry < 0) return;
-        seg.rows = item.rows;
-        seg.row0 = item.row0;
-        seg.q_from = item.first;
-        seg.run = prefix_of(a, seg.entry);
-        const int chunk = part_keys(a, seg.run.n);
-        seg.begin = __builtin_amdgcn_readfirstlane(part * chunk);
-        seg.end = __builtin_amdgcn_readfirstlane(min(seg.run.n, seg.begin + chunk));
-        if (seg.begin >= seg.run.n) return; // (as many parts as that are there for the join)
-        seg.slot = part;
-        rows_segment<DT, D, PAD, MODE>(a, kvh, seg);
+        Segment only{};
+        only.slot = -1;
+        if constexpr (MODE == ROWS_PACKED) {
+            int part = 0;
+            if (a.parts > 1) {
+                part = rest % a.parts;
+                rest /= a.parts;
+            }
+            const TileItem item = tile_item<ROWS>(a, rest);
+            if (item.entry < 0) return;
+            only.entry = item.entry;
+            only.tokens = a.causal ? item.tokens.n : 0;
+            only.q_from = item.tokens.from;
+            tile.rows = item.tokens.n * a.each;
+            tile.row0 = item.row0;
+            only.run = KeyRun{a.table ? a.table + item.entry * a.table_ld : nullptr, item.base, item.keys};
+            only.end = a.causal ? item.keys - item.tokens.n + static_cast<int>(a.by_each.of(min(tile.row0 + ROWS, tile.rows) - 1)) + 1 : item.keys;
+            if (a.parts > 1) {
+                const int chunk = part_keys(a, max(0, only.end));
+                only.begin = part * chunk;
+                only.end = min(only.end, only.begin + chunk);
+                only.slot = part;
+            }
+        } else {
+            const int part = rest % a.parts;
+            const GroupItem item = group_item<ROWS>(a, rest / a.parts);
+            only.entry = __builtin_amdgcn_readfirstlane(item.group);
+            if (only.entry < 0) return;
+            tile.rows = item.rows;
+            tile.row0 = item.row0;
+            only.q_from = item.first;
+            only.run = prefix_of(a, only.entry);
+            only.run.n = __builtin_amdgcn_readfirstlane(only.run.n);
+            const int chunk = part_keys(a, only.run.n);
+            only.begin = part * chunk;
+            only.end = min(only.run.n, only.begin + chunk);
+            if (only.begin >= only.run.n) return; // (as many parts as that are there for the join)
+            only.slot = part;
+        }
+        bool first = true;
+        rows_stream<DT, D, PAD, MODE>(a, tile, [&](Segment &seg) {
+            if (!first) return false;
+            seg = only;
+            first = false;
+            return true;
+        });
     }
 }
 template <int DT, int D, bool PAD, int MODE>
