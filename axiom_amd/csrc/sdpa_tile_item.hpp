@@ -36,14 +36,15 @@ template <int BM> __device__ __forceinline__ GroupItem group_item(const CacheArg
 // Keys of a part of n: whole tiles, a.parts parts at most
 __device__ __forceinline__ int part_keys(const CacheArgs &a, int n) { return max(1, ((n + a.parts - 1) / a.parts + TK - 1) / TK) * TK; }
 
-// Block `index` of all blocks of BM rows, those that walk the most tiles of keys first: a long sequence's last blocks, started last, would keep a few CUs busy
-// after all others are done.  Up to 256 entries: the number of blocks that walk c tiles or more is a sum over the entries, four to a lane, and c is searched for.
-// More: in the order of the entries.  index: uniform.  entry < 0: no such block.
+// Block `index` of all blocks of BM rows.  Up to 64 entries, one to a lane: those that walk the most tiles of keys first, since a long sequence's last blocks, started last, would keep a few CUs
+// busy after all others are done; the number of blocks that walk c tiles or more is a sum over the lanes, and c is searched for (64 chunks of 64 tokens
+// behind 300 keys: 66 us, in the entries' order 80).  More entries: in their order, since the search would take longer than it gains (200 prompts of 82 tokens: 140 us, with four entries to a lane 170).
+// index: uniform.  entry < 0: no such block.
 struct TileItem { int entry, row0; TokenRun tokens; int base, keys; }; // base: of packed keys
 template <int BM> __device__ __forceinline__ TileItem tile_item(const CacheArgs &a, int index) {
     const int lane = threadIdx.x % WAVE;
     int entry = -1, block = 0, from = 0, n = 0, base = 0, keys = 0;
-    if (a.entries > 256) {
+    if (a.entries > WAVE) {
         auto first = [&](int e) { return static_cast<int>(static_cast<int64_t>(clamped(a.cu_q[e], 0, a.total_q)) * a.each / BM + e); };
         entry = last_not_beyond(a.entries, index, first);
         block = index - first(entry);
@@ -54,68 +55,44 @@ template <int BM> __device__ __forceinline__ TileItem tile_item(const CacheArgs 
         base = static_cast<int>(k.base);
         keys = k.n;
     } else {
-        TokenRun tokens[4]; // of this lane's entries
-        int bases[4], most_keys[4], blocks[4];
-        float most = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int e = lane + WAVE * i;
-            tokens[i] = {0, 0};
-            bases[i] = most_keys[i] = blocks[i] = 0;
-            if (WAVE * i < a.entries && e < a.entries) {
-                tokens[i] = tokens_of(a, e);
-                const KeyRun k = keys_of(a, e);
-                bases[i] = static_cast<int>(k.base);
-                most_keys[i] = k.n;
-                blocks[i] = (tokens[i].n * a.each + BM - 1) / BM;
-                if (blocks[i] > 0) most = fmaxf(most, static_cast<float>((k.n + TK - 1) / TK));
-            }
+        TokenRun my_tokens{0, 0};
+        int my_base = 0, my_keys = 0, my_blocks = 0;
+        if (lane < a.entries) {
+            my_tokens = tokens_of(a, lane);
+            const KeyRun k = keys_of(a, lane);
+            my_base = static_cast<int>(k.base);
+            my_keys = k.n;
+            my_blocks = (my_tokens.n * a.each + BM - 1) / BM;
         }
-        auto with = [&](int i, int c) { // blocks of entry i that walk c tiles or more
-            if (c <= 0) return blocks[i];
-            if (most_keys[i] <= TK * (c - 1)) return 0;
-            if (!a.causal) return blocks[i];
-            const int token = TK * (c - 1) - (most_keys[i] - tokens[i].n); // the first one that sees so far
-            if (token <= 0) return blocks[i];
-            return token >= tokens[i].n ? 0 : blocks[i] - token * a.each / BM;
+        auto with = [&](int c) { // blocks of this lane's entry that walk c tiles or more
+            const int token = a.causal ? TK * (c - 1) - (my_keys - my_tokens.n) : TK * (c - 1) < my_keys ? 0 : my_tokens.n; // the first one that sees so far
+            return c <= 0 || token <= 0 ? my_blocks : token >= my_tokens.n ? 0 : my_blocks - token * a.each / BM;
         };
-        auto all_with = [&](int c) {
-            float sum = 0.0f; // (below 2^24: exact)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (WAVE * i < a.entries) sum += static_cast<float>(with(i, c));
-            return __builtin_amdgcn_readfirstlane(static_cast<int>(wave_sum(sum)));
-        };
-        int lo = 0, hi = __builtin_amdgcn_readfirstlane(static_cast<int>(wave_max(most))) + 1; // all_with(lo) > index >= all_with(hi)
+        auto all_with = [&](int c) { return __builtin_amdgcn_readfirstlane(static_cast<int>(wave_sum(static_cast<float>(with(c))))); }; // (below 2^24: exact)
+        // all_with(lo) > index >= all_with(hi)
+        int lo = 0, hi = 1 + __builtin_amdgcn_readfirstlane(static_cast<int>(wave_max(my_blocks > 0 ? static_cast<float>((my_keys + TK - 1) / TK) : 0.0f)));
         if (index >= all_with(0)) return {-1, 0, {0, 0}, 0, 0};
         while (hi - lo > 1) {
             const int mid = (lo + hi) / 2;
             if (all_with(mid) > index) lo = mid;
             else hi = mid;
         }
-        int left = index - all_with(lo + 1); // among those that walk `lo` tiles exactly
+        const int longer = with(lo + 1), mine = with(lo) - longer; // `lo` tiles exactly
+        int upto = mine;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (WAVE * i >= a.entries || entry >= 0) continue;
-            const int mine = with(i, lo) - with(i, lo + 1);
-            int upto = mine;
-#pragma unroll
-            for (int d = 1; d < WAVE; d *= 2) {
-                const int other = __shfl_up(upto, d, WAVE);
-                if (lane >= d) upto += other;
-            }
-            const uint64_t reached = __builtin_amdgcn_ballot_w64(upto > left);
-            if (reached) {
-                const int at = __builtin_ctzll(reached);
-                entry = at + WAVE * i;
-                block = __builtin_amdgcn_readlane(blocks[i] - with(i, lo) + left - (upto - mine), at);
-                from = __builtin_amdgcn_readlane(tokens[i].from, at);
-                n = __builtin_amdgcn_readlane(tokens[i].n, at);
-                base = __builtin_amdgcn_readlane(bases[i], at);
-                keys = __builtin_amdgcn_readlane(most_keys[i], at);
-            } else {
-                left -= __builtin_amdgcn_readlane(upto, WAVE - 1);
-            }
+        for (int d = 1; d < WAVE; d *= 2) {
+            const int other = __shfl_up(upto, d, WAVE);
+            if (lane >= d) upto += other;
+        }
+        const int left = index - all_with(lo + 1);
+        const uint64_t reached = __builtin_amdgcn_ballot_w64(upto > left);
+        if (reached) {
+            entry = __builtin_ctzll(reached);
+            block = __builtin_amdgcn_readlane(my_blocks - longer - upto, entry) + left;
+            from = __builtin_amdgcn_readlane(my_tokens.from, entry);
+            n = __builtin_amdgcn_readlane(my_tokens.n, entry);
+            base = __builtin_amdgcn_readlane(my_base, entry);
+            keys = __builtin_amdgcn_readlane(my_keys, entry);
         }
     }
     auto uniform = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
