@@ -316,14 +316,15 @@ CachePlan step_plan(const CacheArgs &a, int max_kv, int max_prefix) {
     const int64_t most_prefix = a.groups > 0 ? std::min(a.prefix_ld << a.page_shift, MOST_KEYS) : 0;
     // Short sequences stay whole: the join is a launch, 4 - 5 us, and a work-group walks 128 keys a microsecond
     const int64_t walk = std::min<int64_t>(std::max(max_kv, 0), most) + std::min<int64_t>(std::max(max_prefix, 0), most_prefix);
-    p.whole = walk <= 640 && (a.groups == 0 || a.entries * tiles * a.kv_heads <= 512);
+    p.whole = walk <= 640 && (a.groups == 0 || a.entries * tiles * a.kv_heads * walk <= 512 * 640);
     if (p.whole) return p;
-    // shares of the own keys: two work-groups of four waves on each CU; beside prefixes one
-    const int64_t groups = step_groups ? step_groups : a.groups > 0 ? 256 : 512;
+    // parts of a prefix: one work-group for each CU, of 128 rows, in 32 bits two of 16
+    const bool f32 = a.dtype == AXHIP_DTYPE_F32;
+    const int64_t per = f32 ? 16 : 128, blocks = (a.entries * rows + per - 1) / per * a.kv_heads;
+    p.parts = a.groups == 0 ? 0 : static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({64, (f32 ? 512 : 256) / blocks, (std::min<int64_t>(std::max(max_prefix, 1), most_prefix) + 63) / 64})));
+    // shares of the own keys: two work-groups of four waves on each CU, less what prefixes take of them in the same launch
+    const int64_t groups = step_groups ? step_groups : f32 ? 512 : std::max<int64_t>(256, 512 - blocks * p.parts);
     p.shares = static_cast<int>(std::min<int64_t>(std::max<int64_t>(1, groups / (a.kv_heads * tiles)), (most + 127) / 128 * a.entries));
-    // parts of a prefix: one work-group of 128 rows for each CU
-    const int64_t blocks = (a.entries * rows + 127) / 128 * a.kv_heads;
-    p.parts = a.groups == 0 ? 0 : static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({64, 256 / blocks, (most_prefix + 63) / 64})));
     const size_t own = (static_cast<size_t>(2 * p.shares) + (a.groups > 0 ? a.entries : 0)) * a.kv_heads * rows;
     p.bytes = CallScratch::rounded(sizeof(int2_t) * a.entries);
     auto place = [&](size_t floats) { const size_t here = p.bytes; p.bytes = CallScratch::rounded(p.bytes + floats * sizeof(float)); return here; };

@@ -122,6 +122,9 @@ template <int DT, int D, bool PAD, int MODE, class Next> __device__ __forceinlin
     constexpr int VH = F32 ? D / 64 : (NT * 2 + 15) / 16; // 16-byte pieces of a V row that a lane holds (D = 64 in 16 bits: half of one)
     constexpr int VW = F32 ? 4 * VH : NT / 2;             // 32-bit words of that
     static_assert(!F32 || D <= 128, "fp32 head sizes");
+    // Large fp32 heads: a step's K takes the place of the one whose scores are done, its V of the one whose output is (two of each, and the registers do not suffice); those products take long
+    // enough for the loads
+    constexpr bool LEAN = F32 && D > 64;
     extern __shared__ __attribute__((aligned(1024))) unsigned char tile_lds[];
     float *const rows_lds = reinterpret_cast<float *>(tile_lds);
     const int tid = threadIdx.x, lane = tid % WAVE, wave = __builtin_amdgcn_readfirstlane(tid / WAVE), l16 = lane % 16, g = lane / 16;
@@ -187,7 +190,8 @@ template <int DT, int D, bool PAD, int MODE, class Next> __device__ __forceinlin
         }
         return p;
     };
-    auto load = [&](const KeyRun &run, int at, Ids p) __attribute__((always_inline)) { // whether all pages exist
+    auto load = [&](const KeyRun &run, int at, Ids p, auto with_k, auto with_v) __attribute__((always_inline)) { // whether all pages exist
+        constexpr bool K = decltype(with_k)::value, V = decltype(with_v)::value;
         bool exist = true;
 #pragma unroll
         for (int u = 0; u < SUB; ++u) {
@@ -205,9 +209,9 @@ template <int DT, int D, bool PAD, int MODE, class Next> __device__ __forceinlin
                 v += (run.base + vkey) * v_row;
             }
 #pragma unroll
-            for (int j = 0; j < KJ; ++j) kf[u][j] = *reinterpret_cast<const uint4_t *>(k + k_dim[j]);
+            for (int j = 0; K && j < KJ; ++j) kf[u][j] = *reinterpret_cast<const uint4_t *>(k + k_dim[j]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; V && i < 4; ++i) {
                 const unsigned char *vi = v + min(i, run.n - 1 - vkey) * v_row;
                 if constexpr (!F32 && D == 64) {
                     const uint2_t t = *reinterpret_cast<const uint2_t *>(vi + v_dim[0]);
@@ -254,11 +258,14 @@ template <int DT, int D, bool PAD, int MODE, class Next> __device__ __forceinlin
     };
     Ids ids{};
     auto want_ids = [&]() __attribute__((always_inline)) { if (wanted >= 0) ids = ids_at(wanted_next ? nxt.run : cur.run, wanted); };
-    auto load_wanted = [&]() __attribute__((always_inline)) {
+    constexpr std::true_type yes{};
+    constexpr std::false_type no{};
+    auto load_wanted_k = [&]() __attribute__((always_inline)) { if (wanted >= 0) load(wanted_next ? nxt.run : cur.run, wanted, ids, yes, no); };
+    auto load_wanted = [&](auto with_k) __attribute__((always_inline)) { // .. and on to the next one
         loaded = wanted;
         loaded_next = wanted_next;
         if (wanted < 0) return;
-        const bool exist = load(wanted_next ? nxt.run : cur.run, wanted, ids);
+        const bool exist = load(wanted_next ? nxt.run : cur.run, wanted, ids, with_k, yes);
         if (wanted_next) bad_next = bad_next || !exist;
         else bad = bad || !exist;
         behind(loaded, loaded_next);
@@ -269,7 +276,7 @@ template <int DT, int D, bool PAD, int MODE, class Next> __device__ __forceinlin
         wanted_next = wanted < 0;
         if (wanted_next) wanted = has_next ? first_of(nxt) : -1;
         want_ids();
-        load_wanted();
+        load_wanted(yes);
     };
     Queries q = queries_of(cur), q_next{};
     start();
@@ -291,7 +298,7 @@ template <int DT, int D, bool PAD, int MODE, class Next> __device__ __forceinlin
                 for (int c = 0; c < VW; ++c) vc[u][i][c] = vf[u][i][c];
         }
         const int now = loaded;
-        load_wanted();
+        if constexpr (!LEAN) load_wanted(yes);
 
         rows_f32x4 s[SUB];
 #pragma unroll
@@ -307,6 +314,11 @@ template <int DT, int D, bool PAD, int MODE, class Next> __device__ __forceinlin
                     s[u] = rows_mfma<DT>(kc[u][j], q.f[j], s[u]);
                 }
             }
+        if constexpr (LEAN) {
+            __builtin_amdgcn_sched_barrier(0);
+            load_wanted_k();
+            __builtin_amdgcn_sched_barrier(0);
+        }
         if (now + KEYS - 1 > least) {
 #pragma unroll
             for (int u = 0; u < SUB; ++u)
@@ -344,6 +356,10 @@ template <int DT, int D, bool PAD, int MODE, class Next> __device__ __forceinlin
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int t = 0; t < NACC; ++t) oacc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vc[u][i][t]), p[u][i], oacc[t], 0, 0, 0);
+            if constexpr (LEAN) {
+                __builtin_amdgcn_sched_barrier(0);
+                load_wanted(no);
+            }
         } else {
             uint4_t pf; // slot 8 g + e of the second product is key 4 g + e % 4 of sub-tile e / 4
 #pragma unroll
