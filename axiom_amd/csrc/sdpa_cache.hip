@@ -292,11 +292,18 @@ const int tile_waves = [] {
     return e ? atoi(e) : 0;
 }();
 
+// AXHIP_SDPA_F32_ROWS=16|64: rows of a work-group of the fp32 kernel of prompts (measurements only)
+const int f32_rows = [] {
+    const char *e = getenv("AXHIP_SDPA_F32_ROWS");
+    return e ? atoi(e) : 0;
+}();
+
 // How a call is divided, and its temporary memory: what the parts leave for the join.  By the numbers in the arguments and the hints alone: nothing of it depends on addresses or on what the
 // device holds.
 struct CachePlan {
     int shares, parts;
     bool whole;                                         // decoding: one launch, nothing is divided
+    bool apart;                                         // fp32 prompts: 64 rows to a work-group, not 16
     size_t own_out, own_lse, part_out, part_lse, bytes; // places; all of it
 };
 void place_parts(CachePlan &p, const CacheArgs &a, size_t rows) {
@@ -318,7 +325,7 @@ CachePlan step_plan(const CacheArgs &a, int max_kv, int max_prefix) {
     const int64_t walk = std::min<int64_t>(std::max(max_kv, 0), most) + std::min<int64_t>(std::max(max_prefix, 0), most_prefix);
     p.whole = walk <= 640 && (a.groups == 0 || a.entries * tiles * a.kv_heads * walk <= 512 * 640);
     if (p.whole) return p;
-    // parts of a prefix: one work-group for each CU, of 128 rows, in 32 bits two of 16
+    // parts of a prefix: one work-group for each CU, of 128 rows, in 32 bits two
     const bool f32 = a.dtype == AXHIP_DTYPE_F32;
     const int64_t per = f32 ? 16 : 128, blocks = (a.entries * rows + per - 1) / per * a.kv_heads;
     p.parts = a.groups == 0 ? 0 : static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({64, (f32 ? 512 : 256) / blocks, (std::min<int64_t>(std::max(max_prefix, 1), most_prefix) + 63) / 64})));
@@ -350,6 +357,16 @@ CachePlan prompt_plan(const CacheArgs &a, int max_kv) {
             best = time;
             p.parts = parts;
         }
+    }
+    // fp32, nothing divided: work-groups of 16 rows whose waves take a step's keys in turn, or of 64 rows whose waves take 16 each, a quarter of the keys a step.  A work-group takes 6 us beside its
+    // steps, of 2.8 us or 3.8 with others on the CU, and the chip holds 512.  16 -> 64 rows: 64 prompts of 62 tokens, 16 heads of 64, 49 -> 25 us, 8 of 500 89 -> 67; one of 2048, 32 heads of 128, stays:
+    // 435, 494
+    if (a.dtype == AXHIP_DTYPE_F32 && p.parts == 1) {
+        auto time = [&](double count, double step_keys, double step) {
+            return 6 * std::max(1.0, count / 512) + step * std::max(longest / step_keys, count / 512 * std::max(1.0, average / step_keys));
+        };
+        const double keys = a.D <= 64 ? 128 : 64, wide = static_cast<double>(a.total_q * a.each / 64 + (a.entries + 1) / 2) * a.kv_heads;
+        p.apart = f32_rows ? f32_rows == 64 : time(wide, keys / 4, 3.8) < time(blocks, keys, 2.8);
     }
     if (p.parts > 1) place_parts(p, a, static_cast<size_t>(a.total_q) * a.heads);
     return p;
@@ -419,8 +436,8 @@ int axhip_sdpa_packed_ws(const void *q, const void *k, const void *v, void *o, c
     if (rc) return rc;
     const bool f32 = a.dtype == AXHIP_DTYPE_F32, bf16 = a.dtype == AXHIP_DTYPE_BF16;
     if (f32) {
-        last_kernel = plan.parts > 1 ? "f32, parts" : "f32";
-        rc = launch_rows_packed_f32(a, s);
+        last_kernel = plan.parts > 1 ? "f32, parts" : plan.apart ? "f32, apart" : "f32";
+        rc = launch_rows_packed_f32(a, plan.apart, s);
     } else {
         const int64_t blocks = (a.total_q * a.each + 255) / 256 * a.kv_heads;
         const int waves = tile_waves ? tile_waves : blocks >= 192 && plan.parts == 1 ? 8 : 4;

@@ -99,8 +99,9 @@ __device__ inline Share own_share(const CacheArgs &a, int index) {
 }
 
 // What a work-group does: OWN, a share of all own keys (decoding); PACKED, 16 rows of a sequence by cu_q, or a part of their keys (fp32 prompts); PREFIX, a part of a group's prefix for 16 of its
-// rows (fp32); WHOLE, all keys of 16 rows, prefix and own (decoding, not divided)
-enum RowsMode { ROWS_OWN = 0, ROWS_PACKED = 1, ROWS_PREFIX = 2, ROWS_WHOLE = 3 };
+// rows (fp32); WHOLE, all keys of 16 rows, prefix and own (decoding, not divided).  Its four waves take the keys in turn and meet at the end.  APART: as PACKED, 64 rows, 16 to a wave, each of which
+// walks all keys: where there are blocks enough, a quarter of the work-groups, whose start and end cost as much as 250 keys, and nothing to meet for.
+enum RowsMode { ROWS_OWN = 0, ROWS_PACKED = 1, ROWS_PREFIX = 2, ROWS_WHOLE = 3, ROWS_APART = 4 };
 
 // The rows of a work-group: ROWS from row0 on of `rows`, of a sequence or a group; and the keys [begin, end) of one run of keys that it takes next.
 struct RowTile { int kvh, row0, rows; };
@@ -113,15 +114,18 @@ struct Segment {
 
 // Segments come from next(segment), one behind the other, until it answers false.  Their steps are one stream: while a wave works on a step, the next one's K and V are on their way and
 // the page numbers of the one behind that, whether or not they are of the same segment.
-template <int DT, int D, bool PAD, int MODE, class Next> __device__ __forceinline__ void rows_stream(const CacheArgs &a, const RowTile &tile, Next next) {
+template <int DT, int D, bool PAD, int OF, class Next> __device__ __forceinline__ void rows_stream(const CacheArgs &a, const RowTile &tile, Next next) {
+    constexpr bool APART = OF == ROWS_APART;
+    constexpr int MODE = APART ? ROWS_PACKED : OF;
     constexpr bool F32 = DT == AXHIP_DTYPE_F32;
     constexpr int ES = F32 ? 4 : 2;
-    constexpr int SUB = F32 && D > 64 ? 1 : 2, KEYS = 16 * SUB, STRIDE = KEYS * ROWS_WAVES;
+    constexpr int SUB = F32 && D > 64 ? 1 : 2, KEYS = 16 * SUB, STRIDE = APART ? KEYS : KEYS * ROWS_WAVES;
     constexpr int KJ = F32 ? D / 16 : D / 32; // 16-byte pieces of a K row that a lane holds
     constexpr int NT = D / 16;                // 16 bits: output tiles, and elements of V that a lane holds of a key
     constexpr int VH = F32 ? D / 64 : (NT * 2 + 15) / 16; // 16-byte pieces of a V row that a lane holds (D = 64 in 16 bits: half of one)
     constexpr int VW = F32 ? 4 * VH : NT / 2;             // 32-bit words of that
     static_assert(!F32 || D <= 128, "fp32 head sizes");
+    static_assert(!APART || F32, "the results lie as 32-bit ones do");
     // Large fp32 heads: a step's K takes the place of the one whose scores are done, its V of the one whose output is (two of each, and the registers do not suffice); those products take long
     // enough for the loads
     constexpr bool LEAN = F32 && D > 64;
@@ -247,7 +251,7 @@ template <int DT, int D, bool PAD, int MODE, class Next> __device__ __forceinlin
     bool has_next = next(nxt);
     int loaded, wanted;
     bool loaded_next = false, wanted_next = false;
-    auto first_of = [&](const Segment &seg) { const int at = seg.begin + KEYS * wave; return at < seg.end ? at : -1; };
+    auto first_of = [&](const Segment &seg) { const int at = seg.begin + (APART ? 0 : KEYS * wave); return at < seg.end ? at : -1; };
     auto behind = [&](int at, bool of_next) { // the step behind one: into `wanted`
         wanted_next = of_next;
         wanted = at + STRIDE < (of_next ? nxt.end : cur.end) ? at + STRIDE : -1;
@@ -375,6 +379,22 @@ template <int DT, int D, bool PAD, int MODE, class Next> __device__ __forceinlin
         }
     }
 
+    if constexpr (APART) {
+        // ---- a lane holds 4 dims of its row in a place
+        float den = across32(across16(l_run, lanes_add), lanes_add);
+        if (__builtin_amdgcn_ballot_w64(bad)) den = __builtin_nanf("");
+        if (!row_ok) return; // (one segment)
+        const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+        float *const to = static_cast<float *>(a.o) + place_of(cur, row0 + l16).o;
+#pragma unroll
+        for (int h = 0; h < VH; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int d = 64 * h + 16 * g + 4 * i;
+                if (d < dv) *reinterpret_cast<rows_f32x4 *>(to + d) = rows_f32x4{oacc[4 * h][i], oacc[4 * h + 1][i], oacc[4 * h + 2][i], oacc[4 * h + 3][i]} * inv;
+            }
+        return;
+    }
     if (!cur.more) {
     // ---- the four waves' states meet: [wave][row][D + 4], then maxima and denominators
     const float l_tot = across32(across16(l_run, lanes_add), lanes_add);
@@ -523,21 +543,24 @@ template <int DT, int D, bool PAD, int MODE> __device__ __forceinline__ void row
             return true;
         });
     } else {
+        constexpr bool APART = MODE == ROWS_APART;
+        constexpr int BM = APART ? ROWS * ROWS_WAVES : ROWS;
+        const int to_row = APART ? __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE) * ROWS : 0; // (a wave without rows has nothing to wait for)
         Segment only{};
         only.slot = -1;
-        if constexpr (MODE == ROWS_PACKED) {
+        if constexpr (MODE == ROWS_PACKED || MODE == ROWS_APART) {
             int part = 0;
             if (a.parts > 1) {
                 part = rest % a.parts;
                 rest /= a.parts;
             }
-            const TileItem item = tile_item<ROWS>(a, rest);
-            if (item.entry < 0) return;
+            const TileItem item = tile_item<BM>(a, rest);
+            if (item.entry < 0 || item.row0 + to_row >= item.tokens.n * a.each) return;
             only.entry = item.entry;
             only.tokens = a.causal ? item.tokens.n : 0;
             only.q_from = item.tokens.from;
             tile.rows = item.tokens.n * a.each;
-            tile.row0 = item.row0;
+            tile.row0 = item.row0 + to_row;
             only.run = KeyRun{a.table ? a.table + item.entry * a.table_ld : nullptr, item.base, item.keys};
             only.end = a.causal ? item.keys - item.tokens.n + static_cast<int>(a.by_each.of(min(tile.row0 + ROWS, tile.rows) - 1)) + 1 : item.keys;
             if (a.parts > 1) {

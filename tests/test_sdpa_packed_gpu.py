@@ -210,3 +210,30 @@ def test_keys_behind_four_gigabytes():
     k, v = (x[-20:].cpu().double().flip(0).reshape(-1, heads, dim)[:313] for x in (kp, vp))
     want, around, big = ch.attention(q, k, v, 263)
     assert float(((o.cpu().double() - want).abs() - ch.attention_tolerance(want, around, big, 313, dim, "bf16")).max()) <= 0
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("heads,kv_heads,dim,page,by_head", [(16, 8, 64, 0, False), (16, 8, 40, 16, True), (32, 8, 128, 0, False), (14, 7, 100, 8, False), (24, 12, 12, 32, True)])
+def test_many_short_prompts_of_32_bits(causal, heads, kv_heads, dim, page, by_head):
+    """Each wave walks the keys of its own 16 rows (max_kv, a hint, says that there are few): sequences of less than a work-group's 64, empty ones, more keys than queries and fewer."""
+    lengths = [(13 * i) % 61 for i in range(55)] + [64, 65, 1, 0, 130]
+    keys = [n + (3 * i) % 7 - 2 if n > 2 else n for i, n in enumerate(lengths)] if page else lengths
+    p = Problem(lengths, heads, kv_heads, dim, "f32", keys=keys, page=page, by_head=by_head, seed=dim, ld=20)
+    o, kernel = p.run(causal=causal, max_kv=40)
+    assert kernel == "f32, apart"
+    p.check(o, causal)
+    first = o.clone()
+    assert torch.equal(p.run(causal=causal, max_kv=40)[0], first)
+    if page:  # what no sequence holds does not matter; a page that does not exist spoils its sequence alone
+        inside = torch.zeros(p.kp.shape[:2], dtype=torch.bool)
+        for r, n in zip(p.host_table, keys):
+            i = torch.arange(n)
+            inside[r.long()[i // page], i % page] = True
+        p.kp[~inside.cuda()] = math.nan
+        p.vp[~inside.cuda()] = math.inf
+        assert torch.equal(p.run(causal=causal, max_kv=40)[0], first)
+        p.table[55, 0] = p.kp.shape[0]  # (the one of 64)
+        o, at = p.run(causal=causal, max_kv=40)[0], p.cu_q.tolist()
+        assert torch.equal(o[:at[55]], first[:at[55]]) and torch.equal(o[at[56]:], first[at[56]:])
+        sees = torch.arange(64) + keys[55] - 64 >= 0 if causal else torch.ones(64, dtype=torch.bool)
+        assert bool(torch.isnan(o[at[55]:at[56]][sees.cuda()]).all())
