@@ -321,15 +321,16 @@ CachePlan step_plan(const CacheArgs &a, int max_kv, int max_prefix) {
     p.parts = 1;
     const int64_t rows = static_cast<int64_t>(a.new_tokens) * a.each, tiles = (rows + 15) / 16, most = std::min(a.table_ld << a.page_shift, MOST_KEYS);
     const int64_t most_prefix = a.groups > 0 ? std::min(a.prefix_ld << a.page_shift, MOST_KEYS) : 0;
-    // Short sequences stay whole: the join is a launch, 4 - 5 us, and a work-group walks 128 keys a microsecond
+    // Short sequences stay whole: the join is a launch, 4 - 5 us, and a work-group walks 128 keys in 1.1 us.  (One sequence or eight, 32 heads of 128: of 640 keys 11.5 whole, 12.3 - 13.6 in shares; of
+    // 1000 15.5 - 16.1, 12.4 - 13.5.  60 keys behind 400 of a prefix: 4 sequences 11.0 and 13.1, 256 49 and 52, the prefix being read by each.)
     const int64_t walk = std::min<int64_t>(std::max(max_kv, 0), most) + std::min<int64_t>(std::max(max_prefix, 0), most_prefix);
-    p.whole = walk <= 640 && (a.groups == 0 || a.entries * tiles * a.kv_heads * walk <= 512 * 640);
+    p.whole = walk <= 640 && (a.groups == 0 || a.entries * tiles * a.kv_heads * walk <= 3 * 512 * 640);
     if (p.whole) return p;
     // parts of a prefix: one work-group for each CU, of 128 rows, in 32 bits two
     const bool f32 = a.dtype == AXHIP_DTYPE_F32;
     const int64_t per = f32 ? 16 : 128, blocks = (a.entries * rows + per - 1) / per * a.kv_heads;
     p.parts = a.groups == 0 ? 0 : static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({64, (f32 ? 512 : 256) / blocks, (std::min<int64_t>(std::max(max_prefix, 1), most_prefix) + 63) / 64})));
-    // shares of the own keys: two work-groups of four waves on each CU, less what prefixes take of them in the same launch
+    // shares of the own keys: two work-groups of four waves on each CU (64 sequences of 2000: 256 work-groups 105 us, 512 103, 1024 105), less what prefixes take of them in the same launch
     const int64_t groups = step_groups ? step_groups : f32 ? 512 : std::max<int64_t>(256, 512 - blocks * p.parts);
     p.shares = static_cast<int>(std::min<int64_t>(std::max<int64_t>(1, groups / (a.kv_heads * tiles)), (most + 127) / 128 * a.entries));
     const size_t own = (static_cast<size_t>(2 * p.shares) + (a.groups > 0 ? a.entries : 0)) * a.kv_heads * rows;
@@ -440,8 +441,11 @@ int axhip_sdpa_packed_ws(const void *q, const void *k, const void *v, void *o, c
         rc = launch_rows_packed_f32(a, plan.apart, s);
     } else {
         const int64_t blocks = (a.total_q * a.each + 255) / 256 * a.kv_heads;
-        const int waves = tile_waves ? tile_waves : blocks >= 192 && plan.parts == 1 ? 8 : 4;
-        last_kernel = plan.parts > 1 ? "tile, parts" : "tile";
+        // Two work-groups of four waves on a CU start and end beside each other's walk; eight waves of one go in pairs of opposite phases, which long walks of 97 .. 128 dims gain by: 32 heads of
+        // 128, one prompt of 4096 136.6 -> 133.0 us, four of 512 behind 4000 keys 154.8 -> 149.0, 12 of 300 .. 5000 407 -> 399; 12 of 1365 238 either way, 64 of 256 112 -> 129; of 64 dims
+        // 12 of 1365 134 -> 165, of 96 199 -> 207.
+        const int waves = a.D <= 96 || a.D > 128 ? 4 : tile_waves ? tile_waves : blocks >= 256 && params->max_kv > 2048 && plan.parts == 1 ? 8 : 4;
+        last_kernel = plan.parts > 1 ? "tile, parts" : waves == 8 ? "tile, eight waves" : "tile";
         rc = bf16 ? launch_tile_bf16(a, waves, s) : launch_tile_f16(a, waves, s);
     }
     if (!rc && plan.parts > 1) rc = f32 ? launch_join_f32(a, s) : bf16 ? launch_join_bf16(a, s) : launch_join_f16(a, s);

@@ -237,3 +237,26 @@ def test_many_short_prompts_of_32_bits(causal, heads, kv_heads, dim, page, by_he
         assert torch.equal(o[:at[55]], first[:at[55]]) and torch.equal(o[at[56]:], first[at[56]:])
         sees = torch.arange(64) + keys[55] - 64 >= 0 if causal else torch.ones(64, dtype=torch.bool)
         assert bool(torch.isnan(o[at[55]:at[56]][sees.cuda()]).all())
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("heads,kv_heads,dim,page,by_head", [(32, 8, 128, 0, False), (32, 8, 104, 16, True), (16, 8, 128, 64, False)])
+def test_work_groups_of_eight_waves(dt, causal, heads, kv_heads, dim, page, by_head):
+    """(max_kv, a hint, says that walks are long)"""
+    lengths = [(37 * i) % 190 for i in range(40)] + [0, 63, 256, 257, 511] if heads == 32 else [(37 * i) % 190 for i in range(44)] + [1030]
+    keys = [n + (5 * i) % 90 - 20 if n > 20 else n for i, n in enumerate(lengths)] if page else lengths
+    p = Problem(lengths, heads, kv_heads, dim, dt, keys=keys, page=page, by_head=by_head, seed=dim, ld=80)
+    o, kernel = p.run(causal=causal, max_kv=4000)
+    assert kernel == "tile, eight waves"
+    p.check(o, causal)
+    first = o.clone()
+    assert torch.equal(p.run(causal=causal, max_kv=4000)[0], first)
+    if page:
+        inside = torch.zeros(p.kp.shape[:2], dtype=torch.bool)
+        for r, n in zip(p.host_table, keys):
+            i = torch.arange(n)
+            inside[r.long()[i // page], i % page] = True
+        p.kp[~inside.cuda()] = math.nan
+        p.vp[~inside.cuda()] = math.inf
+        assert torch.equal(p.run(causal=causal, max_kv=4000)[0], first)
