@@ -4,6 +4,7 @@
 #include "divisor.hpp"
 
 #include <cmath>
+#include <initializer_list>
 
 namespace axhip {
 namespace {
@@ -218,11 +219,12 @@ int launch_moves(MoveArgs &a, int dtype, bool pairs, int dim, int64_t tokens, in
     const int all = a.heads + 2 * a.kv_heads;
     // Heads of a thread: two share an angle's sines, one where that would leave the chip's 1024 SIMDs without two wavefronts each.  (8192 tokens of 48 heads of 128: two 35.2 us, four 36.4;
     // stores through the caches: one 48.7, two 48.2, four 51.2, eight 52.1.)
-    const bool many = all >= 2 && tokens * all * units >= int64_t(2) * 2 * 64 * 1024;
-    const bool stream = many && tokens * all * dim * static_cast<int64_t>(dtype_size(dtype)) >= STREAMING_OUTPUT_BYTES;
+    const double work = static_cast<double>(tokens) * all * units;
+    const bool many = all >= 2 && work >= 2.0 * 2 * 64 * 1024;
+    const bool stream = many && static_cast<double>(tokens) * all * dim * static_cast<double>(dtype_size(dtype)) >= STREAMING_OUTPUT_BYTES;
     const int per = many ? 2 : 1, groups = (all + per - 1) / per;
+    AXHIP_REQUIRE(static_cast<double>(tokens) * groups * units < 2147483648.0, AXHIP_ERR_UNSUPPORTED, "%s: %lld tokens of %d heads are too many for one launch", who, static_cast<long long>(tokens), all);
     const int64_t total = tokens * groups * units;
-    AXHIP_REQUIRE(total < (int64_t(1) << 31), AXHIP_ERR_UNSUPPORTED, "%s: %lld tokens of %d heads are too many for one launch", who, static_cast<long long>(tokens), all);
     a.units = Divisor(static_cast<uint32_t>(units));
     a.groups = Divisor(static_cast<uint32_t>(groups));
     a.total = static_cast<uint32_t>(total);
@@ -263,7 +265,15 @@ bool sane(const int64_t *strides, int n) {
         if (!sane(strides[i])) return false;
     return true;
 }
+// Rows of `dim` elements that are written: no two of them may share any, so far as two neighbours along one dimension tell
+bool apart(const int64_t *strides, std::initializer_list<int64_t> counts, int dim) {
+    for (int64_t n : counts)
+        if (*strides++ < dim && n > 1) return false;
+    return true;
+}
 bool elements_aligned(const void *p, int dtype) { return (reinterpret_cast<uintptr_t>(p) & (dtype_size(dtype) - 1)) == 0; }
+
+bool pages_apart(const AxhipKvPages &g) { return apart(g.k_strides, {g.n_pages, g.page_size, g.heads}, g.head_dim) && apart(g.v_strides, {g.n_pages, g.page_size, g.heads}, g.head_dim); }
 
 // The widest groups of elements (16 bytes at most) that every address and number given keeps whole.
 struct Width {
@@ -351,7 +361,7 @@ int axhip_rope(const void *x, void *y, const AxhipRopeParams *params, void *stre
     if (rc) return rc;
     AXHIP_REQUIRE(x && y, AXHIP_ERR_INVALID_ARG, "axhip_rope: NULL tensor");
     AXHIP_REQUIRE(elements_aligned(x, p.dtype) && elements_aligned(y, p.dtype), AXHIP_ERR_INVALID_ARG, "axhip_rope: a tensor is not aligned to its elements");
-    AXHIP_REQUIRE((p.tokens == 1 || p.y_strides[0] > 0) && (p.heads == 1 || p.y_strides[1] >= p.head_dim), AXHIP_ERR_INVALID_ARG, "axhip_rope: rows of y overlap");
+    AXHIP_REQUIRE(apart(p.y_strides, {p.tokens, p.heads}, p.head_dim), AXHIP_ERR_INVALID_ARG, "axhip_rope: rows of y overlap");
     AXHIP_REQUIRE(x != y || ((p.tokens == 1 || p.x_strides[0] == p.y_strides[0]) && (p.heads == 1 || p.x_strides[1] == p.y_strides[1])), AXHIP_ERR_INVALID_ARG,
                   "axhip_rope: in place with other strides");
     rc = ensure_init();
@@ -388,10 +398,11 @@ int axhip_kv_append(const void *q, const void *k, const void *v, void *q_out, co
                       (reinterpret_cast<uintptr_t>(p.slots) & 7u) == 0,
                   AXHIP_ERR_INVALID_ARG, "axhip_kv_append: a tensor is not aligned to its elements");
     if (p.heads > 0) {
-        AXHIP_REQUIRE((p.tokens == 1 || p.q_out_strides[0] > 0) && (p.heads == 1 || p.q_out_strides[1] >= g.head_dim), AXHIP_ERR_INVALID_ARG, "axhip_kv_append: rows of q_out overlap");
+        AXHIP_REQUIRE(apart(p.q_out_strides, {p.tokens, p.heads}, g.head_dim), AXHIP_ERR_INVALID_ARG, "axhip_kv_append: rows of q_out overlap");
         AXHIP_REQUIRE(q != q_out || ((p.tokens == 1 || p.q_strides[0] == p.q_out_strides[0]) && (p.heads == 1 || p.q_strides[1] == p.q_out_strides[1])), AXHIP_ERR_INVALID_ARG,
                       "axhip_kv_append: in place with other strides");
     }
+    AXHIP_REQUIRE(pages_apart(g), AXHIP_ERR_INVALID_ARG, "axhip_kv_append: rows of the pages overlap");
     rc = ensure_init();
     if (rc) return rc;
     MoveArgs a{};
@@ -428,6 +439,7 @@ int axhip_kv_copy_pages(const AxhipKvCopyParams *params, void *stream) {
     AXHIP_REQUIRE(p.src && p.dst, AXHIP_ERR_INVALID_ARG, "axhip_kv_copy_pages: NULL src or dst");
     AXHIP_REQUIRE(((reinterpret_cast<uintptr_t>(p.src) | reinterpret_cast<uintptr_t>(p.dst) | reinterpret_cast<uintptr_t>(p.rows)) & 3u) == 0, AXHIP_ERR_INVALID_ARG,
                   "axhip_kv_copy_pages: src, dst or rows are not aligned to their elements");
+    AXHIP_REQUIRE(pages_apart(g) && (p.layers == 1 || (p.k_layer_stride >= g.head_dim && p.v_layer_stride >= g.head_dim)), AXHIP_ERR_INVALID_ARG, "axhip_kv_copy_pages: rows of the pages overlap");
     rc = ensure_init();
     if (rc) return rc;
     CopyArgs a{};
@@ -454,9 +466,9 @@ int axhip_kv_copy_pages(const AxhipKvCopyParams *params, void *stream) {
     const int v = w.bytes(), per = static_cast<int>(dim) * es / v; // pieces of a head
     const int64_t vectors = static_cast<int64_t>(per) * g.heads * g.page_size;
     const int64_t slices = (vectors + 256 * COPY_DEEP - 1) / (256 * COPY_DEEP);
-    const int64_t blocks = slices * p.layers * 2 * p.pairs;
-    AXHIP_REQUIRE(vectors < (int64_t(1) << 31) && slices * p.layers < (int64_t(1) << 31) && p.pairs < (1 << 30) && launch_fits(blocks, 256), AXHIP_ERR_UNSUPPORTED,
+    AXHIP_REQUIRE(vectors < (int64_t(1) << 31) && slices * p.layers < (int64_t(1) << 31) && p.pairs < (1 << 30) && launch_fits(slices * p.layers * 2 * p.pairs, 256), AXHIP_ERR_UNSUPPORTED,
                   "axhip_kv_copy_pages: %d pairs of %d layers are too many for one launch", p.pairs, p.layers);
+    const int64_t blocks = slices * p.layers * 2 * p.pairs;
     a.vectors = static_cast<uint32_t>(vectors);
     a.slices = Divisor(static_cast<uint32_t>(slices));
     a.layers = Divisor(static_cast<uint32_t>(p.layers));
@@ -466,7 +478,7 @@ int axhip_kv_copy_pages(const AxhipKvCopyParams *params, void *stream) {
     const bool dense = row_major || head_major;
     const dim3 grid(static_cast<unsigned>(blocks)), block(256);
     hipStream_t s = resolve_stream(stream);
-    const bool past_caches = vectors * v * p.layers * 2 * p.pairs >= STREAMING_OUTPUT_BYTES;
+    const bool past_caches = static_cast<double>(vectors) * v * p.layers * 2 * p.pairs >= STREAMING_OUTPUT_BYTES;
 #define AXHIP_COPY(V)                                                                                              \
     do {                                                                                                           \
         if (dense && past_caches) hipLaunchKernelGGL((copy_pages_kernel<V, true, true>), grid, block, 0, s, a);         \

@@ -219,6 +219,7 @@ int packed_args(CacheArgs &a, const AxhipSdpaPackedParams *params) {
         a.os[i + 1] = p.o_strides[i];
     }
     if (p.n_seqs == 0 || p.total_q == 0) return AXHIP_OK;
+    AXHIP_REQUIRE((p.total_q == 1 || p.o_strides[0] >= p.head_dim) && (p.heads == 1 || p.o_strides[1] >= p.head_dim), AXHIP_ERR_INVALID_ARG, "axhip_sdpa_packed: rows of o overlap");
     AXHIP_REQUIRE(p.cu_q && int_aligned(p.cu_q), AXHIP_ERR_INVALID_ARG, "axhip_sdpa_packed: NULL or unaligned cu_q");
     if (p.page_table) {
         rc = page_args(who, a, p.pages, p.page_table, p.table_ld, p.kv_lengths);
@@ -257,6 +258,9 @@ int paged_args(CacheArgs &a, const AxhipSdpaPagedParams *params) {
         a.os[i] = p.o_strides[i];
     }
     if (p.n_seqs == 0) return AXHIP_OK;
+    const int64_t dim = p.pages.head_dim;
+    AXHIP_REQUIRE((p.n_seqs == 1 || p.o_strides[0] >= dim) && (p.new_tokens == 1 || p.o_strides[1] >= dim) && (p.heads == 1 || p.o_strides[2] >= dim), AXHIP_ERR_INVALID_ARG,
+                  "axhip_sdpa_paged: rows of o overlap");
     rc = page_args(who, a, p.pages, p.page_table, p.table_ld, p.kv_lengths);
     if (rc) return rc;
     if (p.n_groups > 0) {

@@ -175,3 +175,25 @@ def test_paged_more():
         refused(capi.ERR_INVALID_ARG, lib.axhip_sdpa_paged, *args, C.byref(paged_params()), None)
     refused(capi.ERR_UNSUPPORTED, lib.axhip_sdpa_paged, X, X, C.byref(changed(paged_params(), dict(pages__head_dim=264))), None)
     capi.check(lib.axhip_sdpa_paged(None, None, C.byref(changed(paged_params(), dict(n_seqs=0))), None))
+
+
+@pytest.mark.parametrize("params,change", [
+    (rope_params, dict(y_strides=(32, 64))), (append_params, dict(q_out_strides=(63, 256))), (append_params, dict(pages__k_strides=(2048, 128, 0))), (append_params, dict(pages__v_strides=(2048, 63, 64))),
+    (append_params, dict(pages__k_strides=(0, 128, 64))), (copy_params, dict(pages__k_strides=(32, 128, 64))), (copy_params, dict(pages__v_strides=(2048, 0, 64))), (copy_params, dict(k_layer_stride=0)),
+    (packed_params, dict(o_strides=(256, 32))), (packed_params, dict(o_strides=(0, 64))), (paged_params, dict(o_strides=(0, 256, 64))), (paged_params, dict(o_strides=(256, 256, 63))),
+    (paged_params, dict(new_tokens=2, o_strides=(512, 32, 64)))])
+def test_written_rows_that_overlap(params, change):
+    lib = capi.lib()
+    call = {rope_params: lambda p: lib.axhip_rope(X, 2 * X, p, None), append_params: lambda p: lib.axhip_kv_append(X, X, X, 2 * X, p, None), copy_params: lambda p: lib.axhip_kv_copy_pages(p, None),
+            packed_params: lambda p: lib.axhip_sdpa_packed(X, X, X, X, p, None), paged_params: lambda p: lib.axhip_sdpa_paged(X, X, p, None)}[params]
+    assert "overlap" in refused(capi.ERR_INVALID_ARG, call, C.byref(changed(params(), change)))
+
+
+@pytest.mark.gpu
+def test_more_than_a_launch_takes():
+    """(nothing is launched)"""
+    lib = capi.lib()
+    for tokens in (1 << 33, 1 << 61):
+        refused(capi.ERR_UNSUPPORTED, lib.axhip_rope, X, 2 * X, C.byref(changed(rope_params(), dict(tokens=tokens))), None)
+        refused(capi.ERR_UNSUPPORTED, lib.axhip_kv_append, X, X, X, 2 * X, C.byref(changed(append_params(), dict(tokens=tokens))), None)
+    refused(capi.ERR_UNSUPPORTED, lib.axhip_kv_copy_pages, C.byref(changed(copy_params(), dict(pairs=(1 << 31) - 1, layers=1 << 19))), None)
