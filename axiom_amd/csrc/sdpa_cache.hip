@@ -302,12 +302,19 @@ const int f32_rows = [] {
     return e ? atoi(e) : 0;
 }();
 
+// AXHIP_SDPA_FEW_ROWS=16|128: rows of a work-group of the 16-bit kernels of prompts (measurements only)
+const int few_rows = [] {
+    const char *e = getenv("AXHIP_SDPA_FEW_ROWS");
+    return e ? atoi(e) : 0;
+}();
+
 // How a call is divided, and its temporary memory: what the parts leave for the join.  By the numbers in the arguments and the hints alone: nothing of it depends on addresses or on what the
 // device holds.
 struct CachePlan {
     int shares, parts;
     bool whole;                                         // decoding: one launch, nothing is divided
     bool apart;                                         // fp32 prompts: 64 rows to a work-group, not 16
+    bool few;                                           // 16-bit prompts: 16 rows to a work-group, not 128
     size_t own_out, own_lse, part_out, part_lse, bytes; // places; all of it
 };
 void place_parts(CachePlan &p, const CacheArgs &a, size_t rows) {
@@ -350,9 +357,12 @@ CachePlan step_plan(const CacheArgs &a, int max_kv, int max_prefix) {
 CachePlan prompt_plan(const CacheArgs &a, int max_kv) {
     CachePlan p{};
     p.parts = 1;
-    const int rows = a.dtype == AXHIP_DTYPE_F32 ? 16 : 128;
-    const double blocks = static_cast<double>(a.total_q * a.each / rows + (a.entries + 1) / 2) * a.kv_heads, tile = a.dtype == AXHIP_DTYPE_F32 ? 0.9 : 1.1;
     const int64_t most = std::min(a.table ? a.table_ld << a.page_shift : a.total_kv, MOST_KEYS), longest = std::min<int64_t>(std::max(max_kv, 1), std::max<int64_t>(most, 1));
+    // 16 bits: 16 rows to a work-group, whose waves share the keys, where those fit the chip's 512 places and no walk is long; else tiles of 128 rows.  (128 -> 16 rows: 31 prompts of 14 tokens behind 448
+    // keys, 4 heads on 2, 18.8 -> 12.6 us; one of 1000, 8 heads of 64, 20.1 -> 13.4.  Beyond: 60 of 5 behind 600, 32 heads on 8, 34.7 -> 46.8; one of 2000, 4 heads of 64, 21.1 -> 27.6.)
+    p.few = a.dtype != AXHIP_DTYPE_F32 && (few_rows ? few_rows == 16 : (a.total_q * a.each / 16 + (a.entries + 1) / 2) * a.kv_heads <= 512 && longest <= 1280);
+    const int rows = a.dtype == AXHIP_DTYPE_F32 || p.few ? 16 : 128;
+    const double blocks = static_cast<double>(a.total_q * a.each / rows + (a.entries + 1) / 2) * a.kv_heads, tile = a.dtype == AXHIP_DTYPE_F32 ? 0.9 : p.few ? 0.55 : 1.1;
     const double tokens = static_cast<double>(std::min<int64_t>(longest, a.total_q / std::max(a.entries, 1))), average = a.causal ? static_cast<double>(longest) - tokens / 2 : static_cast<double>(longest);
     const double traffic = static_cast<double>(a.total_q) * a.heads * a.D * 8 / 4e6;
     double best = 0;
@@ -368,7 +378,7 @@ CachePlan prompt_plan(const CacheArgs &a, int max_kv) {
     // 435, 494
     if (a.dtype == AXHIP_DTYPE_F32 && p.parts == 1) {
         auto time = [&](double count, double step_keys, double step) {
-            return 6 * std::max(1.0, count / 512) + step * std::max(longest / step_keys, count / 512 * std::max(1.0, average / step_keys));
+            return 6 * std::max(1.0, count / 512) + step * std::max(std::max(1.0, longest / step_keys), count / 512 * std::max(1.0, average / step_keys));
         };
         const double keys = a.D <= 64 ? 128 : 64, wide = static_cast<double>(a.total_q * a.each / 64 + (a.entries + 1) / 2) * a.kv_heads;
         p.apart = f32_rows ? f32_rows == 64 : time(wide, keys / 4, 3.8) < time(blocks, keys, 2.8);
@@ -449,8 +459,9 @@ int axhip_sdpa_packed_ws(const void *q, const void *k, const void *v, void *o, c
         // 128, one prompt of 4096 136.6 -> 133.0 us, four of 512 behind 4000 keys 154.8 -> 149.0, 12 of 300 .. 5000 407 -> 399; 12 of 1365 238 either way, 64 of 256 112 -> 129; of 64 dims
         // 12 of 1365 134 -> 165, of 96 199 -> 207.
         const int waves = a.D <= 96 || a.D > 128 ? 4 : tile_waves ? tile_waves : blocks >= 256 && params->max_kv > 2048 && plan.parts == 1 ? 8 : 4;
-        last_kernel = plan.parts > 1 ? "tile, parts" : waves == 8 ? "tile, eight waves" : "tile";
-        rc = bf16 ? launch_tile_bf16(a, waves, s) : launch_tile_f16(a, waves, s);
+        last_kernel = plan.few ? plan.parts > 1 ? "few, parts" : "few" : plan.parts > 1 ? "tile, parts" : waves == 8 ? "tile, eight waves" : "tile";
+        if (plan.few) rc = bf16 ? launch_rows_packed_bf16(a, s) : launch_rows_packed_f16(a, s);
+        else rc = bf16 ? launch_tile_bf16(a, waves, s) : launch_tile_f16(a, waves, s);
     }
     if (!rc && plan.parts > 1) rc = f32 ? launch_join_f32(a, s) : bf16 ? launch_join_bf16(a, s) : launch_join_f16(a, s);
     return rc ? rc : scratch.release();

@@ -90,6 +90,8 @@ int launch_prefix_f32(const CacheArgs &a, hipStream_t s);
 int launch_rows_own_bf16(const CacheArgs &a, hipStream_t s);
 int launch_rows_own_f16(const CacheArgs &a, hipStream_t s);
 int launch_rows_own_f32(const CacheArgs &a, hipStream_t s);
+int launch_rows_packed_bf16(const CacheArgs &a, hipStream_t s);
+int launch_rows_packed_f16(const CacheArgs &a, hipStream_t s);
 int launch_rows_packed_f32(const CacheArgs &a, bool apart, hipStream_t s);
 // .. whole sequences, prefix and own keys one behind the other: a step that is not divided
 int launch_rows_whole_bf16(const CacheArgs &a, hipStream_t s);

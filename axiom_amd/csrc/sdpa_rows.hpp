@@ -99,7 +99,7 @@ __device__ inline Share own_share(const CacheArgs &a, int index) {
     return s;
 }
 
-// What a work-group does: OWN, a share of all own keys (decoding); PACKED, 16 rows of a sequence by cu_q, or a part of their keys (fp32 prompts); PREFIX, a part of a group's prefix for 16 of its
+// What a work-group does: OWN, a share of all own keys (decoding); PACKED, 16 rows of a sequence by cu_q, or a part of their keys (prompts of fp32, and of few rows each); PREFIX, a part of a group's prefix for 16 of its
 // rows (fp32); WHOLE, all keys of 16 rows, prefix and own (decoding, not divided).  Its four waves take the keys in turn and meet at the end.  APART: as PACKED, 64 rows, 16 to a wave, each of which
 // walks all keys: where there are blocks enough, a quarter of the work-groups, whose start and end cost as much as 250 keys, and nothing to meet for.
 enum RowsMode { ROWS_OWN = 0, ROWS_PACKED = 1, ROWS_PREFIX = 2, ROWS_WHOLE = 3, ROWS_APART = 4 };
@@ -720,6 +720,8 @@ template <int DT, int MODE> int launch_rows_mode(const CacheArgs &a, int64_t blo
 // the shares of a decoding step's own keys
 template <int DT> int launch_rows_own(const CacheArgs &a, hipStream_t s) { return launch_rows_mode<DT, ROWS_OWN>(a, own_blocks(a), s); }
 template <int DT> int launch_rows_whole(const CacheArgs &a, hipStream_t s) { return launch_rows_mode<DT, ROWS_WHOLE>(a, (static_cast<int64_t>(a.new_tokens) * a.each + ROWS - 1) / ROWS * a.kv_heads * a.entries, s); }
+// rows by cu_q, at most one block more than they need for each entry
+template <int DT> int launch_rows_packed(const CacheArgs &a, hipStream_t s) { return launch_rows_mode<DT, ROWS_PACKED>(a, (a.total_q * a.each / ROWS + a.entries) * a.kv_heads * a.parts, s); }
 template <int DT, int D, bool PACKED> void launch_join_as(const CacheArgs &a, int64_t rows, hipStream_t s) {
     // a work-group to a row where those are few (up to 128 results in the first trip), else a wavefront
     if (rows <= 1024) hipLaunchKernelGGL((sdpa_join_kernel<DT, D, 4, PACKED>), dim3(static_cast<unsigned>(rows)), dim3(256), 0, s, a);

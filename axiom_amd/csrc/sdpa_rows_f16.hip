@@ -2,5 +2,6 @@
 namespace axhip {
 int launch_rows_own_f16(const CacheArgs &a, hipStream_t s) { return launch_rows_own<AXHIP_DTYPE_F16>(a, s); }
 int launch_rows_whole_f16(const CacheArgs &a, hipStream_t s) { return launch_rows_whole<AXHIP_DTYPE_F16>(a, s); }
+int launch_rows_packed_f16(const CacheArgs &a, hipStream_t s) { return launch_rows_packed<AXHIP_DTYPE_F16>(a, s); }
 int launch_join_f16(const CacheArgs &a, hipStream_t s) { return launch_join<AXHIP_DTYPE_F16>(a, s); }
 } // namespace axhip

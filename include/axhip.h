@@ -701,8 +701,8 @@ int axhip_sdpa_paged(const void *q, void *o, const AxhipSdpaPagedParams *params_
 size_t axhip_sdpa_paged_workspace_bytes(const AxhipSdpaPagedParams *params_host);
 int axhip_sdpa_paged_ws(const void *q, void *o, const AxhipSdpaPagedParams *params_host, void *workspace, size_t workspace_bytes,
                         void *stream);
-/* diagnostic: the kernels of the calling thread's last axhip_sdpa_packed ("tile", "tile, eight waves", "tile, parts"; fp32 "f32",
- * "f32, apart", "f32, parts"; keys in parts are joined by a second launch) or axhip_sdpa_paged ("whole"; "shares", "shares, prefix":
+/* diagnostic: the kernels of the calling thread's last axhip_sdpa_packed ("tile", "tile, eight waves", "tile, parts", "few", "few, parts";
+ * fp32 "f32", "f32, apart", "f32, parts"; keys in parts are joined by a second launch) or axhip_sdpa_paged ("whole"; "shares", "shares, prefix":
  * joined alike); of either "generic" (head sizes and strides that the matrix-core kernels do not take), "empty". */
 const char *axhip_sdpa_cache_last_kernel(void);
 

@@ -261,9 +261,9 @@ def test_too_small_workspaces_are_refused():
         assert lib.axhip_sdpa_paged_ws(ch.at(step.q_out), ch.at(step.o), C.byref(step.params[0]), ptr, size, None) == capi.ERR_WORKSPACE
     ch.sync()
     assert bool((step.o == ch.LEFT).all())
-    q = torch.randn(900, 4, 64).bfloat16().cuda()
-    starts = ints([0, 900])
-    p = ch.packed_params(q, q, q, torch.empty_like(q), starts, "bf16", cu_kv=starts, max_kv=900)
+    q = torch.randn(3000, 4, 64).bfloat16().cuda()
+    starts = ints([0, 3000])
+    p = ch.packed_params(q, q, q, torch.empty_like(q), starts, "bf16", cu_kv=starts, max_kv=3000)
     need = lib.axhip_sdpa_packed_workspace_bytes(C.byref(p))
     assert need > 0
     assert lib.axhip_sdpa_packed_ws(ch.at(q), ch.at(q), ch.at(q), ch.at(torch.empty_like(q)), C.byref(p), ch.at(step.ws.bytes), need - 1, None) == capi.ERR_WORKSPACE

@@ -175,7 +175,7 @@ def test_hints_are_hints(dt, page, hint):
     """Keys undivided and in as many parts as there may be: sequences longer and shorter than the hint says, and rows that no sequence owns."""
     p = Problem([40, 0, 3, 150], 4, 2, 96, dt, keys=[900, 5, 0, 1500] if page else None, page=page)
     o, kernel = p.run(max_kv=hint)
-    assert ("parts" in kernel) == (page > 0 and hint > 128)
+    assert kernel.endswith("parts") if page and hint == 10**6 else kernel in ("f32", "few") if hint <= 128 else kernel != "generic"
     p.check(o)
 
 
@@ -260,3 +260,58 @@ def test_work_groups_of_eight_waves(dt, causal, heads, kv_heads, dim, page, by_h
         p.kp[~inside.cuda()] = math.nan
         p.vp[~inside.cuda()] = math.inf
         assert torch.equal(p.run(causal=causal, max_kv=4000)[0], first)
+
+
+MORE = [35, 64, 30, 1, 31, 32, 33] * 6  # enough blocks of rows for work-groups of 128 of them
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lengths", LENGTHS, ids=list(LENGTHS))
+@pytest.mark.parametrize("heads,kv_heads,dim", [(32, 16, 64), (16, 16, 128), (30, 15, 80), (16, 16, 24), (17, 17, 200)])
+def test_prompts_on_tiles(dt, causal, lengths, heads, kv_heads, dim):
+    p = Problem(LENGTHS[lengths] + MORE, heads, kv_heads, dim, dt, seed=dim)
+    o, kernel = p.run(causal=causal)
+    assert kernel == "tile"
+    p.check(o, causal)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("heads,kv_heads,dim,page,by_head", [(32, 16, 64, 16, False), (16, 16, 128, 8, True), (16, 16, 96, 32, False), (17, 17, 40, 128, True), (32, 16, 256, 16, False)])
+def test_chunks_over_pages_on_tiles(dt, causal, heads, kv_heads, dim, page, by_head):
+    """Queries behind what the cache holds, fewer keys than queries, nothing of either; what lies outside does not matter, and a page that does not exist spoils its sequence alone."""
+    lengths = [17, 64, 0, 5, 130, 1, 33] + MORE
+    keys = [300, 64, 40, 3, 141, 90, 0] + [n + (7 * i) % 60 for i, n in enumerate(MORE)]
+    p = Problem(lengths, heads, kv_heads, dim, dt, keys=keys, page=page, by_head=by_head, seed=dim, ld=50)
+    o, kernel = p.run(causal=causal)
+    assert kernel == "tile"
+    p.check(o, causal)
+    first = o.clone()
+    inside = torch.zeros(p.kp.shape[:2], dtype=torch.bool)
+    for r, n in zip(p.host_table, keys):
+        i = torch.arange(n)
+        inside[r.long()[i // page], i % page] = True
+    p.kp[~inside.cuda()] = math.nan
+    p.vp[~inside.cuda()] = math.inf
+    assert torch.equal(p.run(causal=causal)[0], first)
+    p.table[4, 0] = -1
+    o, at = p.run(causal=causal)[0], p.cu_q.tolist()
+    assert torch.equal(o[:at[4]], first[:at[4]]) and torch.equal(o[at[5]:], first[at[5]:]) and bool(torch.isnan(o[at[4]:at[5]]).all())
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("heads,kv_heads,dim,page", [(8, 2, 128, 16), (4, 4, 64, 0), (12, 2, 80, 32), (2, 1, 256, 8), (8, 8, 40, 0)])
+def test_few_rows(dt, causal, heads, kv_heads, dim, page):
+    lengths = [17, 64, 0, 5, 130, 1, 33]
+    keys = [300, 64, 40, 3, 641, 90, 0] if page else lengths
+    p = Problem(lengths, heads, kv_heads, dim, dt, keys=keys, page=page, seed=dim)
+    o, kernel = p.run(causal=causal, max_kv=641)
+    assert kernel == "few"
+    p.check(o, causal)
+    if page:  # divided: one long sequence beside short ones
+        q = Problem([3, 1, 20], heads, kv_heads, dim, dt, keys=[1200, 1000, 20], page=page, seed=dim + 1)
+        o, kernel = q.run(causal=causal, max_kv=1200)
+        assert kernel == "few, parts"
+        q.check(o, causal)
