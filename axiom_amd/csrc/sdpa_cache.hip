@@ -283,12 +283,12 @@ bool form_for_matrix_cores(const CacheArgs &a) {
     const int64_t rows = (a.new_tokens ? static_cast<int64_t>(a.entries) * a.new_tokens : a.total_q) * a.each;
     return rows + int64_t(256) * a.entries < (int64_t(1) << (es == 4 ? 27 : 30));
 }
-// .. and rows can be moved 16 bytes at a time (and offsets inside a piece of 8 rows are 32-bit ones)
+// .. and rows can be moved 16 bytes at a time (and offsets inside a piece of 8 rows are 32-bit ones, and from one page to the next)
 bool for_matrix_cores(const CacheArgs &a) {
     const int es = static_cast<int>(dtype_size(a.dtype));
     uint64_t seen = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) | reinterpret_cast<uintptr_t>(a.o);
     for (int i = 0; i < 3; ++i) seen |= static_cast<uint64_t>(a.qs[i] | a.ks[i] | a.vs[i] | a.os[i]) * es;
-    return form_for_matrix_cores(a) && (seen & 15) == 0 && a.ks[1] < (1 << 26) && a.vs[1] < (1 << 26);
+    return form_for_matrix_cores(a) && (seen & 15) == 0 && a.ks[1] < (1 << 26) && a.vs[1] < (1 << 26) && std::max(a.ks[0], a.vs[0]) * es < (int64_t(1) << 32);
 }
 // AXHIP_SDPA_TILE_WAVES=4|8: waves of a work-group of the tile kernel (measurements only)
 const int tile_waves = [] {
@@ -456,7 +456,7 @@ int axhip_sdpa_packed_ws(const void *q, const void *k, const void *v, void *o, c
     } else {
         const int64_t blocks = (a.total_q * a.each + 255) / 256 * a.kv_heads;
         // Two work-groups of four waves on a CU start and end beside each other's walk; eight waves of one go in pairs of opposite phases, which long walks of 97 .. 128 dims gain by: 32 heads of
-        // 128, one prompt of 4096 136.6 -> 133.0 us, four of 512 behind 4000 keys 154.8 -> 149.0, 12 of 300 .. 5000 407 -> 399; 12 of 1365 238 either way, 64 of 256 112 -> 129; of 64 dims
+        // 128, one prompt of 4096 136.6 -> 133.0 us, four of 512 behind 4000 keys 148.5 -> 144.8, 12 of 300 .. 5000 407 -> 399; 12 of 1365 238 either way, 64 of 256 112 -> 129; of 64 dims
         // 12 of 1365 134 -> 165, of 96 199 -> 207.
         const int waves = a.D <= 96 || a.D > 128 ? 4 : tile_waves ? tile_waves : blocks >= 256 && params->max_kv > 2048 && plan.parts == 1 ? 8 : 4;
         last_kernel = plan.few ? plan.parts > 1 ? "few, parts" : "few" : plan.parts > 1 ? "tile, parts" : waves == 8 ? "tile, eight waves" : "tile";

@@ -11,8 +11,8 @@
 //
 // What the ragged form asks for:
 //  * rows are tokens times the heads that share a key head: one tile of keys serves them all, and a short sequence fills the work-group.
-//  * a piece of a tile that one load instruction fetches (2 to 8 rows) lies in one page, so that its address is wave-uniform: a scalar load of the page's number
-//    a step ahead and scalar arithmetic, no vector instruction a piece.  Only the piece with the last key has lanes to aim elsewhere (at that key: what lies behind it is not read).
+//  * a piece of a tile that one load instruction fetches (2 to 8 rows) lies in one page, so that its address is wave-uniform: the pages' numbers are asked for a step ahead, one to a lane, and
+//    the addresses formed there.  Only the piece with the last key has lanes to aim elsewhere (at that key: what lies behind it is not read).
 //  * work-groups find their rows in the lengths on the device, longest walks first (see tile_item).
 //  * scores are scaled in fp32, in the FMA that subtracts the maximum: q rounded after its scaling, which would save nothing here, adds as much error as the output's rounding does.
 #pragma once
@@ -24,7 +24,6 @@
 namespace axhip {
 
 typedef int tile_int4_t __attribute__((ext_vector_type(4)));
-typedef const __attribute__((address_space(4))) int32_t *scalar_ints; // read by scalar loads
 
 template <bool BF16> __device__ __forceinline__ float16_t tile_mfma(uint4_t a, uint4_t b, float16_t c) {
     if constexpr (BF16) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
@@ -36,9 +35,10 @@ __device__ __forceinline__ uint2_t tile_transposed(const unsigned char *p) {
     typedef __attribute__((address_space(3))) short4_t lds_short4_t;
     return __builtin_bit_cast(uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_t *)(p)));
 }
-// 16 bytes a lane from base + offset straight into LDS: lane i's land at lds_base + 16 i; a lane that is switched off leaves its place as it is
+// 16 bytes a lane from base + offset straight into LDS: lane i's land at lds_base + 16 i; a lane that is switched off leaves its place as it is.  (Five states between a vector instruction that
+// writes the base's registers, such as the reading of a lane, and the load that reads them, which the compiler does not see to here; one behind M0.)
 __device__ __forceinline__ void tile_fetch(uint64_t base_uniform, uint32_t offset, uint32_t lds_base_uniform) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_base_uniform), "v"(offset), "s"(base_uniform) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_base_uniform), "v"(offset), "s"(base_uniform) : "memory");
 }
 // XOR of the 16-byte chunk's place in a row, so that neither 16 rows of one chunk nor the 4 rows of a transposing read meet on a bank
 template <int D> __device__ __forceinline__ int tile_swizzle_k(int row) { return D >= 128 ? (((row & 3) << 2) | ((row >> 2) & 3)) : ((row >> 1) & 7); }
@@ -128,7 +128,6 @@ __device__ __forceinline__ void tile_body(const CacheArgs &a, int index_of_all) 
     // ---- memory -> LDS
     const uint64_t k_base = uniform64(reinterpret_cast<uint64_t>(a.k) + static_cast<uint64_t>(kvh * a.ks[2]) * 2), v_base = uniform64(reinterpret_cast<uint64_t>(a.v) + static_cast<uint64_t>(kvh * a.vs[2]) * 2);
     const uint32_t k_row = static_cast<uint32_t>(a.ks[1]) * 2, v_row = static_cast<uint32_t>(a.vs[1]) * 2;
-    const scalar_ints table = (scalar_ints)(uniform64(reinterpret_cast<uint64_t>(run.table)));
     const int my = lane / CHUNKS; // row of a piece
     uint32_t k_off[NV], v_off[NV];
     int k_chunk[NV], v_chunk[NV];
@@ -144,36 +143,38 @@ __device__ __forceinline__ void tile_body(const CacheArgs &a, int index_of_all) 
     const uint32_t lds_wave = __builtin_amdgcn_readfirstlane(lds_base + RPL * wave * ROWB);
     const int last_piece = (nk - 1) / RPL * RPL;
     bool bad = false;
-    auto piece_of = [&](int tile, int n) { return min(begin + tile * TK + RPL * NW * n + RPL * wave, last_piece); };
-    struct Pages { int id[NLOAD]; };
-    auto pages_at = [&](int tile) { // the pages of this wave's pieces of a tile
-        Pages p;
-#pragma unroll
-        for (int n = 0; n < NLOAD; ++n) p.id[n] = PAGED ? table[piece_of(tile, n) >> a.page_shift] : 0;
-        return p;
-    };
-    auto fetch = [&](uint64_t base, const int64_t (&strides)[3], uint32_t row_bytes, const uint32_t (&off)[NV], const int (&chunk)[NV], int tile, const Pages &p, uint32_t to) __attribute__((always_inline)) {
-#pragma unroll
-        for (int n = 0; n < NLOAD; ++n) {
-            const int piece = piece_of(tile, n);
-            int64_t at;
-            if constexpr (PAGED) {
-                int id = p.id[n];
-                if (static_cast<uint32_t>(id) >= static_cast<uint32_t>(a.n_pages)) {
-                    bad = true;
-                    id = 0;
-                }
-                at = id * strides[0] * 2 + static_cast<int64_t>(piece & ((1 << a.page_shift) - 1)) * row_bytes;
-            } else {
-                at = (run.base + piece) * static_cast<int64_t>(row_bytes);
+    // lane n (modulo NLOAD) has the page of this wave's piece n, and forms its address; the wave takes them from there.  (One scalar instruction after the other for each piece, 20 of them, took a
+    // third of a tile's time with four waves.)
+    const int my_piece = RPL * wave + RPL * NW * (lane % NLOAD);
+    auto page_at = [&](int tile) { return PAGED ? run.table[min(begin + tile * TK + my_piece, last_piece) >> a.page_shift] : 0; };
+    auto fetch = [&](uint64_t base, int64_t page_elements, uint32_t row_bytes, const uint32_t (&off)[NV], const int (&chunk)[NV], int tile, int page, uint32_t to) __attribute__((always_inline)) {
+        uint64_t mine = 0;
+        if constexpr (PAGED) {
+            uint32_t id = static_cast<uint32_t>(page);
+            if (id >= static_cast<uint32_t>(a.n_pages)) {
+                bad = true;
+                id = 0;
             }
-            uint32_t offset = off[n % NV];
-            if (piece == last_piece) offset -= (my - min(my, nk - 1 - last_piece)) * row_bytes;
-            if (chunk[n % NV] * 8 < dv) tile_fetch(uniform64(base + static_cast<uint64_t>(at)), offset, to + n * RPL * NW * ROWB);
+            const uint32_t row_in = static_cast<uint32_t>(min(begin + tile * TK + my_piece, last_piece) & ((1 << a.page_shift) - 1));
+            mine = base + static_cast<uint64_t>(id) * static_cast<uint32_t>(page_elements * 2) + static_cast<uint64_t>(row_in) * row_bytes;
         }
+        auto pieces = [&](auto all_rows) __attribute__((always_inline)) {
+#pragma unroll
+            for (int n = 0; n < NLOAD; ++n) {
+                const int piece = all_rows ? begin + tile * TK + RPL * NW * n + RPL * wave : min(begin + tile * TK + RPL * NW * n + RPL * wave, last_piece);
+                uint64_t at;
+                if constexpr (PAGED) at = (static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(mine >> 32), n))) << 32) | static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(mine), n));
+                else at = uniform64(base + static_cast<uint64_t>((run.base + piece) * static_cast<int64_t>(row_bytes)));
+                uint32_t offset = off[n % NV];
+                if (!all_rows && piece == last_piece) offset -= (my - min(my, nk - 1 - last_piece)) * row_bytes;
+                if (chunk[n % NV] * 8 < dv) tile_fetch(at, offset, to + n * RPL * NW * ROWB);
+            }
+        };
+        if (begin + tile * TK + TK <= last_piece) pieces(std::true_type{});
+        else pieces(std::false_type{});
     };
-    auto load_k = [&](int tile, int buf, const Pages &p) __attribute__((always_inline)) { fetch(k_base, a.ks, k_row, k_off, k_chunk, tile, p, lds_wave + buf * TILEB); };
-    auto load_v = [&](int tile, int buf, const Pages &p) __attribute__((always_inline)) { fetch(v_base, a.vs, v_row, v_off, v_chunk, tile, p, lds_wave + (2 + buf) * TILEB); };
+    auto load_k = [&](int tile, int buf, int page) __attribute__((always_inline)) { fetch(k_base, a.ks[0], k_row, k_off, k_chunk, tile, page, lds_wave + buf * TILEB); };
+    auto load_v = [&](int tile, int buf, int page) __attribute__((always_inline)) { fetch(v_base, a.vs[0], v_row, v_off, v_chunk, tile, page, lds_wave + (2 + buf) * TILEB); };
 
     // ---- LDS fragments (bytes)
     int k_at[KT]; // row ql (+ 32), chunk 2 t + g
@@ -278,12 +279,12 @@ __device__ __forceinline__ void tile_body(const CacheArgs &a, int index_of_all) 
     };
 
     if (ntiles > 0) {
-        Pages here = pages_at(0), next = pages_at(1); // of the tile that V is fetched of next, of the one that K is
+        int here = page_at(0), next = page_at(1); // of the tile that V is fetched of next, of the one that K is
         load_k(0, 0, here);
         load_v(0, 0, here);
         if (ntiles > 1) load_k(1, 1, next);
         here = next;
-        next = pages_at(2);
+        next = page_at(2);
         landed();
         barrier();
 #pragma unroll
@@ -304,7 +305,7 @@ __device__ __forceinline__ void tile_body(const CacheArgs &a, int index_of_all) 
             if (j + 2 < ntiles) load_k(j + 2, PAR, next);
             if (j + 1 < ntiles) load_v(j + 1, 1 - PAR, here);
             here = next;
-            next = pages_at(j + 3);
+            next = page_at(j + 3);
             if (second && active(j)) softmax_phase(j);
             if (active(j)) matrix_phase(tile_lds + (1 - PAR) * TILEB, tile_lds + (2 + PAR) * TILEB);
             if (!second && j + 1 < ntiles && active(j + 1)) softmax_phase(j + 1);
@@ -320,7 +321,8 @@ __device__ __forceinline__ void tile_body(const CacheArgs &a, int index_of_all) 
     if constexpr (PAGED) { // a page that does not exist, seen by any wave
         __syncthreads();
         uint32_t *flags = reinterpret_cast<uint32_t *>(tile_lds);
-        if (lane == 0) flags[wave] = bad;
+        const bool wave_bad = __builtin_amdgcn_ballot_w64(bad) != 0;
+        if (lane == 0) flags[wave] = wave_bad;
         __syncthreads();
         uint32_t any = 0;
 #pragma unroll

@@ -648,7 +648,7 @@ int axhip_kv_copy_pages(const AxhipKvCopyParams *params_host, void *stream);
  * Numbers in cu_q, cu_kv and kv_lengths that lie outside the tensors are clamped to them (total_q and total_kv below 2^30, keys of a
  * sequence up to 2^30); a page that does not exist makes NaN of every query that sees a key of it (of others of its sequence too, at times).
  * o may not overlap the inputs.  max_kv: about how many keys the longest sequence has, which the division of the work goes by and nothing else.
- * 16 bits with head_dim a multiple of 8 up to 256 and pages of 8 rows or more, 16-byte aligned, on the matrix cores; fp32 with head_dim a multiple of 4 up to 128
+ * 16 bits with head_dim a multiple of 8 up to 256 and pages of 8 rows or more, 16-byte aligned, less than 4 GiB apart, on the matrix cores; fp32 with head_dim a multiple of 4 up to 128
  * likewise; everything else up to 256 dims on the generic kernel. */
 typedef struct {
     int32_t dtype;

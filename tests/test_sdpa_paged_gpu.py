@@ -181,3 +181,22 @@ def test_keys_behind_four_gigabytes():
     want, around, big = ch.attention(q[0], torch.cat((k[:313], k[:77])), torch.cat((v[:313], v[:77])), None)
     o, _ = ch.paged(q, kp, vp, table.cuda(), ints([77]), "bf16", starts=ints([0, 1]), prefix_table=table.cuda(), prefix_lengths=ints([313]))
     assert float(((o[0].cpu().double() - want).abs() - ch.attention_tolerance(want, around, big, 390, dim, "bf16")).max()) <= 0
+
+
+def test_pages_four_gigabytes_apart():
+    """(offsets from one page to the next beyond 32 bits: the generic kernel)"""
+    page, heads, dim, apart = 16, 2, 64, (1 << 31) + 64
+    pools = [torch.empty(apart + page * heads * dim, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    kp, vp = (p.as_strided((2, page, heads, dim), (apart, heads * dim, dim, 1)) for p in pools)
+    for i, p in enumerate((kp, vp)):
+        p.copy_(torch.randn(2, page, heads, dim, generator=ch.generator(i)).bfloat16())
+    table = torch.tensor([[1, 0]], dtype=torch.int32)
+    q = torch.randn(1, 2, 4, dim, generator=ch.generator(5)).bfloat16().cuda()
+    k, v = (p.cpu().double().flip(0).reshape(-1, heads, dim)[:27] for p in (kp, vp))
+    want, around, big = ch.attention(q[0], k, v, 25)
+    o, kernel = ch.paged(q, kp, vp, table.cuda(), ints([27]), "bf16")
+    assert kernel == "generic"
+    o2, kernel = ch.packed(q[0], None, None, ints([0, 2]), "bf16", kp=kp, vp=vp, table=table.cuda(), lengths=ints([27]))
+    assert kernel == "generic"
+    for x in (o[0], o2):
+        assert float(((x.cpu().double() - want).abs() - ch.attention_tolerance(want, around, big, 27, dim, "bf16")).max()) <= 0
