@@ -352,17 +352,20 @@ CachePlan step_plan(const CacheArgs &a, int max_kv, int max_prefix) {
     place_parts(p, a, static_cast<size_t>(a.entries) * a.kv_heads * rows);
     return p;
 }
-// Prompts: the keys of a block of rows in parts where there are few blocks for the chip, or a few that are long.  In tiles of 64 keys at 1.1 us (16 rows of fp32: 0.9), the time is that of the
-// longest walk or of all walks over the 512 work-groups that the chip holds, and with parts the join's: a launch and one write and one read of the partial results.
+// Prompts: the keys of a block of rows in parts where there are few blocks for the chip, or a few that are long.  In tiles of 64 keys at 1.5 us (16 rows of 16 bits: 0.55, of fp32: 0.9), the time is
+// that of the longest walk or of all walks over the 512 work-groups that the chip holds, and with parts the join's: a launch and one write and one read of the partial results.  (Three of 333 tokens
+// behind 1500 keys, 16 heads on 4: undivided 45.8 us, in two parts 44.6, in three 39.2, in four 49.7.)
 CachePlan prompt_plan(const CacheArgs &a, int max_kv) {
     CachePlan p{};
     p.parts = 1;
     const int64_t most = std::min(a.table ? a.table_ld << a.page_shift : a.total_kv, MOST_KEYS), longest = std::min<int64_t>(std::max(max_kv, 1), std::max<int64_t>(most, 1));
-    // 16 bits: 16 rows to a work-group, whose waves share the keys, where those fit the chip's 512 places and no walk is long; else tiles of 128 rows.  (128 -> 16 rows: 31 prompts of 14 tokens behind 448
-    // keys, 4 heads on 2, 18.8 -> 12.6 us; one of 1000, 8 heads of 64, 20.1 -> 13.4.  Beyond: 60 of 5 behind 600, 32 heads on 8, 34.7 -> 46.8; one of 2000, 4 heads of 64, 21.1 -> 27.6.)
-    p.few = a.dtype != AXHIP_DTYPE_F32 && (few_rows ? few_rows == 16 : (a.total_q * a.each / 16 + (a.entries + 1) / 2) * a.kv_heads <= 512 && longest <= 1280);
+    // 16 bits: 16 rows to a work-group, whose waves share the keys, where those fit the chip's 512 places and no walk is long (or no entry has more than those 16 rows, on average); else tiles of 128
+    // rows.  (128 -> 16 rows: 31 prompts of 14 tokens behind 448 keys, 4 heads on 2, 18.8 -> 12.6 us; one of 1000, 8 heads of 64, 20.1 -> 13.4; 16 of 4 behind 2000, 32 heads on 8, 47.0 -> 40.2.
+    // Beyond: 60 of 5 behind 600, 32 heads on 8, 34.7 -> 46.8; one of 2000, 4 heads of 64, 21.1 -> 27.6.)
+    const bool fit = (a.total_q * a.each / 16 + (a.entries + 1) / 2) * a.kv_heads <= 512, short_ones = longest <= 1280 || a.total_q * a.each <= int64_t(16) * a.entries;
+    p.few = a.dtype != AXHIP_DTYPE_F32 && (few_rows ? few_rows == 16 : fit && short_ones);
     const int rows = a.dtype == AXHIP_DTYPE_F32 || p.few ? 16 : 128;
-    const double blocks = static_cast<double>(a.total_q * a.each / rows + (a.entries + 1) / 2) * a.kv_heads, tile = a.dtype == AXHIP_DTYPE_F32 ? 0.9 : p.few ? 0.55 : 1.1;
+    const double blocks = static_cast<double>(a.total_q * a.each / rows + (a.entries + 1) / 2) * a.kv_heads, tile = a.dtype == AXHIP_DTYPE_F32 ? 0.9 : p.few ? 0.55 : 1.5;
     const double tokens = static_cast<double>(std::min<int64_t>(longest, a.total_q / std::max(a.entries, 1))), average = a.causal ? static_cast<double>(longest) - tokens / 2 : static_cast<double>(longest);
     const double traffic = static_cast<double>(a.total_q) * a.heads * a.D * 8 / 4e6;
     double best = 0;

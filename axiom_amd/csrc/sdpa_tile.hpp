@@ -158,13 +158,14 @@ __device__ __forceinline__ void tile_body(const CacheArgs &a, int index_of_all) 
             const uint32_t row_in = static_cast<uint32_t>(min(begin + tile * TK + my_piece, last_piece) & ((1 << a.page_shift) - 1));
             mine = base + static_cast<uint64_t>(id) * static_cast<uint32_t>(page_elements * 2) + static_cast<uint64_t>(row_in) * row_bytes;
         }
+        const uint64_t first = PAGED ? 0 : uniform64(base + static_cast<uint64_t>((run.base + begin + tile * TK + RPL * wave) * static_cast<int64_t>(row_bytes)));
         auto pieces = [&](auto all_rows) __attribute__((always_inline)) {
 #pragma unroll
             for (int n = 0; n < NLOAD; ++n) {
                 const int piece = all_rows ? begin + tile * TK + RPL * NW * n + RPL * wave : min(begin + tile * TK + RPL * NW * n + RPL * wave, last_piece);
                 uint64_t at;
                 if constexpr (PAGED) at = (static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(mine >> 32), n))) << 32) | static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(mine), n));
-                else at = uniform64(base + static_cast<uint64_t>((run.base + piece) * static_cast<int64_t>(row_bytes)));
+                else at = first + static_cast<uint64_t>(static_cast<int64_t>(piece - (begin + tile * TK + RPL * wave)) * row_bytes);
                 uint32_t offset = off[n % NV];
                 if (!all_rows && piece == last_piece) offset -= (my - min(my, nk - 1 - last_piece)) * row_bytes;
                 if (chunk[n % NV] * 8 < dv) tile_fetch(at, offset, to + n * RPL * NW * ROWB);
