@@ -288,7 +288,8 @@ bool for_matrix_cores(const CacheArgs &a) {
     const int es = static_cast<int>(dtype_size(a.dtype));
     uint64_t seen = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) | reinterpret_cast<uintptr_t>(a.o);
     for (int i = 0; i < 3; ++i) seen |= static_cast<uint64_t>(a.qs[i] | a.ks[i] | a.vs[i] | a.os[i]) * es;
-    return form_for_matrix_cores(a) && (seen & 15) == 0 && a.ks[1] < (1 << 26) && a.vs[1] < (1 << 26) && std::max(a.ks[0], a.vs[0]) * es < (int64_t(1) << 32);
+    // (page 0 is read in the place of pages that do not exist)
+    return form_for_matrix_cores(a) && (!a.table || a.n_pages > 0) && (seen & 15) == 0 && a.ks[1] < (1 << 26) && a.vs[1] < (1 << 26) && std::max(a.ks[0], a.vs[0]) * es < (int64_t(1) << 32);
 }
 // AXHIP_SDPA_TILE_WAVES=4|8: waves of a work-group of the tile kernel (measurements only)
 const int tile_waves = [] {

@@ -200,3 +200,19 @@ def test_pages_four_gigabytes_apart():
     assert kernel == "generic"
     for x in (o[0], o2):
         assert float(((x.cpu().double() - want).abs() - ch.attention_tolerance(want, around, big, 27, dim, "bf16")).max()) <= 0
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("starts,prefixes", [(None, None), ([0, 2], [5])])
+def test_a_cache_without_pages(dt, starts, prefixes):
+    """Every page is one that does not exist: sequences with keys are not numbers, those without are zeros."""
+    none = torch.empty(0, 16, 2, 64, dtype=ch.DTYPES[dt][1], device="cuda")
+    q = torch.randn(4, 1, 8, 64, generator=ch.generator(3)).to(none.dtype).cuda()
+    table, lens = torch.zeros(4, 200, dtype=torch.int32, device="cuda"), ints([300, 0, 1, 0])
+    how = dict(starts=ints(starts), prefix_table=torch.zeros(1, 8, dtype=torch.int32, device="cuda"), prefix_lengths=ints(prefixes)) if starts else {}
+    o, _ = ch.paged(q, none, none, table, lens, dt, **how)
+    bad = [0, 2] + ([1] if starts else [])
+    good = [i for i in range(4) if i not in bad]
+    assert bool(torch.isnan(o[bad]).all()) and bool((o[good] == 0).all())
+    o, _ = ch.packed(q[:, 0], None, None, ints([0, 1, 2, 3, 4]), dt, kp=none, vp=none, table=table, lengths=lens)
+    assert bool(torch.isnan(o[[0, 2]]).all()) and bool((o[[1, 3]] == 0).all())
