@@ -38,9 +38,10 @@ struct Share { int units, shares, from, to, entry, entry_at; }; // of all; how m
 // By a wavefront; up to 256 sequences four to a lane, more in runs, one to a lane.
 __device__ inline Share own_share(const CacheArgs &a, int index) {
     const int lane = threadIdx.x % WAVE, n = a.entries;
-    auto scan = [&](int v) {
+    auto scan = [&](int v, int count) { // over the first `count` lanes: as many trips as they need
 #pragma unroll
         for (int d = 1; d < WAVE; d *= 2) {
+            if (d >= count) break;
             const int other = __shfl_up(v, d, WAVE);
             if (lane >= d) v += other;
         }
@@ -60,8 +61,9 @@ __device__ inline Share own_share(const CacheArgs &a, int index) {
     for (int i = 0; i < 4; ++i) {
         upto[i] = 0;
         if (i > 0 && (!few || WAVE * i >= n)) continue;
-        upto[i] = total + scan(u[i]);
-        total = __builtin_amdgcn_readlane(upto[i], WAVE - 1);
+        const int count = few ? min(n - WAVE * i, WAVE) : WAVE;
+        upto[i] = total + scan(u[i], count);
+        total = __builtin_amdgcn_readlane(upto[i], count - 1);
     }
     Share s;
     s.units = total;
