@@ -341,7 +341,12 @@ CachePlan step_plan(const CacheArgs &a, int max_kv, int max_prefix) {
     // parts of a prefix: one work-group for each CU, of 128 rows, in 32 bits two
     const bool f32 = a.dtype == AXHIP_DTYPE_F32;
     const int64_t per = f32 ? 16 : 128, blocks = (a.entries * rows + per - 1) / per * a.kv_heads;
-    p.parts = a.groups == 0 ? 0 : static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({64, (f32 ? 512 : 256) / blocks, (std::min<int64_t>(std::max(max_prefix, 1), most_prefix) + 63) / 64})));
+    const int64_t prefix = std::min<int64_t>(std::max(max_prefix, 1), most_prefix);
+    int64_t places = (f32 ? 512 : 256) / blocks;
+    // .. half as many, of up to 1024 keys, beside own keys that take long themselves, by the hint: 64 sequences of 300 keys behind 8192 46.2 -> 44.3 us
+    const double own_us = static_cast<double>(a.entries) * static_cast<double>(std::min<int64_t>(std::max(max_kv, 0), most)) * a.kv_heads * a.D * 4 / 5.2e6;
+    if (!f32 && own_us > 15) places = std::min(places, std::max(128 / blocks, (prefix + 1023) / 1024));
+    p.parts = a.groups == 0 ? 0 : static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({64, places, (prefix + 63) / 64})));
     // shares of the own keys: two work-groups of four waves on each CU (64 sequences of 2000: 256 work-groups 105 us, 512 103, 1024 105), less what prefixes take of them in the same launch
     const int64_t groups = step_groups ? step_groups : f32 ? 512 : std::max<int64_t>(256, 512 - blocks * p.parts);
     p.shares = static_cast<int>(std::min<int64_t>(std::max<int64_t>(1, groups / (a.kv_heads * tiles)), (most + 127) / 128 * a.entries));

@@ -1,5 +1,5 @@
 // A decoding step with prefixes, 16 bits: the tiles of the prefixes and the shares of the own keys in one launch, so that what is bound by the matrix pipe and by a chain of latencies
-// runs beside what is bound by memory: 64 sequences of 300 keys behind 8192, 32 heads on 8 of 128 dims, 40 us and the join's 6 (two launches one behind the other: 58 in all).
+// runs beside what is bound by memory: 64 sequences of 300 keys behind 8192, 32 heads on 8 of 128 dims, 44.5 us with the join (two launches one behind the other: 58).
 #pragma once
 
 #include "sdpa_rows.hpp"
