@@ -47,6 +47,8 @@ class PageBook {
     // Room for so many new tokens behind each sequence: the copies that have to be made first (a page that a sequence is to write to and shares) are added to `copies`.  Either all of
     // them get room, or RuntimeError and nothing changes.  A sequence may be named once.
     void extend(const std::vector<int> &sequences, const std::vector<size_t> &new_tokens, std::vector<Copy> &copies);
+    // .. undone, where nothing has changed since; `copies` are those of that extension alone, and what they would have written to is free again
+    void take_back(const std::vector<int> &sequences, const std::vector<size_t> &new_tokens, const std::vector<Copy> &copies);
     // Pages in use move to the front of the pool, the others' places behind them: the copies that do so, which have been entered already
     std::vector<Copy> compact();
 
@@ -106,6 +108,7 @@ class PagedCache {
         changed();
     }
     size_t length(int sequence) const { return book_.length(sequence); }
+    // Where one of the following fails, on the device too, nothing has changed: sequences, pages and steps are as they were.
     size_t compact(); // how many pages moved
     // Room for new tokens behind each sequence (pages that have to be copied for it are).  Neighbours whose first pages are the same, as forks have them, are read as one prefix
     // when every sequence gets as many tokens.
@@ -121,6 +124,7 @@ class PagedCache {
 
   private:
     void copy(const std::vector<PageBook::Copy> &copies);
+    CacheStep step_of(const std::vector<int> &sequences, const std::vector<size_t> &new_tokens) const;
     void changed();
     void need_current(const CacheStep &step) const;
 

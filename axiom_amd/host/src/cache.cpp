@@ -248,6 +248,24 @@ void PageBook::extend(const std::vector<int> &sequences, const std::vector<size_
     }
 }
 
+void PageBook::take_back(const std::vector<int> &sequences, const std::vector<size_t> &new_tokens, const std::vector<Copy> &copies) {
+    size_t copied = copies.size(); // (in the sequences' order)
+    for (size_t i = sequences.size(); i-- > 0;) {
+        if (new_tokens[i] == 0) continue;
+        Sequence &s = at(sequences[i]);
+        s.length -= new_tokens[i];
+        while (s.pages.size() > (s.length + page_size_ - 1) / page_size_) {
+            drop(s.pages.back());
+            s.pages.pop_back();
+        }
+        if (s.length % page_size_ != 0 && copied > 0 && copies[copied - 1].dst == s.pages.back()) {
+            drop(s.pages.back());
+            s.pages.back() = copies[--copied].src;
+            ++users_[s.pages.back()];
+        }
+    }
+}
+
 std::vector<PageBook::Copy> PageBook::compact() {
     const size_t used = users_.size() - free_.size();
     std::vector<int32_t> to(users_.size(), -1); // where a page moves
@@ -331,9 +349,12 @@ void PagedCache::copy(const std::vector<PageBook::Copy> &copies) {
     AXHIP_CALL(axhip_kv_copy_pages(&p, nullptr));
 }
 
+// (Pages are copied to pages that are free by the old book: until the new one holds, nobody minds what lies there.)
 size_t PagedCache::compact() {
-    const std::vector<PageBook::Copy> copies = book_.compact();
+    PageBook compacted = book_;
+    const std::vector<PageBook::Copy> copies = compacted.compact();
     copy(copies);
+    book_ = std::move(compacted);
     changed();
     return copies.size();
 }
@@ -344,11 +365,22 @@ CacheStep PagedCache::extend(const std::vector<int> &sequences, const std::vecto
         if (n == 0) throw ValueError("PagedCache: a step has a token at least of each of its sequences");
     std::vector<PageBook::Copy> copies;
     book_.extend(sequences, new_tokens, copies);
-    copy(copies);
+    CacheStep step;
+    try {
+        copy(copies);
+        step = step_of(sequences, new_tokens);
+    } catch (...) { // (memory, a launch that is refused)
+        book_.take_back(sequences, new_tokens, copies);
+        throw;
+    }
     changed();
+    step.version = version_;
+    return step;
+}
+
+CacheStep PagedCache::step_of(const std::vector<int> &sequences, const std::vector<size_t> &new_tokens) const {
     const size_t n = sequences.size(), page = book_.page_size();
     CacheStep step;
-    step.version = version_;
     step.sequences = sequences;
     step.new_tokens = new_tokens;
     step.each = new_tokens[0];

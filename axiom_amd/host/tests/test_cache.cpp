@@ -3,6 +3,7 @@
 #include <map>
 #include <set>
 
+#include "axhip.h"
 #include "oracle_util.hpp"
 #include "test_framework.hpp"
 
@@ -180,6 +181,60 @@ TEST(PageBook, RandomOperationsKeepWhatSequencesHold) {
     }
 }
 
+// Extensions that are taken back leave no trace: pages, their users and the order in which free ones are taken are as before
+TEST(PageBook, ExtensionsAreTakenBack) {
+    PageBook book(40, 4), twin(40, 4);
+    std::vector<int> live;
+    uint32_t r = 777;
+    auto any = [&](uint32_t n) {
+        r = r * 1664525u + 1013904223u;
+        return (r >> 12) % n;
+    };
+    for (int turn = 0; turn < 2000; ++turn) {
+        const uint32_t what = any(8);
+        if (what == 0 || live.empty()) {
+            live.push_back(book.add());
+            twin.add();
+        } else if (what == 1) {
+            const int from = live[any(live.size())];
+            live.push_back(book.fork(from));
+            twin.fork(from);
+        } else if (what == 2) {
+            const size_t i = any(live.size()), n = any(book.length(live[i]) + 1);
+            book.truncate(live[i], n);
+            twin.truncate(live[i], n);
+        } else if (what == 3) {
+            const size_t i = any(live.size());
+            book.release(live[i]);
+            twin.release(live[i]);
+            live.erase(live.begin() + i);
+        } else {
+            std::vector<int> batch;
+            std::vector<size_t> more;
+            for (int s : live)
+                if (any(3) == 0) {
+                    batch.push_back(s);
+                    more.push_back(any(6));
+                }
+            const bool keep = any(2) == 0;
+            std::vector<PageBook::Copy> copies;
+            try {
+                book.extend(batch, more, copies);
+            } catch (const RuntimeError &) {
+                continue;
+            }
+            std::vector<PageBook::Copy> same;
+            if (keep) twin.extend(batch, more, same);
+            else book.take_back(batch, more, copies);
+        }
+        ASSERT_TRUE(book.free_pages() == twin.free_pages());
+        for (int s : live) {
+            ASSERT_TRUE(book.length(s) == twin.length(s));
+            ASSERT_TRUE(book.pages(s) == twin.pages(s));
+        }
+    }
+}
+
 TEST(Cache, CpuTensorsAndMismatchesThrow) {
     const Tensor x = Tensor::zeros({2, 4, 8}), i = Tensor::zeros({2}, DType::Int32);
     EXPECT_THROW(ops::rotary(x, i, i), RuntimeError);
@@ -328,4 +383,33 @@ GPU_TEST(Cache, PromptsForksAndSteps) {
         EXPECT_THROW(nn::PagedCache(layers, 64, page, kv, dim, dt).attend(0, last, q), ValueError);
         EXPECT_THROW(cache.attend(0, last, q.astype(DType::Float16)), TypeError);
     }
+}
+
+// Device work that fails (copies of 2^20 layers are refused on the host, before any launch) leaves the book and the steps as they were
+GPU_TEST(Cache, FailedCopiesChangeNothing) {
+    nn::PagedCache cache(size_t(1) << 20, 4, 2, 1, 1, DType::Float32);
+    const Tensor x = axtest::randn({1, 1, 1}, 1).gpu();
+    const int a = cache.add();
+    const nn::CacheStep step = cache.extend({a}, {1});
+    const int b = cache.fork(a);
+    EXPECT_THROW(cache.extend({a, b}, {2, 3}), DeviceError); // one of them is to copy the page that both have
+    for (int s : {a, b}) {
+        EXPECT_EQ(cache.length(s), size_t(1));
+        EXPECT_TRUE(cache.book().pages(s) == (std::vector<int32_t>{0}));
+    }
+    EXPECT_EQ(cache.book().free_pages(), size_t(3));
+    EXPECT_EQ(cache.append(5, step, x, x, x).shape(), x.shape()); // the step is as good as before
+    const int c = cache.add();
+    cache.extend({c}, {1});
+    cache.release(a);
+    cache.release(b);
+    const nn::CacheStep more = cache.extend({c}, {1});
+    EXPECT_THROW(cache.compact(), DeviceError); // page 1 is to move to the place of page 0
+    EXPECT_EQ(cache.length(c), size_t(2));
+    EXPECT_TRUE(cache.book().pages(c) == (std::vector<int32_t>{1}));
+    EXPECT_EQ(cache.book().free_pages(), size_t(3));
+    EXPECT_EQ(cache.append(5, more, x, x, x).shape(), x.shape());
+    const int d = cache.add();
+    cache.extend({d}, {6});
+    EXPECT_TRUE(cache.book().pages(d) == (std::vector<int32_t>{0, 2, 3}));
 }
