@@ -52,6 +52,13 @@ class PageBook {
     // Pages in use move to the front of the pool, the others' places behind them: the copies that do so, which have been entered already
     std::vector<Copy> compact();
 
+    // Neighbours that begin with the same pages, counting whole ones in front of their last new_tokens: the sequences from the group before it up to `end` have the first `pages` pages in
+    // common (0 for one by itself).  Of all divisions, one that leaves the fewest pages to read where each group's common ones are read once.
+    struct Group {
+        size_t end, pages;
+    };
+    std::vector<Group> groups(const std::vector<int> &sequences, const std::vector<size_t> &new_tokens) const;
+
     size_t length(int sequence) const { return at(sequence).length; }
     const std::vector<int32_t> &pages(int sequence) const { return at(sequence).pages; }
     int64_t slot(int sequence, size_t position) const; // page * page_size + row
@@ -111,7 +118,7 @@ class PagedCache {
     // Where one of the following fails, on the device too, nothing has changed: sequences, pages and steps are as they were.
     size_t compact(); // how many pages moved
     // Room for new tokens behind each sequence (pages that have to be copied for it are).  Neighbours whose first pages are the same, as forks have them, are read as one prefix
-    // when every sequence gets as many tokens.
+    // when every sequence gets as many tokens, 16 at most: by PageBook::groups.
     CacheStep extend(const std::vector<int> &sequences, const std::vector<size_t> &new_tokens);
     // Keys and values (tokens, kv_heads, head_dim) of a step into a layer, keys rotated by `turns` (empty: not rotated); the answer is q (tokens, heads, head_dim) rotated alike.
     Tensor append(size_t layer, const CacheStep &step, const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &turns = Tensor(), bool interleaved = false, float amplitude = 1.0f);

@@ -181,6 +181,67 @@ TEST(PageBook, RandomOperationsKeepWhatSequencesHold) {
     }
 }
 
+// Groups of neighbours behind the pages that they share: no other division leaves fewer pages to read, by trying all of them
+TEST(PageBook, GroupsReadTheFewestPages) {
+    uint32_t r = 4242;
+    auto any = [&](uint32_t n) {
+        r = r * 1664525u + 1013904223u;
+        return (r >> 12) % n;
+    };
+    for (int turn = 0; turn < 400; ++turn) {
+        PageBook book(400, 2);
+        std::vector<PageBook::Copy> copies;
+        std::vector<int> batch;
+        const size_t n = 1 + any(8);
+        for (size_t i = 0; i < n; ++i) {
+            if (i == 0 || any(4) == 0) {
+                batch.push_back(book.add());
+            } else { // another one's first tokens
+                batch.push_back(book.fork(batch[any(3) ? any(i) : i - 1]));
+                book.truncate(batch.back(), any(book.length(batch.back()) + 1));
+            }
+            book.extend({batch.back()}, {any(20)}, copies);
+        }
+        std::vector<size_t> more;
+        for (size_t i = 0; i < n; ++i) more.push_back(1 + any(3));
+        book.extend(batch, more, copies);
+        auto whole = [&](size_t i) { return (book.length(batch[i]) - more[i]) / 2; }; // pages in front of the new tokens
+        auto shared = [&](size_t from, size_t end) { // by all of [from, end); one by itself shares none
+            if (end == from + 1) return size_t(0);
+            size_t most = whole(from);
+            for (size_t i = from + 1; i < end; ++i) {
+                size_t same = 0;
+                while (same < std::min(most, whole(i)) && book.pages(batch[i])[same] == book.pages(batch[from])[same]) ++same;
+                most = same;
+            }
+            return most;
+        };
+        size_t most = 0; // pages that need not be read again
+        for (uint32_t cuts = 0; cuts < 1u << (n - 1); ++cuts) {
+            size_t saved = 0, from = 0;
+            for (size_t end = 1; end <= n; ++end)
+                if (end == n || (cuts >> (end - 1) & 1)) {
+                    saved += (end - from - 1) * shared(from, end);
+                    from = end;
+                }
+            most = std::max(most, saved);
+        }
+        size_t saved = 0, from = 0;
+        for (const PageBook::Group &g : book.groups(batch, more)) {
+            ASSERT_TRUE(g.end > from && g.end <= n);
+            ASSERT_TRUE(g.pages == shared(from, g.end));
+            ASSERT_TRUE(g.end == from + 1 || g.pages > 0);
+            saved += (g.end - from - 1) * g.pages;
+            from = g.end;
+        }
+        ASSERT_TRUE(from == n);
+        ASSERT_TRUE(saved == most);
+    }
+    PageBook book(4, 2);
+    EXPECT_TRUE(book.groups({}, {}).empty());
+    EXPECT_THROW(book.groups({0}, {1}), IndexError);
+}
+
 // Extensions that are taken back leave no trace: pages, their users and the order in which free ones are taken are as before
 TEST(PageBook, ExtensionsAreTakenBack) {
     PageBook book(40, 4), twin(40, 4);
@@ -412,4 +473,26 @@ GPU_TEST(Cache, FailedCopiesChangeNothing) {
     const int d = cache.add();
     cache.extend({d}, {6});
     EXPECT_TRUE(cache.book().pages(d) == (std::vector<int32_t>{0, 2, 3}));
+}
+
+// A neighbour that shares little does not take their long prefix from the others, wherever it stands
+GPU_TEST(Cache, PrefixesOfUnequalNeighbours) {
+    const size_t page = 16, kv = 2, dim = 64;
+    nn::PagedCache cache(1, 64, page, kv, dim, DType::BFloat16);
+    const int deep = cache.add();
+    cache.extend({deep}, {20 * page});
+    const int other = cache.fork(deep);
+    cache.truncate(other, page); // the first page only
+    cache.extend({other}, {5 * page});
+    const int second = cache.fork(deep), third = cache.fork(deep);
+    auto lengths = [&](const nn::CacheStep &step) {
+        const Tensor p = step.prefix_lengths.cpu();
+        return std::vector<int32_t>(p.typed_data<int32_t>(), p.typed_data<int32_t>() + p.size());
+    };
+    const int32_t long_one = 20 * page;
+    EXPECT_TRUE(lengths(cache.extend({deep, second, third, other}, {1, 1, 1, 1})) == (std::vector<int32_t>{long_one, 0}));
+    EXPECT_TRUE(lengths(cache.extend({other, third, second, deep}, {1, 1, 1, 1})) == (std::vector<int32_t>{0, long_one}));
+    EXPECT_TRUE(lengths(cache.extend({second, other, third, deep}, {1, 1, 1, 1})) == (std::vector<int32_t>{16, long_one}));
+    const int sixth = cache.fork(other);
+    EXPECT_TRUE(lengths(cache.extend({other, sixth, third, deep}, {1, 1, 1, 1})) == (std::vector<int32_t>{6 * 16, long_one}));
 }
