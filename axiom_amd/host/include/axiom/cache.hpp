@@ -24,8 +24,8 @@ Tensor rotary_turns(size_t rot_dim, double theta = 10000.0, const RotaryScaling 
 Tensor rotary(const Tensor &x, const Tensor &positions, const Tensor &turns, bool interleaved = false, bool inverse = false, float amplitude = 1.0f);
 
 // Attention of sequences side by side: q (tokens, heads, head_dim), k and v (tokens', kv_heads, head_dim), starts Int32 (n + 1) on the GPU: sequence i owns rows starts[i] ..
-// starts[i + 1] - 1.  Causal: the last query of a sequence sees every key of it.  longest_keys: about how many keys the longest sequence has, 0: as many as there are (for the
-// division of the work alone).  Rows of the result that no sequence owns are zeros.
+// starts[i + 1] - 1.  Causal: the last query of a sequence sees every key of it.  longest_keys: about how many keys the longest sequence has (for the division of
+// the work alone), 0: not known, and taken to be up to twice the average.  Rows of the result that no sequence owns are zeros.
 Tensor packed_attention(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &starts_q, const Tensor &starts_kv, bool is_causal = true, float scale = -1.0f, size_t longest_keys = 0);
 
 } // namespace ops

@@ -135,7 +135,9 @@ Tensor packed_attention(const Tensor &q, const Tensor &k, const Tensor &v, const
     p.scale = scale;
     p.total_q = static_cast<int64_t>(q.shape()[0]);
     p.total_kv = static_cast<int64_t>(k.shape()[0]);
-    p.max_kv = static_cast<int32_t>(std::min<size_t>(longest_keys ? longest_keys : k.shape()[0], 1u << 30));
+    // (What the starts hold is on the device: a sequence is taken to have up to twice the average. As many as all together have, 20 prompts of 60 tokens would be computed in three parts and joined.)
+    const size_t total = k.shape()[0], n = starts_q.size() - 1;
+    p.max_kv = static_cast<int32_t>(std::min<size_t>(longest_keys ? longest_keys : n == 0 ? total : std::min(total, 2 * ((total + n - 1) / n)), 1u << 30));
     strides_into(p.q_strides, qs);
     strides_into(p.k_strides, ks);
     strides_into(p.v_strides, vs);

@@ -496,3 +496,19 @@ GPU_TEST(Cache, PrefixesOfUnequalNeighbours) {
     const int sixth = cache.fork(other);
     EXPECT_TRUE(lengths(cache.extend({other, sixth, third, deep}, {1, 1, 1, 1})) == (std::vector<int32_t>{6 * 16, long_one}));
 }
+
+// Without longest_keys the division of the work goes by the number of sequences too, not as though each had all keys
+GPU_TEST(Cache, PackedAttentionWithoutAHint) {
+    auto kernel_of = [](size_t sequences, size_t each, size_t heads, size_t kv, size_t dim, size_t hint) {
+        std::vector<int32_t> starts;
+        for (size_t i = 0; i <= sequences; ++i) starts.push_back(static_cast<int32_t>(i * each));
+        const Tensor q = axtest::randn({sequences * each, heads, dim}, 1).bfloat16().gpu(), k = axtest::randn({sequences * each, kv, dim}, 2).bfloat16().gpu();
+        ops::packed_attention(q, k, k, ints(starts), ints(starts), true, -1.0f, hint);
+        return std::string(axhip_sdpa_cache_last_kernel());
+    };
+    EXPECT_EQ(kernel_of(20, 60, 8, 8, 64, 60), std::string("tile"));
+    EXPECT_EQ(kernel_of(20, 60, 8, 8, 64, 0), std::string("tile"));
+    EXPECT_EQ(kernel_of(64, 256, 32, 8, 128, 256), std::string("tile"));
+    EXPECT_EQ(kernel_of(64, 256, 32, 8, 128, 0), std::string("tile"));
+    EXPECT_EQ(kernel_of(1, 4096, 32, 8, 128, 0), std::string("tile, eight waves")); // (one sequence has them all)
+}
