@@ -126,20 +126,21 @@ __global__ __launch_bounds__(256) void move_heads_kernel(const MoveArgs a) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
         if (!to[i]) continue;
+        // (Which of two products keeps all its bits is written down: left to the compiler, it was not the same one in every variant of the kernel, and a token's result could depend on the batch.)
         if (turns && static_cast<int>(group + i * a.groups.d) < a.heads + a.kv_heads) {
             if constexpr (PAIRS) {
 #pragma unroll
                 for (int j = 0; j < V / 2; ++j) {
                     const float p = get<DT, V>(x[i], 2 * j), r = get<DT, V>(x[i], 2 * j + 1);
-                    put<DT, V>(x[i], 2 * j, p * t[j].c - r * t[j].s);
-                    put<DT, V>(x[i], 2 * j + 1, r * t[j].c + p * t[j].s);
+                    put<DT, V>(x[i], 2 * j, __builtin_fmaf(p, t[j].c, -(r * t[j].s)));
+                    put<DT, V>(x[i], 2 * j + 1, __builtin_fmaf(r, t[j].c, p * t[j].s));
                 }
             } else {
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
                     const float p = get<DT, V>(x[i], j), r = get<DT, V>(y[i], j);
-                    put<DT, V>(x[i], j, p * t[j].c - r * t[j].s);
-                    put<DT, V>(y[i], j, r * t[j].c + p * t[j].s);
+                    put<DT, V>(x[i], j, __builtin_fmaf(p, t[j].c, -(r * t[j].s)));
+                    put<DT, V>(y[i], j, __builtin_fmaf(r, t[j].c, p * t[j].s));
                 }
             }
         }

@@ -155,3 +155,47 @@ def test_copy(dt, by_head, pad, pairs, layers, heads, dim, page, partial):
     capi.check(capi.lib().axhip_kv_copy_pages(C.byref(p), None))
     ch.sync()
     assert torch.equal(kp, want[0]) and torch.equal(vp, want[1])
+
+
+# 64 MiB and more of output, which are stored past the caches, are the same bits as in calls of less
+@pytest.mark.parametrize("dt,heads,dim,rot,tokens", [("bf16", 9, 80, 32, 46700), ("f32", 7, 96, 96, 25001), ("f16", 5, 36, 20, 190001)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rope_of_large_outputs(dt, heads, dim, rot, tokens, interleaved):
+    x = normal(tokens, heads, dim, dt=dt, seed=4)
+    assert x.numel() * x.element_size() >= 64 << 20
+    positions, table = torch.randint(0, 1 << 20, (tokens,), generator=ch.generator(5)).cuda(), ch.turns(rot)
+    how = dict(table=ch.device_turns(table), rot=rot, interleaved=interleaved, dt=dt)
+    y = ch.rope(x, positions, **how)
+    for rows in torch.arange(tokens).split(-(-tokens // 3)):
+        part = slice(int(rows[0]), int(rows[-1]) + 1)
+        assert torch.equal(y[part], ch.rope(x[part], positions[part], **how))
+    some = torch.tensor([0, 1, tokens // 2, tokens - 1])
+    near(y[some.cuda()], *ch.rotated(x[some.cuda()], positions.cpu()[some], table, rot, interleaved), dt)
+    ch.rope(x, positions, **how, out=x)
+    assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dt,heads,kv_heads,dim,rot,tokens,page,by_head", [("bf16", 5, 3, 96, 64, 32003, 16, True), ("f32", 3, 1, 80, 80, 43000, 64, False), ("f16", 7, 2, 128, 0, 24001, 8, False)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_append_of_large_outputs(dt, heads, kv_heads, dim, rot, tokens, page, by_head, interleaved):
+    n_pages = -(-tokens // page) + 3
+    qkv = normal(tokens, heads + 2 * kv_heads, dim, dt=dt, seed=6)
+    assert qkv.numel() * qkv.element_size() >= 64 << 20
+    q, k, v = qkv[:, :heads], qkv[:, heads:heads + kv_heads], qkv[:, heads + kv_heads:]
+    slots = torch.randperm(n_pages * page, generator=ch.generator(7))[:tokens].cuda()
+    slots[-tokens // 16:] = -1
+    positions, table = torch.randint(0, 100000, (tokens,), generator=ch.generator(8)).cuda(), ch.device_turns(ch.turns(rot)) if rot else None
+    got = []
+    for parts in (1, 3):
+        kp, vp = ch.pool(n_pages, page, kv_heads, dim, dt, by_head, seed=9)
+        q_out = torch.full((tokens, heads, dim), ch.LEFT, dtype=qkv.dtype, device="cuda")
+        for rows in torch.arange(tokens).split(-(-tokens // parts)):
+            part = slice(int(rows[0]), int(rows[-1]) + 1)
+            ch.append(q[part], k[part], v[part], q_out[part], kp, vp, slots[part], dt, positions=positions[part] if rot else None, table=table, rot=rot, interleaved=interleaved)
+        got.append((kp, vp, q_out))
+    for one, three in zip(*got):
+        assert torch.equal(one, three)
+    written = slots >= 0
+    assert torch.equal(got[0][1][slots[written] // page, slots[written] % page], v[written])
+    ch.append(q, k, v, q, kp, vp, slots, dt, positions=positions if rot else None, table=table, rot=rot, interleaved=interleaved)  # q in place
+    assert torch.equal(q, q_out)
