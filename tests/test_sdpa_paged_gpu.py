@@ -161,6 +161,22 @@ def test_every_run_gives_the_same_bits(dt):
         assert torch.equal(s.run()[0], first)
 
 
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("groups,new", [(70, 1), (300, 1), (300, 3), (4200, 1)])
+def test_more_groups_than_a_wavefront_has_lanes(dt, groups, new):
+    """Of up to four sequences, every fifth of none, some behind a prefix of no keys; sequences without a group in front and behind."""
+    starts, prefixes = [2], []
+    for g in range(groups):
+        starts.append(starts[-1] + (0 if g % 5 == 4 else (g * 7) % 5 if groups < 1000 else 1 if g % 9 == 0 else 0))
+        prefixes.append(0 if g % 11 == 3 else 1 + (g * 29) % 90)
+    n = starts[-1] + 3
+    s = Step([(i * 37) % 60 for i in range(n)], new, 2, 1, 64, 16, dt, starts=starts, prefixes=prefixes, seed=groups, ld=64)
+    o, kernel = s.run()
+    assert kernel == "shares, prefix"
+    s.kp, s.vp = s.kp.cpu().double(), s.vp.cpu().double()  # (once for all sequences)
+    s.check(o)
+
+
 @pytest.mark.parametrize("dt", ["bf16", "f32"])
 def test_more_sequences_than_a_wavefront_has_lanes(dt):
     for n in (64, 65, 257, 1030):
