@@ -11,7 +11,7 @@ namespace {
 
 // The angle position * turns modulo 2^64 as (cos, sin): the nearest quarter turn is taken off, which leaves |r| <= pi / 4 for the series of
 // both; the first term left out is r^11 / 11! < 1.8e-9 and r^12 / 12! < 1.2e-10.  (An angle formed in 32 bits is 0.004 radians off at
-// position 100000; here the fraction of a turn is cut to 32 bits, 1.5e-9 radians.)
+// position 100000; here the fraction of a turn is rounded to 32 bits, 7e-10 radians.)
 struct CosSin { float c, s; };
 __device__ __forceinline__ CosSin turned(int64_t position, uint64_t turns, float amplitude) {
     const uint32_t at = static_cast<uint32_t>((static_cast<uint64_t>(position) * turns + 0x80000000u) >> 32);

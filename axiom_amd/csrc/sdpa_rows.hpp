@@ -167,7 +167,7 @@ template <int DT, int D, bool PAD, int OF, class Next> __device__ __forceinline_
         return q;
     };
 
-    // ---- K and V from memory.  Rows behind the last key are that key again; dims behind the head size of K are zeros, of V the last ones again.
+    // ---- K and V from memory.  Rows behind the last key are that key again; dims behind the head size: of K zeros, of V the first ones again, whose results nobody stores.
     const unsigned char *kb = static_cast<const unsigned char *>(a.k) + kvh * a.ks[2] * ES, *vb = static_cast<const unsigned char *>(a.v) + kvh * a.vs[2] * ES;
     const int64_t k_page = a.ks[0] * ES, v_page = a.vs[0] * ES, k_row = a.ks[1] * ES, v_row = a.vs[1] * ES;
     int k_dim[KJ], v_dim[VH]; // bytes into a row

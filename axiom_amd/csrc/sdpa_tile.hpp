@@ -6,8 +6,8 @@
 // alternation, the softmax follows.  With eight waves the upper four (one of each SIMD's two) do that in the other order, so that one of the two is
 // in its matrix phase while the other one is in its vector phase.
 //
-// Bound by the vector work between the matrix phases (32 exponentials and 80 other instructions a lane and tile, 930 cycles beside 1024 of MFMAs) and by the power limit: 12 prompts of 16384 tokens,
-// 32 heads on 8 of 128 dims, 400 - 415 us, 0.96 - 0.99 PFLOP/s of the causal half, the matrix pipe busy 47 % of the time at 1.9 GHz.
+// Bound by the vector work between the matrix phases (32 exponentials and 80 other instructions a lane and tile, 930 cycles beside 1024 of MFMAs), which runs beside them for a small part only: 12
+// prompts of 16384 tokens, 32 heads on 8 of 128 dims, 400 - 415 us, 0.96 - 0.99 PFLOP/s of the causal half, matrix pipe and vector instructions busy 47 % of the cycles each, at 1.9 GHz.
 //
 // What the ragged form asks for:
 //  * rows are tokens times the heads that share a key head: one tile of keys serves them all, and a short sequence fills the work-group.

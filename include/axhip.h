@@ -555,8 +555,8 @@ int axhip_sample_ws(const void *logits, int64_t *tokens, float *probs, const Axh
  * whose attention takes keys that lie in one piece per (batch, head), of one length for the batch.
  *
  * Angles are fractions of a full turn in 64 bits: turns[i] = 2^64 f_i / (2 pi), f_i radians a position.  position * turns[i] modulo
- * 2^64 is then the angle of any position, a negative one too, to position * 2^-65 turns: what 64 bits keep of position 2^31, a
- * product of 32-bit numbers loses at position 2^10.
+ * 2^64 is then the angle of any position, a negative one too, to position * 2^-65 turns (2^-34 at position 2^31; a table of 32 bits is
+ * position * 2^-33 off), and the kernels round it to 2^-33.
  * axhip_rope_turns fills such a table on the host (rot_dim / 2 values; no device is needed); copy it to the device once.  f_i =
  * theta^(-2 i / rot_dim), and for contexts longer than the trained `length`:
  *     LINEAR  f_i / factor
@@ -647,7 +647,9 @@ int axhip_kv_copy_pages(const AxhipKvCopyParams *params_host, void *stream);
  * Keys outside a sequence are neither read nor can what lies there matter; a key that a causal query does not see meets a weight of zero and has to be finite in V.
  * Numbers in cu_q, cu_kv and kv_lengths that lie outside the tensors are clamped to them (total_q and total_kv below 2^30, keys of a
  * sequence up to 2^30); a page that does not exist makes NaN of every query that sees a key of it (of others of its sequence too, at times).
- * o may not overlap the inputs.  max_kv: about how many keys the longest sequence has, which the division of the work goes by and nothing else.
+ * o may not overlap the inputs.  max_kv: about how many keys the longest sequence has, which the division of the work goes by and nothing else.  0 says that
+ * they are few, not that nothing is known: one sequence of 8000 keys (a decoding step, 32 heads on 8 of 128) takes 83 us with it and 14 with 8000 or
+ * more.  Where the host does not know lengths, give what there is room for (table_ld * page_size).
  * 16 bits with head_dim a multiple of 8 up to 256 and pages of 8 rows or more, 16-byte aligned, less than 4 GiB apart, on the matrix cores; fp32 with head_dim a multiple of 4 up to 128
  * likewise; everything else up to 256 dims on the generic kernel. */
 typedef struct {
@@ -677,7 +679,7 @@ int axhip_sdpa_packed_ws(const void *q, const void *k, const void *v, void *o, c
  * Shared prefixes: the sequences group_starts[g] .. group_starts[g + 1] - 1 have the prefix_lengths[g] keys in pages
  * prefix_table[g * prefix_ld + ..] in front of their own, all of which every token sees.  They are read once for the group, not once
  * for each of its sequences.  Sequences in front of the first group and behind the last have no prefix; groups may be empty.
- * Everything else as in axhip_sdpa_packed; max_kv and max_prefix are hints alike (own keys, prefix).  Lengths, tables and groups are
+ * Everything else as in axhip_sdpa_packed; max_kv and max_prefix are hints alike (own keys, prefix), 0 among them.  Lengths, tables and groups are
  * read on the device when the kernels run: a captured step replays with what the arrays hold then. */
 typedef struct {
     AxhipKvPages pages;
